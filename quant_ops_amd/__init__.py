@@ -29,6 +29,7 @@ from .int4_matmul import (
     unpack_int32_to_int4,
 )
 from .linear import prepare_w4a4_weight, w4a4_flatquant_linear
+from .mx import mx_dequantize, mx_matmul, mx_quantize, rms_norm_mx_quantize, swiglu_mx_quantize
 from .decompose import get_decompose_dim
 from . import meta_ops  # noqa: F401  (registers fakes once the schemas exist)
 

@@ -27,7 +27,8 @@ INCLUDE = os.path.join(ROOT, "include")
 OBJ = os.path.join(HERE, "_obj")
 
 HIP_SOURCES = ["capi.hip", "flatquant_quant.hip", "flatquant_tile_f16.hip", "flatquant_tile_bf16.hip",
-               "flatquant_f32.hip", "int4_gemm.hip", "int4_gemm_f6.hip", "dequant.hip", "layout.hip", "w4a4_linear.hip"]
+               "flatquant_f32.hip", "int4_gemm.hip", "int4_gemm_f6.hip", "dequant.hip", "layout.hip", "w4a4_linear.hip",
+               "mx_quantize.hip", "mx_gemm.hip"]
 LIB_NAME = "libquant_ops_hip.so"
 TORCH_LIB_NAME = "_quant_ops_torch.so"
 # microbenchmarks of the hardware ceilings (bench.py --ceilings), a library of its own

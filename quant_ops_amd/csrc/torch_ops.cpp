@@ -6,8 +6,9 @@
 // torch.ops.quant_ops.* and graph captures see the same operators. The others
 // are additions of this build: int4_matmul_ex (output dtype choice),
 // int4_matmul_bias (bias in the epilogue), w4a4_linear (the linear layer's
-// quantize + GEMM as one operator) and dequantize_int4 (a device kernel
-// for the reference's Python function).
+// quantize + GEMM as one operator), dequantize_int4 (a device kernel
+// for the reference's Python function) and the microscaled operators (mx_*,
+// *_mx_quantize).
 //
 // Unlike the reference, kernels go to the caller's current HIP stream and the
 // host is never synchronised (cuda_quant_kernel.cu:379-385 synchronised the
@@ -230,6 +231,176 @@ at::Tensor dequantize_int4(const at::Tensor& quantized, const at::Tensor& scales
   return out;
 }
 
+// ---------------------------------------------------------------------------
+// Microscaled formats: codes are uint8 (FP4, two per byte) or float8_e4m3fn
+// (FP8), scales uint8, one per 32 values; rows are padded to whole blocks.
+// ---------------------------------------------------------------------------
+int mx_format(c10::string_view fmt, const char* op) {
+  if (fmt == "mxfp4") return QO_MX_FP4;
+  TORCH_CHECK(fmt == "mxfp8", op, ": fmt must be \"mxfp4\" or \"mxfp8\", got \"", fmt, "\"");
+  return QO_MX_FP8;
+}
+
+int mx_codes_format(const at::Tensor& codes, const char* op, const char* name) {
+  if (codes.scalar_type() == at::kByte) return QO_MX_FP4;
+  TORCH_CHECK(codes.scalar_type() == at::kFloat8_e4m3fn, op, ": ", name,
+              " must be uint8 (FP4 codes) or float8_e4m3fn (FP8 codes), got ", codes.scalar_type());
+  return QO_MX_FP8;
+}
+
+// Empty codes and scales for [tokens, features].
+std::tuple<at::Tensor, at::Tensor> mx_outputs(const at::Tensor& like, int64_t tokens, int64_t features, int format) {
+  const int64_t blocks = (features + 31) / 32;
+  at::Tensor codes = format == QO_MX_FP4 ? at::empty({tokens, 16 * blocks}, like.options().dtype(at::kByte))
+                                         : at::empty({tokens, 32 * blocks}, like.options().dtype(at::kFloat8_e4m3fn));
+  return {codes, at::empty({tokens, blocks}, like.options().dtype(at::kByte))};
+}
+
+void check_rows(const at::Tensor& x, const char* op, const char* name) {
+  TORCH_CHECK(x.dim() == 2, op, ": ", name, " must be 2-D [tokens, features], got ", x.sizes());
+  TORCH_CHECK(x.is_cuda(), op, ": ", name, " must be a GPU tensor");
+  TORCH_CHECK(dtype_code(x.scalar_type()) >= 0, op, ": ", name, " dtype must be float32, float16 or bfloat16, got ",
+              x.scalar_type());
+}
+
+// Rows with unit inner stride that do not overlap; x itself where it has them.
+at::Tensor mx_rows(const at::Tensor& x) {
+  return x.stride(1) == 1 && (x.size(0) <= 1 || x.stride(0) >= x.size(1)) ? x : x.contiguous();
+}
+int64_t mx_ld(const at::Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
+
+std::tuple<at::Tensor, at::Tensor> mx_quantize(const at::Tensor& input, c10::string_view fmt) {
+  check_rows(input, "mx_quantize", "input");
+  const int format = mx_format(fmt, "mx_quantize");
+  c10::DeviceGuard guard(input.device());
+  at::Tensor x = mx_rows(input);
+  auto [codes, scales] = mx_outputs(x, x.size(0), x.size(1), format);
+  check_status(qo_mx_quantize(x.data_ptr(), dtype_code(x.scalar_type()), x.size(0), x.size(1), mx_ld(x), format,
+                              codes.data_ptr(), scales.data_ptr<uint8_t>(), current_stream(x)),
+               "mx_quantize");
+  return {codes, scales};
+}
+
+at::Tensor mx_dequantize(const at::Tensor& codes, const at::Tensor& scales, std::optional<int64_t> features,
+                         std::optional<at::ScalarType> out_dtype) {
+  TORCH_CHECK(codes.is_cuda() && scales.device() == codes.device(), "mx_dequantize: tensors must be on one GPU");
+  TORCH_CHECK(codes.dim() == 2 && scales.dim() == 2, "mx_dequantize: codes and scales must be 2-D");
+  const int format = mx_codes_format(codes, "mx_dequantize", "codes");
+  TORCH_CHECK(scales.scalar_type() == at::kByte, "mx_dequantize: scales must be uint8");
+  const int64_t T = codes.size(0), blocks = scales.size(1);
+  TORCH_CHECK(scales.size(0) == T && codes.size(1) == blocks * (format == QO_MX_FP4 ? 16 : 32),
+              "mx_dequantize: codes ", codes.sizes(), " and scales ", scales.sizes(), " do not match");
+  const int64_t F = features.value_or(32 * blocks);
+  TORCH_CHECK((F + 31) / 32 == blocks && F >= 0, "mx_dequantize: features (", F, ") must fill the ", blocks, " blocks of a row");
+  const at::ScalarType dtype = out_dtype.value_or(at::kFloat);
+  TORCH_CHECK(dtype_code(dtype) >= 0, "mx_dequantize: out_dtype must be float32, float16 or bfloat16");
+  c10::DeviceGuard guard(codes.device());
+  at::Tensor q = codes.contiguous(), s = scales.contiguous();
+  if (reinterpret_cast<uintptr_t>(q.data_ptr()) % 8 != 0) q = q.clone();
+  at::Tensor out = at::empty({T, F}, codes.options().dtype(dtype));
+  check_status(qo_mx_dequantize(q.data_ptr(), s.data_ptr<uint8_t>(), format, T, F, out.data_ptr(), dtype_code(dtype),
+                                current_stream(codes)),
+               "mx_dequantize");
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_mx_impl(const at::Tensor& input, const at::Tensor* residual,
+                                                                const at::Tensor& weight, double eps,
+                                                                c10::string_view fmt, const char* op) {
+  check_rows(input, op, "x");
+  const int format = mx_format(fmt, op);
+  const int64_t T = input.size(0), F = input.size(1);
+  TORCH_CHECK(weight.dim() == 1 && weight.size(0) == F, op, ": weight must hold one value per feature (", F, "), got ",
+              weight.sizes());
+  TORCH_CHECK(weight.device() == input.device() && dtype_code(weight.scalar_type()) >= 0, op,
+              ": weight must be float32, float16 or bfloat16 on x's device");
+  if (residual)
+    TORCH_CHECK(residual->sizes() == input.sizes() && residual->scalar_type() == input.scalar_type() &&
+                    residual->device() == input.device(),
+                op, ": residual must have x's shape, dtype and device");
+  c10::DeviceGuard guard(input.device());
+  at::Tensor x = mx_rows(input), w = weight.contiguous(), res, h;
+  if (residual) {
+    res = mx_rows(*residual);
+    h = at::empty({T, F}, input.options());
+  }
+  auto [codes, scales] = mx_outputs(x, T, F, format);
+  check_status(qo_rms_norm_mx_quantize(x.data_ptr(), residual ? res.data_ptr() : nullptr, dtype_code(x.scalar_type()),
+                                       T, F, mx_ld(x), residual ? mx_ld(res) : 0, w.data_ptr(),
+                                       dtype_code(w.scalar_type()), (float)eps, format, codes.data_ptr(),
+                                       scales.data_ptr<uint8_t>(), residual ? h.data_ptr() : nullptr,
+                                       current_stream(x)),
+               op);
+  return {codes, scales, h};
+}
+
+std::tuple<at::Tensor, at::Tensor> rms_norm_mx_quantize(const at::Tensor& x, const at::Tensor& weight, double eps,
+                                                        c10::string_view fmt) {
+  auto [codes, scales, h] = rms_norm_mx_impl(x, nullptr, weight, eps, fmt, "rms_norm_mx_quantize");
+  return {codes, scales};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_mx_quantize(const at::Tensor& x, const at::Tensor& residual,
+                                                                        const at::Tensor& weight, double eps,
+                                                                        c10::string_view fmt) {
+  return rms_norm_mx_impl(x, &residual, weight, eps, fmt, "add_rms_norm_mx_quantize");
+}
+
+std::tuple<at::Tensor, at::Tensor> swiglu_mx_quantize(const at::Tensor& gate_up, c10::string_view fmt) {
+  check_rows(gate_up, "swiglu_mx_quantize", "gate_up");
+  const int format = mx_format(fmt, "swiglu_mx_quantize");
+  TORCH_CHECK(gate_up.size(1) % 2 == 0, "swiglu_mx_quantize: gate_up must hold two halves, got ", gate_up.sizes());
+  c10::DeviceGuard guard(gate_up.device());
+  at::Tensor x = mx_rows(gate_up);
+  const int64_t T = x.size(0), F = x.size(1) / 2;
+  auto [codes, scales] = mx_outputs(x, T, F, format);
+  check_status(qo_swiglu_mx_quantize(x.data_ptr(), dtype_code(x.scalar_type()), T, F, mx_ld(x), format,
+                                     codes.data_ptr(), scales.data_ptr<uint8_t>(), current_stream(x)),
+               "swiglu_mx_quantize");
+  return {codes, scales};
+}
+
+// Codes whose rows the GEMM can read: 16-byte aligned, unit inner stride, not overlapping.
+at::Tensor mx_gemm_rows(const at::Tensor& codes) {
+  const bool fits = codes.stride(1) == 1 && reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0 &&
+                    (codes.size(0) <= 1 || (codes.stride(0) >= codes.size(1) && codes.stride(0) % 16 == 0));
+  return fits ? codes : codes.clone(at::MemoryFormat::Contiguous);
+}
+
+at::Tensor mx_matmul(const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& b, const at::Tensor& b_scales,
+                     const std::optional<at::Tensor>& bias, std::optional<at::ScalarType> out_dtype) {
+  TORCH_CHECK(a.is_cuda() && a_scales.device() == a.device() && b.device() == a.device() &&
+                  b_scales.device() == a.device(),
+              "mx_matmul: a, b and their scales must be on one GPU");
+  TORCH_CHECK(a.dim() == 2 && a_scales.dim() == 2 && b.dim() == 2 && b_scales.dim() == 2,
+              "mx_matmul: a, b and their scales must be 2-D");
+  const int format = mx_codes_format(a, "mx_matmul", "a");
+  TORCH_CHECK(b.scalar_type() == at::kByte, "mx_matmul: b must be uint8 (FP4 codes), got ", b.scalar_type());
+  TORCH_CHECK(a_scales.scalar_type() == at::kByte && b_scales.scalar_type() == at::kByte,
+              "mx_matmul: scales must be uint8");
+  const int64_t M = a.size(0), N = b.size(0), blocks = a_scales.size(1), K = 32 * blocks;
+  TORCH_CHECK(a_scales.size(0) == M && a.size(1) == (format == QO_MX_FP4 ? K / 2 : K), "mx_matmul: a ", a.sizes(),
+              " and a_scales ", a_scales.sizes(), " do not match");
+  TORCH_CHECK(b_scales.size(0) == N && b_scales.size(1) == blocks && b.size(1) == K / 2, "mx_matmul: b ", b.sizes(),
+              " and b_scales ", b_scales.sizes(), " do not match a's ", blocks, " blocks");
+  const at::ScalarType dtype = out_dtype.value_or(at::kBFloat16);
+  const int od = dtype_code(dtype);
+  TORCH_CHECK(od >= 0, "mx_matmul: out_dtype must be float16, bfloat16 or float32");
+  c10::DeviceGuard guard(a.device());
+  at::Tensor A = mx_gemm_rows(a), B = mx_gemm_rows(b), sa = mx_rows(a_scales), sb = mx_rows(b_scales), bv;
+  if (bias.has_value()) {
+    TORCH_CHECK(bias->device() == a.device() && bias->numel() == N, "mx_matmul: bias must hold N (", N,
+                ") elements on a's device");
+    bv = bias->to(dtype).reshape({N}).contiguous();
+  }
+  at::Tensor out = at::empty({M, N}, a.options().dtype(dtype));
+  check_status(qo_mx_gemm(A.data_ptr(), mx_ld(A), format, sa.data_ptr<uint8_t>(), mx_ld(sa), B.data_ptr(), mx_ld(B),
+                          sb.data_ptr<uint8_t>(), mx_ld(sb), bv.defined() ? bv.data_ptr() : nullptr, out.data_ptr(), od,
+                          N, M, N, K, current_stream(a)),
+               "mx_matmul");
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(quant_ops, m) {
@@ -245,6 +416,16 @@ TORCH_LIBRARY(quant_ops, m) {
   m.def(
       "w4a4_linear(Tensor x, Tensor left_trans, Tensor right_trans, Tensor weight_packed, Tensor weight_scale, "
       "float clip_ratio=1, Tensor? bias=None) -> Tensor");
+  m.def("mx_quantize(Tensor input, str fmt=\"mxfp4\") -> (Tensor, Tensor)");
+  m.def("mx_dequantize(Tensor codes, Tensor scales, int? features=None, ScalarType? out_dtype=None) -> Tensor");
+  m.def("rms_norm_mx_quantize(Tensor x, Tensor weight, float eps=1e-06, str fmt=\"mxfp8\") -> (Tensor, Tensor)");
+  m.def(
+      "add_rms_norm_mx_quantize(Tensor x, Tensor residual, Tensor weight, float eps=1e-06, str fmt=\"mxfp8\") -> "
+      "(Tensor, Tensor, Tensor)");
+  m.def("swiglu_mx_quantize(Tensor gate_up, str fmt=\"mxfp8\") -> (Tensor, Tensor)");
+  m.def(
+      "mx_matmul(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, Tensor? bias=None, "
+      "ScalarType? out_dtype=None) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(quant_ops, CUDA, m) {
@@ -254,4 +435,10 @@ TORCH_LIBRARY_IMPL(quant_ops, CUDA, m) {
   m.impl("dequantize_int4", &dequantize_int4);
   m.impl("int4_matmul_bias", &int4_matmul_bias);
   m.impl("w4a4_linear", &w4a4_linear);
+  m.impl("mx_quantize", &mx_quantize);
+  m.impl("mx_dequantize", &mx_dequantize);
+  m.impl("rms_norm_mx_quantize", &rms_norm_mx_quantize);
+  m.impl("add_rms_norm_mx_quantize", &add_rms_norm_mx_quantize);
+  m.impl("swiglu_mx_quantize", &swiglu_mx_quantize);
+  m.impl("mx_matmul", &mx_matmul);
 }

@@ -2,7 +2,7 @@
 
 Shapes and dtypes follow the reference (``src/quant_ops/meta_ops.py:22-37``):
 int4_matmul -> float16 [M, N]; flatquant_dynamic_quantize -> int32 [T, F/8] or
-int8 [T, F] plus float32 scales [T]. The two operators this build adds get
+int8 [T, F] plus float32 scales [T]. The operators this build adds get
 fakes of their own. Registered only when the native library defined the
 schemas.
 """
@@ -46,3 +46,36 @@ if _loader.KERNELS_AVAILABLE:
     def _dequant_fake(quantized, scales, packed_int32=False):
         feats = quantized.size(1) * (8 if packed_int32 else 1)
         return quantized.new_empty((quantized.size(0), feats), dtype=torch.float32)
+
+    if hasattr(torch.ops.quant_ops, "mx_quantize"):
+
+        def _mx_outputs(like, tokens, feats, fmt):
+            blocks = (feats + 31) // 32
+            codes = (like.new_empty((tokens, 16 * blocks), dtype=torch.uint8) if fmt == "mxfp4"
+                     else like.new_empty((tokens, 32 * blocks), dtype=torch.float8_e4m3fn))
+            return codes, like.new_empty((tokens, blocks), dtype=torch.uint8)
+
+        @torch.library.register_fake("quant_ops::mx_quantize")
+        def _mx_quantize_fake(input, fmt="mxfp4"):
+            return _mx_outputs(input, input.size(0), input.size(1), fmt)
+
+        @torch.library.register_fake("quant_ops::mx_dequantize")
+        def _mx_dequantize_fake(codes, scales, features=None, out_dtype=None):
+            feats = scales.size(1) * 32 if features is None else features
+            return codes.new_empty((codes.size(0), feats), dtype=out_dtype or torch.float32)
+
+        @torch.library.register_fake("quant_ops::rms_norm_mx_quantize")
+        def _rms_norm_mx_fake(x, weight, eps=1e-6, fmt="mxfp8"):
+            return _mx_outputs(x, x.size(0), x.size(1), fmt)
+
+        @torch.library.register_fake("quant_ops::add_rms_norm_mx_quantize")
+        def _add_rms_norm_mx_fake(x, residual, weight, eps=1e-6, fmt="mxfp8"):
+            return (*_mx_outputs(x, x.size(0), x.size(1), fmt), x.new_empty(tuple(x.shape)))
+
+        @torch.library.register_fake("quant_ops::swiglu_mx_quantize")
+        def _swiglu_mx_fake(gate_up, fmt="mxfp8"):
+            return _mx_outputs(gate_up, gate_up.size(0), gate_up.size(1) // 2, fmt)
+
+        @torch.library.register_fake("quant_ops::mx_matmul")
+        def _mx_matmul_fake(a, a_scales, b, b_scales, bias=None, out_dtype=None):
+            return a.new_empty((a.size(0), b.size(0)), dtype=out_dtype or torch.bfloat16)

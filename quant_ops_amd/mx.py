@@ -1,0 +1,168 @@
+"""Microscaled (OCP MX) formats: quantize, dequantize, the product with 4-bit
+weights, and the RMS norm and SwiGLU gate that quantize their result.
+
+Along a row, 32 consecutive values share a scale 2^e, held as the byte e + 127
+(255: NaN), and are coded as ``"mxfp4"`` (FP4 e2m1) or ``"mxfp8"`` (FP8 e4m3).
+A row of F values has B = ceil(F / 32) blocks, the last padded with zeros:
+
+* mxfp4 codes: uint8 [T, 16 B], two per byte, the even value in the low bits;
+* mxfp8 codes: float8_e4m3fn [T, 32 B];
+* scales: uint8 [T, B].
+
+e = floor(log2(largest magnitude)) - 2 (mxfp4) or - 8 (mxfp8), at least -127;
+codes are v / 2^e rounded to nearest even, saturated at 6 or 448. A block that
+holds a NaN or an infinity gets the scale byte 255 and zero codes, and reads
+back (and multiplies) as NaN.
+
+GPU tensors use the HIP kernels through ``torch.ops.quant_ops``; if the HIP
+library is not loaded they raise. Host tensors run the formulas in PyTorch.
+All of it is for inference: codes carry no gradient. None of these functions
+has a counterpart in the reference.
+"""
+from typing import Optional, Tuple
+
+import torch
+
+from . import _loader
+
+BLOCK = 32
+_EMAX = {"mxfp4": 2, "mxfp8": 8}
+_FP4_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def _emax(fmt):
+    if fmt not in _EMAX:
+        raise ValueError(f'fmt must be "mxfp4" or "mxfp8", got {fmt!r}')
+    return _EMAX[fmt]
+
+
+def _rows(x):
+    return x if x.dim() == 2 else x[None] if x.dim() == 1 else x.flatten(0, -2)
+
+
+def _like(t, x):
+    """[T, ...] rows as x's leading dimensions."""
+    return t if x.dim() == 2 else t.reshape(*x.shape[:-1], t.shape[1])
+
+
+def _quantize_pytorch(y, fmt):
+    """Codes and scales of float32 rows y [T, F]."""
+    emax = _emax(fmt)
+    tokens, feats = y.shape
+    blocks = -(-feats // BLOCK)
+    v = torch.nn.functional.pad(y.float(), (0, BLOCK * blocks - feats)).view(tokens, blocks, BLOCK)
+    top = v.abs().amax(2) if blocks else v.new_zeros(tokens, 0)
+    e = torch.where(top == 0, -127, torch.frexp(top)[1] - 1 - emax).clamp(-127, 127)
+    bad = ~torch.isfinite(top)
+    # in float64: 2^e and v / 2^e are exact at every exponent
+    q = torch.where(bad[:, :, None], 0.0, v.double() / torch.ldexp(torch.ones_like(e, dtype=torch.float64), e)[:, :, None])
+    scales = torch.where(bad, 255, e + 127).to(torch.uint8)
+    if fmt == "mxfp8":
+        return q.clamp(-448, 448).float().to(torch.float8_e4m3fn).flatten(1), scales
+    mag = q.abs()
+    step = torch.where(mag < 2, 0.5, torch.where(mag < 4, 1.0, 2.0))
+    near = (torch.round(mag / step) * step).clamp(max=6)
+    grid = torch.tensor(_FP4_VALUES, dtype=torch.float64, device=y.device)
+    code = (torch.searchsorted(grid, near) + 8 * torch.signbit(q)).to(torch.uint8).flatten(1)
+    return code[:, 0::2] | (code[:, 1::2] << 4), scales
+
+
+def _values_pytorch(codes, scales):
+    """float32 [T, 32 B] of codes and scales."""
+    if codes.dtype == torch.uint8:
+        table = torch.tensor(_FP4_VALUES + tuple(-v for v in _FP4_VALUES), device=codes.device)
+        v = table[torch.stack((codes & 15, codes >> 4), 2).long()].flatten(1)
+    else:
+        v = codes.float()
+    s = torch.ldexp(torch.ones_like(scales, dtype=torch.float64), scales.int() - 127)
+    s = torch.where(scales == 255, float("nan"), s).float()
+    return (v.view(*s.shape, BLOCK) * s[:, :, None]).flatten(1)
+
+
+def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4") -> Tuple[torch.Tensor, torch.Tensor]:
+    """Codes and scales of x [..., F] (float32 / float16 / bfloat16)."""
+    _emax(fmt)
+    rows = _rows(x)
+    if x.is_cuda:
+        _loader.require_kernels("mx_quantize")
+        codes, scales = torch.ops.quant_ops.mx_quantize.default(rows, fmt)
+    else:
+        codes, scales = _quantize_pytorch(rows, fmt)
+    return _like(codes, x), _like(scales, x)
+
+
+def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, features: Optional[int] = None,
+                  out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values of codes and scales, [..., features] in out_dtype (each rounded
+    once); features defaults to the padded row length."""
+    q, s = _rows(codes), _rows(scales)
+    if codes.is_cuda:
+        _loader.require_kernels("mx_dequantize")
+        out = torch.ops.quant_ops.mx_dequantize.default(q, s, features, out_dtype)
+    else:
+        feats = BLOCK * s.shape[1] if features is None else features
+        assert -(-feats // BLOCK) == s.shape[1], f"features ({feats}) must fill the {s.shape[1]} blocks of a row"
+        out = _values_pytorch(q, s)[:, :feats].to(out_dtype)
+    return _like(out, codes)
+
+
+def rms_norm_mx_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+                         residual: Optional[torch.Tensor] = None, fmt: str = "mxfp8") -> Tuple[torch.Tensor, ...]:
+    """RMS norm of x (+ residual), quantized: ``(codes, scales)``, and with a
+    residual ``(codes, scales, x + residual)``.
+
+    h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight, all in float32; the
+    sum is returned rounded once to x's dtype. x and residual [..., F] of one
+    dtype, weight [F] of any of the three.
+    """
+    _emax(fmt)
+    rows = _rows(x)
+    res = None if residual is None else _rows(residual)
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"residual {tuple(residual.shape)} must have x's shape {tuple(x.shape)}")
+    if x.is_cuda:
+        _loader.require_kernels("rms_norm_mx_quantize")
+        if res is None:
+            got = torch.ops.quant_ops.rms_norm_mx_quantize.default(rows, weight, float(eps), fmt)
+        else:
+            got = torch.ops.quant_ops.add_rms_norm_mx_quantize.default(rows, res, weight, float(eps), fmt)
+    else:
+        h = rows.float() if res is None else rows.float() + res.float()
+        got = _quantize_pytorch(h / torch.sqrt(h.square().mean(1, keepdim=True) + eps) * weight.float(), fmt)
+        if res is not None:
+            got = (*got, h.to(x.dtype))
+    return tuple(_like(t, x) for t in got)
+
+
+def swiglu_mx_quantize(gate_up: torch.Tensor, fmt: str = "mxfp8") -> Tuple[torch.Tensor, torch.Tensor]:
+    """Codes and scales of silu(g) * u in float32, gate_up [..., 2 F] holding the
+    gate g and then its factor u."""
+    _emax(fmt)
+    rows = _rows(gate_up)
+    if gate_up.is_cuda:
+        _loader.require_kernels("swiglu_mx_quantize")
+        codes, scales = torch.ops.quant_ops.swiglu_mx_quantize.default(rows, fmt)
+    else:
+        if rows.shape[1] % 2:
+            raise ValueError(f"gate_up must hold two halves, got {tuple(gate_up.shape)}")
+        g, u = rows.float().chunk(2, 1)
+        codes, scales = _quantize_pytorch(g / (1 + torch.exp(-g)) * u, fmt)
+    return _like(codes, gate_up), _like(scales, gate_up)
+
+
+def mx_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor,
+              bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``a @ b.T (+ bias)`` of the values that the codes stand for, float32 sums,
+    rounded once to out_dtype.
+
+    a [..., K] mxfp4 or mxfp8 codes with a_scales [..., K/32]; b the weight's
+    mxfp4 codes [N, K/2] with b_scales [N, K/32]; bias [N] (taken in out_dtype).
+    """
+    q, s = _rows(a), _rows(a_scales)
+    if a.is_cuda:
+        _loader.require_kernels("mx_matmul")
+        out = torch.ops.quant_ops.mx_matmul.default(q, s, b, b_scales, bias, out_dtype)
+    else:
+        out = _values_pytorch(q, s) @ _values_pytorch(b, b_scales).t()
+        out = (out if bias is None else out + bias.to(out_dtype).float()).to(out_dtype)
+    return _like(out, a)
