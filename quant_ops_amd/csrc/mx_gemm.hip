@@ -40,15 +40,15 @@ template <class Q>
 constexpr int kMfmaFormat = Q::code == QO_MX_FP4 ? 4 : 0;
 
 // MFMA of weight fragment b (output columns) and activation fragment a
-// (rows): lane l's four sums are row l % 16, columns 4 (l / 16) + 0 .. 3. SEL: the
-// byte of the scale operands.
-template <class QA, int SEL>
+// (rows): lane l's four sums are row l % 16, columns 4 (l / 16) + 0 .. 3. SB, SA:
+// the byte of the scale operands.
+template <class QA, int SB, int SA>
 __device__ inline v4f mx_mfma(const v8i& b, const v8i& a, v4f acc, uint32_t sb, uint32_t sa) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, acc, 4, kMfmaFormat<QA>, SEL, (int)sb, SEL, (int)sa);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, acc, 4, kMfmaFormat<QA>, SB, (int)sb, SA, (int)sa);
 }
 
 // mx_mfma, FP8 fragments in two halves where OT asks for it.
-template <class QA, class OT, int SEL>
+template <class QA, class OT, int SB, int SA>
 __device__ inline v4f mx_mac(const v8i& b, const v8i& a, v4f acc, uint32_t sb, uint32_t sa) {
   if constexpr (kSplitFp8<QA, OT>) {
     v8i hi, lo;
@@ -59,10 +59,10 @@ __device__ inline v4f mx_mac(const v8i& b, const v8i& a, v4f acc, uint32_t sb, u
       hi[i] = (int)(w & mask);
       lo[i] = (int)(w & ~mask);
     }
-    acc = mx_mfma<QA, SEL>(b, lo, acc, sb, sa);
-    return mx_mfma<QA, SEL>(b, hi, acc, sb, sa);
+    acc = mx_mfma<QA, SB, SA>(b, lo, acc, sb, sa);
+    return mx_mfma<QA, SB, SA>(b, hi, acc, sb, sa);
   } else {
-    return mx_mfma<QA, SEL>(b, a, acc, sb, sa);
+    return mx_mfma<QA, SB, SA>(b, a, acc, sb, sa);
   }
 }
 
@@ -154,7 +154,7 @@ mx_gemm_stream(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict_
 #pragma unroll
     for (int j = 0; j < FN; ++j)
 #pragma unroll
-      for (int i = 0; i < FM; ++i) acc[i][j] = mx_mac<QA, OT, 0>(fb[j], fa[i], acc[i][j], sb[j], sa[i]);
+      for (int i = 0; i < FM; ++i) acc[i][j] = mx_mac<QA, OT, 0, 0>(fb[j], fa[i], acc[i][j], sb[j], sa[i]);
   }
 #pragma unroll
   for (int i = 0; i < FM; ++i)
@@ -169,6 +169,280 @@ mx_gemm_stream(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict_
   }
 }
 
+// ---------------------------------------------------------------------------
+// Scale operands of a wave's fragments. Lane f * 16 + r loads the 16 bytes of a
+// quad of k-steps (16 blocks) of row 16 f + r: dword s holds step s's blocks, byte j
+// block j. The MFMA of step s and fragment f wants in lane g * 16 + r byte g of row
+// 16 f + r, so bytes and groups of 16 lanes change places: two rounds of byte
+// permutes and lane swaps, for two steps at a time. Word 2 (s / 2) + f % 2 then
+// holds step s, fragment f in byte 2 (s % 2) + f / 2.
+// ---------------------------------------------------------------------------
+struct MxScales {
+  uint32_t w[4];
+};
+
+// Blocks 16 q .. of the row at p; blocks past the last are 0.
+__device__ inline v4i mx_load_scales(const uint8_t* p, int q, int blocks) {
+  v4i v = {0, 0, 0, 0};
+  p += 16 * (int64_t)q;
+  const int left = blocks - 16 * q;
+  if (left >= 16) {
+    __builtin_memcpy(&v, p, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (left >= 4 * i + 4) {
+        int d;
+        __builtin_memcpy(&d, p + 4 * i, 4);
+        v[i] = d;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+          if (4 * i + j < left) v[i] |= (int)p[4 * i + j] << (8 * j);
+      }
+    }
+  }
+  return v;
+}
+
+__device__ inline MxScales mx_transpose_scales(const v4i& v) {
+  MxScales s;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t x = (uint32_t)v[2 * h], y = (uint32_t)v[2 * h + 1];
+    // (x's low half, y's low half) and the high ones; halves of the upper lane groups change sides
+    const auto p = __builtin_amdgcn_permlane32_swap(__builtin_amdgcn_perm(y, x, 0x05040100u),
+                                                    __builtin_amdgcn_perm(y, x, 0x07060302u), false, false);
+    const auto u = __builtin_amdgcn_permlane16_swap(__builtin_amdgcn_perm(p[1], p[0], 0x06020400u),
+                                                    __builtin_amdgcn_perm(p[1], p[0], 0x07030501u), false, false);
+    s.w[2 * h] = u[0];
+    s.w[2 * h + 1] = u[1];
+  }
+  return s;
+}
+
+// ---------------------------------------------------------------------------
+// mx_gemm_tile: 256 x 256 tiles, eight waves as 4 x 2, each 64 x 128 of the output
+// in 4 x 8 blocks of 16 x 16. Operand rows go from memory into LDS as they are
+// (LDS-DMA), KS k-steps a stage on a ring of STAGES. Waves 0 .. 3 and 4 .. 7
+// alternate, one slot apart, between a load slot (a k-step's LDS reads, the
+// copies of a later stage) and a compute slot (its MFMAs), with a workgroup
+// barrier between slots.
+//
+// A row of a stage is 64 bytes (FP4, one k-step) or 128 (two, or FP8). Its 16-byte
+// chunk c stands at slot c ^ f(row), so that the 16 rows a fragment read touches at
+// once fall into different banks; the copies' source addresses do the
+// permutation, within each row's 64 or 128 contiguous bytes.
+// ---------------------------------------------------------------------------
+template <class Q, int KS>
+struct MxRow {
+  static constexpr int bytes = KS * (Q::code == QO_MX_FP4 ? 64 : 128);
+  static_assert(bytes == 64 || bytes == 128, "row of a stage");
+  static constexpr int per_copy = 1024 / bytes;   // rows of one 64-lane copy
+  // what the slot of row r's chunks is XORed with
+  __device__ static inline int swizzle(int r) { return bytes == 128 ? (r >> 1) & 7 : (r >> 2) & 2; }
+};
+
+template <class QA, class OT, int KS, int STAGES>
+__global__ void __launch_bounds__(512, 1)
+mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ out, int64_t ldc,
+             const typename OT::T* __restrict__ bias, int tiles_m) {
+  using T = typename OT::T;
+  using RA = MxRow<QA, KS>;
+  using RB = MxRow<FP4, KS>;
+  constexpr int BM = 256, BN = 256, W = 8, FM = 4, FN = 8;
+  constexpr int A_BYTES = BM * RA::bytes, BYTES = A_BYTES + BN * RB::bytes;
+  constexpr int TA = A_BYTES / 1024 / W, TB = (BYTES - A_BYTES) / 1024 / W, PER = TA + TB;
+  constexpr bool k16 = sizeof(T) == 2;   // 16-bit outputs go through LDS, float32 from registers
+  constexpr int C_PITCH = BN * 2 + 16;
+  constexpr int RING = STAGES * BYTES, CTILE = k16 ? BM * C_PITCH : 0;
+  static_assert(PER * (STAGES - 1) < 60, "vmcnt range");
+  __shared__ __align__(16) unsigned char ring[RING > CTILE ? RING : CTILE];
+  __shared__ __align__(16) float s_bias[BN];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 1, wn = wave & 1, li = lane & 15, lg = lane >> 4;
+  const bool grp1 = wave >= W / 2;
+  const int M = a.rows, N = b.rows;
+
+  // Each XCD (workgroup j runs on XCD j % 8) a contiguous run of tiles, in groups
+  // of 4 row tiles x every column tile.
+  const int nblk = gridDim.x, xcd = blockIdx.x & 7;
+  const int pid = xcd * (nblk >> 3) + min(xcd, nblk & 7) + (int)(blockIdx.x >> 3);
+  constexpr int GM = 4;
+  const int tiles_n = (N + BN - 1) / BN;
+  const int g = pid / (GM * tiles_n), w = pid % (GM * tiles_n);
+  const int gm = min(GM, tiles_m - g * GM);
+  const int m0 = (g * GM + w % gm) * BM, n0 = (w / gm) * BN;
+
+  // Copy t of this wave fills bytes 1024 (wave + 8 t) .. of its operand's part of
+  // the stage. Rows past the edge repeat the last one (their sums are not
+  // stored); past a row's end its last chunk is repeated (its scales are 0 there).
+  const uint8_t* const a_base = a.codes + (int64_t)m0 * a.ld;
+  const uint8_t* const b_base = b.codes + (int64_t)n0 * b.ld;
+  const int a_end = blocks * (QA::code == QO_MX_FP4 ? 16 : 32) - 16, b_end = blocks * 16 - 16;
+  uint32_t voff[PER];
+  auto copy_row = [&](auto rowc, int t) -> int { return (wave + W * t) * decltype(rowc)::per_copy + lane / (decltype(rowc)::bytes / 16); };
+  auto copy_chunk = [&](auto rowc, int row) -> int { return (lane & (decltype(rowc)::bytes / 16 - 1)) ^ decltype(rowc)::swizzle(row); };
+  const int ca = 16 * copy_chunk(RA{}, copy_row(RA{}, 0)), cb = 16 * copy_chunk(RB{}, copy_row(RB{}, 0));   // the same for every t
+#pragma unroll
+  for (int t = 0; t < PER; ++t)
+    voff[t] = t < TA ? (uint32_t)min(copy_row(RA{}, t), M - 1 - m0) * (uint32_t)a.ld + ca
+                     : (uint32_t)min(copy_row(RB{}, t - TA), N - 1 - n0) * (uint32_t)b.ld + cb;
+  const int nk = (blocks + 3) >> 2, ns = (nk + KS - 1) / KS;
+  const uint32_t ring0 = lds_addr(ring) + 1024 * wave;
+  auto issue = [&](int st, uint32_t buf) {
+    const int oa = st * RA::bytes, ob = st * RB::bytes;
+    // how far this lane's chunk lies past its row's end (0 but in a last, partial stage)
+    const uint32_t over_a = max(oa + ca - a_end, 0), over_b = max(ob + cb - b_end, 0);
+#pragma unroll
+    for (int t = 0; t < PER; ++t) {
+      const uint32_t dst = ring0 + buf + (t < TA ? 8192 * t : A_BYTES + 8192 * (t - TA));
+      if (t < TA) dma16_s(voff[t] - over_a, a_base + oa, __builtin_amdgcn_readfirstlane(dst));
+      else dma16_s(voff[t] - over_b, b_base + ob, __builtin_amdgcn_readfirstlane(dst));
+    }
+  };
+
+  const uint8_t* sp[3];   // scale rows of this lane: A's 64, B's first and second 64
+  sp[0] = a.scales + (int64_t)min(m0 + 64 * wm + lane, M - 1) * a.scales_ld;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) sp[1 + h] = b.scales + (int64_t)min(n0 + 128 * wn + 64 * h + lane, N - 1) * b.scales_ld;
+  v4i raw[3];
+  MxScales sc[3];
+  auto load_scales = [&](int q) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) raw[i] = mx_load_scales(sp[i], q, blocks);
+  };
+
+  // This lane's place in a fragment read (k-step 0 of a stage).
+  const uint32_t xa = (64 * wm + li) * RA::bytes + 16 * (lg ^ RA::swizzle(li));
+  const uint32_t xb = A_BYTES + (128 * wn + li) * RB::bytes + 16 * (lg ^ RB::swizzle(li));
+  v8i fa[FM], fb[FN];
+  auto chunk = [&](uint32_t at) -> v4i { return *reinterpret_cast<const v4i*>(ring + at); };
+  auto load_regs = [&](uint32_t buf, int h) {   // k-step h of the stage: chunks 4 h .., one bit of the slot
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const uint32_t at = buf + 16 * i * RA::bytes;
+      if constexpr (QA::code == QO_MX_FP4) {
+        const v4i x = chunk(at + (xa ^ (64 * h)));
+        fa[i] = v8i{x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+      } else {
+        const v4i x = chunk(at + xa), y = chunk(at + (xa ^ 64));
+        fa[i] = v8i{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const v4i x = chunk(buf + 16 * j * RB::bytes + (xb ^ (64 * h)));
+      fb[j] = v8i{x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+    }
+  };
+  auto bar = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  v4f acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+
+  load_scales(0);
+  if (tid < BN) s_bias[tid] = bias ? (float)bias[min(n0 + tid, N - 1)] : 0.f;
+#pragma unroll
+  for (int st = 0; st < STAGES - 1 + (KS == 2); ++st)
+    if (st < ns) issue(st, st * BYTES);
+  if constexpr (KS == 2) gemm_wait_groups<PER, STAGES - 1>(ns - 1);
+  else gemm_wait_groups<PER, STAGES - 2>(ns - 1);
+  lds_barrier();
+  if (grp1) bar();
+
+  uint32_t buf = 0;   // of the current stage
+  int st = 0;
+  // k-step 4 q + s: load slot, compute slot
+  auto phase = [&](int q, auto stepc) {
+    constexpr int s = decltype(stepc)::value, h = s % KS;
+    const int k = 4 * q + s;
+    if constexpr (s == 0) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) sc[i] = mx_transpose_scales(raw[i]);
+    }
+    load_regs(buf, h);
+    if constexpr (h == 0) {
+      // the stage before this one has been read by every wave: its slot is free
+      const bool first = KS == 2 && st == 0;   // its later stages are under way already
+      const int next = st + STAGES - 1;
+      if (!first && next < ns) issue(next, buf >= BYTES ? buf - BYTES : buf + (STAGES - 1) * BYTES);
+    }
+    if constexpr (s == 0) {
+      if (k + 4 < nk) load_scales(q + 1);
+    }
+    const bool last = h == KS - 1 || k == nk - 1;   // of its stage
+    auto landed = [&]() { gemm_wait_groups<PER, STAGES - 2>(ns - 2 - st); };   // stage st + 1 has
+    if (last && grp1) landed();
+    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+    bar();
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        constexpr int h2 = 2 * (s / 2), b2 = 2 * (s % 2);
+        const uint32_t sb = sc[1 + j / 4].w[h2 + j % 2], sa = sc[0].w[h2 + i % 2];
+        const int e = (j % 4) / 2, f = i / 2;   // byte b2 + e of sb, b2 + f of sa
+        if (e == 0 && f == 0) acc[i][j] = mx_mac<QA, OT, b2, b2>(fb[j], fa[i], acc[i][j], sb, sa);
+        else if (e == 0) acc[i][j] = mx_mac<QA, OT, b2, b2 + 1>(fb[j], fa[i], acc[i][j], sb, sa);
+        else if (f == 0) acc[i][j] = mx_mac<QA, OT, b2 + 1, b2>(fb[j], fa[i], acc[i][j], sb, sa);
+        else acc[i][j] = mx_mac<QA, OT, b2 + 1, b2 + 1>(fb[j], fa[i], acc[i][j], sb, sa);
+      }
+    if (last && !grp1) landed();
+    bar();
+    if (last) {
+      ++st;
+      buf = buf == (STAGES - 1) * BYTES ? 0 : buf + BYTES;
+    }
+  };
+  for (int q = 0; 4 * q < nk; ++q) {
+    phase(q, std::integral_constant<int, 0>{});
+    if (4 * q + 1 < nk) phase(q, std::integral_constant<int, 1>{});
+    if (4 * q + 2 < nk) phase(q, std::integral_constant<int, 2>{});
+    if (4 * q + 3 < nk) phase(q, std::integral_constant<int, 3>{});
+  }
+
+  // acc[i][j][r] is row 64 wm + 16 i + li, column 128 wn + 16 j + 4 lg + r. Group 0 is
+  // one slot ahead: it stages its rows while group 1 runs its last compute
+  // slot, and copies them out while group 1 stages its own.
+  if constexpr (k16) {
+    unsigned char* const c_wave = ring + wm * 64 * C_PITCH + wn * 256;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const v4f bb = *reinterpret_cast<const v4f*>(s_bias + 128 * wn + 16 * j + 4 * lg);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        T v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = OT::cvt(acc[i][j][r] + bb[r]);
+        *reinterpret_cast<v2i*>(c_wave + (16 * i + li) * C_PITCH + 32 * j + 8 * lg) =
+            v2i{(int)(out_bits<OT>(v[0]) | out_bits<OT>(v[1]) << 16), (int)(out_bits<OT>(v[2]) | out_bits<OT>(v[3]) << 16)};
+      }
+    }
+    lds_barrier();
+    const int half = grp1 ? BM / 2 : 0;
+    copy_out_c<BM / 2, BN, 256, OT, true>(ring + half * C_PITCH, C_PITCH, out, ldc, M, N, m0 + half, n0, tid & 255);
+  } else {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const v4f bb = *reinterpret_cast<const v4f*>(s_bias + 128 * wn + 16 * j + 4 * lg);
+        mx_store4<OT>(acc[i][j] + bb, out, ldc, nullptr, M, N, m0 + 64 * wm + 16 * i + li, n0 + 128 * wn + 16 * j + 4 * lg);
+      }
+    lds_barrier();
+  }
+  if (!grp1) bar();
+}
+
 template <class QA, class OT>
 void mx_gemm_launch(const MxOperand& a, const MxOperand& b, int blocks, void* out, int64_t ldc, const void* bias,
                     hipStream_t stream) {
@@ -179,6 +453,12 @@ void mx_gemm_launch(const MxOperand& a, const MxOperand& b, int blocks, void* ou
     const int64_t tiles = ((int64_t)(a.rows + bm - 1) / bm) * ((b.rows + bn - 1) / bn);
     launch(kernel, dim3((unsigned)tiles), dim3(threads), 0, stream, a, b, blocks, o, ldc, bi);
   };
+  constexpr int KS = QA::code == QO_MX_FP4 ? 2 : 1, STAGES = QA::code == QO_MX_FP4 ? 2 : 3;
+  if (a.rows > 64 && blocks > 0 && a.ld < (1 << 23) && b.ld < (1 << 23)) {   // 32-bit offsets within a tile
+    const int tm = (a.rows + 255) / 256, tn = (b.rows + 255) / 256;
+    launch(mx_gemm_tile<QA, OT, KS, STAGES>, dim3((unsigned)(tm * tn)), dim3(512), 0, stream, a, b, blocks, o, ldc, bi, tm);
+    return;
+  }
   if (a.rows <= 16) go(mx_gemm_stream<QA, OT, 1, 1, 1, 8>, 16, 16, 512);
   else go(mx_gemm_stream<QA, OT, 4, 2, 1, 4>, 64, 32, 256);
 }
@@ -210,6 +490,10 @@ extern "C" int qo_mx_gemm(const void* a, int64_t lda, int a_format, const uint8_
   if (lda < row_a || ldb < K / 2 || a_scales_ld < K / 32 || b_scales_ld < K / 32 || ldc < N) {
     qo_set_error("%s: row stride below row length (a %lld, b %lld, scales %lld and %lld, out %lld)", fn, (long long)lda,
                  (long long)ldb, (long long)a_scales_ld, (long long)b_scales_ld, (long long)ldc);
+    return QO_ERR_SHAPE;
+  }
+  if (((M + 63) / 64) * ((N + 31) / 32) > INT32_MAX) {   // more tiles than a grid takes
+    qo_set_error("%s: output too large (M=%lld N=%lld)", fn, (long long)M, (long long)N);
     return QO_ERR_SHAPE;
   }
   if (M == 0 || N == 0) return QO_OK;
