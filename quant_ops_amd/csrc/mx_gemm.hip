@@ -66,6 +66,15 @@ __device__ inline v4f mx_mac(const v8i& b, const v8i& a, v4f acc, uint32_t sb, u
   }
 }
 
+// 32 x 32 blocks of FP4 fragments of 32 rows x 64: lane l has row l % 32, the 16 bytes
+// of block l / 32 and that block's scale in byte S of its operands; its sums
+// are row l % 32, columns 8 e + 4 (l / 32) + 0 .. 3, e = 0 .. 3.
+typedef float v16f __attribute__((ext_vector_type(16)));
+template <int S>
+__device__ inline v16f mx_mfma32(const v8i& b, const v8i& a, v16f acc, uint32_t sb, uint32_t sa) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b, a, acc, 4, 4, S, (int)sb, S, (int)sa);
+}
+
 // The output's four values of one row from column n on, + bias, rounded once.
 template <class OT>
 __device__ inline void mx_store4(v4f v, typename OT::T* out, int64_t ldc, const typename OT::T* bias, int M, int N,
@@ -170,16 +179,9 @@ mx_gemm_stream(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict_
 }
 
 // ---------------------------------------------------------------------------
-// Scale operands of a wave's fragments. Lane f * 16 + r loads the 16 bytes of a
-// quad of k-steps (16 blocks) of row 16 f + r: dword s holds step s's blocks, byte j
-// block j. The MFMA of step s and fragment f wants in lane g * 16 + r byte g of row
-// 16 f + r, so bytes and groups of 16 lanes change places: two rounds of byte
-// permutes and lane swaps, for two steps at a time. Word 2 (s / 2) + f % 2 then
-// holds step s, fragment f in byte 2 (s % 2) + f / 2.
+// Scale operands of a wave's fragments. Lane r loads the 16 bytes of a quad of
+// k-steps (16 blocks) of row r of 64: dword s holds step s's blocks, byte j block j.
 // ---------------------------------------------------------------------------
-struct MxScales {
-  uint32_t w[4];
-};
 
 // Blocks 16 q .. of the row at p; blocks past the last are 0.
 __device__ inline v4i mx_load_scales(const uint8_t* p, int q, int blocks) {
@@ -205,7 +207,32 @@ __device__ inline v4i mx_load_scales(const uint8_t* p, int q, int blocks) {
   return v;
 }
 
-__device__ inline MxScales mx_transpose_scales(const v4i& v) {
+// The same where the row has 16 blocks or more, as one load whatever q (q's
+// blocks, or the row's last 16), and how far to shift what it gave.
+__device__ inline v4i mx_load_scales_end(const uint8_t* p, int q, int blocks) {
+  v4i v;
+  __builtin_memcpy(&v, p + min(16 * q, blocks - 16), 16);
+  return v;
+}
+__device__ inline void mx_shift_scales(v4i& v, int bytes) {   // 1 .. 15, zeros come in
+  const int d = bytes >> 2, r = bytes & 3;
+  uint32_t x[5];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = i + d == 0 ? v[0] : i + d == 1 ? v[1] : i + d == 2 ? v[2] : i + d == 3 ? v[3] : 0;
+  x[4] = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (int)__builtin_amdgcn_alignbyte(x[i + 1], x[i], r);
+}
+
+struct MxScales {
+  uint32_t w[4];
+};
+
+// For fragments of 16 rows x 128: the MFMA of step s and fragment f wants in lane
+// g * 16 + r byte g of row 16 f + r, so bytes and groups of 16 lanes change places:
+// two rounds of byte permutes and lane swaps, for two steps at a time. Word 2 (s / 2)
+// + f % 2 then holds step s, fragment f in byte 2 (s % 2) + f / 2.
+__device__ inline MxScales mx_scales16(const v4i& v) {
   MxScales s;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -217,6 +244,21 @@ __device__ inline MxScales mx_transpose_scales(const v4i& v) {
                                                     __builtin_amdgcn_perm(p[1], p[0], 0x07030501u), false, false);
     s.w[2 * h] = u[0];
     s.w[2 * h + 1] = u[1];
+  }
+  return s;
+}
+
+// For fragments of 32 rows x 64 (half t of a step): lane g * 32 + r wants byte 2 t + g of
+// row 32 f + r. Word 2 (s / 2) + f holds step s, half t in byte 2 (s % 2) + t.
+__device__ inline MxScales mx_scales32(const v4i& v) {
+  MxScales s;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t x = (uint32_t)v[2 * h], y = (uint32_t)v[2 * h + 1];
+    const auto p = __builtin_amdgcn_permlane32_swap(__builtin_amdgcn_perm(y, x, 0x06040200u),
+                                                    __builtin_amdgcn_perm(y, x, 0x07050301u), false, false);
+    s.w[2 * h] = p[0];
+    s.w[2 * h + 1] = p[1];
   }
   return s;
 }
@@ -250,7 +292,8 @@ mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ 
   using T = typename OT::T;
   using RA = MxRow<QA, KS>;
   using RB = MxRow<FP4, KS>;
-  constexpr int BM = 256, BN = 256, W = 8, FM = 4, FN = 8;
+  constexpr int BM = 256, BN = 256, W = 8;
+  constexpr bool k32 = QA::code == QO_MX_FP4;   // 32 x 32 x 64 MFMAs
   constexpr int A_BYTES = BM * RA::bytes, BYTES = A_BYTES + BN * RB::bytes;
   constexpr int TA = A_BYTES / 1024 / W, TB = (BYTES - A_BYTES) / 1024 / W, PER = TA + TB;
   constexpr bool k16 = sizeof(T) == 2;   // 16-bit outputs go through LDS, float32 from registers
@@ -309,31 +352,29 @@ mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ 
   for (int h = 0; h < 2; ++h) sp[1 + h] = b.scales + (int64_t)min(n0 + 128 * wn + 64 * h + lane, N - 1) * b.scales_ld;
   v4i raw[3];
   MxScales sc[3];
-  auto load_scales = [&](int q) {
-#pragma unroll
-    for (int i = 0; i < 3; ++i) raw[i] = mx_load_scales(sp[i], q, blocks);
-  };
 
-  // This lane's place in a fragment read (k-step 0 of a stage).
-  const uint32_t xa = (64 * wm + li) * RA::bytes + 16 * (lg ^ RA::swizzle(li));
-  const uint32_t xb = A_BYTES + (128 * wn + li) * RB::bytes + 16 * (lg ^ RB::swizzle(li));
-  v8i fa[FM], fb[FN];
+  // This lane's place in a fragment read (k-step 0 of a stage): its row of the
+  // first fragment, and its chunk.
+  const int lr = k32 ? lane & 31 : li, lc = k32 ? lane >> 5 : lg;
+  const uint32_t xa = (64 * wm + lr) * RA::bytes + 16 * (lc ^ RA::swizzle(lr));
+  const uint32_t xb = A_BYTES + (128 * wn + lr) * RB::bytes + 16 * (lc ^ RB::swizzle(lr));
+  v8i fa[4], fb[8];   // 16 rows each; 32 x 64: halves 0 and 1 of 32 rows
   auto chunk = [&](uint32_t at) -> v4i { return *reinterpret_cast<const v4i*>(ring + at); };
   auto load_regs = [&](uint32_t buf, int h) {   // k-step h of the stage: chunks 4 h .., one bit of the slot
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const uint32_t at = buf + 16 * i * RA::bytes;
-      if constexpr (QA::code == QO_MX_FP4) {
-        const v4i x = chunk(at + (xa ^ (64 * h)));
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (k32) {
+        const v4i x = chunk(buf + 32 * (i / 2) * RA::bytes + (xa ^ (64 * h + 32 * (i % 2))));
         fa[i] = v8i{x[0], x[1], x[2], x[3], 0, 0, 0, 0};
       } else {
-        const v4i x = chunk(at + xa), y = chunk(at + (xa ^ 64));
+        const v4i x = chunk(buf + 16 * i * RA::bytes + xa), y = chunk(buf + 16 * i * RA::bytes + (xa ^ 64));
         fa[i] = v8i{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
       }
     }
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const v4i x = chunk(buf + 16 * j * RB::bytes + (xb ^ (64 * h)));
+    for (int j = 0; j < 8; ++j) {
+      const v4i x = k32 ? chunk(buf + 32 * (j / 2) * RB::bytes + (xb ^ (64 * h + 32 * (j % 2))))
+                        : chunk(buf + 16 * j * RB::bytes + (xb ^ (64 * h)));
       fb[j] = v8i{x[0], x[1], x[2], x[3], 0, 0, 0, 0};
     }
   };
@@ -343,13 +384,22 @@ mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ 
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  v4f acc[FM][FN];
+  // 16 x 16: acc[i][j] (4 x 8 blocks); 32 x 32: acc32[i][j] (2 x 4)
+  v4f acc[k32 ? 1 : 4][k32 ? 1 : 8];
+  v16f acc32[k32 ? 2 : 1][k32 ? 4 : 1];
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
+  for (auto& row : acc)
 #pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (auto& v : row) v = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (auto& row : acc32)
+#pragma unroll
+    for (auto& v : row)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) v[r] = 0.f;
 
-  load_scales(0);
+#pragma unroll
+  for (int i = 0; i < 3; ++i) raw[i] = mx_load_scales(sp[i], 0, blocks);
   if (tid < BN) s_bias[tid] = bias ? (float)bias[min(n0 + tid, N - 1)] : 0.f;
 #pragma unroll
   for (int st = 0; st < STAGES - 1 + (KS == 2); ++st)
@@ -366,8 +416,13 @@ mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ 
     constexpr int s = decltype(stepc)::value, h = s % KS;
     const int k = 4 * q + s;
     if constexpr (s == 0) {
+      const int past = 16 * (q + 1) - blocks;   // of this quad's blocks
+      if (q > 0 && past > 0) {
 #pragma unroll
-      for (int i = 0; i < 3; ++i) sc[i] = mx_transpose_scales(raw[i]);
+        for (int i = 0; i < 3; ++i) mx_shift_scales(raw[i], past);
+      }
+#pragma unroll
+      for (int i = 0; i < 3; ++i) sc[i] = k32 ? mx_scales32(raw[i]) : mx_scales16(raw[i]);
     }
     load_regs(buf, h);
     if constexpr (h == 0) {
@@ -377,26 +432,40 @@ mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ 
       if (!first && next < ns) issue(next, buf >= BYTES ? buf - BYTES : buf + (STAGES - 1) * BYTES);
     }
     if constexpr (s == 0) {
-      if (k + 4 < nk) load_scales(q + 1);
+      if (k + 4 < nk) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) raw[i] = mx_load_scales_end(sp[i], q + 1, blocks);
+      }
     }
     const bool last = h == KS - 1 || k == nk - 1;   // of its stage
-    auto landed = [&]() { gemm_wait_groups<PER, STAGES - 2>(ns - 2 - st); };   // stage st + 1 has
-    if (last && grp1) landed();
+    if (last) gemm_wait_groups<PER, STAGES - 2>(ns - 2 - st);   // stage st + 1 has landed
     __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
     bar();
+    constexpr int word = 2 * (s / 2), byte = 2 * (s % 2);
+    if constexpr (k32) {
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        constexpr int h2 = 2 * (s / 2), b2 = 2 * (s % 2);
-        const uint32_t sb = sc[1 + j / 4].w[h2 + j % 2], sa = sc[0].w[h2 + i % 2];
-        const int e = (j % 4) / 2, f = i / 2;   // byte b2 + e of sb, b2 + f of sa
-        if (e == 0 && f == 0) acc[i][j] = mx_mac<QA, OT, b2, b2>(fb[j], fa[i], acc[i][j], sb, sa);
-        else if (e == 0) acc[i][j] = mx_mac<QA, OT, b2, b2 + 1>(fb[j], fa[i], acc[i][j], sb, sa);
-        else if (f == 0) acc[i][j] = mx_mac<QA, OT, b2 + 1, b2>(fb[j], fa[i], acc[i][j], sb, sa);
-        else acc[i][j] = mx_mac<QA, OT, b2 + 1, b2 + 1>(fb[j], fa[i], acc[i][j], sb, sa);
-      }
-    if (last && !grp1) landed();
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t sb = sc[1 + j / 2].w[word + j % 2], sa = sc[0].w[word + i];
+            acc32[i][j] = t == 0 ? mx_mfma32<byte>(fb[2 * j], fa[2 * i], acc32[i][j], sb, sa)
+                                 : mx_mfma32<byte + 1>(fb[2 * j + 1], fa[2 * i + 1], acc32[i][j], sb, sa);
+          }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t sb = sc[1 + j / 4].w[word + j % 2], sa = sc[0].w[word + i % 2];
+          const int e = (j % 4) / 2, f = i / 2;   // byte + e of sb, byte + f of sa
+          if (e == 0 && f == 0) acc[i][j] = mx_mac<QA, OT, byte, byte>(fb[j], fa[i], acc[i][j], sb, sa);
+          else if (e == 0) acc[i][j] = mx_mac<QA, OT, byte, byte + 1>(fb[j], fa[i], acc[i][j], sb, sa);
+          else if (f == 0) acc[i][j] = mx_mac<QA, OT, byte + 1, byte>(fb[j], fa[i], acc[i][j], sb, sa);
+          else acc[i][j] = mx_mac<QA, OT, byte + 1, byte + 1>(fb[j], fa[i], acc[i][j], sb, sa);
+        }
+    }
     bar();
     if (last) {
       ++st;
@@ -410,34 +479,47 @@ mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ 
     if (4 * q + 3 < nk) phase(q, std::integral_constant<int, 3>{});
   }
 
-  // acc[i][j][r] is row 64 wm + 16 i + li, column 128 wn + 16 j + 4 lg + r. Group 0 is
-  // one slot ahead: it stages its rows while group 1 runs its last compute
-  // slot, and copies them out while group 1 stages its own.
+  // Each lane's sums come in fours of consecutive columns: 16 x 16 blocks hold row
+  // 16 i + li, columns 16 j + 4 lg ..; 32 x 32 row 32 i + lane % 32, columns 32 j + 8 e +
+  // 4 (lane / 32) .., e = 0 .. 3.
+  auto fours = [&](auto&& f) {
+    if constexpr (k32) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const v16f& v = acc32[i][j];
+            f(32 * i + lr, 32 * j + 8 * e + 4 * lc, v4f{v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]});
+          }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f(16 * i + li, 16 * j + 4 * lg, acc[i][j]);
+    }
+  };
+  // Group 0 is one slot ahead: it stages its rows while group 1 runs its last
+  // compute slot, and copies them out while group 1 stages its own.
   if constexpr (k16) {
     unsigned char* const c_wave = ring + wm * 64 * C_PITCH + wn * 256;
+    fours([&](int row, int col, const v4f& x) {
+      const v4f bb = *reinterpret_cast<const v4f*>(s_bias + 128 * wn + col);
+      T v[4];
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const v4f bb = *reinterpret_cast<const v4f*>(s_bias + 128 * wn + 16 * j + 4 * lg);
-#pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        T v[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = OT::cvt(acc[i][j][r] + bb[r]);
-        *reinterpret_cast<v2i*>(c_wave + (16 * i + li) * C_PITCH + 32 * j + 8 * lg) =
-            v2i{(int)(out_bits<OT>(v[0]) | out_bits<OT>(v[1]) << 16), (int)(out_bits<OT>(v[2]) | out_bits<OT>(v[3]) << 16)};
-      }
-    }
+      for (int r = 0; r < 4; ++r) v[r] = OT::cvt(x[r] + bb[r]);
+      *reinterpret_cast<v2i*>(c_wave + row * C_PITCH + 2 * col) =
+          v2i{(int)(out_bits<OT>(v[0]) | out_bits<OT>(v[1]) << 16), (int)(out_bits<OT>(v[2]) | out_bits<OT>(v[3]) << 16)};
+    });
     lds_barrier();
     const int half = grp1 ? BM / 2 : 0;
     copy_out_c<BM / 2, BN, 256, OT, true>(ring + half * C_PITCH, C_PITCH, out, ldc, M, N, m0 + half, n0, tid & 255);
   } else {
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        const v4f bb = *reinterpret_cast<const v4f*>(s_bias + 128 * wn + 16 * j + 4 * lg);
-        mx_store4<OT>(acc[i][j] + bb, out, ldc, nullptr, M, N, m0 + 64 * wm + 16 * i + li, n0 + 128 * wn + 16 * j + 4 * lg);
-      }
+    fours([&](int row, int col, const v4f& x) {
+      const v4f bb = *reinterpret_cast<const v4f*>(s_bias + 128 * wn + col);
+      mx_store4<OT>(x + bb, out, ldc, nullptr, M, N, m0 + 64 * wm + row, n0 + 128 * wn + col);
+    });
     lds_barrier();
   }
   if (!grp1) bar();
