@@ -418,7 +418,8 @@ int qo_transpose_int32(const int32_t* in, int64_t in_ld, int64_t rows, int64_t c
  * 2^e, held as the byte e + 127, and are coded as FP4 e2m1 or FP8 e4m3. A row
  * of F values has B = ceil(F / 32) blocks, the last padded with zeros: B scale
  * bytes, and 16 B bytes of FP4 codes (two per byte, the even value in the low
- * bits) or 32 B bytes of FP8 codes. No counterpart in the reference.
+ * bits) or 32 B bytes of FP8 codes. Rows of codes are contiguous, rows of scales
+ * scales_ld bytes apart. No counterpart in the reference.
  *
  * e = floor(log2(largest magnitude)) - 2 (FP4, largest value 6) or - 8 (FP8,
  * 448), at least -127 (all-zero blocks: -127); codes are v / 2^e rounded to
@@ -431,22 +432,23 @@ enum qo_mx_format { QO_MX_FP4 = 0, QO_MX_FP8 = 1 };
 #define QO_MX_MAX_FEATURES (1LL << 30)
 
 /*
- * Quantize rows: codes and scales (contiguous rows, as above) of x [tokens,
- * features] of x_dtype (F32, F16, BF16), row stride x_ld elements.
+ * Quantize rows: codes and scales (as above) of x [tokens, features] of x_dtype
+ * (F32, F16, BF16), row stride x_ld elements.
  *
- * Errors: QO_ERR_SHAPE for negative or too large sizes or x_ld < features;
+ * Errors: QO_ERR_SHAPE for negative or too large sizes, x_ld < features or
+ * scales_ld < B;
  * QO_ERR_DTYPE for other dtype or format codes; QO_ERR_ALIGNMENT if codes is
  * not 8-byte aligned; QO_ERR_NULL_POINTER.
  */
 int qo_mx_quantize(const void* x, int x_dtype, int64_t tokens, int64_t features, int64_t x_ld, int format,
-                   void* codes, uint8_t* scales, void* stream);
+                   void* codes, uint8_t* scales, int64_t scales_ld, void* stream);
 
 /*
- * The values of codes and scales (contiguous rows): out [tokens, features] of
- * out_dtype, contiguous, code * 2^e rounded once. Errors as qo_mx_quantize.
+ * The values of codes and scales: out [tokens, features] of out_dtype,
+ * contiguous, code * 2^e rounded once. Errors as qo_mx_quantize.
  */
-int qo_mx_dequantize(const void* codes, const uint8_t* scales, int format, int64_t tokens, int64_t features,
-                     void* out, int out_dtype, void* stream);
+int qo_mx_dequantize(const void* codes, const uint8_t* scales, int64_t scales_ld, int format, int64_t tokens,
+                     int64_t features, void* out, int out_dtype, void* stream);
 
 /*
  * RMS norm with the residual's addition, quantized: h = x + residual (residual
@@ -463,7 +465,8 @@ int qo_mx_dequantize(const void* codes, const uint8_t* scales, int format, int64
  */
 int qo_rms_norm_mx_quantize(const void* x, const void* residual, int x_dtype, int64_t tokens, int64_t features,
                             int64_t x_ld, int64_t residual_ld, const void* weight, int weight_dtype, float eps,
-                            int format, void* codes, uint8_t* scales, void* residual_out, void* stream);
+                            int format, void* codes, uint8_t* scales, int64_t scales_ld, void* residual_out,
+                            void* stream);
 
 /*
  * SwiGLU, quantized: codes and scales of y = g / (1 + exp(-g)) * u, where row t
@@ -471,7 +474,7 @@ int qo_rms_norm_mx_quantize(const void* x, const void* residual, int x_dtype, in
  * stride ld elements (at least 2 * features). Errors as qo_mx_quantize.
  */
 int qo_swiglu_mx_quantize(const void* gate_up, int dtype, int64_t tokens, int64_t features, int64_t ld, int format,
-                          void* codes, uint8_t* scales, void* stream);
+                          void* codes, uint8_t* scales, int64_t scales_ld, void* stream);
 
 /*
  * The product of microscaled operands: out[m, n] = rnd(sum_k a[m, k] * b[n, k] +
@@ -480,16 +483,26 @@ int qo_swiglu_mx_quantize(const void* gate_up, int dtype, int64_t tokens, int64_
  *   a, b      codes of [M, K] in a_format and of the weight [N, K] in FP4; row
  *             strides lda, ldb in bytes; both pointers and strides multiples
  *             of 16
- *   a_scales  scale bytes [M, K/32], row stride a_scales_ld; b_scales [N, K/32]
+ *   a_scales  scale bytes [M, K/32], row stride a_scales_ld; b_scales [N, K/32]. With
+ *             more than QO_MX_GEMM_FEW_ROWS rows both pointers and strides must be
+ *             multiples of 16, and every row readable up to the next multiple of 16
+ *             bytes (what stands there does not count)
  *   bias      NULL or [N] of out_dtype
  *   out       [M, N] of out_dtype (F32, F16, BF16), row stride ldc elements
  *   K         a multiple of 32 (the padded row length)
+ *   workspace NULL or device memory, 16-byte aligned, that lets products with few
+ *             tiles split K: used where workspace_bytes is at least
+ *             qo_mx_gemm_workspace_size(M, N, K, a_format) (0: not split). Only this
+ *             call's kernels read and write it; calls that share one must be ordered
  *
  * Errors: QO_ERR_SHAPE, QO_ERR_DTYPE, QO_ERR_ALIGNMENT, QO_ERR_NULL_POINTER.
  */
+#define QO_MX_GEMM_FEW_ROWS 16
 int qo_mx_gemm(const void* a, int64_t lda, int a_format, const uint8_t* a_scales, int64_t a_scales_ld,
                const void* b, int64_t ldb, const uint8_t* b_scales, int64_t b_scales_ld, const void* bias,
-               void* out, int out_dtype, int64_t ldc, int64_t M, int64_t N, int64_t K, void* stream);
+               void* out, int out_dtype, int64_t ldc, int64_t M, int64_t N, int64_t K, void* workspace,
+               int64_t workspace_bytes, void* stream);
+int64_t qo_mx_gemm_workspace_size(int64_t M, int64_t N, int64_t K, int a_format);
 
 #ifdef __cplusplus
 }

@@ -25,7 +25,8 @@ EXPORTED = ("qo_status_string", "qo_version", "qo_last_error", "qo_set_kernel_ro
             "qo_int4_gemm_f6_prepare", "qo_int4_gemm_f6_run", "qo_int4_gemm_f6_operand_bytes",
             "qo_int4_gemm_f6_convert", "qo_int4_gemm_f6_run2", "qo_w4a4_linear_f6w", "qo_w4a4_linear", "qo_w4a4_linear_ws", "qo_w4a4_linear_noalloc", "qo_dequantize_int4",
             "qo_pack_int4_to_int32", "qo_pack_int4_clamped", "qo_unpack_int32_to_int4", "qo_transpose_int32",
-            "qo_mx_quantize", "qo_mx_dequantize", "qo_rms_norm_mx_quantize", "qo_swiglu_mx_quantize", "qo_mx_gemm")
+            "qo_mx_quantize", "qo_mx_dequantize", "qo_rms_norm_mx_quantize", "qo_swiglu_mx_quantize", "qo_mx_gemm",
+            "qo_mx_gemm_workspace_size")
 
 # QO_ROUTE_* bits of qo_set_kernel_routing (include/quant_ops_hip.h)
 ROUTE = {"FQ_GENERIC": 1 << 0, "FQ_NO_WAVE": 1 << 1, "FQ_NO_DUO": 1 << 2, "FQ_NO_FEW": 1 << 3,
@@ -110,17 +111,19 @@ def lib():
         fn.restype = c_int
         fn.argtypes = [c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp]
     L.qo_mx_quantize.restype = c_int
-    L.qo_mx_quantize.argtypes = [c_vp, c_int, c_i64, c_i64, c_i64, c_int, c_vp, c_vp, c_vp]
+    L.qo_mx_quantize.argtypes = [c_vp, c_int, c_i64, c_i64, c_i64, c_int, c_vp, c_vp, c_i64, c_vp]
     L.qo_mx_dequantize.restype = c_int
-    L.qo_mx_dequantize.argtypes = [c_vp, c_vp, c_int, c_i64, c_i64, c_vp, c_int, c_vp]
+    L.qo_mx_dequantize.argtypes = [c_vp, c_vp, c_i64, c_int, c_i64, c_i64, c_vp, c_int, c_vp]
     L.qo_rms_norm_mx_quantize.restype = c_int
     L.qo_rms_norm_mx_quantize.argtypes = [c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_int, c_f, c_int,
-                                          c_vp, c_vp, c_vp, c_vp]
+                                          c_vp, c_vp, c_i64, c_vp, c_vp]
     L.qo_swiglu_mx_quantize.restype = c_int
-    L.qo_swiglu_mx_quantize.argtypes = [c_vp, c_int, c_i64, c_i64, c_i64, c_int, c_vp, c_vp, c_vp]
+    L.qo_swiglu_mx_quantize.argtypes = [c_vp, c_int, c_i64, c_i64, c_i64, c_int, c_vp, c_vp, c_i64, c_vp]
     L.qo_mx_gemm.restype = c_int
     L.qo_mx_gemm.argtypes = [c_vp, c_i64, c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_int, c_i64,
-                             c_i64, c_i64, c_i64, c_vp]
+                             c_i64, c_i64, c_i64, c_vp, c_i64, c_vp]
+    L.qo_mx_gemm_workspace_size.restype = c_i64
+    L.qo_mx_gemm_workspace_size.argtypes = [c_i64, c_i64, c_i64, c_int]
     _lib = L
     return L
 
@@ -455,12 +458,18 @@ def _ptr(t):
     return ctypes.c_void_p(t.data_ptr() if t is not None else None)
 
 
+def _row_stride(t):
+    """Stride of a matrix whose rows do not overlap (a single row has one too)."""
+    return max(t.stride(0), t.shape[1])
+
+
 def mx_buffers(tokens, features, fmt, device):
-    """Empty codes and scales for [tokens, features] rows."""
+    """Empty codes and scales for [tokens, features] rows (scale rows 16 bytes' multiples apart)."""
     blocks = (features + 31) // 32
+    pad = (blocks + 15) // 16 * 16
     codes = (torch.empty((tokens, 16 * blocks), dtype=torch.uint8, device=device) if fmt == "mxfp4" else
              torch.empty((tokens, 32 * blocks), dtype=torch.float8_e4m3fn, device=device))
-    return codes, torch.empty((tokens, blocks), dtype=torch.uint8, device=device)
+    return codes, torch.empty((tokens, pad), dtype=torch.uint8, device=device)[:, :blocks]
 
 
 def mx_quantize(x, fmt="mxfp4", codes=None, scales=None, stream=None):
@@ -469,15 +478,15 @@ def mx_quantize(x, fmt="mxfp4", codes=None, scales=None, stream=None):
     if codes is None:
         codes, scales = mx_buffers(t, f, fmt, x.device)
     _check(lib().qo_mx_quantize(_ptr(x), _TORCH_CODE[x.dtype], t, f, _ld(x), _MX_CODE[fmt], _ptr(codes), _ptr(scales),
-                                _stream(stream)))
+                                _row_stride(scales), _stream(stream)))
     return codes, scales
 
 
 def mx_dequantize(codes, scales, features, out_dtype=torch.float32, stream=None):
-    """Call ``qo_mx_dequantize`` on contiguous codes and scales."""
+    """Call ``qo_mx_dequantize`` on contiguous codes."""
     fmt = MX_FP4 if codes.dtype == torch.uint8 else MX_FP8
     out = torch.empty((codes.shape[0], features), dtype=out_dtype, device=codes.device)
-    _check(lib().qo_mx_dequantize(_ptr(codes), _ptr(scales), fmt, codes.shape[0], features, _ptr(out),
+    _check(lib().qo_mx_dequantize(_ptr(codes), _ptr(scales), _row_stride(scales), fmt, codes.shape[0], features, _ptr(out),
                                   _TORCH_CODE[out_dtype], _stream(stream)))
     return out
 
@@ -492,7 +501,7 @@ def rms_norm_mx_quantize(x, weight, eps=1e-6, residual=None, fmt="mxfp8", residu
     _check(lib().qo_rms_norm_mx_quantize(_ptr(x), _ptr(residual), _TORCH_CODE[x.dtype], t, f, _ld(x),
                                          _ld(residual) if residual is not None else 0, _ptr(weight),
                                          _TORCH_CODE[weight.dtype], float(eps), _MX_CODE[fmt], _ptr(codes),
-                                         _ptr(scales), _ptr(residual_out), _stream(stream)))
+                                         _ptr(scales), _row_stride(scales), _ptr(residual_out), _stream(stream)))
     return codes, scales, residual_out
 
 
@@ -501,17 +510,26 @@ def swiglu_mx_quantize(gate_up, fmt="mxfp8", stream=None):
     t, f = gate_up.shape[0], gate_up.shape[1] // 2
     codes, scales = mx_buffers(t, f, fmt, gate_up.device)
     _check(lib().qo_swiglu_mx_quantize(_ptr(gate_up), _TORCH_CODE[gate_up.dtype], t, f, _ld(gate_up), _MX_CODE[fmt],
-                                       _ptr(codes), _ptr(scales), _stream(stream)))
+                                       _ptr(codes), _ptr(scales), _row_stride(scales), _stream(stream)))
     return codes, scales
 
 
-def mx_gemm(a, a_scales, b, b_scales, bias=None, out_dtype=torch.bfloat16, out=None, stream=None):
+def mx_gemm_workspace_size(m, n, k, fmt):
+    """``qo_mx_gemm_workspace_size``."""
+    return int(lib().qo_mx_gemm_workspace_size(m, n, k, _MX_CODE[fmt]))
+
+
+def mx_gemm(a, a_scales, b, b_scales, bias=None, out_dtype=torch.bfloat16, out=None, stream=None, workspace=None):
     """Call ``qo_mx_gemm``: a (uint8 or float8_e4m3fn codes) [M, ..], b uint8 [N, K/2], rows 16-byte
-    aligned; bias in the output dtype."""
+    aligned; bias in the output dtype. ``workspace``: a uint8 device tensor, or True to allocate one."""
     m, n, blocks = a.shape[0], b.shape[0], a_scales.shape[1]
+    if workspace is True:
+        need = mx_gemm_workspace_size(m, n, 32 * blocks, "mxfp4" if a.dtype == torch.uint8 else "mxfp8")
+        workspace = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
     if out is None:
         out = torch.empty((m, n), dtype=out_dtype, device=a.device)
-    _check(lib().qo_mx_gemm(_ptr(a), _ld(a), MX_FP4 if a.dtype == torch.uint8 else MX_FP8, _ptr(a_scales), _ld(a_scales),
-                            _ptr(b), _ld(b), _ptr(b_scales), _ld(b_scales), _ptr(bias), _ptr(out),
-                            _TORCH_CODE[out.dtype], _ld(out), m, n, 32 * blocks, _stream(stream)))
+    _check(lib().qo_mx_gemm(_ptr(a), _ld(a), MX_FP4 if a.dtype == torch.uint8 else MX_FP8, _ptr(a_scales), _row_stride(a_scales),
+                            _ptr(b), _ld(b), _ptr(b_scales), _row_stride(b_scales), _ptr(bias), _ptr(out),
+                            _TORCH_CODE[out.dtype], _ld(out), m, n, 32 * blocks, _ptr(workspace),
+                            workspace.numel() if workspace is not None else 0, _stream(stream)))
     return out

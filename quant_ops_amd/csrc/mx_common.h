@@ -120,7 +120,8 @@ __device__ inline void store8(typename D::T* p, int64_t n, const float (&v)[8]) 
 // Codes and scale of the block whose eight values v this lane holds beside the
 // other three lanes of its quad (chunk c of a row, c / 4 the block).
 template <class Q>
-__device__ inline void mx_store8(const float (&v)[8], uint8_t* codes, uint8_t* scales, int64_t row, int blocks, int c) {
+__device__ inline void mx_store8(const float (&v)[8], uint8_t* codes, uint8_t* scales, int64_t scales_ld,
+                                 int64_t row, int blocks, int c) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
@@ -130,7 +131,7 @@ __device__ inline void mx_store8(const float (&v)[8], uint8_t* codes, uint8_t* s
   uint32_t* out = reinterpret_cast<uint32_t*>(codes + (row * blocks * 4 + c) * (4 * Q::words));
 #pragma unroll
   for (int i = 0; i < Q::words; ++i) out[i] = w[i];
-  if ((c & 3) == 0) scales[row * blocks + (c >> 2)] = (uint8_t)byte;
+  if ((c & 3) == 0) scales[row * scales_ld + (c >> 2)] = (uint8_t)byte;
 }
 
 }  // namespace qo

@@ -7,6 +7,9 @@
 // Fragments of 16 rows x 128 values (four blocks): lane l = r + 16 g has row r.
 // FP4: the 16 bytes of block g. FP8: bytes 16 g .. of the row's 128 and 64 + 16 g ..
 // (half of two blocks each). Either way its scale operand is block g's.
+#include <algorithm>
+
+#include "dispatch_rules.h"
 #include "int4_common.h"
 #include "mx_common.h"
 
@@ -54,8 +57,10 @@ __device__ inline v4f mx_mac(const v8i& b, const v8i& a, v4f acc, uint32_t sb, u
     v8i hi, lo;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t w = (uint32_t)a[i], top = w & 0x40404040u;   // exponent field's high bit
-      const uint32_t mask = (top << 1) | (top + (top - (top >> 6)));   // 0xFF in each byte that has it
+      // 0xFF in each byte whose exponent field has its high bit (shifted to the sign, which the
+      // permute's selectors 8 .. 11 spread over a byte)
+      const uint32_t w = (uint32_t)a[i];
+      const uint32_t mask = __builtin_amdgcn_perm(w << 1, w << 9, 0x0B090A08u);
       hi[i] = (int)(w & mask);
       lo[i] = (int)(w & ~mask);
     }
@@ -94,134 +99,171 @@ __device__ inline void mx_store4(v4f v, typename OT::T* out, int64_t ldc, const 
 }
 
 // ---------------------------------------------------------------------------
-// mx_gemm_stream: a workgroup makes 16 FM x 16 FN outputs; its W waves split the
-// k-steps (of 128) in contiguous runs, load their fragments straight into
-// registers, U steps at a time, and add their sums in LDS in a fixed order.
+// mx_gemm_stream: up to 16 rows (or rows too long for the tiled kernels' 32-bit offsets).
+// A workgroup makes tiles of 16 x 16 FN outputs, one after the other; its W waves split
+// the quads of k-steps (16 blocks) in contiguous runs, load fragments and scales
+// straight into registers, and add their sums in LDS in a fixed order. Bound by
+// the weight's bytes from memory: a wave has the next quad's on the way while it
+// multiplies one, across the end of a tile as well. RESIDENT: a wave has one quad
+// at most, and keeps a's fragments of it.
 // ---------------------------------------------------------------------------
-template <class QA, class OT, int FM, int FN, int U, int W>
-__global__ void __launch_bounds__(64 * W)
+template <class QA, class OT, int FN, int W, bool RESIDENT>
+__global__ void __launch_bounds__(64 * W, FN == 1 ? 4 : 2)
 mx_gemm_stream(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ out, int64_t ldc,
-               const typename OT::T* __restrict__ bias) {
-  constexpr int F = FM * FN;
-  __shared__ __align__(16) v4f part[W][F][64];
+               const typename OT::T* __restrict__ bias, int64_t tiles) {
+  constexpr bool k8 = QA::code == QO_MX_FP8;
+  constexpr int AB = k8 ? 128 : 64;   // bytes of a row of a for a k-step
+  __shared__ __align__(16) v4f part[2][W][FN][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, lg = lane >> 4;
   const int tiles_n = (b.rows + 16 * FN - 1) / (16 * FN);
-  const int m0 = (int)(blockIdx.x / tiles_n) * 16 * FM, n0 = (int)(blockIdx.x % tiles_n) * 16 * FN;
 
-  // rows past the edge read the last row; their sums are not stored
-  const uint8_t *ac[FM], *as[FM], *bc[FN], *bs[FN];
-#pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int64_t r = min(m0 + 16 * i + li, a.rows - 1);
-    ac[i] = a.codes + r * a.ld + 16 * lg;
-    as[i] = a.scales + r * a.scales_ld;
-  }
-#pragma unroll
-  for (int j = 0; j < FN; ++j) {
-    const int64_t r = min(n0 + 16 * j + li, b.rows - 1);
-    bc[j] = b.codes + r * b.ld + 16 * lg;
-    bs[j] = b.scales + r * b.scales_ld;
-  }
-
-  v4f acc[FM][FN];
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-
-  // step t's fragment; past the last block: zeros with scale 1
-  auto frag4 = [&](const uint8_t* p, int t) -> v8i {
-    v4i x = {0, 0, 0, 0};
-    if (4 * t + lg < blocks) x = *reinterpret_cast<const v4i*>(p + 64 * (int64_t)t);
-    return v8i{x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+  struct A {
+    v4i c[k8 ? 8 : 4], s;
   };
-  auto frag8 = [&](const uint8_t* p, int t) -> v8i {
-    v4i x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-    if (4 * t + (lg >> 1) < blocks) x = *reinterpret_cast<const v4i*>(p + 128 * (int64_t)t);
-    if (4 * t + 2 + (lg >> 1) < blocks) y = *reinterpret_cast<const v4i*>(p + 128 * (int64_t)t + 64);
-    return v8i{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+  struct B {
+    v4i c[FN][4], s[FN];
   };
-  auto scale = [&](const uint8_t* p, int t) -> uint32_t { return 4 * t + lg < blocks ? p[4 * t + lg] : 127u; };
-
-  const int nk = (blocks + 3) >> 2;
-  const int t0 = (int)((int64_t)nk * wave / W), t1 = (int)((int64_t)nk * (wave + 1) / W);
-  for (int t = t0; t < t1; ++t) {
-    v8i fa[FM], fb[FN];
-    uint32_t sa[FM], sb[FN];
+  // Sixteen bytes of a code row, zeros past its last block; the 16 scale bytes of quad q, 0 past the last.
+  auto get = [&](const uint8_t* p, int block, auto wholec) -> v4i {
+    if constexpr (decltype(wholec)::value) return *reinterpret_cast<const v4i*>(p);
+    return block < blocks ? *reinterpret_cast<const v4i*>(p) : v4i{0, 0, 0, 0};
+  };
+  auto scales = [&](const uint8_t* p, int q, auto wholec) -> v4i {
+    v4i v = {0, 0, 0, 0};
+    p += 16 * (int64_t)q;
+    if constexpr (decltype(wholec)::value) {
+      __builtin_memcpy(&v, p, 16);
+    } else {
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      fb[j] = frag4(bc[j], t);
-      sb[j] = scale(bs[j], t);
+      for (int i = 0; i < 16; ++i)
+        if (16 * q + i < blocks) v[i / 4] |= (int)((uint32_t)p[i] << (8 * (i % 4)));
     }
+    return v;
+  };
+  // Rows past the edge read the last row; their sums are not stored.
+  auto load_a = [&](int64_t tile, int q, A& x) {
+    const int64_t r = min((int)(tile / tiles_n) * 16 + li, a.rows - 1);
+    const uint8_t *p = a.codes + r * a.ld + 16 * lg + 4 * AB * (int64_t)q, *ps = a.scales + r * a.scales_ld;
+    auto go = [&](auto wholec) {
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      if constexpr (QA::code == QO_MX_FP4) fa[i] = frag4(ac[i], t);
-      else fa[i] = frag8(ac[i], t);
-      sa[i] = scale(as[i], t);
-    }
+      for (int s = 0; s < 4; ++s) {
+        const int t = 4 * q + s;
+        if constexpr (k8) {
+          x.c[2 * s] = get(p + AB * s, 4 * t + (lg >> 1), wholec);
+          x.c[2 * s + 1] = get(p + AB * s + 64, 4 * t + 2 + (lg >> 1), wholec);
+        } else {
+          x.c[s] = get(p + AB * s, 4 * t + lg, wholec);
+        }
+      }
+      x.s = scales(ps, q, wholec);
+    };
+    if (16 * q + 16 <= blocks) go(std::true_type{});
+    else go(std::false_type{});
+  };
+  auto load_b = [&](int64_t tile, int q, B& x) {
+    auto go = [&](auto wholec) {
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
+      for (int j = 0; j < FN; ++j) {
+        const int64_t r = min((int)(tile % tiles_n) * 16 * FN + 16 * j + li, b.rows - 1);
+        const uint8_t* p = b.codes + r * b.ld + 16 * lg + 256 * (int64_t)q;
 #pragma unroll
-      for (int i = 0; i < FM; ++i) acc[i][j] = mx_mac<QA, OT, 0, 0>(fb[j], fa[i], acc[i][j], sb[j], sa[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j) part[wave][i * FN + j][lane] = acc[i][j];
-  __syncthreads();
-  for (int f = wave; f < F; f += W) {
-    v4f v = part[0][f][lane];
-#pragma unroll
-    for (int w = 1; w < W; ++w) v += part[w][f][lane];
-    mx_store4<OT>(v, out, ldc, bias, a.rows, b.rows, m0 + 16 * (f / FN) + li, n0 + 16 * (f % FN) + 4 * lg);
-  }
-}
+        for (int s = 0; s < 4; ++s) x.c[j][s] = get(p + 64 * s, 16 * q + 4 * s + lg, wholec);
+        x.s[j] = scales(b.scales + r * b.scales_ld, q, wholec);
+      }
+    };
+    if (16 * q + 16 <= blocks) go(std::true_type{});
+    else go(std::false_type{});
+  };
 
-// ---------------------------------------------------------------------------
-// Scale operands of a wave's fragments. Lane r loads the 16 bytes of a quad of
-// k-steps (16 blocks) of row r of 64: dword s holds step s's blocks, byte j block j.
-// ---------------------------------------------------------------------------
-
-// Blocks 16 q .. of the row at p; blocks past the last are 0.
-__device__ inline v4i mx_load_scales(const uint8_t* p, int q, int blocks) {
-  v4i v = {0, 0, 0, 0};
-  p += 16 * (int64_t)q;
-  const int left = blocks - 16 * q;
-  if (left >= 16) {
-    __builtin_memcpy(&v, p, 16);
-  } else {
+  v4f acc[FN];
+  auto multiply = [&](const A& x, const B& y) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (left >= 4 * i + 4) {
-        int d;
-        __builtin_memcpy(&d, p + 4 * i, 4);
-        v[i] = d;
+    for (int s = 0; s < 4; ++s) {
+      v8i fa;
+      if constexpr (k8) {
+        const v4i &l = x.c[2 * s], &h = x.c[2 * s + 1];
+        fa = v8i{l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
       } else {
+        fa = v8i{x.c[s][0], x.c[s][1], x.c[s][2], x.c[s][3], 0, 0, 0, 0};
+      }
 #pragma unroll
-        for (int j = 0; j < 3; ++j)
-          if (4 * i + j < left) v[i] |= (int)p[4 * i + j] << (8 * j);
+      for (int j = 0; j < FN; ++j) {
+        const v4i& c = y.c[j][s];
+        // in two halves whatever the output: the matrix cores wait for memory here
+        acc[j] = mx_mac<QA, OutF32, 0, 0>(v8i{c[0], c[1], c[2], c[3], 0, 0, 0, 0}, fa, acc[j], (uint32_t)y.s[j][s] >> (8 * lg),
+                                      (uint32_t)x.s[s] >> (8 * lg));
       }
     }
+  };
+
+  const int nq = (blocks + 15) >> 4;
+  const int q0 = (int)((int64_t)nq * wave / W), q1 = (int)((int64_t)nq * (wave + 1) / W);
+  int64_t tile = blockIdx.x;
+  int q = q0, parity = 0;
+  A x;
+  auto clear = [&]() {
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
+  };
+  // One quad (cur is its weight) or, for a wave without any, one tile; false at the end.
+  auto turn = [&](B& cur, B& next) -> bool {
+    if (q0 < q1) {
+      if (!RESIDENT) load_a(tile, q, x);
+      const bool more = q + 1 < q1;
+      const int64_t then = more ? tile : tile + gridDim.x;
+      if (then < tiles) load_b(then, more ? q + 1 : q0, next);
+      if constexpr (RESIDENT && k8) {   // the halves of a's codes anew for each tile: kept, they leave room for one workgroup a CU
+#pragma unroll
+        for (auto& c : x.c) asm volatile("" : "+v"(c));
+      }
+      multiply(x, cur);
+      if (more) {
+        ++q;
+        return true;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < FN; ++j) part[parity][wave][j][lane] = acc[j];
+    __builtin_amdgcn_sched_barrier(0);
+    lds_barrier();   // loads stay under way; part's other half is free once all waves are past the next one
+    __builtin_amdgcn_sched_barrier(0);
+    if (wave < FN) {
+      v4f v = part[parity][0][wave][lane];
+#pragma unroll
+      for (int w = 1; w < W; ++w) v += part[parity][w][wave][lane];
+      mx_store4<OT>(v, out, ldc, bias, a.rows, b.rows, (int)(tile / tiles_n) * 16 + li,
+                    (int)(tile % tiles_n) * 16 * FN + 16 * wave + 4 * lg);
+    }
+    clear();
+    parity ^= 1;
+    q = q0;
+    tile += gridDim.x;
+    return tile < tiles;
+  };
+  clear();
+  B y, z;
+  if (q0 < q1) {
+    load_b(tile, q0, y);
+    if (RESIDENT) load_a(tile, q0, x);
   }
-  return v;
+  while (turn(y, z) && turn(z, y)) {
+  }
 }
 
-// The same where the row has 16 blocks or more, as one load whatever q (q's
-// blocks, or the row's last 16), and how far to shift what it gave.
-__device__ inline v4i mx_load_scales_end(const uint8_t* p, int q, int blocks) {
-  v4i v;
-  __builtin_memcpy(&v, p + min(16 * q, blocks - 16), 16);
-  return v;
-}
-__device__ inline void mx_shift_scales(v4i& v, int bytes) {   // 1 .. 15, zeros come in
-  const int d = bytes >> 2, r = bytes & 3;
-  uint32_t x[5];
+// ---------------------------------------------------------------------------
+// Scale operands of a wave's fragments. The tiled kernels copy the 16 bytes of a
+// quad of k-steps (16 blocks) of every row of the tile into LDS. Lane r reads
+// those of row r of 64: dword s holds step s's blocks, byte j block j.
+// ---------------------------------------------------------------------------
+
+// Clears the last `past` (1 .. 15) of the 16 bytes: blocks that the row does not have.
+__device__ inline void mx_clear_scales(v4i& v, int past) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = i + d == 0 ? v[0] : i + d == 1 ? v[1] : i + d == 2 ? v[2] : i + d == 3 ? v[3] : 0;
-  x[4] = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (int)__builtin_amdgcn_alignbyte(x[i + 1], x[i], r);
+  for (int i = 0; i < 4; ++i) {
+    const int gone = past - 4 * (3 - i);   // of this dword's bytes, from the top
+    v[i] = gone >= 4 ? 0 : gone <= 0 ? v[i] : (int)((uint32_t)v[i] & (0xFFFFFFFFu >> (8 * gone)));
+  }
 }
 
 struct MxScales {
@@ -264,17 +306,12 @@ __device__ inline MxScales mx_scales32(const v4i& v) {
 }
 
 // ---------------------------------------------------------------------------
-// mx_gemm_tile: 256 x 256 tiles, eight waves as 4 x 2, each 64 x 128 of the output
-// in 4 x 8 blocks of 16 x 16. Operand rows go from memory into LDS as they are
-// (LDS-DMA), KS k-steps a stage on a ring of STAGES. Waves 0 .. 3 and 4 .. 7
-// alternate, one slot apart, between a load slot (a k-step's LDS reads, the
-// copies of a later stage) and a compute slot (its MFMAs), with a workgroup
-// barrier between slots.
-//
-// A row of a stage is 64 bytes (FP4, one k-step) or 128 (two, or FP8). Its 16-byte
-// chunk c stands at slot c ^ f(row), so that the 16 rows a fragment read touches at
-// once fall into different banks; the copies' source addresses do the
-// permutation, within each row's 64 or 128 contiguous bytes.
+// How the tiled kernels hold operands in LDS: rows go there as they are (LDS-DMA), KS
+// k-steps a stage. A row of a stage is 64 bytes (FP4, one k-step) or 128 (two, or FP8);
+// a copy of 64-byte rows costs as much as one of 128-byte rows (64 GB/s a CU against
+// 127: each row is a line of L2). Its 16-byte chunk c stands at slot c ^ f(row), so
+// that the rows a fragment read touches at once fall into different banks; the
+// copies' source addresses do the permutation, within each row's 64 or 128 contiguous bytes.
 // ---------------------------------------------------------------------------
 template <class Q, int KS>
 struct MxRow {
@@ -285,15 +322,36 @@ struct MxRow {
   __device__ static inline int swizzle(int r) { return bytes == 128 ? (r >> 1) & 7 : (r >> 2) & 2; }
 };
 
-template <class QA, class OT, int KS, int STAGES>
+// Tile of workgroup blockIdx.x: each XCD (workgroup j runs on XCD j % 8) a contiguous run
+// of tiles, in groups of up to GM row tiles x every column tile.
+struct MxTile {
+  int m, n;
+};
+template <int GM>
+__device__ inline MxTile mx_tile_of(int tiles_m, int tiles_n) {
+  const int nblk = gridDim.x, xcd = blockIdx.x & 7;
+  const int pid = xcd * (nblk >> 3) + min(xcd, nblk & 7) + (int)(blockIdx.x >> 3);
+  const int g = pid / (GM * tiles_n), w = pid % (GM * tiles_n);
+  const int gm = min(GM, tiles_m - g * GM);
+  return {g * GM + w % gm, w / gm};
+}
+
+// ---------------------------------------------------------------------------
+// mx_gemm_tile: FP8 x FP4, 256 x 256 tiles, eight waves as 4 x 2, each 64 x 128 of the output
+// in 4 x 8 blocks of 16 x 16; stages of one k-step on a ring of three. Waves 0 .. 3
+// and 4 .. 7 alternate, one slot apart, between a load slot (a k-step's LDS reads,
+// the copies of stage t + 2) and a compute slot (its MFMAs), with a workgroup barrier
+// between slots. 4096 x 4096 x 14336: 160 us, 3.0 PFLOP/s, the matrix cores busy 76 % of the
+// time at the 2.0 GHz that the board's power limit leaves (registers only: 4.25).
+// ---------------------------------------------------------------------------
+template <class OT>
 __global__ void __launch_bounds__(512, 1)
 mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ out, int64_t ldc,
              const typename OT::T* __restrict__ bias, int tiles_m) {
   using T = typename OT::T;
-  using RA = MxRow<QA, KS>;
-  using RB = MxRow<FP4, KS>;
-  constexpr int BM = 256, BN = 256, W = 8;
-  constexpr bool k32 = QA::code == QO_MX_FP4;   // 32 x 32 x 64 MFMAs
+  using RA = MxRow<FP8, 1>;
+  using RB = MxRow<FP4, 1>;
+  constexpr int BM = 256, BN = 256, W = 8, STAGES = 3;
   constexpr int A_BYTES = BM * RA::bytes, BYTES = A_BYTES + BN * RB::bytes;
   constexpr int TA = A_BYTES / 1024 / W, TB = (BYTES - A_BYTES) / 1024 / W, PER = TA + TB;
   constexpr bool k16 = sizeof(T) == 2;   // 16-bit outputs go through LDS, float32 from registers
@@ -301,6 +359,7 @@ mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ 
   constexpr int RING = STAGES * BYTES, CTILE = k16 ? BM * C_PITCH : 0;
   static_assert(PER * (STAGES - 1) < 60, "vmcnt range");
   __shared__ __align__(16) unsigned char ring[RING > CTILE ? RING : CTILE];
+  __shared__ __align__(16) unsigned char s_scales[(BM + BN) * 16];   // a quad's: A's rows, B's rows
   __shared__ __align__(16) float s_bias[BN];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -308,22 +367,15 @@ mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ 
   const bool grp1 = wave >= W / 2;
   const int M = a.rows, N = b.rows;
 
-  // Each XCD (workgroup j runs on XCD j % 8) a contiguous run of tiles, in groups
-  // of 4 row tiles x every column tile.
-  const int nblk = gridDim.x, xcd = blockIdx.x & 7;
-  const int pid = xcd * (nblk >> 3) + min(xcd, nblk & 7) + (int)(blockIdx.x >> 3);
-  constexpr int GM = 4;
-  const int tiles_n = (N + BN - 1) / BN;
-  const int g = pid / (GM * tiles_n), w = pid % (GM * tiles_n);
-  const int gm = min(GM, tiles_m - g * GM);
-  const int m0 = (g * GM + w % gm) * BM, n0 = (w / gm) * BN;
+  const MxTile tile = mx_tile_of<4>(tiles_m, (N + BN - 1) / BN);
+  const int m0 = tile.m * BM, n0 = tile.n * BN;
 
   // Copy t of this wave fills bytes 1024 (wave + 8 t) .. of its operand's part of
   // the stage. Rows past the edge repeat the last one (their sums are not
   // stored); past a row's end its last chunk is repeated (its scales are 0 there).
   const uint8_t* const a_base = a.codes + (int64_t)m0 * a.ld;
   const uint8_t* const b_base = b.codes + (int64_t)n0 * b.ld;
-  const int a_end = blocks * (QA::code == QO_MX_FP4 ? 16 : 32) - 16, b_end = blocks * 16 - 16;
+  const int a_end = blocks * 32 - 16, b_end = blocks * 16 - 16;
   uint32_t voff[PER];
   auto copy_row = [&](auto rowc, int t) -> int { return (wave + W * t) * decltype(rowc)::per_copy + lane / (decltype(rowc)::bytes / 16); };
   auto copy_chunk = [&](auto rowc, int row) -> int { return (lane & (decltype(rowc)::bytes / 16 - 1)) ^ decltype(rowc)::swizzle(row); };
@@ -332,7 +384,7 @@ mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ 
   for (int t = 0; t < PER; ++t)
     voff[t] = t < TA ? (uint32_t)min(copy_row(RA{}, t), M - 1 - m0) * (uint32_t)a.ld + ca
                      : (uint32_t)min(copy_row(RB{}, t - TA), N - 1 - n0) * (uint32_t)b.ld + cb;
-  const int nk = (blocks + 3) >> 2, ns = (nk + KS - 1) / KS;
+  const int nk = (blocks + 3) >> 2;
   const uint32_t ring0 = lds_addr(ring) + 1024 * wave;
   auto issue = [&](int st, uint32_t buf) {
     const int oa = st * RA::bytes, ob = st * RB::bytes;
@@ -346,35 +398,37 @@ mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ 
     }
   };
 
-  const uint8_t* sp[3];   // scale rows of this lane: A's 64, B's first and second 64
-  sp[0] = a.scales + (int64_t)min(m0 + 64 * wm + lane, M - 1) * a.scales_ld;
+  // Scales: each wave copies 64 rows, A's 0 .. 255 then B's.
+  const uint8_t* const s_base = wave < 4 ? a.scales + (int64_t)m0 * a.scales_ld : b.scales + (int64_t)n0 * b.scales_ld;
+  const uint32_t s_off = wave < 4 ? (uint32_t)min(64 * wave + lane, M - 1 - m0) * (uint32_t)a.scales_ld
+                                  : (uint32_t)min(64 * (wave - 4) + lane, N - 1 - n0) * (uint32_t)b.scales_ld;
+  const uint32_t s_dst = __builtin_amdgcn_readfirstlane(lds_addr(s_scales) + 1024 * wave);
+  auto issue_scales = [&](int q) { dma16_s(s_off, s_base + 16 * (int64_t)q, s_dst); };
+  MxScales sc[3];   // A's 64 rows, B's first and second 64
+  auto load_scales = [&](int q) {
+    const int past = 16 * (q + 1) - blocks;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) sp[1 + h] = b.scales + (int64_t)min(n0 + 128 * wn + 64 * h + lane, N - 1) * b.scales_ld;
-  v4i raw[3];
-  MxScales sc[3];
+    for (int i = 0; i < 3; ++i) {
+      v4i v = *reinterpret_cast<const v4i*>(s_scales + 16 * ((i == 0 ? 64 * wm : BM + 128 * wn + 64 * (i - 1)) + lane));
+      if (past > 0) mx_clear_scales(v, past);
+      sc[i] = mx_scales16(v);
+    }
+  };
 
-  // This lane's place in a fragment read (k-step 0 of a stage): its row of the
-  // first fragment, and its chunk.
-  const int lr = k32 ? lane & 31 : li, lc = k32 ? lane >> 5 : lg;
-  const uint32_t xa = (64 * wm + lr) * RA::bytes + 16 * (lc ^ RA::swizzle(lr));
-  const uint32_t xb = A_BYTES + (128 * wn + lr) * RB::bytes + 16 * (lc ^ RB::swizzle(lr));
-  v8i fa[4], fb[8];   // 16 rows each; 32 x 64: halves 0 and 1 of 32 rows
+  // This lane's place in a fragment read: its row of the first fragment, and its chunk.
+  const uint32_t xa = (64 * wm + li) * RA::bytes + 16 * (lg ^ RA::swizzle(li));
+  const uint32_t xb = A_BYTES + (128 * wn + li) * RB::bytes + 16 * (lg ^ RB::swizzle(li));
+  v8i fa[4], fb[8];
   auto chunk = [&](uint32_t at) -> v4i { return *reinterpret_cast<const v4i*>(ring + at); };
-  auto load_regs = [&](uint32_t buf, int h) {   // k-step h of the stage: chunks 4 h .., one bit of the slot
+  auto load_regs = [&](uint32_t buf) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (k32) {
-        const v4i x = chunk(buf + 32 * (i / 2) * RA::bytes + (xa ^ (64 * h + 32 * (i % 2))));
-        fa[i] = v8i{x[0], x[1], x[2], x[3], 0, 0, 0, 0};
-      } else {
-        const v4i x = chunk(buf + 16 * i * RA::bytes + xa), y = chunk(buf + 16 * i * RA::bytes + (xa ^ 64));
-        fa[i] = v8i{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-      }
+      const v4i x = chunk(buf + 16 * i * RA::bytes + xa), y = chunk(buf + 16 * i * RA::bytes + (xa ^ 64));
+      fa[i] = v8i{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const v4i x = k32 ? chunk(buf + 32 * (j / 2) * RB::bytes + (xb ^ (64 * h + 32 * (j % 2))))
-                        : chunk(buf + 16 * j * RB::bytes + (xb ^ (64 * h)));
+      const v4i x = chunk(buf + 16 * j * RB::bytes + xb);
       fb[j] = v8i{x[0], x[1], x[2], x[3], 0, 0, 0, 0};
     }
   };
@@ -384,93 +438,53 @@ mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ 
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  // 16 x 16: acc[i][j] (4 x 8 blocks); 32 x 32: acc32[i][j] (2 x 4)
-  v4f acc[k32 ? 1 : 4][k32 ? 1 : 8];
-  v16f acc32[k32 ? 2 : 1][k32 ? 4 : 1];
+  v4f acc[4][8];
 #pragma unroll
   for (auto& row : acc)
 #pragma unroll
     for (auto& v : row) v = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (auto& row : acc32)
-#pragma unroll
-    for (auto& v : row)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = 0.f;
 
-#pragma unroll
-  for (int i = 0; i < 3; ++i) raw[i] = mx_load_scales(sp[i], 0, blocks);
+  issue_scales(0);
   if (tid < BN) s_bias[tid] = bias ? (float)bias[min(n0 + tid, N - 1)] : 0.f;
 #pragma unroll
-  for (int st = 0; st < STAGES - 1 + (KS == 2); ++st)
-    if (st < ns) issue(st, st * BYTES);
-  if constexpr (KS == 2) gemm_wait_groups<PER, STAGES - 1>(ns - 1);
-  else gemm_wait_groups<PER, STAGES - 2>(ns - 1);
+  for (int k = 0; k < STAGES - 1; ++k)
+    if (k < nk) issue(k, k * BYTES);
+  gemm_wait_groups<PER, STAGES - 2>(nk - 1);
   lds_barrier();
   if (grp1) bar();
 
   uint32_t buf = 0;   // of the current stage
-  int st = 0;
   // k-step 4 q + s: load slot, compute slot
   auto phase = [&](int q, auto stepc) {
-    constexpr int s = decltype(stepc)::value, h = s % KS;
+    constexpr int s = decltype(stepc)::value;
     const int k = 4 * q + s;
-    if constexpr (s == 0) {
-      const int past = 16 * (q + 1) - blocks;   // of this quad's blocks
-      if (q > 0 && past > 0) {
-#pragma unroll
-        for (int i = 0; i < 3; ++i) mx_shift_scales(raw[i], past);
-      }
-#pragma unroll
-      for (int i = 0; i < 3; ++i) sc[i] = k32 ? mx_scales32(raw[i]) : mx_scales16(raw[i]);
-    }
-    load_regs(buf, h);
-    if constexpr (h == 0) {
-      // the stage before this one has been read by every wave: its slot is free
-      const bool first = KS == 2 && st == 0;   // its later stages are under way already
-      const int next = st + STAGES - 1;
-      if (!first && next < ns) issue(next, buf >= BYTES ? buf - BYTES : buf + (STAGES - 1) * BYTES);
-    }
-    if constexpr (s == 0) {
-      if (k + 4 < nk) {
-#pragma unroll
-        for (int i = 0; i < 3; ++i) raw[i] = mx_load_scales_end(sp[i], q + 1, blocks);
-      }
-    }
-    const bool last = h == KS - 1 || k == nk - 1;   // of its stage
-    if (last) gemm_wait_groups<PER, STAGES - 2>(ns - 2 - st);   // stage st + 1 has landed
+    if constexpr (s == 0) load_scales(q);
+    load_regs(buf);
+    // the stage before this one has been read by every wave: its slot is free
+    if (k + STAGES - 1 < nk) issue(k + STAGES - 1, buf >= BYTES ? buf - BYTES : buf + (STAGES - 1) * BYTES);
+    // Every wave has read this quad's scales two slots ago; the next quad's land
+    // by the end of step 3 (they are older than its copies).
+    const bool more = s == 2 && 4 * (q + 1) < nk;
+    if (more) issue_scales(q + 1);
+    // stage k + 1 has landed
+    if (more && nk - 2 - k >= STAGES - 2) gemm_wait_vmcnt<PER * (STAGES - 2) + 1>();
+    else gemm_wait_groups<PER, STAGES - 2>(nk - 2 - k);
     __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
     bar();
     constexpr int word = 2 * (s / 2), byte = 2 * (s % 2);
-    if constexpr (k32) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t sb = sc[1 + j / 2].w[word + j % 2], sa = sc[0].w[word + i];
-            acc32[i][j] = t == 0 ? mx_mfma32<byte>(fb[2 * j], fa[2 * i], acc32[i][j], sb, sa)
-                                 : mx_mfma32<byte + 1>(fb[2 * j + 1], fa[2 * i + 1], acc32[i][j], sb, sa);
-          }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t sb = sc[1 + j / 4].w[word + j % 2], sa = sc[0].w[word + i % 2];
-          const int e = (j % 4) / 2, f = i / 2;   // byte + e of sb, byte + f of sa
-          if (e == 0 && f == 0) acc[i][j] = mx_mac<QA, OT, byte, byte>(fb[j], fa[i], acc[i][j], sb, sa);
-          else if (e == 0) acc[i][j] = mx_mac<QA, OT, byte, byte + 1>(fb[j], fa[i], acc[i][j], sb, sa);
-          else if (f == 0) acc[i][j] = mx_mac<QA, OT, byte + 1, byte>(fb[j], fa[i], acc[i][j], sb, sa);
-          else acc[i][j] = mx_mac<QA, OT, byte + 1, byte + 1>(fb[j], fa[i], acc[i][j], sb, sa);
-        }
-    }
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t sb = sc[1 + j / 4].w[word + j % 2], sa = sc[0].w[word + i % 2];
+        const int e = (j % 4) / 2, f = i / 2;   // byte + e of sb, byte + f of sa
+        if (e == 0 && f == 0) acc[i][j] = mx_mac<FP8, OT, byte, byte>(fb[j], fa[i], acc[i][j], sb, sa);
+        else if (e == 0) acc[i][j] = mx_mac<FP8, OT, byte, byte + 1>(fb[j], fa[i], acc[i][j], sb, sa);
+        else if (f == 0) acc[i][j] = mx_mac<FP8, OT, byte + 1, byte>(fb[j], fa[i], acc[i][j], sb, sa);
+        else acc[i][j] = mx_mac<FP8, OT, byte + 1, byte + 1>(fb[j], fa[i], acc[i][j], sb, sa);
+      }
     bar();
-    if (last) {
-      ++st;
-      buf = buf == (STAGES - 1) * BYTES ? 0 : buf + BYTES;
-    }
+    buf = buf == (STAGES - 1) * BYTES ? 0 : buf + BYTES;
   };
   for (int q = 0; 4 * q < nk; ++q) {
     phase(q, std::integral_constant<int, 0>{});
@@ -479,26 +493,12 @@ mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ 
     if (4 * q + 3 < nk) phase(q, std::integral_constant<int, 3>{});
   }
 
-  // Each lane's sums come in fours of consecutive columns: 16 x 16 blocks hold row
-  // 16 i + li, columns 16 j + 4 lg ..; 32 x 32 row 32 i + lane % 32, columns 32 j + 8 e +
-  // 4 (lane / 32) .., e = 0 .. 3.
+  // A lane's sums: row 16 i + li, four columns from 16 j + 4 lg on.
   auto fours = [&](auto&& f) {
-    if constexpr (k32) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const v16f& v = acc32[i][j];
-            f(32 * i + lr, 32 * j + 8 * e + 4 * lc, v4f{v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]});
-          }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f(16 * i + li, 16 * j + 4 * lg, acc[i][j]);
-    }
+      for (int i = 0; i < 4; ++i) f(16 * i + li, 16 * j + 4 * lg, acc[i][j]);
   };
   // Group 0 is one slot ahead: it stages its rows while group 1 runs its last
   // compute slot, and copies them out while group 1 stages its own.
@@ -525,33 +525,548 @@ mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ 
   if (!grp1) bar();
 }
 
-template <class QA, class OT>
-void mx_gemm_launch(const MxOperand& a, const MxOperand& b, int blocks, void* out, int64_t ldc, const void* bias,
-                    hipStream_t stream) {
+// ---------------------------------------------------------------------------
+// mx_gemm_mid: BM x BN tiles (128 x 128, 128 x 64 or 64 x 64) by four waves (2 x 2), two
+// workgroups to a CU, for products whose 256 x 256 tiles would leave CUs idle. FP4:
+// stages of two k-steps (128-byte rows) and 32 x 32 MFMAs; FP8: one k-step, 16 x 16.
+// A wave reads step s + 1's fragments into a second register set while it
+// multiplies step s, so a step costs one barrier: it says that step s + 1 has landed and
+// that every wave holds step s in registers, which frees a stage that ends
+// there for copies.
+//
+// With few tiles the k-steps are split (blockIdx.y, whole quads): each part leaves its
+// float32 sums in `parts`, in the order of its registers, and mx_gemm_join adds
+// them in a fixed order.
+// ---------------------------------------------------------------------------
+template <class QA, int BM, int BN>
+struct MxMid {
+  static constexpr bool k32 = QA::code == QO_MX_FP4;
+  static constexpr int KS = k32 ? 2 : 1;
+  // As many stages as let two workgroups share a CU's LDS: a small tile's step is
+  // short, and its copies need as long.
+  static constexpr int STAGES = BM + BN == 256 ? (k32 ? 2 : 3) : BM + BN == 192 ? 3 : (k32 ? 4 : 6);
+  static constexpr int WM = BM / 2, WN = BN / 2;      // a wave's outputs
+  static constexpr int SIDE = k32 ? 32 : 16;          // of an MFMA's block
+  static constexpr int FM = WM / SIDE, FN = WN / SIDE, FOURS = SIDE * SIDE / 256;
+  static constexpr int VALUES = FM * FN * FOURS;      // fours of sums of a lane
+  // Lane's sums number f (of VALUES): its row and first column in the tile.
+  __device__ static inline int row(int f, int wm, int lane) { return WM * wm + SIDE * (f / FOURS / FN) + (lane & (SIDE - 1)); }
+  __device__ static inline int col(int f, int wn, int lane) {
+    return WN * wn + SIDE * (f / FOURS % FN) + (k32 ? 8 * (f % FOURS) + 4 * (lane >> 5) : 4 * (lane >> 4));
+  }
+};
+
+// A tile's sums (four waves, 2 x 2) + bias to out: 16-bit values through LDS, in 16-byte
+// pieces of rows, float32 from registers. s_bias holds the tile's columns.
+template <class QA, class OT, int BM, int BN>
+__device__ inline void mx_mid_store(const v4f (&acc)[MxMid<QA, BM, BN>::VALUES], unsigned char* c_tile, const float* s_bias,
+                                    typename OT::T* out, int64_t ldc, int M, int N, int m0, int n0, int tid) {
+  using G = MxMid<QA, BM, BN>;
   using T = typename OT::T;
-  T* o = reinterpret_cast<T*>(out);
-  const T* bi = reinterpret_cast<const T*>(bias);
-  auto go = [&](auto kernel, int bm, int bn, int threads) {
-    const int64_t tiles = ((int64_t)(a.rows + bm - 1) / bm) * ((b.rows + bn - 1) / bn);
-    launch(kernel, dim3((unsigned)tiles), dim3(threads), 0, stream, a, b, blocks, o, ldc, bi);
+  constexpr int C_PITCH = BN * 2 + 16;
+  const int lane = tid & 63, wm = (tid >> 6) >> 1, wn = (tid >> 6) & 1;
+#pragma unroll
+  for (int f = 0; f < G::VALUES; ++f) {
+    const int r = G::row(f, wm, lane), c = G::col(f, wn, lane);
+    const v4f v = acc[f] + *reinterpret_cast<const v4f*>(s_bias + c);
+    if constexpr (sizeof(T) == 2) {
+      T o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = OT::cvt(v[e]);
+      *reinterpret_cast<v2i*>(c_tile + r * C_PITCH + 2 * c) =
+          v2i{(int)(out_bits<OT>(o[0]) | out_bits<OT>(o[1]) << 16), (int)(out_bits<OT>(o[2]) | out_bits<OT>(o[3]) << 16)};
+    } else {
+      mx_store4<OT>(v, out, ldc, nullptr, M, N, m0 + r, n0 + c);
+    }
+  }
+  if constexpr (sizeof(T) == 2) {
+    lds_barrier();
+    copy_out_c<BM, BN, 256, OT>(c_tile, C_PITCH, out, ldc, M, N, m0, n0, tid);
+  }
+}
+
+template <class QA, class OT, int BM, int BN>
+__global__ void __launch_bounds__(256, 2)
+mx_gemm_mid(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ out, int64_t ldc,
+            const typename OT::T* __restrict__ bias, int tiles_m, v4f* __restrict__ parts) {
+  using G = MxMid<QA, BM, BN>;
+  constexpr int W = 4, KS = G::KS, STAGES = G::STAGES;
+  using RA = MxRow<QA, KS>;
+  using RB = MxRow<FP4, KS>;
+  constexpr int A_BYTES = BM * RA::bytes, BYTES = A_BYTES + BN * RB::bytes;
+  constexpr int TA = A_BYTES / 1024 / W, TB = BN * RB::bytes / 1024 / W, PER = TA + TB;
+  constexpr int RING = STAGES * BYTES;
+  static_assert(TA * 4096 == A_BYTES && TB * 4096 == BYTES - A_BYTES, "whole copies");
+  constexpr int C_BYTES = sizeof(typename OT::T) == 2 ? BM * (BN * 2 + 16) : 0;
+  static_assert(C_BYTES + BN * 4 <= RING, "staged output and bias");
+  constexpr int SCALES = (BM + BN) * 16;
+  __shared__ __align__(16) unsigned char ring[RING];
+  __shared__ __align__(16) unsigned char s_scales[2 * SCALES];   // even and odd quads'
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 1, wn = wave & 1, lr = lane & (G::SIDE - 1), lc = lane / G::SIDE;
+  const int M = a.rows, N = b.rows;
+  const MxTile tile = mx_tile_of<8>(tiles_m, (N + BN - 1) / BN);
+  const int m0 = tile.m * BM, n0 = tile.n * BN;
+
+  // This part's quads of k-steps. Stages past the last repeat it: blocks past a row's
+  // end, whose scales are 0, add nothing.
+  const int all = (blocks + 15) >> 4;
+  const int q0 = (int)((int64_t)all * blockIdx.y / gridDim.y), nq = (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y) - q0;
+  const int st0 = 4 / KS * q0, last_stage = (blocks - 1) / (4 * KS);
+
+  // Copies as in mx_gemm_tile.
+  const uint8_t* const a_base = a.codes + (int64_t)m0 * a.ld;
+  const uint8_t* const b_base = b.codes + (int64_t)n0 * b.ld;
+  const int a_end = blocks * (QA::code == QO_MX_FP4 ? 16 : 32) - 16, b_end = blocks * 16 - 16;
+  uint32_t voff[PER];
+  auto copy_row = [&](auto rowc, int t) -> int { return (wave + W * t) * decltype(rowc)::per_copy + lane / (decltype(rowc)::bytes / 16); };
+  auto copy_chunk = [&](auto rowc, int row) -> int { return (lane & (decltype(rowc)::bytes / 16 - 1)) ^ decltype(rowc)::swizzle(row); };
+  const int ca = 16 * copy_chunk(RA{}, copy_row(RA{}, 0)), cb = 16 * copy_chunk(RB{}, copy_row(RB{}, 0));
+#pragma unroll
+  for (int t = 0; t < PER; ++t)
+    voff[t] = t < TA ? (uint32_t)min(copy_row(RA{}, t), M - 1 - m0) * (uint32_t)a.ld + ca
+                     : (uint32_t)min(copy_row(RB{}, t - TA), N - 1 - n0) * (uint32_t)b.ld + cb;
+  const uint32_t ring0 = lds_addr(ring) + 1024 * wave;
+  auto issue = [&](int st, uint32_t buf) {
+    st = min(st0 + st, last_stage);
+    const int oa = st * RA::bytes, ob = st * RB::bytes;
+    const uint32_t over_a = max(oa + ca - a_end, 0), over_b = max(ob + cb - b_end, 0);
+#pragma unroll
+    for (int t = 0; t < PER; ++t) {
+      const uint32_t dst = ring0 + buf + (t < TA ? 4096 * t : A_BYTES + 4096 * (t - TA));
+      if (t < TA) dma16_s(voff[t] - over_a, a_base + oa, __builtin_amdgcn_readfirstlane(dst));
+      else dma16_s(voff[t] - over_b, b_base + ob, __builtin_amdgcn_readfirstlane(dst));
+    }
   };
-  constexpr int KS = QA::code == QO_MX_FP4 ? 2 : 1, STAGES = QA::code == QO_MX_FP4 ? 2 : 3;
-  if (a.rows > 64 && blocks > 0 && a.ld < (1 << 23) && b.ld < (1 << 23)) {   // 32-bit offsets within a tile
-    const int tm = (a.rows + 255) / 256, tn = (b.rows + 255) / 256;
-    launch(mx_gemm_tile<QA, OT, KS, STAGES>, dim3((unsigned)(tm * tn)), dim3(512), 0, stream, a, b, blocks, o, ldc, bi, tm);
+
+  // Scales: BM / 64 waves copy 64 rows of A each, the next BN / 64 B's; spare waves repeat the last.
+  constexpr int SA = BM / 64, SB = BN / 64;
+  const int sw = min(wave, SA + SB - 1);
+  const uint8_t* const s_base = sw < SA ? a.scales + (int64_t)m0 * a.scales_ld : b.scales + (int64_t)n0 * b.scales_ld;
+  const uint32_t s_off = sw < SA ? (uint32_t)min(64 * sw + lane, M - 1 - m0) * (uint32_t)a.scales_ld
+                                 : (uint32_t)min(64 * (sw - SA) + lane, N - 1 - n0) * (uint32_t)b.scales_ld;
+  const uint32_t s_dst = __builtin_amdgcn_readfirstlane(lds_addr(s_scales) + 1024 * sw);
+  auto issue_scales = [&](int q) {   // quads past the last repeat it
+    dma16_s(s_off, s_base + 16 * (int64_t)min(q0 + q, all - 1), __builtin_amdgcn_readfirstlane(s_dst + (q & 1) * SCALES));
+  };
+  MxScales sc[2];
+  auto load_scales = [&](int q) {
+    const int past = 16 * (q0 + q + 1) - blocks;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // a wave of fewer than 64 rows uses the first lanes' (the others read any row of the tile)
+      const int row = i == 0 ? min(G::WM * wm + lane, BM - 1) : BM + min(G::WN * wn + lane, BN - 1);
+      v4i v = *reinterpret_cast<const v4i*>(s_scales + (q & 1) * SCALES + 16 * row);
+      if (past > 0) mx_clear_scales(v, past);
+      sc[i] = G::k32 ? mx_scales32(v) : mx_scales16(v);
+    }
+  };
+
+  const uint32_t xa = (G::WM * wm + lr) * RA::bytes + 16 * (lc ^ RA::swizzle(lr));
+  const uint32_t xb = A_BYTES + (G::WN * wn + lr) * RB::bytes + 16 * (lc ^ RB::swizzle(lr));
+  constexpr int H = G::k32 ? 2 : 1;   // fragments of a block of rows and a k-step
+  v8i fa[2][G::FM * H], fb[2][G::FN * H];
+  auto chunk = [&](uint32_t at) -> v4i { return *reinterpret_cast<const v4i*>(ring + at); };
+  auto load_regs = [&](uint32_t buf, auto halfc, auto setc) {   // k-step `half` of the stage
+    constexpr int set = decltype(setc)::value, half = decltype(halfc)::value;
+#pragma unroll
+    for (int i = 0; i < G::FM * H; ++i) {
+      const uint32_t at = buf + G::SIDE * (i / H) * RA::bytes;
+      const v4i x = chunk(at + (xa ^ (64 * half + 32 * (i % H))));
+      if constexpr (G::k32) {
+        fa[set][i] = v8i{x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+      } else {
+        const v4i y = chunk(at + (xa ^ 64));
+        fa[set][i] = v8i{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < G::FN * H; ++j) {
+      const v4i x = chunk(buf + G::SIDE * (j / H) * RB::bytes + (xb ^ (64 * half + 32 * (j % H))));
+      fb[set][j] = v8i{x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+    }
+  };
+
+  v4f acc[G::k32 ? 1 : G::VALUES];
+  v16f acc32[G::k32 ? G::FM * G::FN : 1];
+#pragma unroll
+  for (auto& v : acc) v = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (auto& v : acc32)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) v[r] = 0.f;
+
+  const float my_bias = bias ? (float)bias[min(n0 + min(tid, BN - 1), N - 1)] : 0.f;
+  issue_scales(0);
+#pragma unroll
+  for (int st = 0; st < STAGES; ++st) {
+    if (st == STAGES - 1) issue_scales(1);   // before the last copies, as in every quad's step 3
+    issue(st, st * BYTES);
+  }
+  gemm_wait_vmcnt<PER * (STAGES - 1) + 1>();   // the first stage and scales have landed
+  lds_barrier();
+  load_regs(0, std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
+
+  uint32_t buf = 0;   // the stage of step s
+  auto phase = [&](int q, auto stepc, auto lastc) {
+    constexpr int s = decltype(stepc)::value, h = s % KS, T = s / KS, PQ = 4 / KS;   // stage T of the quad's PQ
+    constexpr bool LAST = decltype(lastc)::value;
+    // Stage T + 1 has landed; the later ones may be under way, and the scales copied
+    // before the last stage of the quad before (stage STAGES - 1 from this quad's
+    // first) where that may be: not where step 0, which has no wait when KS = 2, needs
+    // them. The last quad has no copies of its own past its end.
+    if constexpr (h == KS - 1) {
+      constexpr int issued = LAST ? std::max(STAGES - 1, std::min(T + STAGES - 1, PQ - 1)) : T + STAGES - 1;
+      constexpr int flying = std::max(issued - (T + 1), 0);
+      gemm_wait_vmcnt<PER * flying + (issued - flying < STAGES - 1 && !(KS == 2 && T == PQ - 1) ? 1 : 0)>();
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    lds_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (s == 0) load_scales(q);
+    const uint32_t next = buf == (STAGES - 1) * BYTES ? 0 : buf + BYTES;
+    if constexpr (!(LAST && s == 3))
+      load_regs(h == KS - 1 ? next : buf, std::integral_constant<int, (s + 1) % KS>{}, std::integral_constant<int, (s + 1) & 1>{});
+    if constexpr (!LAST && s == 3) issue_scales(q + 2);   // this quad's are in registers
+    if constexpr (h == KS - 1 && (!LAST || T + STAGES < PQ)) issue(PQ * q + T + STAGES, buf);   // so is this stage
+    constexpr int set = s & 1, word = 2 * (s / 2), byte = 2 * (s % 2);
+    if constexpr (G::k32) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < G::FN; ++j)
+#pragma unroll
+          for (int i = 0; i < G::FM; ++i) {
+            v16f& v = acc32[i * G::FN + j];
+            const uint32_t sb = sc[1].w[word + j], sa = sc[0].w[word + i];
+            v = t == 0 ? mx_mfma32<byte>(fb[set][2 * j], fa[set][2 * i], v, sb, sa)
+                       : mx_mfma32<byte + 1>(fb[set][2 * j + 1], fa[set][2 * i + 1], v, sb, sa);
+          }
+    } else {
+#pragma unroll
+      for (int j = 0; j < G::FN; ++j)
+#pragma unroll
+        for (int i = 0; i < G::FM; ++i) {
+          v4f& v = acc[i * G::FN + j];
+          const uint32_t sb = sc[1].w[word + j % 2], sa = sc[0].w[word + i % 2];
+          const int e = j / 2, f = i / 2;   // byte + e of sb, byte + f of sa
+          if (e == 0 && f == 0) v = mx_mac<QA, OT, byte, byte>(fb[set][j], fa[set][i], v, sb, sa);
+          else if (e == 0) v = mx_mac<QA, OT, byte, byte + 1>(fb[set][j], fa[set][i], v, sb, sa);
+          else if (f == 0) v = mx_mac<QA, OT, byte + 1, byte>(fb[set][j], fa[set][i], v, sb, sa);
+          else v = mx_mac<QA, OT, byte + 1, byte + 1>(fb[set][j], fa[set][i], v, sb, sa);
+        }
+    }
+    if constexpr (h == KS - 1) buf = next;
+  };
+  auto quad = [&](int q, auto lastc) {
+    phase(q, std::integral_constant<int, 0>{}, lastc);
+    phase(q, std::integral_constant<int, 1>{}, lastc);
+    phase(q, std::integral_constant<int, 2>{}, lastc);
+    phase(q, std::integral_constant<int, 3>{}, lastc);
+  };
+  for (int q = 0; q < nq - 1; ++q) quad(q, std::false_type{});
+  quad(nq - 1, std::true_type{});
+  gemm_wait_vmcnt<0>();
+  lds_barrier();   // every wave has read its last step and nothing is under way: the ring is free
+
+  v4f sums[G::VALUES];
+#pragma unroll
+  for (int f = 0; f < G::VALUES; ++f) {
+    if constexpr (G::k32) {
+      const v16f& v = acc32[f / 4];
+      sums[f] = v4f{v[4 * (f % 4)], v[4 * (f % 4) + 1], v[4 * (f % 4) + 2], v[4 * (f % 4) + 3]};
+    } else {
+      sums[f] = acc[f];
+    }
+  }
+  if (parts) {
+    v4f* p = parts + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * (BM * BN / 4) + tid;
+#pragma unroll
+    for (int f = 0; f < G::VALUES; ++f) p[256 * f] = sums[f];
     return;
   }
-  if (a.rows <= 16) go(mx_gemm_stream<QA, OT, 1, 1, 1, 8>, 16, 16, 512);
-  else go(mx_gemm_stream<QA, OT, 4, 2, 1, 4>, 64, 32, 256);
+  float* const s_bias = reinterpret_cast<float*>(ring + C_BYTES);
+  if (tid < BN) s_bias[tid] = my_bias;
+  lds_barrier();
+  mx_mid_store<QA, OT, BM, BN>(sums, ring, s_bias, out, ldc, M, N, m0, n0, tid);
+}
+
+// The parts of mx_gemm_mid's split products, added in order (workgroup = tile).
+template <class QA, class OT, int BM, int BN>
+__global__ void __launch_bounds__(256)
+mx_gemm_join(const v4f* __restrict__ parts, int splits, typename OT::T* __restrict__ out, int64_t ldc,
+             const typename OT::T* __restrict__ bias, int M, int N, int tiles_m) {
+  using G = MxMid<QA, BM, BN>;
+  __shared__ __align__(16) unsigned char c_tile[sizeof(typename OT::T) == 2 ? BM * (BN * 2 + 16) : 16];
+  __shared__ __align__(16) float s_bias[BN];
+  const int tid = threadIdx.x;
+  const MxTile tile = mx_tile_of<8>(tiles_m, (N + BN - 1) / BN);
+  const int m0 = tile.m * BM, n0 = tile.n * BN;
+  if (tid < BN) s_bias[tid] = bias ? (float)bias[min(n0 + tid, N - 1)] : 0.f;
+  const v4f* p = parts + (int64_t)blockIdx.x * (BM * BN / 4) + tid;
+  const int64_t part = (int64_t)gridDim.x * (BM * BN / 4);
+  v4f sums[G::VALUES];
+#pragma unroll
+  for (int f = 0; f < G::VALUES; ++f) sums[f] = p[256 * f];
+  for (int z = 1; z < splits; ++z)
+#pragma unroll
+    for (int f = 0; f < G::VALUES; ++f) sums[f] += p[z * part + 256 * f];
+  __syncthreads();
+  mx_mid_store<QA, OT, BM, BN>(sums, c_tile, s_bias, out, ldc, M, N, m0, n0, tid);
+}
+
+// ---------------------------------------------------------------------------
+// mx_gemm_wide: FP4 x FP4, 256 x 256 tiles by four waves (2 x 2, one to a SIMD), each
+// 128 x 128 in 4 x 4 blocks of 32 x 32: a wave's LDS reads then serve twice the
+// products of a 64 x 128 wave's. Stages of two k-steps (128-byte rows) on a ring of two.
+// While a wave multiplies step j it reads step j + 1's fragments into a second
+// register set and, in odd steps, copies the stage after the next, one LDS
+// or copy instruction between every two MFMAs; a step costs one barrier.
+// ---------------------------------------------------------------------------
+template <class OT>
+__global__ void __launch_bounds__(256, 1)
+mx_gemm_wide(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ out, int64_t ldc,
+             const typename OT::T* __restrict__ bias, int tiles_m) {
+  using T = typename OT::T;
+  using R = MxRow<FP4, 2>;
+  constexpr int BM = 256, BN = 256, W = 4;
+  constexpr int A_BYTES = BM * R::bytes, BYTES = 2 * A_BYTES;
+  constexpr int PER = BYTES / 1024 / W;   // copies of a wave for a stage: A's, then B's
+  constexpr bool k16 = sizeof(T) == 2;
+  constexpr int C_PITCH = BN * 2 + 16, RING = 2 * BYTES, CTILE = k16 ? BM * C_PITCH : 0;
+  __shared__ __align__(16) unsigned char ring[RING > CTILE ? RING : CTILE];
+  __shared__ __align__(16) unsigned char s_scales[(BM + BN) * 16];   // a quad's: A's rows, B's rows
+  __shared__ __align__(16) float s_bias[BN];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 1, wn = wave & 1, lr = lane & 31, lc = lane >> 5;
+  const int M = a.rows, N = b.rows;
+
+  const MxTile tile = mx_tile_of<4>(tiles_m, (N + BN - 1) / BN);
+  const int m0 = tile.m * BM, n0 = tile.n * BN;
+
+  // Copies as in mx_gemm_tile: copy t of this wave fills rows 8 (wave + 4 t) .. of A or B.
+  const uint8_t* const a_base = a.codes + (int64_t)m0 * a.ld;
+  const uint8_t* const b_base = b.codes + (int64_t)n0 * b.ld;
+  const int end = blocks * 16 - 16;
+  const int cc = 16 * ((lane & 7) ^ R::swizzle(8 * wave + (lane >> 3)));
+  uint32_t voff[PER];
+#pragma unroll
+  for (int t = 0; t < PER; ++t) {
+    const int row = 8 * (wave + W * (t % (PER / 2))) + (lane >> 3);
+    voff[t] = t < PER / 2 ? (uint32_t)min(row, M - 1 - m0) * (uint32_t)a.ld + cc : (uint32_t)min(row, N - 1 - n0) * (uint32_t)b.ld + cc;
+  }
+  // The loop runs whole quads of k-steps: stages past the last repeat it, and the
+  // blocks past a row's end, whose scales are 0, add nothing.
+  const int nq = (blocks + 15) >> 4, last_stage = (blocks - 1) >> 3;
+  const uint32_t ring0 = lds_addr(ring) + 1024 * wave;
+  auto copy = [&](int t, int st, uint32_t buf, uint32_t over) {
+    const uint32_t dst = ring0 + buf + (t < PER / 2 ? 4096 * t : A_BYTES + 4096 * (t - PER / 2));
+    dma16_s(voff[t] - over, (t < PER / 2 ? a_base : b_base) + st * R::bytes, __builtin_amdgcn_readfirstlane(dst));
+  };
+  auto over_of = [&](int st) -> uint32_t { return max(st * R::bytes + cc - end, 0); };
+
+  // Scales: wave w copies rows 128 w .. of A's then B's.
+  const bool s_a = wave < 2;
+  const uint8_t* const s_base = s_a ? a.scales + (int64_t)m0 * a.scales_ld : b.scales + (int64_t)n0 * b.scales_ld;
+  uint32_t s_off[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int row = 128 * (wave & 1) + 64 * h + lane;
+    s_off[h] = s_a ? (uint32_t)min(row, M - 1 - m0) * (uint32_t)a.scales_ld : (uint32_t)min(row, N - 1 - n0) * (uint32_t)b.scales_ld;
+  }
+  const uint32_t s_dst = lds_addr(s_scales) + 2048 * wave;
+  auto issue_scales = [&](int q) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) dma16_s(s_off[h], s_base + 16 * (int64_t)q, __builtin_amdgcn_readfirstlane(s_dst + 1024 * h));
+  };
+  v4i raw[4];        // A's two 64 rows, B's two
+  MxScales sc[4];
+  auto read_scales = [&](int i) { raw[i] = *reinterpret_cast<const v4i*>(s_scales + 16 * (i < 2 ? 128 * wm + 64 * i + lane : BM + 128 * wn + 64 * (i - 2) + lane)); };
+  auto set_scales = [&](int q) {
+    const int past = 16 * (q + 1) - blocks;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (past > 0) mx_clear_scales(raw[i], past);
+      sc[i] = mx_scales32(raw[i]);
+    }
+  };
+
+  const uint32_t x = lr * R::bytes + 16 * (lc ^ R::swizzle(lr));
+  v4i fa[2][8], fb[2][8];   // [set][2 * block of 32 rows + half]
+  // fragment f of step k: A's 0 .. 7, B's 8 .. 15
+  auto read = [&](int k, int f, v4i& to) {
+    const uint32_t at = ((k >> 1) & 1) * BYTES + (f < 8 ? 128 * wm * R::bytes : A_BYTES + 128 * wn * R::bytes) + 32 * ((f % 8) / 2) * R::bytes;
+    to = *reinterpret_cast<const v4i*>(ring + at + (x ^ (64 * (k & 1) + 32 * (f % 2))));
+  };
+  auto wide = [](const v4i& v) -> v8i { return v8i{v[0], v[1], v[2], v[3], 0, 0, 0, 0}; };
+
+  v16f acc[4][4];
+#pragma unroll
+  for (auto& row : acc)
+#pragma unroll
+    for (auto& v : row)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) v[r] = 0.f;
+
+  issue_scales(0);
+  if (tid < BN) s_bias[tid] = bias ? (float)bias[min(n0 + tid, N - 1)] : 0.f;
+#pragma unroll
+  for (int st = 0; st < 2; ++st) {
+    const int from = min(st, last_stage);
+    const uint32_t over = over_of(from);
+#pragma unroll
+    for (int t = 0; t < PER; ++t) copy(t, from, st * BYTES, over);
+  }
+  gemm_wait_vmcnt<PER>();
+  lds_barrier();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) read_scales(i);
+#pragma unroll
+  for (int f = 0; f < 16; ++f) read(0, f, f < 8 ? fa[0][f] : fb[0][f - 8]);
+  gemm_wait_vmcnt<0>();
+
+  // Step 4 q + s: LAST: of the last quad.
+  auto phase = [&](int q, auto stepc, auto lastc) {
+    constexpr int s = decltype(stepc)::value, set = s & 1;
+    constexpr bool LAST = decltype(lastc)::value, reads = !(LAST && s == 3), copies = !LAST && s % 2 == 1;
+    if constexpr (s == 0) set_scales(q);
+    lds_barrier();   // step s + 1 has landed for every wave, and every wave holds step s
+    // odd steps: the stage that ends has been read whole, its slot takes the stage after the next
+    const int next = min(2 * q + s / 2 + 2, last_stage);
+    const uint32_t over = copies ? over_of(next) : 0;
+    if constexpr (!LAST && s == 2) issue_scales(q + 1);   // landed by this step's end
+    constexpr int word = 2 * (s / 2), byte = 2 * (s % 2);
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {   // two MFMAs, one read, one copy
+      if constexpr (reads) read(s + 1, u, u < 8 ? fa[set ^ 1][u] : fb[set ^ 1][u - 8]);
+      if constexpr (copies) copy(u, next, (s / 2) * BYTES, over);
+      if constexpr (!LAST && s == 3)
+        if (u % 4 == 3) read_scales(u / 4);
+      __builtin_amdgcn_sched_barrier(0);
+      const int t = u / 8, j = (u % 8) / 2;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = 2 * (u % 2) + e;
+        const uint32_t sb = sc[2 + j / 2].w[word + j % 2], sa = sc[i / 2].w[word + i % 2];
+        acc[i][j] = t == 0 ? mx_mfma32<byte>(wide(fb[set][2 * j]), wide(fa[set][2 * i]), acc[i][j], sb, sa)
+                           : mx_mfma32<byte + 1>(wide(fb[set][2 * j + 1]), wide(fa[set][2 * i + 1]), acc[i][j], sb, sa);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (!LAST && s % 2 == 0) gemm_wait_vmcnt<0>();   // the stage that the next step reads from, and scales
+  };
+  auto quad = [&](int q, auto lastc) {
+    phase(q, std::integral_constant<int, 0>{}, lastc);
+    phase(q, std::integral_constant<int, 1>{}, lastc);
+    phase(q, std::integral_constant<int, 2>{}, lastc);
+    phase(q, std::integral_constant<int, 3>{}, lastc);
+  };
+  for (int q = 0; q < nq - 1; ++q) quad(q, std::false_type{});
+  quad(nq - 1, std::true_type{});
+  lds_barrier();
+
+  // acc[i][j][4 e + r] is row 128 wm + 32 i + lane % 32, column 128 wn + 32 j + 8 e + 4 (lane / 32) + r.
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = 128 * wn + 32 * j + 8 * e + 4 * lc;
+      const v4f bb = *reinterpret_cast<const v4f*>(s_bias + c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 128 * wm + 32 * i + lr;
+        const v4f v = v4f{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]} + bb;
+        if constexpr (k16) {
+          T o[4];
+#pragma unroll
+          for (int z = 0; z < 4; ++z) o[z] = OT::cvt(v[z]);
+          *reinterpret_cast<v2i*>(ring + r * C_PITCH + 2 * c) =
+              v2i{(int)(out_bits<OT>(o[0]) | out_bits<OT>(o[1]) << 16), (int)(out_bits<OT>(o[2]) | out_bits<OT>(o[3]) << 16)};
+        } else {
+          mx_store4<OT>(v, out, ldc, nullptr, M, N, m0 + r, n0 + c);
+        }
+      }
+    }
+  if constexpr (k16) {
+    lds_barrier();
+    copy_out_c<BM, BN, 256, OT, true>(ring, C_PITCH, out, ldc, M, N, m0, n0, tid);
+  }
+}
+
+template <class QA, class OT>
+void mx_gemm_launch(const MxOperand& a, const MxOperand& b, int blocks, void* out, int64_t ldc, const void* bias,
+                    void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  using T = typename OT::T;
+  constexpr bool k8 = QA::code == QO_MX_FP8;
+  T* const o = reinterpret_cast<T*>(out);
+  const T* const bi = reinterpret_cast<const T*>(bias);
+  const int M = a.rows, N = b.rows;
+  auto tiled = [&](auto kernel, int bm, int bn, int threads, int splits, auto... more) {
+    const int tm = (M + bm - 1) / bm;
+    launch(kernel, dim3((unsigned)(tm * ((N + bn - 1) / bn)), splits), dim3(threads), 0, stream, a, b, blocks, o, ldc, bi, tm, more...);
+  };
+  auto mid = [&](auto bmc, auto bnc, int splits) {
+    constexpr int BM = decltype(bmc)::value, BN = decltype(bnc)::value;
+    v4f* const parts = splits > 1 ? reinterpret_cast<v4f*>(workspace) : nullptr;
+    tiled(mx_gemm_mid<QA, OT, BM, BN>, BM, BN, 256, splits, parts);
+    if (splits > 1) {
+      const int tm = (M + BM - 1) / BM;
+      launch(mx_gemm_join<QA, OT, BM, BN>, dim3((unsigned)(tm * ((N + BN - 1) / BN))), dim3(256), 0, stream, parts, splits, o,
+             ldc, bi, M, N, tm);
+    }
+  };
+  if (M > QO_MX_GEMM_FEW_ROWS && blocks > 0 && a.ld <= kMxMostRow && b.ld <= kMxMostRow) {
+    MxPlan plan = mx_plan(M, N, blocks, k8, device_cu_count(), true);
+    if (plan.splits > 1 && (!workspace || workspace_bytes < mx_plan_bytes(plan, M, N)))
+      plan = mx_plan(M, N, blocks, k8, device_cu_count(), false);
+    constexpr std::integral_constant<int, 128> c128{};
+    constexpr std::integral_constant<int, 64> c64{};
+    switch (plan.tile) {
+      case kMxTile256:
+        if constexpr (k8) tiled(mx_gemm_tile<OT>, 256, 256, 512, 1);
+        else tiled(mx_gemm_wide<OT>, 256, 256, 256, 1);
+        return;
+      case kMxTile128: return mid(c128, c128, plan.splits);
+      case kMxTile128x64: return mid(c128, c64, plan.splits);
+      default: return mid(c64, c64, plan.splits);
+    }
+  }
+  auto stream_rows = [&](auto fnc, auto wc, auto residentc, int per_cu) {
+    constexpr int FN = decltype(fnc)::value, W = decltype(wc)::value;
+    const int64_t tiles = (int64_t)((M + 15) / 16) * ((N + 16 * FN - 1) / (16 * FN));
+    const int64_t grid = std::min<int64_t>(tiles, (int64_t)per_cu * device_cu_count());
+    launch(mx_gemm_stream<QA, OT, FN, W, decltype(residentc)::value>, dim3((unsigned)grid), dim3(64 * W), 0, stream, a, b,
+           blocks, o, ldc, bi, tiles);
+  };
+  // us, weight from memory: up to 8 quads (one to a wave, one row of tiles: a's fragments
+  // stay) 8 waves, two workgroups a CU: 16 x 28672 x 4096 FP8 17.7 (one pair of columns 19.4,
+  // four workgroups 20.9). Longer: 16 waves, 1 x 4096 x 14336 FP8 10.0 (8 waves 14.0);
+  // with pairs of columns for every CU 8 waves, which read a half as often: 16 x 8192 x 28672
+  // FP8 38 (16 waves 50), 1 x 28672 x 8192 34 either way.
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 8> w8{};
+  if (blocks <= 128 && M <= 16) stream_rows(one, w8, std::true_type{}, 2);
+  else if (N >= 32 * device_cu_count()) stream_rows(std::integral_constant<int, 2>{}, w8, std::false_type{}, 2);
+  else stream_rows(one, std::integral_constant<int, 16>{}, std::false_type{}, 1);
 }
 
 }  // namespace
 
 }  // namespace qo
 
+extern "C" int64_t qo_mx_gemm_workspace_size(int64_t M, int64_t N, int64_t K, int a_format) {
+  using namespace qo;
+  if (M <= QO_MX_GEMM_FEW_ROWS || N < 1 || K < 32 || M > QO_MX_MAX_FEATURES || N > QO_MX_MAX_FEATURES || K > kMxMostRow) return 0;
+  const MxPlan plan = mx_plan(M, N, (K + 31) / 32, a_format == QO_MX_FP8, device_cu_count(), true);
+  return plan.splits > 1 ? mx_plan_bytes(plan, M, N) : 0;
+}
+
 extern "C" int qo_mx_gemm(const void* a, int64_t lda, int a_format, const uint8_t* a_scales, int64_t a_scales_ld,
                           const void* b, int64_t ldb, const uint8_t* b_scales, int64_t b_scales_ld, const void* bias,
-                          void* out, int out_dtype, int64_t ldc, int64_t M, int64_t N, int64_t K, void* stream) {
+                          void* out, int out_dtype, int64_t ldc, int64_t M, int64_t N, int64_t K, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
   using namespace qo;
   const char* fn = "qo_mx_gemm";
   if (M < 0 || N < 0 || K < 0 || K % 32 != 0 || M > QO_MX_MAX_FEATURES || N > QO_MX_MAX_FEATURES ||
@@ -587,6 +1102,16 @@ extern "C" int qo_mx_gemm(const void* a, int64_t lda, int a_format, const uint8_
     qo_set_error("%s: codes and their row strides must be multiples of 16 bytes", fn);
     return QO_ERR_ALIGNMENT;
   }
+  if (M > QO_MX_GEMM_FEW_ROWS && K > 0 &&
+      ((uintptr_t)a_scales % 16 != 0 || (uintptr_t)b_scales % 16 != 0 || a_scales_ld % 16 != 0 || b_scales_ld % 16 != 0)) {
+    qo_set_error("%s: scales and their row strides must be multiples of 16 bytes (more than %d rows)", fn,
+                 QO_MX_GEMM_FEW_ROWS);
+    return QO_ERR_ALIGNMENT;
+  }
+  if ((uintptr_t)workspace % 16 != 0) {
+    qo_set_error("%s: workspace must be 16-byte aligned", fn);
+    return QO_ERR_ALIGNMENT;
+  }
   const MxOperand A = {reinterpret_cast<const uint8_t*>(a), lda, a_scales, a_scales_ld, (int)M};
   const MxOperand B = {reinterpret_cast<const uint8_t*>(b), ldb, b_scales, b_scales_ld, (int)N};
   launch_begin();
@@ -594,9 +1119,9 @@ extern "C" int qo_mx_gemm(const void* a, int64_t lda, int a_format, const uint8_
     using QA = decltype(q);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const int blocks = (int)(K / 32);
-    if (out_dtype == QO_DTYPE_F32) mx_gemm_launch<QA, OutF32>(A, B, blocks, out, ldc, bias, s);
-    else if (out_dtype == QO_DTYPE_F16) mx_gemm_launch<QA, OutF16>(A, B, blocks, out, ldc, bias, s);
-    else mx_gemm_launch<QA, OutBF16>(A, B, blocks, out, ldc, bias, s);
+    if (out_dtype == QO_DTYPE_F32) mx_gemm_launch<QA, OutF32>(A, B, blocks, out, ldc, bias, workspace, workspace_bytes, s);
+    else if (out_dtype == QO_DTYPE_F16) mx_gemm_launch<QA, OutF16>(A, B, blocks, out, ldc, bias, workspace, workspace_bytes, s);
+    else mx_gemm_launch<QA, OutBF16>(A, B, blocks, out, ldc, bias, workspace, workspace_bytes, s);
   };
   if (a_format == QO_MX_FP4) with_out(FP4{});
   else with_out(FP8{});

@@ -29,7 +29,7 @@ __device__ inline void for_rows(const RowMap& map, int64_t tokens, F&& f) {
 template <class D, class Q, int U>
 __global__ void __launch_bounds__(256)
 mx_quantize_kernel(const typename D::T* __restrict__ x, int64_t ld, int64_t tokens, int64_t features, int blocks,
-                   RowMap map, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+                   RowMap map, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t scales_ld) {
   for_rows<U>(map, tokens, [&](int64_t row, int step, int c) {
     float v[U][8];
 #pragma unroll
@@ -37,7 +37,7 @@ mx_quantize_kernel(const typename D::T* __restrict__ x, int64_t ld, int64_t toke
       if (row + u * step < tokens) load8<D>(x + (row + u * step) * ld + 8 * c, features - 8 * c, v[u]);
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (row + u * step < tokens) mx_store8<Q>(v[u], codes, scales, row + u * step, blocks, c);
+      if (row + u * step < tokens) mx_store8<Q>(v[u], codes, scales, scales_ld, row + u * step, blocks, c);
   });
 }
 
@@ -46,7 +46,7 @@ mx_quantize_kernel(const typename D::T* __restrict__ x, int64_t ld, int64_t toke
 template <class D, class Q, int U>
 __global__ void __launch_bounds__(256)
 swiglu_mx_kernel(const typename D::T* __restrict__ x, int64_t ld, int64_t tokens, int64_t features, int blocks,
-                 RowMap map, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+                 RowMap map, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t scales_ld) {
   for_rows<U>(map, tokens, [&](int64_t row, int step, int c) {
     float g[U][8], up[U][8];
 #pragma unroll
@@ -61,14 +61,14 @@ swiglu_mx_kernel(const typename D::T* __restrict__ x, int64_t ld, int64_t tokens
       if (row + u * step < tokens) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[u][i] = g[u][i] / (1.f + expf(-g[u][i])) * up[u][i];
-        mx_store8<Q>(g[u], codes, scales, row + u * step, blocks, c);
+        mx_store8<Q>(g[u], codes, scales, scales_ld, row + u * step, blocks, c);
       }
   });
 }
 
 template <class D, class Q, int U>
 __global__ void __launch_bounds__(256)
-mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t tokens,
+mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t scales_ld, int64_t tokens,
                      int64_t features, int blocks, RowMap map, typename D::T* __restrict__ out) {
   for_rows<U>(map, tokens, [&](int64_t row, int step, int c) {
     uint32_t w[U][Q::words], byte[U];
@@ -77,7 +77,7 @@ mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restric
       if (row + u * step < tokens) {
         const int64_t r = row + u * step;
         __builtin_memcpy(w[u], codes + (r * blocks * 4 + c) * (4 * Q::words), sizeof(w[u]));
-        byte[u] = scales[r * blocks + (c >> 2)];
+        byte[u] = scales[r * scales_ld + (c >> 2)];
       }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(THREADS)
 rms_norm_mx_kernel(const typename D::T* __restrict__ x, int64_t ld, const typename D::T* res,
                    int64_t res_ld, const void* __restrict__ weight, int weight_dtype, int64_t tokens,
                    int64_t features, int blocks, float eps, uint8_t* __restrict__ codes,
-                   uint8_t* __restrict__ scales, typename D::T* res_out) {
+                   uint8_t* __restrict__ scales, int64_t scales_ld, typename D::T* res_out) {
   constexpr int W = THREADS / 64, N = NV ? NV : 1;
   __shared__ float part[W];
   const int tid = threadIdx.x, chunks = 4 * blocks;
@@ -146,7 +146,7 @@ rms_norm_mx_kernel(const typename D::T* __restrict__ x, int64_t ld, const typena
       weights(c, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = v[i] * r * w[i];
-      mx_store8<Q>(v, codes, scales, row, blocks, c);
+      mx_store8<Q>(v, codes, scales, scales_ld, row, blocks, c);
     };
     if constexpr (NV > 0) {
 #pragma unroll
@@ -193,9 +193,14 @@ bool known_dtype(int c) { return c == QO_DTYPE_F32 || c == QO_DTYPE_F16 || c == 
 bool known_format(int c) { return c == QO_MX_FP4 || c == QO_MX_FP8; }
 
 // Checks that the entry points share; QO_OK with *empty set where there is nothing to do.
-int check(const char* fn, int64_t tokens, int64_t features, int dtype, int format, bool* empty) {
+int check(const char* fn, int64_t tokens, int64_t features, int dtype, int format, int64_t scales_ld, bool* empty) {
   if (tokens < 0 || features < 0 || features > QO_MX_MAX_FEATURES) {
     qo_set_error("%s: invalid sizes tokens=%lld features=%lld", fn, (long long)tokens, (long long)features);
+    return QO_ERR_SHAPE;
+  }
+  if (scales_ld < (features + 31) / 32) {
+    qo_set_error("%s: scales_ld %lld below the %lld blocks of a row", fn, (long long)scales_ld,
+                 (long long)((features + 31) / 32));
     return QO_ERR_SHAPE;
   }
   if (!known_dtype(dtype)) {
@@ -225,11 +230,11 @@ int misaligned(const char* fn, const char* what) {
 }  // namespace qo
 
 extern "C" int qo_mx_quantize(const void* x, int x_dtype, int64_t tokens, int64_t features, int64_t x_ld, int format,
-                              void* codes, uint8_t* scales, void* stream) {
+                              void* codes, uint8_t* scales, int64_t scales_ld, void* stream) {
   using namespace qo;
   const char* fn = "qo_mx_quantize";
   bool empty;
-  const int st = check(fn, tokens, features, x_dtype, format, &empty);
+  const int st = check(fn, tokens, features, x_dtype, format, scales_ld, &empty);
   if (st != QO_OK) return st;
   if (x_ld < features) {
     qo_set_error("%s: row stride %lld below row length %lld", fn, (long long)x_ld, (long long)features);
@@ -246,18 +251,18 @@ extern "C" int qo_mx_quantize(const void* x, int x_dtype, int64_t tokens, int64_
       const Grid g = row_grid(tokens, 4 * blocks, 1);
       launch(mx_quantize_kernel<D, decltype(q), 1>, g.grid, dim3(256), 0, reinterpret_cast<hipStream_t>(stream),
              reinterpret_cast<const typename D::T*>(x), x_ld, tokens, features, blocks, g.map,
-             reinterpret_cast<uint8_t*>(codes), scales);
+             reinterpret_cast<uint8_t*>(codes), scales, scales_ld);
     });
   });
   return launch_result(fn);
 }
 
-extern "C" int qo_mx_dequantize(const void* codes, const uint8_t* scales, int format, int64_t tokens,
-                                int64_t features, void* out, int out_dtype, void* stream) {
+extern "C" int qo_mx_dequantize(const void* codes, const uint8_t* scales, int64_t scales_ld, int format,
+                                int64_t tokens, int64_t features, void* out, int out_dtype, void* stream) {
   using namespace qo;
   const char* fn = "qo_mx_dequantize";
   bool empty;
-  const int st = check(fn, tokens, features, out_dtype, format, &empty);
+  const int st = check(fn, tokens, features, out_dtype, format, scales_ld, &empty);
   if (st != QO_OK) return st;
   if (empty) return QO_OK;
   if (!codes || !scales || !out) return null_pointer(fn);
@@ -269,7 +274,7 @@ extern "C" int qo_mx_dequantize(const void* codes, const uint8_t* scales, int fo
     with_format(format, [&](auto q) {
       const Grid g = row_grid(tokens, (features + 7) / 8, 1);
       launch(mx_dequantize_kernel<D, decltype(q), 1>, g.grid, dim3(256), 0, reinterpret_cast<hipStream_t>(stream),
-             reinterpret_cast<const uint8_t*>(codes), scales, tokens, features, blocks, g.map,
+             reinterpret_cast<const uint8_t*>(codes), scales, scales_ld, tokens, features, blocks, g.map,
              reinterpret_cast<typename D::T*>(out));
     });
   });
@@ -277,11 +282,11 @@ extern "C" int qo_mx_dequantize(const void* codes, const uint8_t* scales, int fo
 }
 
 extern "C" int qo_swiglu_mx_quantize(const void* gate_up, int dtype, int64_t tokens, int64_t features, int64_t ld,
-                                     int format, void* codes, uint8_t* scales, void* stream) {
+                                     int format, void* codes, uint8_t* scales, int64_t scales_ld, void* stream) {
   using namespace qo;
   const char* fn = "qo_swiglu_mx_quantize";
   bool empty;
-  const int st = check(fn, tokens, features, dtype, format, &empty);
+  const int st = check(fn, tokens, features, dtype, format, scales_ld, &empty);
   if (st != QO_OK) return st;
   if (ld < 2 * features) {
     qo_set_error("%s: row stride %lld below row length %lld", fn, (long long)ld, (long long)(2 * features));
@@ -298,7 +303,7 @@ extern "C" int qo_swiglu_mx_quantize(const void* gate_up, int dtype, int64_t tok
       const Grid g = row_grid(tokens, 4 * blocks, 1);
       launch(swiglu_mx_kernel<D, decltype(q), 1>, g.grid, dim3(256), 0, reinterpret_cast<hipStream_t>(stream),
              reinterpret_cast<const typename D::T*>(gate_up), ld, tokens, features, blocks, g.map,
-             reinterpret_cast<uint8_t*>(codes), scales);
+             reinterpret_cast<uint8_t*>(codes), scales, scales_ld);
     });
   });
   return launch_result(fn);
@@ -307,11 +312,11 @@ extern "C" int qo_swiglu_mx_quantize(const void* gate_up, int dtype, int64_t tok
 extern "C" int qo_rms_norm_mx_quantize(const void* x, const void* residual, int x_dtype, int64_t tokens,
                                        int64_t features, int64_t x_ld, int64_t residual_ld, const void* weight,
                                        int weight_dtype, float eps, int format, void* codes, uint8_t* scales,
-                                       void* residual_out, void* stream) {
+                                       int64_t scales_ld, void* residual_out, void* stream) {
   using namespace qo;
   const char* fn = "qo_rms_norm_mx_quantize";
   bool empty;
-  const int st = check(fn, tokens, features, x_dtype, format, &empty);
+  const int st = check(fn, tokens, features, x_dtype, format, scales_ld, &empty);
   if (st != QO_OK) return st;
   if (!known_dtype(weight_dtype)) {
     qo_set_error("%s: unsupported weight dtype code %d", fn, weight_dtype);
@@ -335,7 +340,8 @@ extern "C" int qo_rms_norm_mx_quantize(const void* x, const void* residual, int 
       auto go = [&](auto kernel, int threads) {
         launch(kernel, grid, dim3(threads), 0, reinterpret_cast<hipStream_t>(stream), reinterpret_cast<const T*>(x),
                x_ld, reinterpret_cast<const T*>(residual), residual_ld, weight, weight_dtype, tokens, features, blocks,
-               eps, reinterpret_cast<uint8_t*>(codes), scales, residual ? reinterpret_cast<T*>(residual_out) : nullptr);
+               eps, reinterpret_cast<uint8_t*>(codes), scales, scales_ld,
+               residual ? reinterpret_cast<T*>(residual_out) : nullptr);
       };
       using Q = decltype(q);
       go(rms_norm_mx_kernel<D, Q, 256, 0>, 256);

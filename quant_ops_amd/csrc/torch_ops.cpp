@@ -248,13 +248,16 @@ int mx_codes_format(const at::Tensor& codes, const char* op, const char* name) {
   return QO_MX_FP8;
 }
 
-// Empty codes and scales for [tokens, features].
+// Empty codes and scales for [tokens, features]. Rows of scales stand a multiple of
+// 16 bytes apart, as mx_matmul reads them.
 std::tuple<at::Tensor, at::Tensor> mx_outputs(const at::Tensor& like, int64_t tokens, int64_t features, int format) {
   const int64_t blocks = (features + 31) / 32;
   at::Tensor codes = format == QO_MX_FP4 ? at::empty({tokens, 16 * blocks}, like.options().dtype(at::kByte))
                                          : at::empty({tokens, 32 * blocks}, like.options().dtype(at::kFloat8_e4m3fn));
-  return {codes, at::empty({tokens, blocks}, like.options().dtype(at::kByte))};
+  at::Tensor scales = at::empty({tokens, (blocks + 15) / 16 * 16}, like.options().dtype(at::kByte));
+  return {codes, blocks % 16 == 0 ? scales : scales.narrow(1, 0, blocks)};
 }
+int64_t mx_scales_ld(const at::Tensor& s) { return std::max(s.stride(0), s.size(1)); }
 
 void check_rows(const at::Tensor& x, const char* op, const char* name) {
   TORCH_CHECK(x.dim() == 2, op, ": ", name, " must be 2-D [tokens, features], got ", x.sizes());
@@ -276,7 +279,7 @@ std::tuple<at::Tensor, at::Tensor> mx_quantize(const at::Tensor& input, c10::str
   at::Tensor x = mx_rows(input);
   auto [codes, scales] = mx_outputs(x, x.size(0), x.size(1), format);
   check_status(qo_mx_quantize(x.data_ptr(), dtype_code(x.scalar_type()), x.size(0), x.size(1), mx_ld(x), format,
-                              codes.data_ptr(), scales.data_ptr<uint8_t>(), current_stream(x)),
+                              codes.data_ptr(), scales.data_ptr<uint8_t>(), mx_scales_ld(scales), current_stream(x)),
                "mx_quantize");
   return {codes, scales};
 }
@@ -295,10 +298,10 @@ at::Tensor mx_dequantize(const at::Tensor& codes, const at::Tensor& scales, std:
   const at::ScalarType dtype = out_dtype.value_or(at::kFloat);
   TORCH_CHECK(dtype_code(dtype) >= 0, "mx_dequantize: out_dtype must be float32, float16 or bfloat16");
   c10::DeviceGuard guard(codes.device());
-  at::Tensor q = codes.contiguous(), s = scales.contiguous();
+  at::Tensor q = codes.contiguous(), s = mx_rows(scales);
   if (reinterpret_cast<uintptr_t>(q.data_ptr()) % 8 != 0) q = q.clone();
   at::Tensor out = at::empty({T, F}, codes.options().dtype(dtype));
-  check_status(qo_mx_dequantize(q.data_ptr(), s.data_ptr<uint8_t>(), format, T, F, out.data_ptr(), dtype_code(dtype),
+  check_status(qo_mx_dequantize(q.data_ptr(), s.data_ptr<uint8_t>(), mx_scales_ld(s), format, T, F, out.data_ptr(), dtype_code(dtype),
                                 current_stream(codes)),
                "mx_dequantize");
   return out;
@@ -328,7 +331,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_mx_impl(const at::Tensor
   check_status(qo_rms_norm_mx_quantize(x.data_ptr(), residual ? res.data_ptr() : nullptr, dtype_code(x.scalar_type()),
                                        T, F, mx_ld(x), residual ? mx_ld(res) : 0, w.data_ptr(),
                                        dtype_code(w.scalar_type()), (float)eps, format, codes.data_ptr(),
-                                       scales.data_ptr<uint8_t>(), residual ? h.data_ptr() : nullptr,
+                                       scales.data_ptr<uint8_t>(), mx_scales_ld(scales), residual ? h.data_ptr() : nullptr,
                                        current_stream(x)),
                op);
   return {codes, scales, h};
@@ -355,7 +358,7 @@ std::tuple<at::Tensor, at::Tensor> swiglu_mx_quantize(const at::Tensor& gate_up,
   const int64_t T = x.size(0), F = x.size(1) / 2;
   auto [codes, scales] = mx_outputs(x, T, F, format);
   check_status(qo_swiglu_mx_quantize(x.data_ptr(), dtype_code(x.scalar_type()), T, F, mx_ld(x), format,
-                                     codes.data_ptr(), scales.data_ptr<uint8_t>(), current_stream(x)),
+                                     codes.data_ptr(), scales.data_ptr<uint8_t>(), mx_scales_ld(scales), current_stream(x)),
                "swiglu_mx_quantize");
   return {codes, scales};
 }
@@ -365,6 +368,22 @@ at::Tensor mx_gemm_rows(const at::Tensor& codes) {
   const bool fits = codes.stride(1) == 1 && reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0 &&
                     (codes.size(0) <= 1 || (codes.stride(0) >= codes.size(1) && codes.stride(0) % 16 == 0));
   return fits ? codes : codes.clone(at::MemoryFormat::Contiguous);
+}
+
+// Scales as the GEMM of `rows` rows reads them: with many, 16-byte aligned rows that are
+// readable up to a multiple of 16 bytes.
+at::Tensor mx_gemm_scales(const at::Tensor& scales, int64_t rows) {
+  at::Tensor s = mx_rows(scales);
+  if (rows <= QO_MX_GEMM_FEW_ROWS) return s;
+  const int64_t n = s.size(0), blocks = s.size(1), pad = (blocks + 15) / 16 * 16;
+  const int64_t stored = (int64_t)s.storage().nbytes() - s.storage_offset();
+  if (reinterpret_cast<uintptr_t>(s.data_ptr()) % 16 == 0 && mx_scales_ld(s) % 16 == 0 &&
+      (n - 1) * mx_scales_ld(s) + pad <= stored)
+    return s;
+  at::Tensor padded = at::empty({n, pad}, s.options());
+  at::Tensor view = padded.narrow(1, 0, blocks);
+  view.copy_(s);
+  return view;
 }
 
 at::Tensor mx_matmul(const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& b, const at::Tensor& b_scales,
@@ -387,16 +406,18 @@ at::Tensor mx_matmul(const at::Tensor& a, const at::Tensor& a_scales, const at::
   const int od = dtype_code(dtype);
   TORCH_CHECK(od >= 0, "mx_matmul: out_dtype must be float16, bfloat16 or float32");
   c10::DeviceGuard guard(a.device());
-  at::Tensor A = mx_gemm_rows(a), B = mx_gemm_rows(b), sa = mx_rows(a_scales), sb = mx_rows(b_scales), bv;
+  at::Tensor A = mx_gemm_rows(a), B = mx_gemm_rows(b), sa = mx_gemm_scales(a_scales, M), sb = mx_gemm_scales(b_scales, M), bv;
   if (bias.has_value()) {
     TORCH_CHECK(bias->device() == a.device() && bias->numel() == N, "mx_matmul: bias must hold N (", N,
                 ") elements on a's device");
     bv = bias->to(dtype).reshape({N}).contiguous();
   }
   at::Tensor out = at::empty({M, N}, a.options().dtype(dtype));
-  check_status(qo_mx_gemm(A.data_ptr(), mx_ld(A), format, sa.data_ptr<uint8_t>(), mx_ld(sa), B.data_ptr(), mx_ld(B),
-                          sb.data_ptr<uint8_t>(), mx_ld(sb), bv.defined() ? bv.data_ptr() : nullptr, out.data_ptr(), od,
-                          N, M, N, K, current_stream(a)),
+  const int64_t ws_bytes = qo_mx_gemm_workspace_size(M, N, K, format);
+  at::Tensor ws = gemm_workspace(ws_bytes, a);
+  check_status(qo_mx_gemm(A.data_ptr(), mx_ld(A), format, sa.data_ptr<uint8_t>(), mx_scales_ld(sa), B.data_ptr(),
+                          mx_ld(B), sb.data_ptr<uint8_t>(), mx_scales_ld(sb), bv.defined() ? bv.data_ptr() : nullptr, out.data_ptr(), od,
+                          N, M, N, K, ws.defined() ? ws.data_ptr() : nullptr, ws_bytes, current_stream(a)),
                "mx_matmul");
   return out;
 }

@@ -53,7 +53,7 @@ if _loader.KERNELS_AVAILABLE:
             blocks = (feats + 31) // 32
             codes = (like.new_empty((tokens, 16 * blocks), dtype=torch.uint8) if fmt == "mxfp4"
                      else like.new_empty((tokens, 32 * blocks), dtype=torch.float8_e4m3fn))
-            return codes, like.new_empty((tokens, blocks), dtype=torch.uint8)
+            return codes, like.new_empty((tokens, (blocks + 15) // 16 * 16), dtype=torch.uint8)[:, :blocks]
 
         @torch.library.register_fake("quant_ops::mx_quantize")
         def _mx_quantize_fake(input, fmt="mxfp4"):

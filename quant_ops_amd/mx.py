@@ -7,7 +7,8 @@ A row of F values has B = ceil(F / 32) blocks, the last padded with zeros:
 
 * mxfp4 codes: uint8 [T, 16 B], two per byte, the even value in the low bits;
 * mxfp8 codes: float8_e4m3fn [T, 32 B];
-* scales: uint8 [T, B].
+* scales: uint8 [T, B]; those made on the GPU stand a multiple of 16 bytes apart
+  by rows, as the product of many rows reads them (others are copied).
 
 e = floor(log2(largest magnitude)) - 2 (mxfp4) or - 8 (mxfp8), at least -127;
 codes are v / 2^e rounded to nearest even, saturated at 6 or 448. A block that

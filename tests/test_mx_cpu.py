@@ -91,27 +91,30 @@ def test_c_abi_checks():
     """Every refusal of the C entry points comes before a launch (the addresses are never read)."""
     lib = capi.lib()
     A = 4096   # an aligned, unused address
-    quantize = lambda x=A, dt=1, t=4, f=64, ld=64, fmt=0, c=A, s=A: lib.qo_mx_quantize(_p(x), dt, t, f, ld, fmt, _p(c), _p(s), _p(None))  # noqa: E731
+    quantize = lambda x=A, dt=1, t=4, f=64, ld=64, fmt=0, c=A, s=A, sl=2: lib.qo_mx_quantize(_p(x), dt, t, f, ld, fmt, _p(c), _p(s), sl, _p(None))  # noqa: E731
     assert quantize(t=0) == 0 and quantize(f=0) == 0
-    assert quantize(t=-1) == 2 and quantize(f=2 ** 31) == 2 and quantize(ld=63) == 2
+    assert quantize(t=-1) == 2 and quantize(f=2 ** 31, sl=2 ** 26) == 2 and quantize(ld=63) == 2 and quantize(sl=1) == 2
     assert quantize(dt=3) == 3 and quantize(fmt=2) == 3 and quantize(fmt=-1) == 3
     assert quantize(x=None) == 1 and quantize(c=None) == 1 and quantize(s=None) == 1
     assert quantize(c=A + 4) == 4 and b"aligned" in lib.qo_last_error()
-    deq = lambda c=A, s=A, fmt=0, t=4, f=64, o=A, dt=0: lib.qo_mx_dequantize(_p(c), _p(s), fmt, t, f, _p(o), dt, _p(None))  # noqa: E731
+    deq = lambda c=A, s=A, fmt=0, t=4, f=64, o=A, dt=0: lib.qo_mx_dequantize(_p(c), _p(s), 2, fmt, t, f, _p(o), dt, _p(None))  # noqa: E731
     assert deq(t=0) == 0 and deq(f=-1) == 2 and deq(dt=4) == 3 and deq(fmt=7) == 3 and deq(o=None) == 1 and deq(c=A + 2) == 4
     norm = lambda x=A, r=None, dt=1, t=4, f=64, ld=64, rld=64, w=A, wd=0, fmt=1, c=A, s=A, ro=None: lib.qo_rms_norm_mx_quantize(  # noqa: E731
-        _p(x), _p(r), dt, t, f, ld, rld, _p(w), wd, 1e-6, fmt, _p(c), _p(s), _p(ro), _p(None))
+        _p(x), _p(r), dt, t, f, ld, rld, _p(w), wd, 1e-6, fmt, _p(c), _p(s), 2, _p(ro), _p(None))
     assert norm(t=0) == 0 and norm(ld=63) == 2 and norm(r=A, rld=63, ro=A) == 2 and norm(wd=3) == 3 and norm(dt=9) == 3
     assert norm(w=None) == 1 and norm(r=A) == 1 and norm(c=A + 1) == 4
-    gate = lambda x=A, dt=1, t=4, f=64, ld=128, fmt=1, c=A, s=A: lib.qo_swiglu_mx_quantize(_p(x), dt, t, f, ld, fmt, _p(c), _p(s), _p(None))  # noqa: E731
+    gate = lambda x=A, dt=1, t=4, f=64, ld=128, fmt=1, c=A, s=A: lib.qo_swiglu_mx_quantize(_p(x), dt, t, f, ld, fmt, _p(c), _p(s), 2, _p(None))  # noqa: E731
     assert gate(t=0) == 0 and gate(ld=127) == 2 and gate(dt=3) == 3 and gate(x=None) == 1 and gate(c=A + 4) == 4
-    gemm = lambda a=A, lda=32, fa=0, sa=A, sal=2, b=A, ldb=32, sb=A, sbl=2, bias=None, o=A, od=2, ldc=8, M=4, N=8, K=64: lib.qo_mx_gemm(  # noqa: E731
-        _p(a), lda, fa, _p(sa), sal, _p(b), ldb, _p(sb), sbl, _p(bias), _p(o), od, ldc, M, N, K, _p(None))
+    gemm = lambda a=A, lda=32, fa=0, sa=A, sal=2, b=A, ldb=32, sb=A, sbl=2, bias=None, o=A, od=2, ldc=8, M=4, N=8, K=64, ws=None: lib.qo_mx_gemm(  # noqa: E731
+        _p(a), lda, fa, _p(sa), sal, _p(b), ldb, _p(sb), sbl, _p(bias), _p(o), od, ldc, M, N, K, _p(ws), 0, _p(None))
     assert gemm(M=0) == 0 and gemm(N=0) == 0
     assert gemm(K=65) == 2 and gemm(K=-32) == 2 and gemm(M=-1) == 2 and gemm(ldc=7) == 2 and gemm(lda=16) == 2 and gemm(ldb=16) == 2
     assert gemm(fa=1) == 2 and gemm(sal=1) == 2 and gemm(sbl=1) == 2      # FP8 rows are twice as long
     assert gemm(fa=2) == 3 and gemm(od=3) == 3
     assert gemm(a=None) == 1 and gemm(o=None) == 1 and gemm(sb=None) == 1
+    # more than 16 rows: scale rows of 16-byte multiples
+    assert gemm(M=17) == 4 and gemm(M=17, sal=16, sbl=8) == 4 and gemm(M=17, sal=16, sbl=16, sa=A + 8) == 4
+    assert gemm(M=17, sal=16, sbl=16, ws=A + 8) == 4
     assert gemm(a=A + 8) == 4 and gemm(b=A + 1) == 4 and gemm(lda=40) == 4 and gemm(ldb=33) == 4
 
 
