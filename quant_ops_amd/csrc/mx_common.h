@@ -69,50 +69,76 @@ __device__ inline void mx_codes8(const float (&v)[8], uint32_t byte, uint32_t (&
   }
 }
 
-// The values of eight codes.
+// The values of the codes in a word: eight (FP4) or four (FP8).
 template <class Q>
-__device__ inline void mx_values8(const uint32_t (&w)[Q::words], uint32_t byte, float (&v)[8]) {
+__device__ inline void mx_word_values(uint32_t w, uint32_t byte, float (&v)[8 / Q::words]) {
   const float scale = __builtin_bit_cast(float, byte << 23);   // field 255 reads as NaN
-  v2f p[4];
+  v2f p[4 / Q::words];
   if constexpr (Q::code == QO_MX_FP4) {
-    p[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], scale, 0);
-    p[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], scale, 1);
-    p[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], scale, 2);
-    p[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], scale, 3);
+    p[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0);
+    p[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 1);
+    p[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 2);
+    p[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 3);
   } else {
-    p[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[0], scale, false);
-    p[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[0], scale, true);
-    p[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[1], scale, false);
-    p[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[1], scale, true);
+    p[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, false);
+    p[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, true);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = p[i / 2][i % 2];
+  for (int i = 0; i < 8 / Q::words; ++i) v[i] = p[i / 2][i % 2];
 }
 
-// Eight elements from p, the first n of them (the rest 0). Whole pieces are one
-// 16-byte load (two for float32) at any alignment, which global loads allow.
+// Elements 8 c .. of a row of n (the rest 0). Whole pieces are one 16-byte load (two
+// for float32) at any alignment, which global loads allow. WHOLE: n is a
+// multiple of 8, so a piece is there or not; the load then has no branch (a
+// piece past the end reads the row's first and drops it), and loads of several
+// pieces are under way together.
 template <class D>
-__device__ inline void load8(const typename D::T* p, int64_t n, float (&v)[8]) {
+struct Raw8 {
   typename D::T t[8];
-  if (n >= 8) {
-    __builtin_memcpy(t, p, sizeof(t));
+};
+template <class D, bool WHOLE>
+__device__ inline Raw8<D> load8(const typename D::T* row, int c, int64_t n) {
+  Raw8<D> r;
+  if constexpr (WHOLE) {
+    __builtin_memcpy(r.t, row + (8 * c < n ? 8 * c : 0), sizeof(r.t));
   } else {
+    const typename D::T* p = row + 8 * c;
+    if (8 * c + 8 <= n) {
+      __builtin_memcpy(r.t, p, sizeof(r.t));
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = i < n ? p[i] : (typename D::T)0.f;
+      for (int i = 0; i < 8; ++i) r.t[i] = 8 * c + i < n ? p[i] : (typename D::T)0.f;
+    }
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = D::to_f(t[i]);
+  return r;
 }
-template <class D>
-__device__ inline void store8(typename D::T* p, int64_t n, const float (&v)[8]) {
-  typename D::T t[8];
+template <class D, bool WHOLE>
+__device__ inline void values8(const Raw8<D>& r, int c, int64_t n, float (&v)[8]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = D::from_f(v[i]);
-  if (n >= 8) {
-    __builtin_memcpy(p, t, sizeof(t));
+  for (int i = 0; i < 8; ++i) v[i] = !WHOLE || 8 * c < n ? D::to_f(r.t[i]) : 0.f;
+}
+
+// N values to the N elements at p, the first n of them; NT: as non-temporal 16-byte stores where p allows.
+template <class D, int N, bool NT = false>
+__device__ inline void store_row(typename D::T* p, int64_t n, const float (&v)[N]) {
+  typename D::T t[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) t[i] = D::from_f(v[i]);
+  if (n >= N) {
+    if constexpr (NT) {
+      static_assert(sizeof(t) % 16 == 0, "whole pieces");
+#pragma unroll
+      for (int h = 0; h < (int)sizeof(t) / 16; ++h) {
+        v4i w;
+        __builtin_memcpy(&w, reinterpret_cast<const char*>(t) + 16 * h, 16);
+        __builtin_nontemporal_store(w, reinterpret_cast<v4i*>(p) + h);
+      }
+    } else {
+      __builtin_memcpy(p, t, sizeof(t));
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < N; ++i)
       if (i < n) p[i] = t[i];
   }
 }
