@@ -628,16 +628,19 @@ mx_gemm_mid(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ o
     voff[t] = t < TA ? (uint32_t)min(copy_row(RA{}, t), M - 1 - m0) * (uint32_t)a.ld + ca
                      : (uint32_t)min(copy_row(RB{}, t - TA), N - 1 - n0) * (uint32_t)b.ld + cb;
   const uint32_t ring0 = lds_addr(ring) + 1024 * wave;
-  auto issue = [&](int st, uint32_t buf) {
+  struct From {
+    int oa, ob;
+    uint32_t over_a, over_b;
+  };
+  auto from = [&](int st) -> From {
     st = min(st0 + st, last_stage);
     const int oa = st * RA::bytes, ob = st * RB::bytes;
-    const uint32_t over_a = max(oa + ca - a_end, 0), over_b = max(ob + cb - b_end, 0);
-#pragma unroll
-    for (int t = 0; t < PER; ++t) {
-      const uint32_t dst = ring0 + buf + (t < TA ? 4096 * t : A_BYTES + 4096 * (t - TA));
-      if (t < TA) dma16_s(voff[t] - over_a, a_base + oa, __builtin_amdgcn_readfirstlane(dst));
-      else dma16_s(voff[t] - over_b, b_base + ob, __builtin_amdgcn_readfirstlane(dst));
-    }
+    return {oa, ob, (uint32_t)max(oa + ca - a_end, 0), (uint32_t)max(ob + cb - b_end, 0)};
+  };
+  auto copy = [&](int t, const From& f, uint32_t buf) {
+    const uint32_t dst = ring0 + buf + (t < TA ? 4096 * t : A_BYTES + 4096 * (t - TA));
+    if (t < TA) dma16_s(voff[t] - f.over_a, a_base + f.oa, __builtin_amdgcn_readfirstlane(dst));
+    else dma16_s(voff[t] - f.over_b, b_base + f.ob, __builtin_amdgcn_readfirstlane(dst));
   };
 
   // Scales: BM / 64 waves copy 64 rows of A each, the next BN / 64 B's; spare waves repeat the last.
@@ -668,23 +671,21 @@ mx_gemm_mid(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ o
   constexpr int H = G::k32 ? 2 : 1;   // fragments of a block of rows and a k-step
   v8i fa[2][G::FM * H], fb[2][G::FN * H];
   auto chunk = [&](uint32_t at) -> v4i { return *reinterpret_cast<const v4i*>(ring + at); };
-  auto load_regs = [&](uint32_t buf, auto halfc, auto setc) {   // k-step `half` of the stage
-    constexpr int set = decltype(setc)::value, half = decltype(halfc)::value;
-#pragma unroll
-    for (int i = 0; i < G::FM * H; ++i) {
-      const uint32_t at = buf + G::SIDE * (i / H) * RA::bytes;
-      const v4i x = chunk(at + (xa ^ (64 * half + 32 * (i % H))));
+  constexpr int NA = G::FM * H, NB = G::FN * H;
+  auto read = [&](int f, uint32_t buf, int half, v8i (&ta)[NA], v8i (&tb)[NB]) {   // fragment f of k-step `half` of the stage: A's, then B's
+    if (f < NA) {
+      const uint32_t at = buf + G::SIDE * (f / H) * RA::bytes;
+      const v4i x = chunk(at + (xa ^ (64 * half + 32 * (f % H))));
       if constexpr (G::k32) {
-        fa[set][i] = v8i{x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+        ta[f] = v8i{x[0], x[1], x[2], x[3], 0, 0, 0, 0};
       } else {
         const v4i y = chunk(at + (xa ^ 64));
-        fa[set][i] = v8i{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        ta[f] = v8i{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
       }
-    }
-#pragma unroll
-    for (int j = 0; j < G::FN * H; ++j) {
+    } else {
+      const int j = f - NA;
       const v4i x = chunk(buf + G::SIDE * (j / H) * RB::bytes + (xb ^ (64 * half + 32 * (j % H))));
-      fb[set][j] = v8i{x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+      tb[j] = v8i{x[0], x[1], x[2], x[3], 0, 0, 0, 0};
     }
   };
 
@@ -702,11 +703,14 @@ mx_gemm_mid(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ o
 #pragma unroll
   for (int st = 0; st < STAGES; ++st) {
     if (st == STAGES - 1) issue_scales(1);   // before the last copies, as in every quad's step 3
-    issue(st, st * BYTES);
+    const From f = from(st);
+#pragma unroll
+    for (int t = 0; t < PER; ++t) copy(t, f, st * BYTES);
   }
   gemm_wait_vmcnt<PER * (STAGES - 1) + 1>();   // the first stage and scales have landed
   lds_barrier();
-  load_regs(0, std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
+#pragma unroll
+  for (int f = 0; f < NA + NB; ++f) read(f, 0, 0, fa[0], fb[0]);
 
   uint32_t buf = 0;   // the stage of step s
   auto phase = [&](int q, auto stepc, auto lastc) {
@@ -726,36 +730,40 @@ mx_gemm_mid(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ o
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (s == 0) load_scales(q);
     const uint32_t next = buf == (STAGES - 1) * BYTES ? 0 : buf + BYTES;
-    if constexpr (!(LAST && s == 3))
-      load_regs(h == KS - 1 ? next : buf, std::integral_constant<int, (s + 1) % KS>{}, std::integral_constant<int, (s + 1) & 1>{});
+    constexpr bool reads = !(LAST && s == 3), copies = h == KS - 1 && (!LAST || T + STAGES < PQ);
     if constexpr (!LAST && s == 3) issue_scales(q + 2);   // this quad's are in registers
-    if constexpr (h == KS - 1 && (!LAST || T + STAGES < PQ)) issue(PQ * q + T + STAGES, buf);   // so is this stage
-    constexpr int set = s & 1, word = 2 * (s / 2), byte = 2 * (s % 2);
-    if constexpr (G::k32) {
+    From f = {};
+    if constexpr (copies) f = from(PQ * q + T + STAGES);   // into this stage's slot: it is in registers
+    constexpr int set = s & 1, word = 2 * (s / 2), byte = 2 * (s % 2), MF = G::FM * G::FN * H;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+    for (int u = 0; u < MF; ++u) {   // the next step's reads and the copies, spread between the MFMAs
+      if constexpr (reads) {
 #pragma unroll
-        for (int j = 0; j < G::FN; ++j)
+        for (int r = u * (NA + NB) / MF; r < (u + 1) * (NA + NB) / MF; ++r)
+          read(r, h == KS - 1 ? next : buf, (s + 1) % KS, fa[set ^ 1], fb[set ^ 1]);
+      }
+      if constexpr (copies) {
 #pragma unroll
-          for (int i = 0; i < G::FM; ++i) {
-            v16f& v = acc32[i * G::FN + j];
-            const uint32_t sb = sc[1].w[word + j], sa = sc[0].w[word + i];
-            v = t == 0 ? mx_mfma32<byte>(fb[set][2 * j], fa[set][2 * i], v, sb, sa)
-                       : mx_mfma32<byte + 1>(fb[set][2 * j + 1], fa[set][2 * i + 1], v, sb, sa);
-          }
-    } else {
-#pragma unroll
-      for (int j = 0; j < G::FN; ++j)
-#pragma unroll
-        for (int i = 0; i < G::FM; ++i) {
-          v4f& v = acc[i * G::FN + j];
-          const uint32_t sb = sc[1].w[word + j % 2], sa = sc[0].w[word + i % 2];
-          const int e = j / 2, f = i / 2;   // byte + e of sb, byte + f of sa
-          if (e == 0 && f == 0) v = mx_mac<QA, OT, byte, byte>(fb[set][j], fa[set][i], v, sb, sa);
-          else if (e == 0) v = mx_mac<QA, OT, byte, byte + 1>(fb[set][j], fa[set][i], v, sb, sa);
-          else if (f == 0) v = mx_mac<QA, OT, byte + 1, byte>(fb[set][j], fa[set][i], v, sb, sa);
-          else v = mx_mac<QA, OT, byte + 1, byte + 1>(fb[set][j], fa[set][i], v, sb, sa);
-        }
+        for (int t = u * PER / MF; t < (u + 1) * PER / MF; ++t) copy(t, f, buf);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (G::k32) {
+        const int t = u / (G::FM * G::FN), j = u % (G::FM * G::FN) / G::FM, i = u % G::FM;
+        v16f& v = acc32[i * G::FN + j];
+        const uint32_t sb = sc[1].w[word + j], sa = sc[0].w[word + i];
+        v = t == 0 ? mx_mfma32<byte>(fb[set][2 * j], fa[set][2 * i], v, sb, sa)
+                   : mx_mfma32<byte + 1>(fb[set][2 * j + 1], fa[set][2 * i + 1], v, sb, sa);
+      } else {
+        const int j = u / G::FM, i = u % G::FM;
+        v4f& v = acc[i * G::FN + j];
+        const uint32_t sb = sc[1].w[word + j % 2], sa = sc[0].w[word + i % 2];
+        const int e = j / 2, g = i / 2;   // byte + e of sb, byte + g of sa
+        if (e == 0 && g == 0) v = mx_mac<QA, OT, byte, byte>(fb[set][j], fa[set][i], v, sb, sa);
+        else if (e == 0) v = mx_mac<QA, OT, byte, byte + 1>(fb[set][j], fa[set][i], v, sb, sa);
+        else if (g == 0) v = mx_mac<QA, OT, byte + 1, byte>(fb[set][j], fa[set][i], v, sb, sa);
+        else v = mx_mac<QA, OT, byte + 1, byte + 1>(fb[set][j], fa[set][i], v, sb, sa);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (h == KS - 1) buf = next;
   };

@@ -80,15 +80,22 @@ def _values_pytorch(codes, scales):
     return (v.view(*s.shape, BLOCK) * s[:, :, None]).flatten(1)
 
 
+# The operators' overloads, looked up once (a lookup costs as much as a check).
+_OPS = ("mx_quantize", "mx_dequantize", "rms_norm_mx_quantize", "add_rms_norm_mx_quantize", "swiglu_mx_quantize", "mx_matmul")
+_op = {name: getattr(torch.ops.quant_ops, name).default for name in _OPS} if _loader.KERNELS_AVAILABLE else {}
+
+
+def _gpu(name):
+    _loader.require_kernels(name)
+    return _op[name]
+
+
 def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4") -> Tuple[torch.Tensor, torch.Tensor]:
     """Codes and scales of x [..., F] (float32 / float16 / bfloat16)."""
-    _emax(fmt)
+    if x.is_cuda and x.dim() == 2:
+        return _gpu("mx_quantize")(x, fmt)
     rows = _rows(x)
-    if x.is_cuda:
-        _loader.require_kernels("mx_quantize")
-        codes, scales = torch.ops.quant_ops.mx_quantize.default(rows, fmt)
-    else:
-        codes, scales = _quantize_pytorch(rows, fmt)
+    codes, scales = _gpu("mx_quantize")(rows, fmt) if x.is_cuda else _quantize_pytorch(rows, fmt)
     return _like(codes, x), _like(scales, x)
 
 
@@ -96,10 +103,11 @@ def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, features: Optional[
                   out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values of codes and scales, [..., features] in out_dtype (each rounded
     once); features defaults to the padded row length."""
+    if codes.is_cuda and codes.dim() == 2:
+        return _gpu("mx_dequantize")(codes, scales, features, out_dtype)
     q, s = _rows(codes), _rows(scales)
     if codes.is_cuda:
-        _loader.require_kernels("mx_dequantize")
-        out = torch.ops.quant_ops.mx_dequantize.default(q, s, features, out_dtype)
+        out = _gpu("mx_dequantize")(q, s, features, out_dtype)
     else:
         feats = BLOCK * s.shape[1] if features is None else features
         assert -(-feats // BLOCK) == s.shape[1], f"features ({feats}) must fill the {s.shape[1]} blocks of a row"
@@ -116,17 +124,17 @@ def rms_norm_mx_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-
     sum is returned rounded once to x's dtype. x and residual [..., F] of one
     dtype, weight [F] of any of the three.
     """
-    _emax(fmt)
+    if x.is_cuda and x.dim() == 2:
+        if residual is None:
+            return _gpu("rms_norm_mx_quantize")(x, weight, eps, fmt)
+        return _gpu("add_rms_norm_mx_quantize")(x, residual, weight, eps, fmt)
     rows = _rows(x)
     res = None if residual is None else _rows(residual)
     if residual is not None and residual.shape != x.shape:
         raise ValueError(f"residual {tuple(residual.shape)} must have x's shape {tuple(x.shape)}")
     if x.is_cuda:
-        _loader.require_kernels("rms_norm_mx_quantize")
-        if res is None:
-            got = torch.ops.quant_ops.rms_norm_mx_quantize.default(rows, weight, float(eps), fmt)
-        else:
-            got = torch.ops.quant_ops.add_rms_norm_mx_quantize.default(rows, res, weight, float(eps), fmt)
+        got = (_gpu("rms_norm_mx_quantize")(rows, weight, eps, fmt) if res is None else
+               _gpu("add_rms_norm_mx_quantize")(rows, res, weight, eps, fmt))
     else:
         h = rows.float() if res is None else rows.float() + res.float()
         got = _quantize_pytorch(h / torch.sqrt(h.square().mean(1, keepdim=True) + eps) * weight.float(), fmt)
@@ -138,11 +146,11 @@ def rms_norm_mx_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-
 def swiglu_mx_quantize(gate_up: torch.Tensor, fmt: str = "mxfp8") -> Tuple[torch.Tensor, torch.Tensor]:
     """Codes and scales of silu(g) * u in float32, gate_up [..., 2 F] holding the
     gate g and then its factor u."""
-    _emax(fmt)
+    if gate_up.is_cuda and gate_up.dim() == 2:
+        return _gpu("swiglu_mx_quantize")(gate_up, fmt)
     rows = _rows(gate_up)
     if gate_up.is_cuda:
-        _loader.require_kernels("swiglu_mx_quantize")
-        codes, scales = torch.ops.quant_ops.swiglu_mx_quantize.default(rows, fmt)
+        codes, scales = _gpu("swiglu_mx_quantize")(rows, fmt)
     else:
         if rows.shape[1] % 2:
             raise ValueError(f"gate_up must hold two halves, got {tuple(gate_up.shape)}")
@@ -159,10 +167,11 @@ def mx_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales
     a [..., K] mxfp4 or mxfp8 codes with a_scales [..., K/32]; b the weight's
     mxfp4 codes [N, K/2] with b_scales [N, K/32]; bias [N] (taken in out_dtype).
     """
+    if a.is_cuda and a.dim() == 2:
+        return _gpu("mx_matmul")(a, a_scales, b, b_scales, bias, out_dtype)
     q, s = _rows(a), _rows(a_scales)
     if a.is_cuda:
-        _loader.require_kernels("mx_matmul")
-        out = torch.ops.quant_ops.mx_matmul.default(q, s, b, b_scales, bias, out_dtype)
+        out = _gpu("mx_matmul")(q, s, b, b_scales, bias, out_dtype)
     else:
         out = _values_pytorch(q, s) @ _values_pytorch(b, b_scales).t()
         out = (out if bias is None else out + bias.to(out_dtype).float()).to(out_dtype)
