@@ -102,9 +102,9 @@ inline F6Tile f6_tile(int64_t M, int64_t N, int64_t K, bool f32, int64_t cus) {
 // workgroups (two to a CU but for 256 x 256) times k-steps (128 values, quads of
 // four) times what a step takes for one workgroup on a CU and for two, and what a
 // launch, a round and the join of parts take besides. Measured with the weight from
-// memory, 4096 columns, FP4 / FP8: 256 x 256 920 / 1330 a step; 128 x 128 480 / 590
-// alone, 640 / 930 for two; 128 x 64 260 / 430, 480 / 730; 64 x 64 150 / 220, 300 / 430.
-// Whole products, us, FP4: 1024 x 4096 x 14336 94 on 256 x 256, 59 on 128 x 128, 58 on
+// memory, 4096 columns, FP4 / FP8: 256 x 256 920 / 1330 a step; 128 x 128 380 / 590
+// alone (480 with the few stages of two), 640 / 930 for two; 128 x 64 260 / 430, 480 / 730; 64 x 64 150 / 220, 300 / 430.
+// Whole products, us, FP4: 1024 x 4096 x 14336 94 on 256 x 256, 47 on 128 x 128, 58 on
 // 128 x 64; 512 x 4096 x 4096 13.7 on 128 x 64, 15.6 on 64 x 64; 128 x 4096 x 14336 on 64 x 64
 // 26.7 in one part, 19.2 in two; 64 x 4096 x 14336 27.5 in one, 15.2 in four; 256 x 4096 x 4096
 // 9.9 in one, 13.8 in two.
@@ -116,26 +116,29 @@ struct MxPlan {
 constexpr int64_t kMxMostRow = 1 << 22;   // bytes between rows: offsets within a tile take 32 bits
 inline int64_t mx_tile_rows(MxTileKind t) { return t == kMxTile256 ? 256 : t == kMxTile64 ? 64 : 128; }
 inline int64_t mx_tile_cols(MxTileKind t) { return t == kMxTile256 ? 256 : t == kMxTile128 ? 128 : 64; }
+inline int64_t mx_tiles(MxTileKind t, int64_t M, int64_t N) {
+  return ((M + mx_tile_rows(t) - 1) / mx_tile_rows(t)) * ((N + mx_tile_cols(t) - 1) / mx_tile_cols(t));
+}
 inline int64_t mx_plan_bytes(const MxPlan& p, int64_t M, int64_t N) {
-  const int64_t bm = mx_tile_rows(p.tile), bn = mx_tile_cols(p.tile);
-  return p.splits * ((M + bm - 1) / bm) * ((N + bn - 1) / bn) * bm * bn * 4;
+  return p.splits * mx_tiles(p.tile, M, N) * mx_tile_rows(p.tile) * mx_tile_cols(p.tile) * 4;
 }
 inline MxPlan mx_plan(int64_t M, int64_t N, int64_t blocks, bool fp8, int64_t cus, bool may_split) {
-  static const int64_t kStep[2][4][2] = {{{920, 920}, {480, 640}, {260, 480}, {150, 300}},
-                                         {{1330, 1330}, {590, 930}, {430, 730}, {220, 430}}};
+  // alone on a CU in the only round and in a last one, and two
+  static const int64_t kStep[2][4][3] = {{{920, 920, 920}, {380, 480, 640}, {260, 260, 480}, {150, 150, 300}},
+                                         {{1330, 1330, 1330}, {590, 590, 930}, {430, 430, 730}, {220, 220, 430}}};
   const int64_t quads = (blocks + 15) / 16;
   MxPlan best = {kMxTile256, 1};
   int64_t least = INT64_MAX;
   for (int t = kMxTile256; t <= kMxTile64; ++t) {
     const MxTileKind kind = (MxTileKind)t;
-    const int64_t bm = mx_tile_rows(kind), bn = mx_tile_cols(kind), tiles = ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+    const int64_t tiles = mx_tiles(kind, M, N);
     const int64_t slots = kind == kMxTile256 ? cus : 2 * cus;
     for (int splits = 1; splits <= 8; splits *= 2) {
       if (splits > 1 && (!may_split || kind == kMxTile256 || quads < 2 * splits)) break;
       const int64_t n = tiles * splits, steps = 4 * ((quads + splits - 1) / splits);
       const int64_t full = n / slots, rest = n % slots;
-      int64_t ns = 4000 + full * (steps * kStep[fp8][t][1] + 4000);
-      if (rest) ns += steps * kStep[fp8][t][rest > cus] + 4000;
+      int64_t ns = 4000 + full * (steps * kStep[fp8][t][2] + 4000);
+      if (rest) ns += steps * kStep[fp8][t][rest > cus ? 2 : full > 0] + 4000;
       if (kind == kMxTile256) ns += (full + (rest != 0)) * 6000;   // a round's output waits for memory
       if (splits > 1) ns += 4000 + splits * M * N * 8 / 3500;      // parts written and read at 3.5 TB/s
       if (ns < least) least = ns, best = {kind, splits};

@@ -545,6 +545,11 @@ struct MxMid {
   // As many stages as let two workgroups share a CU's LDS: a small tile's step is
   // short, and its copies need as long.
   static constexpr int STAGES = BM + BN == 256 ? (k32 ? 2 : 3) : BM + BN == 192 ? 3 : (k32 ? 4 : 6);
+  // Of a workgroup that has a CU to itself: a stage comes in 0.8 us, its products take
+  // half of that. us for FP4 1024 x 4096 x 14336 (256 tiles) 47.2 against 57.9, and with
+  // two workgroups' work on a CU 28.1 against 22.1 (333 x 11008 x 4096). FP8, whose
+  // products take twice as long, and smaller tiles gain nothing.
+  static constexpr int ALONE = BM + BN == 256 && k32 ? 4 : STAGES;
   static constexpr int WM = BM / 2, WN = BN / 2;      // a wave's outputs
   static constexpr int SIDE = k32 ? 32 : 16;          // of an MFMA's block
   static constexpr int FM = WM / SIDE, FN = WN / SIDE, FOURS = SIDE * SIDE / 256;
@@ -585,18 +590,19 @@ __device__ inline void mx_mid_store(const v4f (&acc)[MxMid<QA, BM, BN>::VALUES],
   }
 }
 
-template <class QA, class OT, int BM, int BN>
-__global__ void __launch_bounds__(256, 2)
+template <class QA, class OT, int BM, int BN, int STAGES>
+__global__ void __launch_bounds__(256, (STAGES > MxMid<QA, BM, BN>::STAGES ? 1 : 2))
 mx_gemm_mid(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ out, int64_t ldc,
             const typename OT::T* __restrict__ bias, int tiles_m, v4f* __restrict__ parts) {
   using G = MxMid<QA, BM, BN>;
-  constexpr int W = 4, KS = G::KS, STAGES = G::STAGES;
+  constexpr int W = 4, KS = G::KS;
   using RA = MxRow<QA, KS>;
   using RB = MxRow<FP4, KS>;
   constexpr int A_BYTES = BM * RA::bytes, BYTES = A_BYTES + BN * RB::bytes;
   constexpr int TA = A_BYTES / 1024 / W, TB = BN * RB::bytes / 1024 / W, PER = TA + TB;
   constexpr int RING = STAGES * BYTES;
   static_assert(TA * 4096 == A_BYTES && TB * 4096 == BYTES - A_BYTES, "whole copies");
+  static_assert(STAGES <= 4 / KS + 2, "a quad's scales are older than the copies under way in the quad before's last stage");
   constexpr int C_BYTES = sizeof(typename OT::T) == 2 ? BM * (BN * 2 + 16) : 0;
   static_assert(C_BYTES + BN * 4 <= RING, "staged output and bias");
   constexpr int SCALES = (BM + BN) * 16;
@@ -653,16 +659,22 @@ mx_gemm_mid(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ o
   auto issue_scales = [&](int q) {   // quads past the last repeat it
     dma16_s(s_off, s_base + 16 * (int64_t)min(q0 + q, all - 1), __builtin_amdgcn_readfirstlane(s_dst + (q & 1) * SCALES));
   };
+  v4i raw[2];   // the next quad's: A's, B's
   MxScales sc[2];
-  auto load_scales = [&](int q) {
-    const int past = 16 * (q0 + q + 1) - blocks;
+  auto read_scales = [&](int q) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       // a wave of fewer than 64 rows uses the first lanes' (the others read any row of the tile)
       const int row = i == 0 ? min(G::WM * wm + lane, BM - 1) : BM + min(G::WN * wn + lane, BN - 1);
-      v4i v = *reinterpret_cast<const v4i*>(s_scales + (q & 1) * SCALES + 16 * row);
-      if (past > 0) mx_clear_scales(v, past);
-      sc[i] = G::k32 ? mx_scales32(v) : mx_scales16(v);
+      raw[i] = *reinterpret_cast<const v4i*>(s_scales + (q & 1) * SCALES + 16 * row);
+    }
+  };
+  auto set_scales = [&](int q) {
+    const int past = 16 * (q0 + q + 1) - blocks;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (past > 0) mx_clear_scales(raw[i], past);
+      sc[i] = G::k32 ? mx_scales32(raw[i]) : mx_scales16(raw[i]);
     }
   };
 
@@ -711,6 +723,7 @@ mx_gemm_mid(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ o
   lds_barrier();
 #pragma unroll
   for (int f = 0; f < NA + NB; ++f) read(f, 0, 0, fa[0], fb[0]);
+  read_scales(0);
 
   uint32_t buf = 0;   // the stage of step s
   auto phase = [&](int q, auto stepc, auto lastc) {
@@ -718,34 +731,36 @@ mx_gemm_mid(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ o
     constexpr bool LAST = decltype(lastc)::value;
     // Stage T + 1 has landed; the later ones may be under way, and the scales copied
     // before the last stage of the quad before (stage STAGES - 1 from this quad's
-    // first) where that may be: not where step 0, which has no wait when KS = 2, needs
-    // them. The last quad has no copies of its own past its end.
+    // first) where that may be: not in the last stage, where the next quad's are read.
+    // The last quad has no copies of its own past its end.
     if constexpr (h == KS - 1) {
       constexpr int issued = LAST ? std::max(STAGES - 1, std::min(T + STAGES - 1, PQ - 1)) : T + STAGES - 1;
       constexpr int flying = std::max(issued - (T + 1), 0);
-      gemm_wait_vmcnt<PER * flying + (issued - flying < STAGES - 1 && !(KS == 2 && T == PQ - 1) ? 1 : 0)>();
+      gemm_wait_vmcnt<PER * flying + (issued - flying < STAGES - 1 && T != PQ - 1 ? 1 : 0)>();
     }
+    if constexpr (s == 0) set_scales(q);
     __builtin_amdgcn_sched_barrier(0);
     lds_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (s == 0) load_scales(q);
     const uint32_t next = buf == (STAGES - 1) * BYTES ? 0 : buf + BYTES;
     constexpr bool reads = !(LAST && s == 3), copies = h == KS - 1 && (!LAST || T + STAGES < PQ);
     if constexpr (!LAST && s == 3) issue_scales(q + 2);   // this quad's are in registers
     From f = {};
     if constexpr (copies) f = from(PQ * q + T + STAGES);   // into this stage's slot: it is in registers
-    constexpr int set = s & 1, word = 2 * (s / 2), byte = 2 * (s % 2), MF = G::FM * G::FN * H;
+    constexpr int set = s & 1, word = 2 * (s / 2), byte = 2 * (s % 2), MF = G::FM * G::FN * H, RF = MF / 2;
 #pragma unroll
-    for (int u = 0; u < MF; ++u) {   // the next step's reads and the copies, spread between the MFMAs
+    for (int u = 0; u < MF; ++u) {   // the next step's reads, in the first half, and the copies between the MFMAs
       if constexpr (reads) {
 #pragma unroll
-        for (int r = u * (NA + NB) / MF; r < (u + 1) * (NA + NB) / MF; ++r)
+        for (int r = std::min(u * (NA + NB) / RF, NA + NB); r < std::min((u + 1) * (NA + NB) / RF, NA + NB); ++r)
           read(r, h == KS - 1 ? next : buf, (s + 1) % KS, fa[set ^ 1], fb[set ^ 1]);
       }
       if constexpr (copies) {
 #pragma unroll
         for (int t = u * PER / MF; t < (u + 1) * PER / MF; ++t) copy(t, f, buf);
       }
+      if constexpr (!LAST && s == 3)
+        if (u == MF / 2) read_scales(q + 1);
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (G::k32) {
         const int t = u / (G::FM * G::FN), j = u % (G::FM * G::FN) / G::FM, i = u % G::FM;
@@ -1015,10 +1030,13 @@ void mx_gemm_launch(const MxOperand& a, const MxOperand& b, int blocks, void* ou
     const int tm = (M + bm - 1) / bm;
     launch(kernel, dim3((unsigned)(tm * ((N + bn - 1) / bn)), splits), dim3(threads), 0, stream, a, b, blocks, o, ldc, bi, tm, more...);
   };
-  auto mid = [&](auto bmc, auto bnc, int splits) {
+  auto mid = [&](auto bmc, auto bnc, const MxPlan& plan) {
     constexpr int BM = decltype(bmc)::value, BN = decltype(bnc)::value;
+    const int splits = plan.splits;
     v4f* const parts = splits > 1 ? reinterpret_cast<v4f*>(workspace) : nullptr;
-    tiled(mx_gemm_mid<QA, OT, BM, BN>, BM, BN, 256, splits, parts);
+    constexpr int STAGES = MxMid<QA, BM, BN>::STAGES, ALONE = MxMid<QA, BM, BN>::ALONE;
+    if (splits * mx_tiles(plan.tile, M, N) <= device_cu_count()) tiled(mx_gemm_mid<QA, OT, BM, BN, ALONE>, BM, BN, 256, splits, parts);
+    else tiled(mx_gemm_mid<QA, OT, BM, BN, STAGES>, BM, BN, 256, splits, parts);
     if (splits > 1) {
       const int tm = (M + BM - 1) / BM;
       launch(mx_gemm_join<QA, OT, BM, BN>, dim3((unsigned)(tm * ((N + BN - 1) / BN))), dim3(256), 0, stream, parts, splits, o,
@@ -1036,9 +1054,9 @@ void mx_gemm_launch(const MxOperand& a, const MxOperand& b, int blocks, void* ou
         if constexpr (k8) tiled(mx_gemm_tile<OT>, 256, 256, 512, 1);
         else tiled(mx_gemm_wide<OT>, 256, 256, 256, 1);
         return;
-      case kMxTile128: return mid(c128, c128, plan.splits);
-      case kMxTile128x64: return mid(c128, c64, plan.splits);
-      default: return mid(c64, c64, plan.splits);
+      case kMxTile128: return mid(c128, c128, plan);
+      case kMxTile128x64: return mid(c128, c64, plan);
+      default: return mid(c64, c64, plan);
     }
   }
   auto stream_rows = [&](auto fnc, auto wc, auto residentc, int per_cu) {

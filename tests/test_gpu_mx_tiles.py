@@ -23,7 +23,8 @@ CASES = [
     (65, 16391, 1, "mxfp4", "128", 1),
     (129, 11007, 5, "mxfp4", "128", 1),
     (77, 16391, 35, "mxfp4", "128", 1),
-    (65, 16391, 257, "mxfp4", "128", 2),          # 17 quads: parts of 8 and 9
+    (65, 16391, 257, "mxfp4", "128", 1),          # 17 quads, one tile to a CU
+    (77, 8201, 513, "mxfp4", "128", 2),           # 33: parts of 16 and 17
     (65, 8201, 448, "mxfp4", "128", 4),
     (65, 4097, 896, "mxfp4", "128", 8),
     (65, 8201, 3, "mxfp4", "128x64", 1),
