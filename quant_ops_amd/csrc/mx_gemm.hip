@@ -105,7 +105,8 @@ __device__ inline void mx_store4(v4f v, typename OT::T* out, int64_t ldc, const 
 // straight into registers, and add their sums in LDS in a fixed order. Bound by
 // the weight's bytes from memory: a wave has the next quad's on the way while it
 // multiplies one, across the end of a tile as well. RESIDENT: a wave has one quad
-// at most, and keeps a's fragments of it.
+// at most, and keeps a's fragments of it. 16 x 28672 x 4096 FP4 15.6 us (62 MB of weight,
+// 4.1 TB/s), FP8 18.7; 1 x 4096 x 14336 9.1 and 10.8.
 // ---------------------------------------------------------------------------
 template <class QA, class OT, int FN, int W, bool RESIDENT>
 __global__ void __launch_bounds__(64 * W, FN == 1 ? 4 : 2)
@@ -532,7 +533,15 @@ mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ 
 // A wave reads step s + 1's fragments into a second register set while it
 // multiplies step s, so a step costs one barrier: it says that step s + 1 has landed and
 // that every wave holds step s in registers, which frees a stage that ends
-// there for copies.
+// there for copies. The next step's reads stand between the first half of the MFMAs (all
+// of them: 333 x 11008 x 4096 FP4 22.9 us, half 22.1). Two groups of four waves on one
+// tile, each half of the k-steps and joined in LDS, measured no better: FP4 1024 x 4096
+// x 14336 51 us (four waves with as much LDS 47), FP8 69 (72).
+//
+// us with the weight from memory: 1024 x 4096 x 14336 FP4 47 (2.5 PFLOP/s), FP8 72;
+// 333 x 11008 x 4096 22 and 30; 64 x 28672 x 4096 21 and 24. A step waits for its
+// copies and for its slowest wave: FP8 on 128 x 128, weights in the cache, has the matrix
+// cores busy 52 % of the time.
 //
 // With few tiles the k-steps are split (blockIdx.y, whole quads): each part leaves its
 // float32 sums in `parts`, in the order of its registers, and mx_gemm_join adds
@@ -845,7 +854,10 @@ mx_gemm_join(const v4f* __restrict__ parts, int splits, typename OT::T* __restri
 // products of a 64 x 128 wave's. Stages of two k-steps (128-byte rows) on a ring of two.
 // While a wave multiplies step j it reads step j + 1's fragments into a second
 // register set and, in odd steps, copies the stage after the next, one LDS
-// or copy instruction between every two MFMAs; a step costs one barrier.
+// or copy instruction between every two MFMAs; a step costs one barrier. 4096 x 4096 x
+// 14336 107-115 us, 4.2-4.5 PFLOP/s (registers only 6.1, at the clock that the board's
+// power limit leaves); 4096 x 14336 x 4096 136-142 us: a round's output (33 MB) waits for
+// memory. The last, half full round as 128 x 128 tiles of a second launch: 3 % less.
 // ---------------------------------------------------------------------------
 template <class OT>
 __global__ void __launch_bounds__(256, 1)
