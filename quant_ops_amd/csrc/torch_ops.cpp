@@ -14,6 +14,7 @@
 // host is never synchronised (cuda_quant_kernel.cu:379-385 synchronised the
 // stream after launching on the legacy default stream).
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
@@ -248,14 +249,21 @@ int mx_codes_format(const at::Tensor& codes, const char* op, const char* name) {
   return QO_MX_FP8;
 }
 
+// Uninitialized rows from the caching allocator, without the dispatcher's way to it (of the
+// host's time of a small call, which bounds it, a tenth).
+at::Tensor mx_empty(int64_t rows, int64_t columns, at::ScalarType dtype, at::Device device) {
+  return at::detail::empty_cuda({rows, columns}, dtype, device, std::nullopt);
+}
+
 // Empty codes and scales for [tokens, features]. Rows of scales stand a multiple of
-// 16 bytes apart, as mx_matmul reads them.
+// 16 bytes apart, as mx_matmul reads them: the tensor is made with the padding and narrowed.
 std::tuple<at::Tensor, at::Tensor> mx_outputs(const at::Tensor& like, int64_t tokens, int64_t features, int format) {
-  const int64_t blocks = (features + 31) / 32;
-  at::Tensor codes = format == QO_MX_FP4 ? at::empty({tokens, 16 * blocks}, like.options().dtype(at::kByte))
-                                         : at::empty({tokens, 32 * blocks}, like.options().dtype(at::kFloat8_e4m3fn));
-  at::Tensor scales = at::empty({tokens, (blocks + 15) / 16 * 16}, like.options().dtype(at::kByte));
-  return {codes, blocks % 16 == 0 ? scales : scales.narrow(1, 0, blocks)};
+  const int64_t blocks = (features + 31) / 32, pad = (blocks + 15) / 16 * 16;
+  at::Tensor codes = format == QO_MX_FP4 ? mx_empty(tokens, 16 * blocks, at::kByte, like.device())
+                                         : mx_empty(tokens, 32 * blocks, at::kFloat8_e4m3fn, like.device());
+  at::Tensor scales = mx_empty(tokens, pad, at::kByte, like.device());
+  if (pad != blocks) scales.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef{tokens, blocks}, at::IntArrayRef{pad, 1});
+  return {std::move(codes), std::move(scales)};
 }
 int64_t mx_scales_ld(const at::Tensor& s) { return std::max(s.stride(0), s.size(1)); }
 
@@ -300,7 +308,7 @@ at::Tensor mx_dequantize(const at::Tensor& codes, const at::Tensor& scales, std:
   c10::DeviceGuard guard(codes.device());
   at::Tensor q = codes.contiguous(), s = mx_rows(scales);
   if (reinterpret_cast<uintptr_t>(q.data_ptr()) % 8 != 0) q = q.clone();
-  at::Tensor out = at::empty({T, F}, codes.options().dtype(dtype));
+  at::Tensor out = mx_empty(T, F, dtype, codes.device());
   check_status(qo_mx_dequantize(q.data_ptr(), s.data_ptr<uint8_t>(), mx_scales_ld(s), format, T, F, out.data_ptr(), dtype_code(dtype),
                                 current_stream(codes)),
                "mx_dequantize");
@@ -325,7 +333,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_mx_impl(const at::Tensor
   at::Tensor x = mx_rows(input), w = weight.contiguous(), res, h;
   if (residual) {
     res = mx_rows(*residual);
-    h = at::empty({T, F}, input.options());
+    h = mx_empty(T, F, input.scalar_type(), input.device());
   }
   auto [codes, scales] = mx_outputs(x, T, F, format);
   check_status(qo_rms_norm_mx_quantize(x.data_ptr(), residual ? res.data_ptr() : nullptr, dtype_code(x.scalar_type()),
@@ -412,7 +420,7 @@ at::Tensor mx_matmul(const at::Tensor& a, const at::Tensor& a_scales, const at::
                 ") elements on a's device");
     bv = bias->to(dtype).reshape({N}).contiguous();
   }
-  at::Tensor out = at::empty({M, N}, a.options().dtype(dtype));
+  at::Tensor out = mx_empty(M, N, dtype, a.device());
   const int64_t ws_bytes = qo_mx_gemm_workspace_size(M, N, K, format);
   at::Tensor ws = gemm_workspace(ws_bytes, a);
   check_status(qo_mx_gemm(A.data_ptr(), mx_ld(A), format, sa.data_ptr<uint8_t>(), mx_scales_ld(sa), B.data_ptr(),
