@@ -1055,7 +1055,8 @@ void mx_gemm_launch(const MxOperand& a, const MxOperand& b, int blocks, void* ou
              ldc, bi, M, N, tm);
     }
   };
-  if (M > QO_MX_GEMM_FEW_ROWS && blocks > 0 && a.ld <= kMxMostRow && b.ld <= kMxMostRow) {
+  if (M > QO_MX_GEMM_FEW_ROWS && blocks > 0 && std::max(a.ld, b.ld) <= kMxMostRow &&
+      std::max(a.scales_ld, b.scales_ld) <= kMxMostRow) {
     MxPlan plan = mx_plan(M, N, blocks, k8, device_cu_count(), true);
     if (plan.splits > 1 && (!workspace || workspace_bytes < mx_plan_bytes(plan, M, N)))
       plan = mx_plan(M, N, blocks, k8, device_cu_count(), false);

@@ -134,6 +134,19 @@ def test_rows_far_apart(gpu, fmt):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+def test_scale_rows_far_apart(gpu, fmt):
+    """Rows of scales whose distances within a tile pass 32 bits."""
+    m, n, blocks, stride = 130, 45, 40, 34 << 20
+    (a, sa), (b, sb) = _operand(m, blocks, fmt, 1), _operand(n, blocks, "mxfp4", 2)
+    raw = torch.empty((m - 1) * stride + 48, dtype=torch.uint8, device=gpu)
+    far = raw.as_strided((m, blocks), (stride, 1))
+    far.copy_(sa)
+    out = qo.mx_matmul(a.to(gpu), far, b.to(gpu), sb.to(gpu), out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    _check_product(out, a, sa, b, sb)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("feats", [4096, 4104, 8192, 8200, 16384, 16392, 24576, 24584, 32768, 32776, 4099, 8190, 33001])
 def test_norm_lengths(gpu, feats, fmt):
     """Both sides of every line between the norm's variants; odd lengths."""
