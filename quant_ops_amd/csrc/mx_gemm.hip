@@ -990,7 +990,7 @@ mx_gemm_wide(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ 
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (!LAST && s % 2 == 0) gemm_wait_vmcnt<0>();   // the stage that the next step reads from, and scales
+    if constexpr (s == 0 || (!LAST && s == 2)) gemm_wait_vmcnt<0>();   // the stage that the next step reads from, and scales
   };
   auto quad = [&](int q, auto lastc) {
     phase(q, std::integral_constant<int, 0>{}, lastc);
