@@ -539,9 +539,8 @@ mx_gemm_tile(MxOperand a, MxOperand b, int blocks, typename OT::T* __restrict__ 
 // x 14336 51 us (four waves with as much LDS 47), FP8 69 (72).
 //
 // us with the weight from memory: 1024 x 4096 x 14336 FP4 47 (2.5 PFLOP/s), FP8 72;
-// 333 x 11008 x 4096 22 and 30; 64 x 28672 x 4096 21 and 24. A step waits for its
-// copies and for its slowest wave: FP8 on 128 x 128, weights in the cache, has the matrix
-// cores busy 52 % of the time.
+// 333 x 11008 x 4096 22 and 29; 64 x 28672 x 4096 21 and 24. The copies bound it: without
+// them in the loop FP8 1024 x 4096 x 14336 takes 41 us, without the LDS reads 72.
 //
 // With few tiles the k-steps are split (blockIdx.y, whole quads): each part leaves its
 // float32 sums in `parts`, in the order of its registers, and mx_gemm_join adds
@@ -571,7 +570,10 @@ struct MxMid {
 };
 
 // A tile's sums (four waves, 2 x 2) + bias to out: 16-bit values through LDS, in 16-byte
-// pieces of rows, float32 from registers. s_bias holds the tile's columns.
+// pieces of rows, float32 from registers. s_bias holds the tile's columns. Non-temporal
+// stores: 1024 x 4096 x 4096 FP8 25.4 -> 22.0 us, 333 x 11008 x 4096 29.8 -> 29.0, a gated
+// MLP block, whose next kernel reads them, the same; in mx_gemm_wide 4096 x 14336 x 4096
+// 149 -> 144, mx_gemm_tile 194 -> 187.
 template <class QA, class OT, int BM, int BN>
 __device__ inline void mx_mid_store(const v4f (&acc)[MxMid<QA, BM, BN>::VALUES], unsigned char* c_tile, const float* s_bias,
                                     typename OT::T* out, int64_t ldc, int M, int N, int m0, int n0, int tid) {
@@ -595,7 +597,7 @@ __device__ inline void mx_mid_store(const v4f (&acc)[MxMid<QA, BM, BN>::VALUES],
   }
   if constexpr (sizeof(T) == 2) {
     lds_barrier();
-    copy_out_c<BM, BN, 256, OT>(c_tile, C_PITCH, out, ldc, M, N, m0, n0, tid);
+    copy_out_c<BM, BN, 256, OT, true>(c_tile, C_PITCH, out, ldc, M, N, m0, n0, tid);
   }
 }
 
@@ -856,8 +858,11 @@ mx_gemm_join(const v4f* __restrict__ parts, int splits, typename OT::T* __restri
 // register set and, in odd steps, copies the stage after the next, one LDS
 // or copy instruction between every two MFMAs; a step costs one barrier. 4096 x 4096 x
 // 14336 107-115 us, 4.2-4.5 PFLOP/s (registers only 6.1, at the clock that the board's
-// power limit leaves); 4096 x 14336 x 4096 136-142 us: a round's output (33 MB) waits for
-// memory. The last, half full round as 128 x 128 tiles of a second launch: 3 % less.
+// power limit leaves); 4096 x 14336 x 4096 136-144 us: a round's output (33 MB) waits for
+// memory (without its stores 127). The last, half full round as 128 x 128 tiles of a second
+// launch: 3 % less. One workgroup a CU that goes from tile to tile, the next tile's first
+// copies ahead of its stores from registers: the sums leave no registers for that, and
+// what it spills takes 202 us.
 // ---------------------------------------------------------------------------
 template <class OT>
 __global__ void __launch_bounds__(256, 1)
