@@ -44,12 +44,15 @@ mx_quantize_kernel(const typename D::T* __restrict__ x, int64_t ld, int64_t toke
 // g / (1 + exp(-g)) to a few units of float32, in a third of the instructions of
 // expf and a full division (which bound the kernel). The power's argument -g log2(e)
 // is split in its rounded product and the rest; above 128 the power is
-// infinite and the quotient 0, as the formula has it. The reciprocal is taken of
-// a quarter of the sum, so that it never leaves the normal range.
+// infinite and the quotient 0, as the formula has it. From g = 128 on the power adds
+// nothing to 1: the argument stops there, so that the split of the largest g is no
+// inf - inf. The reciprocal is taken of a quarter of the sum, so that it never
+// leaves the normal range.
 __device__ inline float mx_silu(float g) {
   constexpr float kLog2e = 1.44269502f, kRest = 1.92596303e-8f, kLn2 = 0.693147182f;   // log2(e) = kLog2e + kRest
-  const float hi = -g * kLog2e;
-  const float lo = fmaf(-g, kRest, fmaf(-g, kLog2e, -hi));
+  const float t = fminf(g, 128.f);   // a NaN is in the last line's g still
+  const float hi = -t * kLog2e;
+  const float lo = fmaf(-t, kRest, fmaf(-t, kLog2e, -hi));
   const float p = __builtin_amdgcn_exp2f(hi);
   const float e = hi >= 128.f ? __builtin_inff() : fmaf(p, lo * kLn2, p);
   return (0.25f * g) * __builtin_amdgcn_rcpf(fmaf(e, 0.25f, 0.25f));

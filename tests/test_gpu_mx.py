@@ -209,6 +209,18 @@ def test_swiglu_large_gates(gpu):
     assert bool((scales[-2:] == 255).all()) and bool((codes[-2:].view(torch.uint8) == 0).all())
 
 
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+def test_swiglu_largest_gates(gpu, dtype):
+    """Gates up to the type's largest, where g log2(e) leaves float32: silu(g) is g, or 0 below."""
+    top = torch.finfo(dtype).max
+    g = torch.tensor([128.0, 1e10, 2.0 ** 127, 2.3e38, 2.4e38, 3e38, top, -1e10, -2.0 ** 127, -3e38, -top]).to(dtype)
+    x = torch.cat([g[:, None].expand(-1, 32), torch.full((len(g), 32), 2.0 ** -10, dtype=dtype)], 1).contiguous()
+    codes, scales = qo.swiglu_mx_quantize(x.to(gpu), "mxfp8")
+    torch.cuda.synchronize()
+    y = (g.double().clamp(min=0) * 2.0 ** -10)[:, None].expand(-1, 32)
+    _check_near(y, 8 * U, "mxfp8", codes, scales)
+
+
 def _operand(rows, blocks, fmt, seed, lo=118, hi=136):
     """Random codes (every finite one) and scale bytes."""
     g = torch.Generator().manual_seed(seed)
