@@ -1,4 +1,4 @@
-"""The microscaled operators from their definition, in 64 bits (checker only; no
+"""The microscaled operators from their definition, in 64 bits (for tests; no
 counterpart in the reference).
 
 Written apart from the package: exponents from ``math.frexp``-style arithmetic
