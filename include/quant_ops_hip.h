@@ -478,7 +478,7 @@ int qo_swiglu_mx_quantize(const void* gate_up, int dtype, int64_t tokens, int64_
 
 /*
  * The product of microscaled operands: out[m, n] = rnd(sum_k a[m, k] * b[n, k] +
- * bias[n]) with float32 sums, on the scaled matrix cores.
+ * bias[n]) with float32 sums of exact products, on the scaled matrix cores.
  *
  *   a, b      codes of [M, K] in a_format and of the weight [N, K] in FP4; row
  *             strides lda, ldb in bytes; both pointers and strides multiples

@@ -161,8 +161,8 @@ def swiglu_mx_quantize(gate_up: torch.Tensor, fmt: str = "mxfp8") -> Tuple[torch
 
 def mx_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor,
               bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """``a @ b.T (+ bias)`` of the values that the codes stand for, float32 sums,
-    rounded once to out_dtype.
+    """``a @ b.T (+ bias)`` of the values that the codes stand for, float32 sums of
+    exact products, rounded once to out_dtype.
 
     a [..., K] mxfp4 or mxfp8 codes with a_scales [..., K/32]; b the weight's
     mxfp4 codes [N, K/2] with b_scales [N, K/32]; bias [N] (taken in out_dtype).
