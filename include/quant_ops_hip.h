@@ -453,7 +453,8 @@ int qo_mx_dequantize(const void* codes, const uint8_t* scales, int64_t scales_ld
 /*
  * RMS norm with the residual's addition, quantized: h = x + residual (residual
  * NULL: h = x), y = h / sqrt(mean(h^2) + eps) * weight, codes and scales of y.
- * h, the mean and y are float32.
+ * h and y are float32 (y rounded once from the formula's value, whose mean is held
+ * in 64 bits).
  *
  *   x, residual   [tokens, features] of x_dtype, row strides x_ld, residual_ld
  *   weight        [features] of weight_dtype (F32, F16, BF16)

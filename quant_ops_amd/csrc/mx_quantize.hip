@@ -102,14 +102,15 @@ mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restric
 }
 
 // One row per workgroup, in registers: h = x + residual, the mean of h^2, then
-// y = h / sqrt(mean + eps) * weight and its codes. Statistics, h and y are
-// float32; h is rounded once, to x's type, where it is stored. Of T threads (a
-// multiple of 64 up to MOST), thread t holds chunks t, t + T, .. (NV of them, T the
-// least that covers the row); rows longer than that, or of no whole pieces, are
-// read twice (NV = 0). The factor 1 / sqrt and its product with h carry their roundings
-// along, at no cost in time: y is off by its last rounding and half the sum's error, and
-// 14 to 18 of 8192 x 4096 FP8 codes are not those of the exact y. 8192 x 4096 bf16 with a residual: 45 us, 5.2 TB/s, on 512 threads of one chunk (256 of
-// two 50, 128 of four 60, 1024, half of them idle, 106; read twice 59).
+// y = h / sqrt(mean + eps) * weight and its codes. h and y are float32. The sum of
+// squares and the mean are held in 64 bits, and the factor 1 / sqrt and its products with h
+// carry their roundings along, so y is the formula's value rounded once (beside memory's
+// time at no cost: 8192 x 4096 as with float32 sums; products in 64 bits 15 % more). h is
+// rounded once, to x's type, where it is stored. Of T threads (a multiple of 64 up to MOST),
+// thread t holds chunks t, t + T, .. (NV of them, T the least that covers the row); rows
+// longer than that, or of no whole pieces, are read twice (NV = 0). 8192 x 4096 bf16 with a
+// residual: 45 us, 5.2 TB/s, on 512 threads of one chunk (256 of two 50, 128 of four 60,
+// 1024, half of them idle, 106; read twice 59).
 template <class D, class Q, int MOST, int NV>
 __global__ void __launch_bounds__(MOST)
 rms_norm_mx_kernel(const typename D::T* __restrict__ x, int64_t ld, const typename D::T* res, int64_t res_ld,
@@ -118,7 +119,7 @@ rms_norm_mx_kernel(const typename D::T* __restrict__ x, int64_t ld, const typena
                    int64_t scales_ld, typename D::T* res_out) {
   constexpr int N = NV ? NV : 1;
   constexpr bool WHOLE = NV > 0;
-  __shared__ float part[MOST / 64];
+  __shared__ double part[MOST / 64];
   const int tid = threadIdx.x, T = blockDim.x, chunks = 4 * blocks;
   auto weights = [&](int c, float(&w)[8]) {
     if (weight_dtype == QO_DTYPE_F32) values8<F32T, WHOLE>(load8<F32T, WHOLE>(reinterpret_cast<const float*>(weight), c, features), c, features, w);
@@ -127,7 +128,7 @@ rms_norm_mx_kernel(const typename D::T* __restrict__ x, int64_t ld, const typena
   };
   for (int64_t row = blockIdx.x; row < tokens; row += gridDim.x) {
     Raw8<D> rx[N], rr[N];
-    float sum = 0.f;
+    double sum = 0.0;
     auto load = [&](int c, int j) {
       rx[j] = load8<D, WHOLE>(x + row * ld, c, features);
       if (res) rr[j] = load8<D, WHOLE>(res + row * res_ld, c, features);
@@ -140,10 +141,12 @@ rms_norm_mx_kernel(const typename D::T* __restrict__ x, int64_t ld, const typena
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] += r[i];
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = opaque(v[i]);   // else all chunks of h become one tuple, which spills
     };
     auto squares = [&](const float(&v)[8]) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fmaf(v[i], v[i], sum);
+      for (int i = 0; i < 8; ++i) sum = fma((double)v[i], (double)v[i], sum);
     };
     float h[N][8];
     if constexpr (NV > 0) {
@@ -166,25 +169,26 @@ rms_norm_mx_kernel(const typename D::T* __restrict__ x, int64_t ld, const typena
     if (T > 64) {
       if ((tid & 63) == 0) part[tid >> 6] = sum;
       __syncthreads();
-      sum = 0.f;
+      sum = 0.0;
       for (int i = 0; i < T >> 6; ++i) sum += part[i];
       __syncthreads();   // part is written again for the next row
     }
-    // 1 / sqrt(mean + eps) as r + rest: the rest by a Newton step in 64 bits (0 where r is 0 or infinite)
-    const double mean = (double)sum * per_feature + (double)eps;
-    const float r = 1.f / sqrtf((float)mean);
+    // 1 / sqrt(mean + eps) as r + rest: the rest by a Newton step in 64 bits, which leaves 2^-45 of it (0
+    // where r is 0 or infinite)
+    const double mean = sum * per_feature + (double)eps;
+    const float r = __builtin_amdgcn_rsqf((float)mean);
     const float step = (float)(0.5 * r * (1.0 - mean * r * r)), rest = step == step ? step : 0.f;
-    auto finish = [&](int c, float(&v)[8]) {
+    auto finish = [&](int c, const float(&v)[8]) {
       // whole pieces stream to memory (16-byte aligned: the host's check)
-      if (res_out && 8 * c < features) store_row<D, 8, WHOLE>(res_out + row * features + 8 * c, features - 8 * c, v);
-      float w[8];
+      if (res_out && 8 * c < features) store_row<D, 8, WHOLE>(res_out + row * features + 8 * c, WHOLE ? 8 : features - 8 * c, v);
+      float w[8], y[8];
       weights(c, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {   // (v r + its rounding + v rest) w
         const float q = v[i] * r, more = fmaf(v[i], rest, fmaf(v[i], r, -q));
-        v[i] = fmaf(q, w[i], more * w[i]);
+        y[i] = fmaf(q, w[i], more * w[i]);
       }
-      mx_store8<Q>(v, codes, scales, scales_ld, row, blocks, c);
+      mx_store8<Q>(y, codes, scales, scales_ld, row, blocks, c);
     };
     if constexpr (NV > 0) {
 #pragma unroll

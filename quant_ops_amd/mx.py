@@ -120,8 +120,8 @@ def rms_norm_mx_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-
     """RMS norm of x (+ residual), quantized: ``(codes, scales)``, and with a
     residual ``(codes, scales, x + residual)``.
 
-    h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight, all in float32; the
-    sum is returned rounded once to x's dtype. x and residual [..., F] of one
+    h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight in float32 (on the
+    GPU y is rounded once); the sum is returned rounded once to x's dtype. x and residual [..., F] of one
     dtype, weight [F] of any of the three.
     """
     if x.is_cuda and x.dim() == 2:
