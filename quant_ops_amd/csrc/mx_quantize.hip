@@ -104,13 +104,13 @@ mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restric
 // One row per workgroup, in registers: h = x + residual, the mean of h^2, then
 // y = h / sqrt(mean + eps) * weight and its codes. h and y are float32. The sum of
 // squares and the mean are held in 64 bits, and the factor 1 / sqrt and its products with h
-// carry their roundings along, so y is the formula's value rounded once (beside memory's
-// time at no cost: 8192 x 4096 as with float32 sums; products in 64 bits 15 % more). h is
-// rounded once, to x's type, where it is stored. Of T threads (a multiple of 64 up to MOST),
-// thread t holds chunks t, t + T, .. (NV of them, T the least that covers the row); rows
-// longer than that, or of no whole pieces, are read twice (NV = 0). 8192 x 4096 bf16 with a
-// residual: 45 us, 5.2 TB/s, on 512 threads of one chunk (256 of two 50, 128 of four 60,
-// 1024, half of them idle, 106; read twice 59).
+// carry their roundings along, so y is the formula's value rounded once, also where the
+// squares leave float32 (beside memory's time at no cost: 8192 x 4096 as with float32 sums;
+// products in 64 bits 15 % more). h is rounded once, to x's type, where it is stored. Of T
+// threads (a multiple of 64 up to MOST), thread t holds chunks t, t + T, .. (NV of them, T
+// the least that covers the row); rows longer than that, or of no whole pieces, are read
+// twice (NV = 0). 8192 x 4096 bf16 with a residual: 45 us, 5.2 TB/s, on 512 threads of one
+// chunk (256 of two 50, 128 of four 60, 1024, half of them idle, 106; read twice 59).
 template <class D, class Q, int MOST, int NV>
 __global__ void __launch_bounds__(MOST)
 rms_norm_mx_kernel(const typename D::T* __restrict__ x, int64_t ld, const typename D::T* res, int64_t res_ld,
@@ -173,19 +173,21 @@ rms_norm_mx_kernel(const typename D::T* __restrict__ x, int64_t ld, const typena
       for (int i = 0; i < T >> 6; ++i) sum += part[i];
       __syncthreads();   // part is written again for the next row
     }
-    // 1 / sqrt(mean + eps) as r + rest: the rest by a Newton step in 64 bits, which leaves 2^-45 of it (0
-    // where r is 0 or infinite)
+    // 1 / sqrt(mean + eps) = fit (r + rest): the rest by a Newton step in 64 bits, which leaves 2^-45 of
+    // it (0 where r is 0 or infinite). fit is 1, or the power of two that brings the squares into float32.
     const double mean = sum * per_feature + (double)eps;
-    const float r = __builtin_amdgcn_rsqf((float)mean);
-    const float step = (float)(0.5 * r * (1.0 - mean * r * r)), rest = step == step ? step : 0.f;
+    const float fit = mean > 0x1p100 ? 0x1p-80f : mean < 0x1p-100 ? 0x1p96f : 1.f;
+    const double m = mean * fit * fit;
+    const float r = __builtin_amdgcn_rsqf((float)m);
+    const float step = (float)(0.5 * r * (1.0 - m * r * r)), rest = step == step ? step : 0.f;
     auto finish = [&](int c, const float(&v)[8]) {
       // whole pieces stream to memory (16-byte aligned: the host's check)
       if (res_out && 8 * c < features) store_row<D, 8, WHOLE>(res_out + row * features + 8 * c, WHOLE ? 8 : features - 8 * c, v);
       float w[8], y[8];
       weights(c, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {   // (v r + its rounding + v rest) w
-        const float q = v[i] * r, more = fmaf(v[i], rest, fmaf(v[i], r, -q));
+      for (int i = 0; i < 8; ++i) {   // (u r + its rounding + u rest) w
+        const float u = v[i] * fit, q = u * r, more = fmaf(u, rest, fmaf(u, r, -q));
         y[i] = fmaf(q, w[i], more * w[i]);
       }
       mx_store8<Q>(y, codes, scales, scales_ld, row, blocks, c);

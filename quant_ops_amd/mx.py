@@ -120,8 +120,8 @@ def rms_norm_mx_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-
     """RMS norm of x (+ residual), quantized: ``(codes, scales)``, and with a
     residual ``(codes, scales, x + residual)``.
 
-    h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight in float32 (on the
-    GPU y is rounded once); the sum is returned rounded once to x's dtype. x and residual [..., F] of one
+    h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight, both rounded once to
+    float32; the sum is returned rounded once to x's dtype. x and residual [..., F] of one
     dtype, weight [F] of any of the three.
     """
     if x.is_cuda and x.dim() == 2:
@@ -137,7 +137,8 @@ def rms_norm_mx_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-
                _gpu("add_rms_norm_mx_quantize")(rows, res, weight, eps, fmt))
     else:
         h = rows.float() if res is None else rows.float() + res.float()
-        got = _quantize_pytorch(h / torch.sqrt(h.square().mean(1, keepdim=True) + eps) * weight.float(), fmt)
+        wide = h.double()   # squares leave float32 where h does not
+        got = _quantize_pytorch((wide / torch.sqrt(wide.square().mean(1, keepdim=True) + eps) * weight.double()).float(), fmt)
         if res is not None:
             got = (*got, h.to(x.dtype))
     return tuple(_like(t, x) for t in got)

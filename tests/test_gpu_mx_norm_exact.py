@@ -1,5 +1,5 @@
 """GPU tests of the microscaled RMS norm's arithmetic: y is the formula's value rounded once to
-float32."""
+float32, whatever the row's sum of squares."""
 import pytest
 import torch
 
@@ -36,6 +36,23 @@ def test_codes_beside_a_tie(gpu, feats, fmt):
     codes, scales = qo.rms_norm_mx_quantize(h.to(gpu), w.to(gpu), 1e-6, fmt=fmt)
     torch.cuda.synchronize()
     _check_near(om.rms_norm(h, w, torch.tensor(1e-6).double())[1], ONCE, fmt, codes, scales)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("feats", [100, 4096, 8192, 40000])
+def test_squares_past_float32(gpu, feats, dtype, fmt):
+    """Rows whose squares leave float32 at either end: their norm is a row of ordinary size.
+    (2^-70 with eps 0: squares of 2^-140; 2^90: of 2^180, a sum's mean past 2^127 as well.)"""
+    x = torch.randn(6, feats, generator=torch.Generator().manual_seed(feats))
+    for rows, power in ((slice(0, 2), 90), (slice(2, 4), -70), (slice(4, 6), 122)):
+        x[rows] *= 2.0 ** power
+    x = x.to(dtype)
+    w = torch.linspace(0.5, 1.5, feats)
+    print(f"[gpu-mx-norm] large and small rows, {feats} {dtype} {fmt}", flush=True)
+    codes, scales = qo.rms_norm_mx_quantize(x.to(gpu), w.to(gpu), 0.0, fmt=fmt)
+    torch.cuda.synchronize()
+    _check_near(om.rms_norm(x, w, 0.0)[1], ONCE, fmt, codes, scales)
 
 
 @pytest.mark.parametrize("with_residual", (False, True))
