@@ -80,13 +80,18 @@ def _values_pytorch(codes, scales):
     return (v.view(*s.shape, BLOCK) * s[:, :, None]).flatten(1)
 
 
-# The operators' overloads, looked up once (a lookup costs as much as a check).
+# The operators' overloads, looked up once (a lookup costs as much as a check). A library
+# built before these operators lacks them: the package imports with it all the same.
 _OPS = ("mx_quantize", "mx_dequantize", "rms_norm_mx_quantize", "add_rms_norm_mx_quantize", "swiglu_mx_quantize", "mx_matmul")
-_op = {name: getattr(torch.ops.quant_ops, name).default for name in _OPS} if _loader.KERNELS_AVAILABLE else {}
+_op = {name: getattr(torch.ops.quant_ops, name).default for name in _OPS
+       if _loader.KERNELS_AVAILABLE and hasattr(torch.ops.quant_ops, name)}
 
 
 def _gpu(name):
     _loader.require_kernels(name)
+    if name not in _op:
+        raise RuntimeError(f"{name}: the loaded library ({_loader.TORCH_LIB_PATH}) does not have it; "
+                           "rebuild with python -m quant_ops_amd._build")
     return _op[name]
 
 
