@@ -122,6 +122,9 @@ inline int64_t mx_tile_cols(MxTileKind t) { return t == kMxTile256 ? 256 : t == 
 inline int64_t mx_tiles(MxTileKind t, int64_t M, int64_t N) {
   return ((M + mx_tile_rows(t) - 1) / mx_tile_rows(t)) * ((N + mx_tile_cols(t) - 1) / mx_tile_cols(t));
 }
+// Whether each of a plan's workgroups has a CU to itself: 128 x 128 FP4 tiles then take the room of two for
+// a ring of twice the stages (measured at MxMid::ALONE).
+inline bool mx_alone(const MxPlan& p, int64_t M, int64_t N, int64_t cus) { return p.splits * mx_tiles(p.tile, M, N) <= cus; }
 inline int64_t mx_plan_bytes(const MxPlan& p, int64_t M, int64_t N) {
   return p.splits * mx_tiles(p.tile, M, N) * mx_tile_rows(p.tile) * mx_tile_cols(p.tile) * 4;
 }

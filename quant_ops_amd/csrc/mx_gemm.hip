@@ -1079,7 +1079,7 @@ void mx_gemm_launch(const MxOperand& a, const MxOperand& b, int blocks, void* ou
     const int splits = plan.splits;
     v4f* const parts = splits > 1 ? reinterpret_cast<v4f*>(workspace) : nullptr;
     constexpr int STAGES = MxMid<QA, BM, BN>::STAGES, ALONE = MxMid<QA, BM, BN>::ALONE;
-    if (splits * mx_tiles(plan.tile, M, N) <= device_cu_count()) tiled(mx_gemm_mid<QA, OT, BM, BN, ALONE>, BM, BN, 256, splits, parts);
+    if (mx_alone(plan, M, N, device_cu_count())) tiled(mx_gemm_mid<QA, OT, BM, BN, ALONE>, BM, BN, 256, splits, parts);
     else tiled(mx_gemm_mid<QA, OT, BM, BN, STAGES>, BM, BN, 256, splits, parts);
     if (splits > 1) {
       const int tm = (M + BM - 1) / BM;
