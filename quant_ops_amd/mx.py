@@ -46,6 +46,31 @@ def _like(t, x):
     return t if x.dim() == 2 else t.reshape(*x.shape[:-1], t.shape[1])
 
 
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _check(ok, message):
+    """Host tensors are refused where the GPU operators refuse them."""
+    if not ok:
+        raise ValueError(message)
+
+
+def _check_float(t, name):
+    _check(t.dtype in _FLOATS, f"{name} dtype must be float32, float16 or bfloat16, got {t.dtype}")
+
+
+def _check_codes(codes, scales, name):
+    _check(codes.dtype in (torch.uint8, torch.float8_e4m3fn),
+           f"{name} must be uint8 (FP4 codes) or float8_e4m3fn (FP8 codes), got {codes.dtype}")
+    _check(scales.dtype == torch.uint8, f"{name}'s scales must be uint8, got {scales.dtype}")
+    _check(codes.shape == (scales.shape[0], scales.shape[1] * (BLOCK // 2 if codes.dtype == torch.uint8 else BLOCK)),
+           f"{name} {tuple(codes.shape)} and its scales {tuple(scales.shape)} do not match")
+
+
+def _check_out(out_dtype):
+    _check(out_dtype in _FLOATS, f"out_dtype must be float32, float16 or bfloat16, got {out_dtype}")
+
+
 def _quantize_pytorch(y, fmt):
     """Codes and scales of float32 rows y [T, F]."""
     emax = _emax(fmt)
@@ -100,7 +125,11 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4") -> Tuple[torch.Tensor, torc
     if x.is_cuda and x.dim() == 2:
         return _gpu("mx_quantize")(x, fmt)
     rows = _rows(x)
-    codes, scales = _gpu("mx_quantize")(rows, fmt) if x.is_cuda else _quantize_pytorch(rows, fmt)
+    if x.is_cuda:
+        codes, scales = _gpu("mx_quantize")(rows, fmt)
+    else:
+        _check_float(x, "input")
+        codes, scales = _quantize_pytorch(rows, fmt)
     return _like(codes, x), _like(scales, x)
 
 
@@ -114,6 +143,8 @@ def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, features: Optional[
     if codes.is_cuda:
         out = _gpu("mx_dequantize")(q, s, features, out_dtype)
     else:
+        _check_codes(q, s, "codes")
+        _check_out(out_dtype)
         feats = BLOCK * s.shape[1] if features is None else features
         assert -(-feats // BLOCK) == s.shape[1], f"features ({feats}) must fill the {s.shape[1]} blocks of a row"
         out = _values_pytorch(q, s)[:, :feats].to(out_dtype)
@@ -141,6 +172,10 @@ def rms_norm_mx_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-
         got = (_gpu("rms_norm_mx_quantize")(rows, weight, eps, fmt) if res is None else
                _gpu("add_rms_norm_mx_quantize")(rows, res, weight, eps, fmt))
     else:
+        _check_float(x, "x")
+        _check_float(weight, "weight")
+        _check(weight.shape == rows.shape[1:], f"weight must hold one value per feature ({rows.shape[1]}), got {tuple(weight.shape)}")
+        _check(res is None or res.dtype == x.dtype, "residual must have x's dtype")
         h = rows.float() if res is None else rows.float() + res.float()
         wide = h.double()   # squares leave float32 where h does not
         got = _quantize_pytorch((wide / torch.sqrt(wide.square().mean(1, keepdim=True) + eps) * weight.double()).float(), fmt)
@@ -158,8 +193,8 @@ def swiglu_mx_quantize(gate_up: torch.Tensor, fmt: str = "mxfp8") -> Tuple[torch
     if gate_up.is_cuda:
         codes, scales = _gpu("swiglu_mx_quantize")(rows, fmt)
     else:
-        if rows.shape[1] % 2:
-            raise ValueError(f"gate_up must hold two halves, got {tuple(gate_up.shape)}")
+        _check_float(gate_up, "gate_up")
+        _check(rows.shape[1] % 2 == 0, f"gate_up must hold two halves, got {tuple(gate_up.shape)}")
         g, u = rows.float().chunk(2, 1)
         codes, scales = _quantize_pytorch(g / (1 + torch.exp(-g)) * u, fmt)
     return _like(codes, gate_up), _like(scales, gate_up)
@@ -179,6 +214,12 @@ def mx_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales
     if a.is_cuda:
         out = _gpu("mx_matmul")(q, s, b, b_scales, bias, out_dtype)
     else:
+        _check_codes(q, s, "a")
+        _check_codes(b, b_scales, "b")
+        _check(b.dtype == torch.uint8, f"b must be uint8 (FP4 codes), got {b.dtype}")
+        _check(b_scales.shape[1] == s.shape[1], f"b's scales {tuple(b_scales.shape)} do not match a's {s.shape[1]} blocks")
+        _check(bias is None or bias.numel() == b.shape[0], f"bias must hold N ({b.shape[0]}) elements")
+        _check_out(out_dtype)
         out = _values_pytorch(q, s) @ _values_pytorch(b, b_scales).t()
-        out = (out if bias is None else out + bias.to(out_dtype).float()).to(out_dtype)
+        out = (out if bias is None else out + bias.to(out_dtype).float().reshape(-1)).to(out_dtype)
     return _like(out, a)
