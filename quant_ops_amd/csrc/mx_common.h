@@ -16,7 +16,6 @@ namespace qo {
 
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef short v2s __attribute__((ext_vector_type(2)));
-typedef float v8f __attribute__((ext_vector_type(8)));
 
 struct FP4 {
   static constexpr int code = QO_MX_FP4, emax = 2, words = 1;   // words: dwords of 8 codes
