@@ -463,6 +463,11 @@ def _row_stride(t):
     return max(t.stride(0), t.shape[1])
 
 
+def _unit_rows(t):
+    """t, or a copy of it, with unit inner stride."""
+    return t if t is None or t.stride(-1) == 1 else t.contiguous()
+
+
 def mx_buffers(tokens, features, fmt, device):
     """Empty codes and scales for [tokens, features] rows (scale rows 16 bytes' multiples apart)."""
     blocks = (features + 31) // 32
@@ -473,8 +478,9 @@ def mx_buffers(tokens, features, fmt, device):
 
 
 def mx_quantize(x, fmt="mxfp4", codes=None, scales=None, stream=None):
-    """Call ``qo_mx_quantize`` on x [T, F] (unit inner stride); returns (codes, scales)."""
+    """Call ``qo_mx_quantize`` on x [T, F]; returns (codes, scales)."""
     t, f = x.shape
+    x = _unit_rows(x)
     if codes is None:
         codes, scales = mx_buffers(t, f, fmt, x.device)
     _check(lib().qo_mx_quantize(_ptr(x), _TORCH_CODE[x.dtype], t, f, _ld(x), _MX_CODE[fmt], _ptr(codes), _ptr(scales),
@@ -483,7 +489,8 @@ def mx_quantize(x, fmt="mxfp4", codes=None, scales=None, stream=None):
 
 
 def mx_dequantize(codes, scales, features, out_dtype=torch.float32, stream=None):
-    """Call ``qo_mx_dequantize`` on contiguous codes."""
+    """Call ``qo_mx_dequantize``."""
+    codes, scales = codes.contiguous(), _unit_rows(scales)
     fmt = MX_FP4 if codes.dtype == torch.uint8 else MX_FP8
     out = torch.empty((codes.shape[0], features), dtype=out_dtype, device=codes.device)
     _check(lib().qo_mx_dequantize(_ptr(codes), _ptr(scales), _row_stride(scales), fmt, codes.shape[0], features, _ptr(out),
@@ -493,8 +500,10 @@ def mx_dequantize(codes, scales, features, out_dtype=torch.float32, stream=None)
 
 def rms_norm_mx_quantize(x, weight, eps=1e-6, residual=None, fmt="mxfp8", residual_out=None, stream=None):
     """Call ``qo_rms_norm_mx_quantize``; returns (codes, scales, residual_out or None).
-    ``residual_out`` may be a contiguous ``residual`` itself."""
+    ``residual_out`` (contiguous) may be a contiguous ``residual`` itself."""
     t, f = x.shape
+    x, residual, weight = _unit_rows(x), _unit_rows(residual), weight.contiguous()
+    assert residual_out is None or residual_out.is_contiguous()
     codes, scales = mx_buffers(t, f, fmt, x.device)
     if residual is not None and residual_out is None:
         residual_out = torch.empty((t, f), dtype=x.dtype, device=x.device)
@@ -508,6 +517,7 @@ def rms_norm_mx_quantize(x, weight, eps=1e-6, residual=None, fmt="mxfp8", residu
 def swiglu_mx_quantize(gate_up, fmt="mxfp8", stream=None):
     """Call ``qo_swiglu_mx_quantize`` on [T, 2 F]; returns (codes, scales)."""
     t, f = gate_up.shape[0], gate_up.shape[1] // 2
+    gate_up = _unit_rows(gate_up)
     codes, scales = mx_buffers(t, f, fmt, gate_up.device)
     _check(lib().qo_swiglu_mx_quantize(_ptr(gate_up), _TORCH_CODE[gate_up.dtype], t, f, _ld(gate_up), _MX_CODE[fmt],
                                        _ptr(codes), _ptr(scales), _row_stride(scales), _stream(stream)))
@@ -521,13 +531,17 @@ def mx_gemm_workspace_size(m, n, k, fmt):
 
 def mx_gemm(a, a_scales, b, b_scales, bias=None, out_dtype=torch.bfloat16, out=None, stream=None, workspace=None):
     """Call ``qo_mx_gemm``: a (uint8 or float8_e4m3fn codes) [M, ..], b uint8 [N, K/2], rows 16-byte
-    aligned; bias in the output dtype. ``workspace``: a uint8 device tensor, or True to allocate one."""
+    aligned; bias is taken in the output dtype. ``workspace``: a uint8 device tensor, or True to allocate one."""
     m, n, blocks = a.shape[0], b.shape[0], a_scales.shape[1]
     if workspace is True:
         need = mx_gemm_workspace_size(m, n, 32 * blocks, "mxfp4" if a.dtype == torch.uint8 else "mxfp8")
         workspace = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
     if out is None:
         out = torch.empty((m, n), dtype=out_dtype, device=a.device)
+    assert out.stride(1) == 1 or n == 1
+    a, a_scales, b, b_scales = (_unit_rows(t) for t in (a, a_scales, b, b_scales))
+    if bias is not None:
+        bias = bias.to(out.dtype).contiguous()
     _check(lib().qo_mx_gemm(_ptr(a), _ld(a), MX_FP4 if a.dtype == torch.uint8 else MX_FP8, _ptr(a_scales), _row_stride(a_scales),
                             _ptr(b), _ld(b), _ptr(b_scales), _row_stride(b_scales), _ptr(bias), _ptr(out),
                             _TORCH_CODE[out.dtype], _ld(out), m, n, 32 * blocks, _ptr(workspace),
