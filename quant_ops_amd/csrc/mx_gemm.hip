@@ -1,8 +1,9 @@
 // The product of microscaled operands (mx_common.h) on gfx950's scaled matrix
 // cores: out[m, n] = rnd(sum_k a[m, k] b[n, k] + bias[n]), a in FP4 or FP8, the
 // weight b in FP4, each value its code times its block's scale.
-// v_mfma_scale_f32_16x16x128_f8f6f4 takes both formats and the scale bytes as
-// they are and sums in float32.
+// v_mfma_scale_f32_16x16x128_f8f6f4 and, for tiles of FP4 x FP4,
+// v_mfma_scale_f32_32x32x64_f8f6f4 (mx_mfma32) take both formats and the scale
+// bytes as they are and sum in float32.
 //
 // Fragments of 16 rows x 128 values (four blocks): lane l = r + 16 g has row r.
 // FP4: the 16 bytes of block g. FP8: bytes 16 g .. of the row's 128 and 64 + 16 g ..
@@ -100,8 +101,8 @@ __device__ inline void mx_store4(v4f v, typename OT::T* out, int64_t ldc, const 
 // straight into registers, and add their sums in LDS in a fixed order. Bound by
 // the weight's bytes from memory: a wave has the next quad's on the way while it
 // multiplies one, across the end of a tile as well. RESIDENT: a wave has one quad
-// at most, and keeps a's fragments of it. 16 x 28672 x 4096 FP4 15.6 us (62 MB of weight,
-// 4.1 TB/s), FP8 18.7; 1 x 4096 x 14336 9.1 and 10.8.
+// at most, and keeps a's fragments of it. 16 x 28672 x 4096 FP4 15.1 us (62 MB of weight,
+// 4.1 TB/s), FP8 18.6; 1 x 4096 x 14336 8.8 and 10.7.
 // ---------------------------------------------------------------------------
 template <class QA, class OT, int FN, int W, bool RESIDENT>
 __global__ void __launch_bounds__(64 * W, FN == 1 ? 4 : 2)
@@ -588,9 +589,9 @@ struct MxMid {
 
 // A tile's sums (four waves, 2 x 2) + bias to out: 16-bit values through LDS, in 16-byte
 // pieces of rows, float32 from registers. s_bias holds the tile's columns. Non-temporal
-// stores: 1024 x 4096 x 4096 FP8 25.4 -> 22.0 us, 333 x 11008 x 4096 29.8 -> 29.0, a gated
-// MLP block, whose next kernel reads them, the same; in mx_gemm_wide 4096 x 14336 x 4096
-// 149 -> 144, mx_gemm_tile 194 -> 187.
+// stores (measured with one MFMA a product): 1024 x 4096 x 4096 FP8 25.4 -> 22.0 us, 333 x
+// 11008 x 4096 29.8 -> 29.0, a gated MLP block, whose next kernel reads them, the same; in
+// mx_gemm_wide 4096 x 14336 x 4096 149 -> 144, mx_gemm_tile 194 -> 187.
 template <class QA, class OT, int BM, int BN>
 __device__ inline void mx_mid_store(const v4f (&acc)[MxMid<QA, BM, BN>::VALUES], unsigned char* c_tile, const float* s_bias,
                                     typename OT::T* out, int64_t ldc, int M, int N, int m0, int n0, int tid) {
@@ -884,9 +885,9 @@ mx_gemm_join(const v4f* __restrict__ parts, int splits, typename OT::T* __restri
 // While a wave multiplies step j it reads step j + 1's fragments into a second
 // register set and, in odd steps, copies the stage after the next, one LDS
 // or copy instruction between every two MFMAs; a step costs one barrier. 4096 x 4096 x
-// 14336 107-115 us, 4.2-4.5 PFLOP/s (registers only 6.1, at the clock that the board's
-// power limit leaves); 4096 x 14336 x 4096 136-144 us: a round's output (33 MB) waits for
-// memory (without its stores 127). The last, half full round as 128 x 128 tiles of a second
+// 14336 115 us, 4.2 PFLOP/s (one wave a SIMD in registers only 6.0, at the clock that the
+// board's power limit leaves); 4096 x 14336 x 4096 148 us, 139 with operands in cache: a
+// round's output (33 MB) waits for memory (without its stores 127). The last, half full round as 128 x 128 tiles of a second
 // launch: 3 % less. One workgroup a CU that goes from tile to tile, the next tile's first
 // copies ahead of its stores from registers: the sums leave no registers for that, and
 // what it spills takes 202 us.
@@ -1112,10 +1113,10 @@ void mx_gemm_launch(const MxOperand& a, const MxOperand& b, int blocks, void* ou
            blocks, o, ldc, bi, tiles);
   };
   // us, weight from memory: up to 8 quads (one to a wave, one row of tiles: a's fragments
-  // stay) 8 waves, two workgroups a CU: 16 x 28672 x 4096 FP8 17.7 (one pair of columns 19.4,
-  // four workgroups 20.9). Longer: 16 waves, 1 x 4096 x 14336 FP8 10.0 (8 waves 14.0);
-  // with pairs of columns for every CU 8 waves, which read a half as often: 16 x 8192 x 28672
-  // FP8 38 (16 waves 50), 1 x 28672 x 8192 34 either way.
+  // stay) 8 waves, two workgroups a CU: 16 x 28672 x 4096 FP8 18.6 (with one pair of columns a
+  // tenth more, with four workgroups 18 %). Longer: 16 waves, 1 x 4096 x 14336 FP8 10.7 (8 waves
+  // 40 % more); with pairs of columns for every CU 8 waves, which read a half as often: 16 x 8192
+  // x 28672 FP8 37 (16 waves a third more), 1 x 28672 x 8192 34 either way.
   constexpr std::integral_constant<int, 1> one{};
   constexpr std::integral_constant<int, 8> w8{};
   if (blocks <= 128 && M <= 16) stream_rows(one, w8, std::true_type{}, 2);
