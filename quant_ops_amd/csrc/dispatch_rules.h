@@ -107,11 +107,13 @@ inline F6Tile f6_tile(int64_t M, int64_t N, int64_t K, bool f32, int64_t cus) {
 // Whole products, us, FP4: 1024 x 4096 x 14336 94 on 256 x 256, 47 on 128 x 128, 58 on
 // 128 x 64; 512 x 4096 x 4096 13.7 on 128 x 64, 15.6 on 64 x 64; 128 x 4096 x 14336 on 64 x 64
 // 26.7 in one part, 19.2 in two; 64 x 4096 x 14336 27.5 in one, 15.2 in four; 256 x 4096 x 4096
-// 9.9 in one, 13.8 in two. A last round of more workgroups than CUs is priced as if each CU had two, which is
-// long where few have (258 tiles of 128 x 128, 333 x 11008 x 4096 FP4: by a third). FP8's steps are those of one MFMA a product; its kernels have two, and take
-// 2200; 700, 1340 for two; 570, 890; 370, 570. That is much the same factor for all: of 17 products of 32 to
-// 2048 rows the choice is the fastest for 15 and within 3 % for the others, and where the longer steps would
-// choose otherwise (30 of 165 sizes over the range) theirs is 1.2 times as slow to 1.2 times as fast, the same on average.
+// 9.9 in one, 13.8 in two. A last round of more workgroups than CUs is priced as if each CU
+// had two, which is long where few have (258 tiles of 128 x 128, 333 x 11008 x 4096 FP4: by a
+// third). FP8's steps are those of one MFMA a product; its kernels have two, and take 2200;
+// 700, 1340 for two; 570, 890; 370, 570. That is much the same factor for all: of 17 products
+// of 32 to 2048 rows the choice is the fastest for 15 and within 3 % for the others, and where
+// the longer steps would choose otherwise (30 of 165 sizes over the range) their choice takes
+// 0.83 to 1.19 times as long, on average the same.
 enum MxTileKind { kMxTile256, kMxTile128, kMxTile128x64, kMxTile64 };
 struct MxPlan {
   MxTileKind tile;
