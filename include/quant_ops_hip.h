@@ -505,6 +505,101 @@ int qo_mx_gemm(const void* a, int64_t lda, int a_format, const uint8_t* a_scales
                int64_t workspace_bytes, void* stream);
 int64_t qo_mx_gemm_workspace_size(int64_t M, int64_t N, int64_t K, int a_format);
 
+/*
+ * A paged key/value cache held in 4 bits. One vector of head_dim values per token and KV
+ * head, asymmetric: with v clamped to +-65504, lo = fp16(min v), s = fp16((max v - lo) / 15)
+ * and c = (v - lo) / s rounded to nearest even and clamped to 0 .. 15 (s = 0: c = 0); it reads
+ * as lo + s c. A vector that holds a NaN or an infinity has s = lo = NaN and c = 0. A token's
+ * slot is page * page_size + its place in the page. Contiguous, codes and params 16-byte
+ * aligned; P is page_size, D head_dim:
+ *
+ *   k_codes  uint8 [pages, kv_heads, P, D/2]         byte j: value 2j in the low bits, 2j+1 in the high
+ *   v_codes  uint8 [pages, kv_heads, P/16, D/2, 16]  the same bytes, 16 tokens side by side
+ *   params   fp16 [pages, 2, kv_heads, P/16, 2, 16]  keys, values; s, lo; 16 tokens side by side
+ *
+ * page_size is a power of two from 16 to QO_KV4_MAX_PAGE, head_dim 64, 96, 128, 192 or 256,
+ * pages at most 2^31 - 1, kv_heads 16384; calls take up to QO_KV4_MAX_TOKENS tokens. No
+ * counterpart in the reference.
+ */
+typedef struct qo_kv4_cache {
+  void* k_codes;
+  void* v_codes;
+  void* params;
+  int64_t pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+} qo_kv4_cache;
+#define QO_KV4_MAX_PAGE 4096
+#define QO_KV4_MAX_TOKENS (1LL << 27)
+
+/* Vectors of [tokens, heads, head_dim] at any strides (in elements), unit inner stride. */
+typedef struct qo_heads {
+  const void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+} qo_heads;
+
+/*
+ * Append tokens: k and v [tokens, kv_heads, head_dim] of dtype (F32, F16, BF16) are quantized
+ * into the cache at slots [tokens], k after the position rotation, and q [tokens, q_heads,
+ * head_dim] (may be NULL) is rotated into q_out (contiguous, of dtype).
+ *
+ *   slots         a slot outside the cache (a negative one too) leaves the token out; the
+ *                 others must differ (of two tokens with one slot the cache may hold a mix)
+ *   positions     [tokens], NULL without a rotation; a position outside the table gives NaN
+ *   cos_, sin_    [table_rows, rot / 2], NULL without a rotation (rot 0; q must be NULL then)
+ *   rot           the first values of a vector that are rotated: a multiple of 8 up to head_dim
+ *   interleaved   0: pairs (i, i + rot/2), else (2i, 2i + 1). (a, b) turns to (a cos - b sin,
+ *                 b cos + a sin), rounded to float32 (q then to dtype)
+ *
+ * Only the appended tokens' codes and parameters change. Errors: QO_ERR_SHAPE,
+ * QO_ERR_DTYPE, QO_ERR_ALIGNMENT, QO_ERR_NULL_POINTER.
+ */
+int qo_kv4_append(const qo_kv4_cache* cache, const qo_heads* q, const qo_heads* k, const qo_heads* v, int dtype,
+                  int64_t tokens, int q_heads, const int64_t* slots, const int64_t* positions, const float* cos_,
+                  const float* sin_, int64_t table_rows, int rot, int interleaved, void* q_out, void* stream);
+
+/*
+ * Read slots back: k_out, v_out [tokens, kv_heads, head_dim] of out_dtype, contiguous, lo + s c
+ * in float32, then rounded to out_dtype (F16: within +-65504); zeros for slots outside the cache. Errors as
+ * qo_kv4_append.
+ */
+int qo_kv4_read(const qo_kv4_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out,
+                int out_dtype, void* stream);
+
+/*
+ * Causal attention of q [tokens, q_heads, head_dim] (q_heads a multiple of kv_heads; query head
+ * h reads KV head h / (q_heads / kv_heads)) over the cached keys and values:
+ * out = softmax(scale q k^T) v in float32 sums, rounded to dtype, [tokens, q_heads, head_dim]
+ * contiguous.
+ *
+ *   page_table  int32 [sequences, table_width], row stride table_ld: pages of each sequence in
+ *               order. A visible token on a page outside the cache makes its queries NaN
+ *   lengths     int32 [sequences]: cached tokens, those of the queries included (negative: 0).
+ *               One above table_width * page_size makes the sequence's queries NaN
+ *   q_starts    int32 [sequences + 1], ascending from 0: sequence b has the queries
+ *               q_starts[b] .. q_starts[b + 1] - 1, or NULL: tokens / sequences each. Rows from
+ *               the last entry on are zeros
+ *   window      0, or the number of tokens a query sees up to its own
+ *
+ * Query i of n of a sequence of L tokens stands at p = L - n + i and sees the tokens up to p,
+ * of a window those above p - window. A query that sees none gives zeros. scale is positive.
+ *
+ *   workspace   NULL or device memory, 16-byte aligned, that lets few queries share long
+ *               sequences among workgroups: used where workspace_bytes is at least
+ *               qo_kv4_attention_workspace_size of the same sizes (0: not shared). Only
+ *               this call's kernels read and write it; calls that share one must be ordered
+ *
+ * Errors: QO_ERR_SHAPE, QO_ERR_DTYPE, QO_ERR_ALIGNMENT, QO_ERR_NULL_POINTER.
+ */
+int qo_kv4_attention(const qo_kv4_cache* cache, const qo_heads* q, int dtype, int64_t tokens, int q_heads,
+                     const int32_t* page_table, int64_t table_ld, int64_t table_width, const int32_t* lengths,
+                     const int32_t* q_starts, int64_t sequences, float scale, int64_t window, void* out,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+int64_t qo_kv4_attention_workspace_size(const qo_kv4_cache* cache, int64_t tokens, int q_heads, int64_t table_width,
+                                        int64_t sequences, int has_starts, int64_t window);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,7 +26,8 @@ EXPORTED = ("qo_status_string", "qo_version", "qo_last_error", "qo_set_kernel_ro
             "qo_int4_gemm_f6_convert", "qo_int4_gemm_f6_run2", "qo_w4a4_linear_f6w", "qo_w4a4_linear", "qo_w4a4_linear_ws", "qo_w4a4_linear_noalloc", "qo_dequantize_int4",
             "qo_pack_int4_to_int32", "qo_pack_int4_clamped", "qo_unpack_int32_to_int4", "qo_transpose_int32",
             "qo_mx_quantize", "qo_mx_dequantize", "qo_rms_norm_mx_quantize", "qo_swiglu_mx_quantize", "qo_mx_gemm",
-            "qo_mx_gemm_workspace_size")
+            "qo_mx_gemm_workspace_size", "qo_kv4_append", "qo_kv4_read", "qo_kv4_attention",
+            "qo_kv4_attention_workspace_size")
 
 # QO_ROUTE_* bits of qo_set_kernel_routing (include/quant_ops_hip.h)
 ROUTE = {"FQ_GENERIC": 1 << 0, "FQ_NO_WAVE": 1 << 1, "FQ_NO_DUO": 1 << 2, "FQ_NO_FEW": 1 << 3,
@@ -34,6 +35,20 @@ ROUTE = {"FQ_GENERIC": 1 << 0, "FQ_NO_WAVE": 1 << 1, "FQ_NO_DUO": 1 << 2, "FQ_NO
          "LINEAR_NO_READ_AHEAD": 1 << 7, "GEMM_NO_F6": 1 << 8}
 
 _TORCH_CODE = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
+
+
+class KV4Struct(ctypes.Structure):
+    """``qo_kv4_cache``."""
+
+    _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("params", ctypes.c_void_p),
+                ("pages", ctypes.c_int64), ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32)]
+
+
+class HeadsStruct(ctypes.Structure):
+    """``qo_heads``."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
 
 
 class QuantOpsError(RuntimeError):
@@ -124,6 +139,17 @@ def lib():
                              c_i64, c_i64, c_i64, c_vp, c_i64, c_vp]
     L.qo_mx_gemm_workspace_size.restype = c_i64
     L.qo_mx_gemm_workspace_size.argtypes = [c_i64, c_i64, c_i64, c_int]
+    c_cache, c_heads = ctypes.POINTER(KV4Struct), ctypes.POINTER(HeadsStruct)
+    L.qo_kv4_append.restype = c_int
+    L.qo_kv4_append.argtypes = [c_cache, c_heads, c_heads, c_heads, c_int, c_i64, c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_int,
+                                c_int, c_vp, c_vp]
+    L.qo_kv4_read.restype = c_int
+    L.qo_kv4_read.argtypes = [c_cache, c_vp, c_i64, c_vp, c_vp, c_int, c_vp]
+    L.qo_kv4_attention.restype = c_int
+    L.qo_kv4_attention.argtypes = [c_cache, c_heads, c_int, c_i64, c_int, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_f, c_i64,
+                                   c_vp, c_vp, c_i64, c_vp]
+    L.qo_kv4_attention_workspace_size.restype = c_i64
+    L.qo_kv4_attention_workspace_size.argtypes = [c_cache, c_i64, c_int, c_i64, c_i64, c_int, c_i64]
     _lib = L
     return L
 
@@ -546,4 +572,61 @@ def mx_gemm(a, a_scales, b, b_scales, bias=None, out_dtype=torch.bfloat16, out=N
                             _ptr(b), _ld(b), _ptr(b_scales), _row_stride(b_scales), _ptr(bias), _ptr(out),
                             _TORCH_CODE[out.dtype], _ld(out), m, n, 32 * blocks, _ptr(workspace),
                             workspace.numel() if workspace is not None else 0, _stream(stream)))
+    return out
+
+
+def kv4_struct(cache):
+    """``qo_kv4_cache`` of the three tensors (``quant_ops_amd.KV4Cache``)."""
+    k, v, params = cache
+    assert k.is_contiguous() and v.is_contiguous() and params.is_contiguous()
+    return KV4Struct(k.data_ptr(), v.data_ptr(), params.data_ptr(), k.shape[0], k.shape[2], k.shape[1], 2 * k.shape[3])
+
+
+def _heads(x):
+    return None if x is None else ctypes.byref(HeadsStruct(x.data_ptr(), x.stride(0), x.stride(1)))
+
+
+def kv4_append(cache, k, v, slots, positions=None, cos=None, sin=None, q=None, interleaved=False, stream=None):
+    """Call ``qo_kv4_append``; returns the rotated q or None."""
+    k, v, q = _unit_rows(k), _unit_rows(v), _unit_rows(q)
+    slots = slots.contiguous()
+    positions, cos, sin = (None if t is None else t.contiguous() for t in (positions, cos, sin))
+    out = None if q is None else torch.empty(tuple(q.shape), dtype=q.dtype, device=q.device)
+    _check(lib().qo_kv4_append(ctypes.byref(kv4_struct(cache)), _heads(q), _heads(k), _heads(v), _TORCH_CODE[k.dtype],
+                               k.shape[0], 0 if q is None else q.shape[1], _ptr(slots), _ptr(positions), _ptr(cos), _ptr(sin),
+                               0 if cos is None else cos.shape[0], 0 if cos is None else 2 * cos.shape[1], int(interleaved),
+                               _ptr(out), _stream(stream)))
+    return out
+
+
+def kv4_read(cache, slots, out_dtype=torch.float32, stream=None):
+    """Call ``qo_kv4_read``; returns (k, v)."""
+    slots = slots.contiguous()
+    shape = (slots.shape[0], cache[0].shape[1], 2 * cache[0].shape[3])
+    k, v = (torch.empty(shape, dtype=out_dtype, device=slots.device) for _ in range(2))
+    _check(lib().qo_kv4_read(ctypes.byref(kv4_struct(cache)), _ptr(slots), slots.shape[0], _ptr(k), _ptr(v),
+                             _TORCH_CODE[out_dtype], _stream(stream)))
+    return k, v
+
+
+def kv4_attention_workspace_size(cache, tokens, q_heads, table_width, sequences, has_starts=False, window=0):
+    """``qo_kv4_attention_workspace_size``."""
+    return int(lib().qo_kv4_attention_workspace_size(ctypes.byref(kv4_struct(cache)), tokens, q_heads, table_width, sequences,
+                                                     int(has_starts), window))
+
+
+def kv4_attention(q, cache, page_table, lengths, scale, q_starts=None, window=0, out=None, workspace=None, stream=None):
+    """Call ``qo_kv4_attention``. ``workspace``: a uint8 device tensor, or True to allocate one."""
+    q, page_table, lengths = _unit_rows(q), _unit_rows(page_table), lengths.contiguous()
+    batch, width = page_table.shape
+    if workspace is True:
+        need = kv4_attention_workspace_size(cache, q.shape[0], q.shape[1], width, batch, q_starts is not None, window)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    if out is None:
+        out = torch.empty(tuple(q.shape), dtype=q.dtype, device=q.device)
+    assert out.is_contiguous() and (q_starts is None or q_starts.is_contiguous())
+    _check(lib().qo_kv4_attention(ctypes.byref(kv4_struct(cache)), _heads(q), _TORCH_CODE[q.dtype], q.shape[0], q.shape[1],
+                                  _ptr(page_table), _ld(page_table), width, _ptr(lengths), _ptr(q_starts), batch, float(scale),
+                                  window, _ptr(out), _ptr(workspace), workspace.numel() if workspace is not None else 0,
+                                  _stream(stream)))
     return out

@@ -1,0 +1,595 @@
+// Causal attention over the 4-bit cache of kv4_common.h, on its codes: with k = lo + s c,
+// q . k = s (q . c) + lo sum(q), and with v the same, sum_t p v = sum_t (p s) c + sum_t p lo,
+// so both products run on the codes, which fp16 holds exactly, and the parameters are applied
+// to scores, in float32.
+//
+// A wave takes 64 tokens a step (four tiles of 16) and 16 NB rows (a row: one query of one of
+// the heads that share a KV head). v_mfma_f32_16x16x32_f16 computes S^T = K Q^T (A: codes of 16
+// tokens, B: queries) and O^T += V^T P^T (A: codes of 16 pairs' values, B: weights). Lane
+// l = r + 16 g of an operand holds eight consecutive k of row r, a lane of the result rows
+// 4 g .. 4 g + 3 of column r; the order of k is free as long as both operands have it. So
+//   * S^T's row 4 a + i of its tile u is token 16 a + 4 u + i: lane group g ends up with tokens
+//     16 g .. 16 g + 15, the k that it supplies to the second product from the 16 bytes of
+//     tile g of the values, and the weights never change lanes;
+//   * values of a vector (k of the first product) and tokens (of the second) come in the order
+//     in which masks take codes out of a word, and the queries and weights are put in it.
+//
+// A code is made fp16 by masking alone: its four bits at the bottom of an fp16 are the subnormal
+// c 2^-24, at bits 4 .. 7 c 2^-20. The matrix core keeps subnormals, but what it drops of a sum
+// of products (probed) goes by an exponent that a subnormal's leading zeros do not lower: with
+// bits 0 .. 3 the sums are off by 1e-7 of their terms' magnitudes, with bits 4 .. 7 by 2e-9.
+// 16-bit queries take both places (five instructions for eight codes), float32 the second alone
+// (seven).
+//
+// Queries: brought by a power of two for each row to a largest magnitude in [2^14, 2^15), 16-bit
+// values are exact in fp16 (those below 2^-28 of the largest lose bits); float32 takes two fp16
+// parts (22 bits). Weights: p s 2^15 / S, where S is a power of two that no scale of the tokens so
+// far exceeds, is at most 2^15, and rounded to fp16 (half a step 2^-12, beside bf16's 2^-9 of
+// the output) or, for fp16 and float32, to two parts. Maximum, sums and outputs are float32.
+#include "dispatch_rules.h"
+#include "kv4_common.h"
+
+namespace qo {
+
+namespace {
+
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.44269504f;
+constexpr float kInf = __builtin_inff();
+
+struct Attention {
+  KV4 cache;
+  const void* q;
+  int64_t q_token, q_head;
+  void* out;
+  const int32_t* table;
+  int64_t table_ld;
+  int64_t width;              // pages of a row of the table
+  const int32_t* lengths;
+  const int32_t* q_starts;    // or null: `each` queries a sequence
+  int64_t tokens, sequences, each;
+  int q_heads, group;
+  float scale;
+  int64_t window;             // 0: none
+  int64_t tiles;              // row tiles of all sequences
+  int splits;
+  float* part;                // [splits][tokens * q_heads][DIM], then [splits][tokens * q_heads][2]
+};
+
+// Reductions over the four lane groups (lanes r, r + 16, r + 32, r + 48).
+__device__ inline float bits_float(uint32_t u) { return __builtin_bit_cast(float, u); }
+template <class F>
+__device__ inline float groups_reduce(float v, F&& f) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const v2u a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const float w = f(bits_float(a[0]), bits_float(a[1]));
+  const uint32_t x = __builtin_bit_cast(uint32_t, w);
+  const v2u b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return f(bits_float(b[0]), bits_float(b[1]));
+}
+__device__ inline float groups_max(float v) {
+  return groups_reduce(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ inline float groups_sum(float v) {
+  return groups_reduce(v, [](float a, float b) { return a + b; });
+}
+
+// Eight codes of a word as fp16: even ones times kEven, odd ones times kOdd, in the order
+// 0, 4, 1, 5, 2, 6, 3, 7.
+constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;
+template <bool FINE>
+struct Codes {
+  static constexpr float kEven = FINE ? 0x1p-20f : 0x1p-24f, kOdd = 0x1p-20f;
+  __device__ static inline v8h of(uint32_t w) {
+    const uint32_t h = w >> 8;
+    if constexpr (FINE) return __builtin_bit_cast(v8h, (v4u){(w << 4) & kHigh, w & kHigh, (w >> 4) & kHigh, h & kHigh});
+    else return __builtin_bit_cast(v8h, (v4u){w & kLow, w & kHigh, h & kLow, h & kHigh});
+  }
+  // The low (odd: high) halves of eight bytes, in the order 0, 2, 1, 3, 4, 6, 5, 7.
+  __device__ static inline v8h even(uint32_t a, uint32_t b) {
+    if constexpr (FINE)
+      return __builtin_bit_cast(v8h, (v4u){(a << 4) & kHigh, (a >> 4) & kHigh, (b << 4) & kHigh, (b >> 4) & kHigh});
+    else return __builtin_bit_cast(v8h, (v4u){a & kLow, (a >> 8) & kLow, b & kLow, (b >> 8) & kLow});
+  }
+  __device__ static inline v8h odd(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(v8h, (v4u){a & kHigh, (a >> 8) & kHigh, b & kHigh, (b >> 8) & kHigh});
+  }
+};
+
+__device__ inline uint32_t pk_max_u16(uint32_t a, uint32_t b) {
+  typedef unsigned short v2u16 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2u16, a), __builtin_bit_cast(v2u16, b)));
+}
+
+// Where a tile of 16 tokens stands: its page (0 for one outside the cache) and the place of its first token.
+struct Tile {
+  int64_t page;
+  int place;
+  bool bad;
+};
+__device__ inline Tile tile_at(const Attention& a, const int32_t* table, int64_t t) {
+  const int64_t at = t >> a.cache.shift;
+  const int64_t page = at < a.width ? table[at] : 0;   // beyond: past the tokens, masked
+  const bool bad = page < 0 || page >= a.cache.pages;
+  return {bad ? 0 : page, (int)(t & ((1 << a.cache.shift) - 1)), bad};
+}
+
+// One row's end: the token after the last that it sees, and the first.
+struct Sees {
+  int64_t first, last;
+};
+
+template <class D, int DIM, int NB, int NQ, int NP, bool FINE>
+__global__ void __launch_bounds__(256)
+kv4_attention_kernel(Attention a) {
+  constexpr int NS = DIM / 32;        // k-steps of a score, words of a key's codes in a lane
+  constexpr int NF = DIM / 32;        // blocks of 16 pairs of values
+  constexpr int ROWS = 16 * NB, TILE = 4 * ROWS;
+  using C = Codes<FINE>;
+  using T = typename D::T;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int heads = a.cache.heads;
+  int64_t block = blockIdx.x;
+  const int head = (int)(block % heads);
+  block /= heads;
+  const int64_t tile = block % a.tiles;
+  const int split = (int)(block / a.tiles);
+
+  // The tile's sequence, its queries and the tile's first row. Tiles of ragged sequences are
+  // counted from q_starts[b] * group / TILE + b on, which leaves room for every one's last.
+  int64_t b, start, count, row0;
+  auto begin_of = [&](int64_t i) {   // i >= 0; sequence 0 starts at 0, the rows behind the last are one more
+    const int64_t s = i == 0 ? 0 : (int64_t)a.q_starts[i];
+    return s < 0 ? 0 : s > a.tokens ? a.tokens : s;
+  };
+  if (a.q_starts) {
+    int64_t n = 0;
+    for (int64_t base = 0; base <= a.sequences; base += 64) {
+      const int64_t i = base + lane;
+      const bool before = i <= a.sequences && begin_of(i) * a.group / TILE + i <= tile;
+      const int got = __popcll(__ballot(before));
+      n += got;
+      if (got < 64) break;
+    }
+    b = n - 1;
+    start = begin_of(b);
+    const int64_t end = b < a.sequences ? begin_of(b + 1) : a.tokens;
+    count = end > start ? end - start : 0;
+    row0 = (tile - (start * a.group / TILE + b)) * TILE;
+  } else {
+    const int64_t per = (a.each * a.group + TILE - 1) / TILE;
+    b = tile / per;
+    start = b * a.each;
+    count = a.each;
+    row0 = (tile % per) * TILE;
+  }
+  const int64_t all = count * a.group;
+  if (row0 < 0 || row0 >= all) return;   // below 0: q_starts that do not ascend
+  const int rows = (int)(all - row0 < TILE ? all - row0 : TILE);
+
+  const int64_t capacity = a.width << a.cache.shift;
+  int64_t length = b < a.sequences ? a.lengths[b] : 0;
+  const bool poison = length > capacity;
+  if (length < 0 || poison) length = 0;
+
+  // The waves' rows; waves with the same rows take turns at their tokens.
+  const int blocks = (rows + ROWS - 1) / ROWS;
+  const int sharing = blocks == 1 ? 4 : blocks == 2 ? 2 : 1;
+  const int mine = wave / sharing, turn_of = wave % sharing;
+  const bool active = mine < blocks;
+  const int64_t first_row = row0 + (active ? mine : 0) * ROWS;
+  const int64_t last_row = first_row + ROWS < row0 + rows ? first_row + ROWS - 1 : row0 + rows - 1;
+  auto sees = [&](int64_t row) {
+    const int64_t p = length - count + row / a.group;
+    const int64_t first = a.window && p + 1 > a.window ? p + 1 - a.window : 0;
+    return Sees{first, length ? (p + 1 > 0 ? p + 1 : 0) : 0};
+  };
+  const Sees top = sees(first_row), bottom = sees(last_row);
+
+  const int64_t row_of_lane[2] = {first_row + r <= last_row ? first_row + r : last_row,
+                                  first_row + 16 + r <= last_row ? first_row + 16 + r : last_row};
+  Sees see[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) see[n] = sees(row_of_lane[n]);
+
+  // Queries as fp16 parts in the order of Codes::of, the odd codes' factor taken out.
+  v8h qf[NQ][NB][NS];
+  float factor[NB], qsum[NB];   // of the exponent of two; sum of a query, in units of its scores
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int64_t row = row_of_lane[n];
+    const T* q = reinterpret_cast<const T*>(a.q) + (start + row / a.group) * a.q_token +
+                 (head * a.group + row % a.group) * a.q_head;
+    float x[NS][8], most = 0.f;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      T t[8];
+      __builtin_memcpy(t, q + (g * NS + s) * 8, sizeof(t));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[s][i] = D::to_f(t[i]);
+        most = fmaxf(most, fabsf(x[s][i]));
+      }
+    }
+    most = groups_max(most);
+    int e = 15 - __builtin_amdgcn_frexp_expf(most);   // 2^14 <= most 2^e < 2^15
+    e = most > 0.f && most < kInf ? min(max(e, -100), 60) : 0;
+    float sum = 0.f;
+    constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = ldexpf(x[s][kOrder[i]], e);
+        sum += v;
+        const float w = kOrder[i] & 1 ? v * (C::kEven / C::kOdd) : v;
+        qf[0][n][s][i] = (_Float16)w;
+        if constexpr (NQ > 1) qf[1][n][s][i] = (_Float16)(w - (float)(_Float16)w);
+      }
+    qsum[n] = most < kInf ? groups_sum(sum) * C::kEven : __builtin_nanf("");   // an infinity's scores are NaN
+    factor[n] = fmaxf(ldexpf(a.scale * kLog2e, -e) * (1.f / C::kEven), 0x1p-126f);   // 0 times a masked score: no number
+  }
+
+  v4f o[NB][NF][2];
+  float most[NB], at[NB], total[NB], least[NB];   // largest score; exponent of weight 1; sums of weights, and times minima
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    most[n] = -kInf;
+    at[n] = total[n] = least[n] = 0.f;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) o[n][f][0] = o[n][f][1] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+  int scale_exp = -14;
+
+  const int64_t begin = top.first & ~(int64_t)63;
+  const int64_t steps = bottom.last > begin ? (bottom.last - begin + 63) / 64 : 0;
+  const int64_t per_split = (steps + a.splits - 1) / a.splits;
+  const int64_t to = (split + 1) * per_split < steps ? (split + 1) * per_split : steps;
+  const int32_t* table = a.table + (b < a.sequences ? b : 0) * a.table_ld;
+  for (int64_t step = split * per_split + turn_of; active && step < to; step += sharing) {
+    const int64_t t0 = begin + 64 * step;
+    // keys: lane row r reads token 16 (r / 4) + 4 u + r % 4 of tile u, its words of group g
+    const Tile kt = tile_at(a, table, t0 + 16 * (r >> 2)), vt = tile_at(a, table, t0 + 16 * g);
+    const uint8_t* kp = a.cache.key(kt.page, head, kt.place + (r & 3), DIM) + g * (4 * NS);
+    const uint8_t* vp = a.cache.value_tile(vt.page, head, vt.place, DIM) + r * 16;
+    uint32_t kw[4][NS];
+    v4u vw[NF];
+    v4u kpar[4], vpar[4];   // scales (two words of eight), minima
+#pragma unroll
+    for (int u = 0; u < 4; ++u) __builtin_memcpy(kw[u], kp + u * 4 * (DIM / 2), sizeof(kw[u]));
+    const v4u* pk = reinterpret_cast<const v4u*>(a.cache.param_tile(vt.page, 0, head, vt.place));
+    const v4u* pv = reinterpret_cast<const v4u*>(a.cache.param_tile(vt.page, 1, head, vt.place));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) kpar[i] = pk[i], vpar[i] = pv[i];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) vw[f] = *reinterpret_cast<const v4u*>(vp + f * 256);
+
+    const bool whole = t0 + 64 <= top.last && t0 >= bottom.first && !__any(vt.bad);
+    _Float16 ks[16], kl[16], vs[16], vl[16];
+    __builtin_memcpy(ks, kpar, 32);
+    __builtin_memcpy(kl, kpar + 2, 32);
+    __builtin_memcpy(vs, vpar, 32);
+    __builtin_memcpy(vl, vpar + 2, 32);
+    if (!whole) {
+      // tokens that no row sees may hold anything; those on a bad page are NaN
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int64_t t = t0 + 16 * g + i;
+        const bool seen = t >= top.first && t < bottom.last;
+        const _Float16 nan = (_Float16)__builtin_nanf(""), zero = (_Float16)0.f;
+        ks[i] = !seen ? zero : vt.bad ? nan : ks[i];
+        kl[i] = !seen ? zero : vt.bad ? nan : kl[i];
+        vs[i] = !seen ? zero : vt.bad ? nan : vs[i];
+        vl[i] = !seen ? zero : vt.bad ? nan : vl[i];
+      }
+    }
+    uint32_t big = 0;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      uint32_t two;
+      __builtin_memcpy(&two, vs + i, 4);
+      big = pk_max_u16(big, two & 0x7FFF7FFFu);
+    }
+    // the exponent of the largest scale, over the step's tokens (as bits, which order like it)
+    const uint32_t field = (uint32_t)groups_max((float)(max(big & 0xFFFFu, big >> 16) >> 10));
+    const int exp_now = max(scale_exp, __builtin_amdgcn_readfirstlane((int)field) - 14);
+
+    v4f sc[NB][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) sc[n][u] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const v8h c = C::of(kw[u][s]);
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int h = 0; h < NQ; ++h)
+            sc[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, qf[h][n][s], sc[n][u], 0, 0, 0);
+      }
+    }
+    v8h ph[NB][2], pl[NB][2];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      float now = most[n];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float y = fmaf((float)ks[4 * u + i], sc[n][u][i], (float)kl[4 * u + i] * qsum[n]);
+          if (!whole) {
+            const int64_t t = t0 + 16 * g + 4 * u + i;
+            if (t >= see[n].last || t < see[n].first) y = -kInf;
+          }
+          sc[n][u][i] = y;
+          now = fmaxf(now, y);
+        }
+      now = groups_max(now);
+      if (__any(now > most[n]) || exp_now > scale_exp) {
+        const float next = now == -kInf ? 0.f : fmaf(factor[n], now, (float)(exp_now - 15));
+        const float shrink = most[n] == -kInf ? 1.f : __builtin_amdgcn_exp2f(at[n] - next);   // before: all sums 0
+        most[n] = now;
+        at[n] = next;
+        total[n] *= shrink;
+        least[n] *= shrink;
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            o[n][f][0][i] *= shrink;
+            o[n][f][1][i] *= shrink;
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // tokens 8 z .. 8 z + 7 of the lane in the order of Codes::even
+          constexpr int kSlot[4] = {0, 2, 1, 3};
+          const int z = u >> 1, j = 4 * (u & 1) + kSlot[i];
+          const float p = __builtin_amdgcn_exp2f(fmaf(factor[n], sc[n][u][i], -at[n]));
+          float s = (float)vs[4 * u + i], lo = (float)vl[4 * u + i];
+          if (!whole && sc[n][u][i] == -kInf) s = lo = 0.f;   // a masked token's NaN stays out
+          total[n] += p;
+          least[n] = fmaf(p, lo, least[n]);
+          const _Float16 h = (_Float16)(p * s);
+          ph[n][z][j] = h;
+          if constexpr (NP > 1) pl[n][z][j] = (_Float16)fmaf(p, s, -(float)h);
+        }
+    }
+    scale_exp = exp_now;
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        const v8h even = C::even(vw[f][2 * z], vw[f][2 * z + 1]), odd = C::odd(vw[f][2 * z], vw[f][2 * z + 1]);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          o[n][f][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, ph[n][z], o[n][f][0], 0, 0, 0);
+          o[n][f][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, ph[n][z], o[n][f][1], 0, 0, 0);
+          if constexpr (NP > 1) {
+            o[n][f][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, pl[n][z], o[n][f][0], 0, 0, 0);
+            o[n][f][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, pl[n][z], o[n][f][1], 0, 0, 0);
+          }
+        }
+      }
+  }
+
+  // Outputs in units of the weights, and the sums of all lanes. A wave that saw nothing has
+  // the exponent -inf, so that it counts for nothing beside another.
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    total[n] = groups_sum(total[n]);
+    least[n] = groups_sum(least[n]);
+    if (most[n] == -kInf && total[n] == 0.f) at[n] = -kInf;
+    if (poison) total[n] = __builtin_nanf(""), at[n] = 0.f;
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o[n][f][0][i] = fmaf(o[n][f][0][i], 1.f / C::kEven, least[n]);
+        o[n][f][1][i] = fmaf(o[n][f][1][i], 1.f / C::kOdd, least[n]);
+      }
+  }
+  // Waves that shared rows: half of them hand theirs to the others, twice for four.
+  __shared__ float join[2][64][NB * NF * 8 + 2 * NB + 1];   // one float more: lanes in different banks
+  for (int step = sharing / 2; step > 0; step /= 2) {
+    // of two waves that share rows and stand `step` turns apart the later gives
+    const int slot = sharing == 4 ? (turn_of % step) : mine;
+    float* box = join[slot & 1][lane];
+    if (active && turn_of >= step && turn_of < 2 * step) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        box[2 * n] = at[n];
+        box[2 * n + 1] = total[n];
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) box[2 * NB + (n * NF + f) * 8 + i] = o[n][f][i >> 2][i & 3];
+      }
+    }
+    __syncthreads();
+    if (active && turn_of < step) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const float other = box[2 * n], both = fmaxf(at[n], other);
+        const float x = at[n] == -kInf ? 0.f : __builtin_amdgcn_exp2f(at[n] - both);
+        const float y = other == -kInf ? 0.f : __builtin_amdgcn_exp2f(other - both);
+        at[n] = both;
+        total[n] = total[n] * x + box[2 * n + 1] * y;
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            o[n][f][i >> 2][i & 3] = o[n][f][i >> 2][i & 3] * x + box[2 * NB + (n * NF + f) * 8 + i] * y;
+      }
+    }
+    __syncthreads();
+  }
+  if (!active || turn_of) return;
+  const int64_t total_rows = a.tokens * a.q_heads;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int64_t row = first_row + 16 * n + r;
+    if (row > last_row) continue;
+    const int64_t at_row = (start + row / a.group) * a.q_heads + head * a.group + row % a.group;
+    if (a.splits > 1) {
+      const int64_t slot = split * total_rows + at_row;
+      float* to_o = a.part + slot * DIM;
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = o[n][f][i & 1][i >> 1];
+        __builtin_memcpy(to_o + 32 * f + 8 * g, v, sizeof(v));
+      }
+      if (g == 0) {
+        float* ml = a.part + a.splits * total_rows * DIM + slot * 2;
+        ml[0] = at[n];
+        ml[1] = total[n];
+      }
+    } else {
+      T* to_o = reinterpret_cast<T*>(a.out) + at_row * DIM;
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = D::from_f(total[n] == 0.f ? 0.f : o[n][f][i & 1][i >> 1] / total[n]);
+        __builtin_memcpy(to_o + 32 * f + 8 * g, v, sizeof(v));
+      }
+    }
+  }
+}
+
+// Parts of a row's tokens to its output. A thread takes four values.
+template <class D, int DIM>
+__global__ void __launch_bounds__(256)
+kv4_attention_join(const float* __restrict__ part, int splits, int64_t rows, typename D::T* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / (DIM / 4);
+  if (row >= rows) return;
+  const float* ml = part + splits * rows * DIM + row * 2;
+  float most = -kInf;
+  for (int s = 0; s < splits; ++s) most = fmaxf(most, ml[s * rows * 2]);
+  float total = 0.f;
+  v4f sum = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; ++s) {
+    const float at = ml[s * rows * 2];
+    if (at == -kInf) continue;
+    const float w = __builtin_amdgcn_exp2f(at - most);
+    const v4f v = *reinterpret_cast<const v4f*>(part + (s * rows + row) * DIM + (i % (DIM / 4)) * 4);
+    total = fmaf(w, ml[s * rows * 2 + 1], total);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] = fmaf(w, v[j], sum[j]);
+  }
+  typename D::T t[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) t[j] = D::from_f(total == 0.f ? 0.f : sum[j] / total);
+  __builtin_memcpy(out + row * DIM + (i % (DIM / 4)) * 4, t, sizeof(t));
+}
+
+template <class F>
+void with_dim(int dim, F&& f) {
+  if (dim == 64) f(std::integral_constant<int, 64>{});
+  else if (dim == 96) f(std::integral_constant<int, 96>{});
+  else if (dim == 128) f(std::integral_constant<int, 128>{});
+  else if (dim == 192) f(std::integral_constant<int, 192>{});
+  else f(std::integral_constant<int, 256>{});
+}
+
+}  // namespace
+
+}  // namespace qo
+
+extern "C" int64_t qo_kv4_attention_workspace_size(const qo_kv4_cache* cache, int64_t tokens, int q_heads,
+                                                   int64_t table_width, int64_t sequences, int has_starts,
+                                                   int64_t window) {
+  using namespace qo;
+  if (!cache || cache->kv_heads < 1 || tokens < 1 || q_heads < cache->kv_heads || sequences < 1) return 0;
+  const Kv4Plan p = kv4_plan(tokens, q_heads, cache->kv_heads, cache->head_dim, table_width * cache->page_size,
+                             sequences, has_starts != 0, window, device_cu_count());
+  return p.splits > 1 ? p.splits * tokens * q_heads * (cache->head_dim + 2) * 4 : 0;
+}
+
+extern "C" int qo_kv4_attention(const qo_kv4_cache* cache, const qo_heads* q, int dtype, int64_t tokens, int q_heads,
+                                const int32_t* page_table, int64_t table_ld, int64_t table_width,
+                                const int32_t* lengths, const int32_t* q_starts, int64_t sequences, float scale,
+                                int64_t window, void* out, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace qo;
+  const char* fn = "qo_kv4_attention";
+  KV4 c;
+  const int st = kv4_cache(fn, cache, &c);
+  if (st != QO_OK) return st;
+  if (tokens < 0 || tokens > QO_KV4_MAX_TOKENS || sequences < 0 || sequences > QO_KV4_MAX_TOKENS || table_width < 0 ||
+      table_width > INT32_MAX || table_ld < table_width) {
+    qo_set_error("%s: invalid sizes tokens=%lld sequences=%lld table %lld wide, row stride %lld", fn, (long long)tokens,
+                 (long long)sequences, (long long)table_width, (long long)table_ld);
+    return QO_ERR_SHAPE;
+  }
+  if (q_heads < 1 || q_heads > 16384 || q_heads % c.heads != 0) {
+    qo_set_error("%s: q_heads (%d) must be a multiple of kv_heads (%d)", fn, q_heads, c.heads);
+    return QO_ERR_SHAPE;
+  }
+  if (!q_starts && (sequences == 0 ? tokens != 0 : tokens % sequences != 0)) {
+    qo_set_error("%s: %lld queries of %lld sequences need q_starts", fn, (long long)tokens, (long long)sequences);
+    return QO_ERR_SHAPE;
+  }
+  if (!(scale > 0.f && scale < 3.4e38f) || window < 0) {
+    qo_set_error("%s: scale must be positive and window not negative, got %g and %lld", fn, (double)scale,
+                 (long long)window);
+    return QO_ERR_SHAPE;
+  }
+  if (dtype != QO_DTYPE_F32 && dtype != QO_DTYPE_F16 && dtype != QO_DTYPE_BF16) {
+    qo_set_error("%s: unsupported dtype code %d", fn, dtype);
+    return QO_ERR_DTYPE;
+  }
+  if (tokens == 0) return QO_OK;
+  if (!q || !q->data || !out || (sequences && !lengths) || (sequences && table_width && !page_table)) {
+    qo_set_error("%s: NULL pointer argument", fn);
+    return QO_ERR_NULL_POINTER;
+  }
+  if (workspace && (uintptr_t)workspace % 16 != 0) {
+    qo_set_error("%s: workspace must be 16-byte aligned", fn);
+    return QO_ERR_ALIGNMENT;
+  }
+  Kv4Plan plan = kv4_plan(tokens, q_heads, c.heads, cache->head_dim, table_width * cache->page_size, sequences,
+                          q_starts != nullptr, window, device_cu_count());
+  if (plan.splits > 1 &&
+      (!workspace || workspace_bytes < plan.splits * tokens * q_heads * (cache->head_dim + 2) * 4))
+    plan.splits = 1;
+  const int64_t grid = plan.tiles * c.heads * plan.splits;
+  if (grid > (1 << 24) - 1) {   // 256 threads each
+    qo_set_error("%s: too many rows for one call (%lld workgroups)", fn, (long long)grid);
+    return QO_ERR_SHAPE;
+  }
+  Attention a = {c, q->data, q->token_stride, q->head_stride, out, page_table, table_ld, table_width, lengths, q_starts,
+                 tokens, sequences, sequences ? tokens / sequences : 0, q_heads, q_heads / c.heads, scale, window,
+                 plan.tiles, plan.splits, reinterpret_cast<float*>(workspace)};
+  if (c.pages == 0) a.width = 0;   // nothing to read
+  launch_begin();
+  auto go = [&](auto d, auto parts_q, auto parts_p, auto fine) {
+    using D = decltype(d);
+    constexpr int NQ = decltype(parts_q)::value, NP = decltype(parts_p)::value;
+    constexpr bool FINE = decltype(fine)::value;
+    with_dim(cache->head_dim, [&](auto dim) {
+      constexpr int DIM = decltype(dim)::value;
+      hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+      if (plan.row_blocks == 1) launch(kv4_attention_kernel<D, DIM, 1, NQ, NP, FINE>, dim3((unsigned)grid), dim3(256), 0, s, a);
+      else if constexpr (DIM <= 128) launch(kv4_attention_kernel<D, DIM, 2, NQ, NP, FINE>, dim3((unsigned)grid), dim3(256), 0, s, a);
+      if (plan.splits > 1) {
+        const int64_t rows = tokens * q_heads;
+        launch(kv4_attention_join<D, DIM>, dim3((unsigned)((rows * (DIM / 4) + 255) / 256)), dim3(256), 0, s,
+               reinterpret_cast<const float*>(workspace), plan.splits, rows, reinterpret_cast<typename D::T*>(out));
+      }
+    });
+  };
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  if (dtype == QO_DTYPE_BF16) go(BF16T{}, One{}, One{}, std::false_type{});
+  else if (dtype == QO_DTYPE_F16) go(F16T{}, One{}, Two{}, std::false_type{});
+  else go(F32T{}, Two{}, Two{}, std::true_type{});
+  return launch_result(fn);
+}

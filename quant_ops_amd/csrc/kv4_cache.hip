@@ -1,0 +1,346 @@
+// Appending keys and values to the 4-bit cache of kv4_common.h, with the position rotation on
+// the way, and reading them back.
+#include "kv4_common.h"
+
+namespace qo {
+
+int kv4_cache(const char* fn, const qo_kv4_cache* c, KV4* out) {
+  if (!c) {
+    qo_set_error("%s: NULL cache", fn);
+    return QO_ERR_NULL_POINTER;
+  }
+  if (!kv4_head_dim(c->head_dim)) {
+    qo_set_error("%s: head_dim must be 64, 96, 128, 192 or 256, got %d", fn, (int)c->head_dim);
+    return QO_ERR_SHAPE;
+  }
+  const int p = c->page_size;
+  if (p < 16 || p > QO_KV4_MAX_PAGE || (p & (p - 1))) {
+    qo_set_error("%s: page_size must be a power of two from 16 to %d, got %d", fn, QO_KV4_MAX_PAGE, p);
+    return QO_ERR_SHAPE;
+  }
+  if (c->pages < 0 || c->pages > INT32_MAX || c->kv_heads < 1 || c->kv_heads > 16384) {
+    qo_set_error("%s: invalid sizes pages=%lld kv_heads=%d", fn, (long long)c->pages, (int)c->kv_heads);
+    return QO_ERR_SHAPE;
+  }
+  if (c->pages && (!c->k_codes || !c->v_codes || !c->params)) {
+    qo_set_error("%s: NULL pointer in the cache", fn);
+    return QO_ERR_NULL_POINTER;
+  }
+  if (((uintptr_t)c->k_codes | (uintptr_t)c->v_codes | (uintptr_t)c->params) % 16 != 0) {
+    qo_set_error("%s: the cache's pointers must be 16-byte aligned", fn);
+    return QO_ERR_ALIGNMENT;
+  }
+  int shift = 4;
+  while ((1 << shift) < p) ++shift;
+  *out = {reinterpret_cast<uint8_t*>(c->k_codes), reinterpret_cast<uint8_t*>(c->v_codes),
+          reinterpret_cast<_Float16*>(c->params), c->pages, shift, c->kv_heads};
+  return QO_OK;
+}
+
+namespace {
+
+// Lanes of a vector: eight values each, a power of two of them (those past the vector idle).
+template <int DIM>
+constexpr int kLanes = DIM <= 64 ? 8 : DIM <= 128 ? 16 : 32;
+
+// N elements at p (16 bytes at most, at any alignment).
+template <class D, int N>
+__device__ inline void load_values(const typename D::T* p, float* v) {
+  typename D::T t[N];
+  __builtin_memcpy(t, p, sizeof(t));
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = D::to_f(t[i]);
+}
+
+template <int LANES, class F>
+__device__ inline float lanes_reduce(float v, F&& f) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) v = f(v, __shfl_xor(v, o, LANES));
+  return v;
+}
+
+// A token's rotation: angles of position p, or NaN where the table does not reach.
+struct Angles {
+  const int64_t* positions;
+  const float* cos_;
+  const float* sin_;
+  int64_t rows;
+  int rot, interleaved;
+};
+
+// Eight values of a vector and where they stand: `at` the first four, `more` the others. In
+// the rotated part a lane has four pairs.
+struct Place {
+  int at, more;
+  bool turned;
+};
+__device__ inline Place place_of(int lane, const Angles& a) {
+  if (8 * lane >= a.rot || a.interleaved) return {8 * lane, 8 * lane + 4, 8 * lane < a.rot};
+  return {4 * lane, a.rot / 2 + 4 * lane, true};
+}
+
+// (a, b) -> (a cos - b sin, b cos + a sin). A product of two float32 is exact in 64 bits, so
+// the results are the formula's, rounded to 64 bits and then to 32: whoever computes it in
+// 64 bits gets the same codes.
+__device__ inline void turn(float& a, float& b, float c, float s) {
+  const double x = (double)a * c - (double)b * s, y = (double)b * c + (double)a * s;
+  a = (float)x;
+  b = (float)y;
+}
+
+// Codes of a vector's eight values and its parameters. Borders between codes are decided in
+// 64 bits: n = floor of an estimate of (v - lo) / s is the quotient's floor, or beside it
+// where the quotient is next to a whole number, and either way v - lo against s (n + 1/2),
+// which is exact, says whether the nearest code is n or n + 1.
+template <int LANES>
+__device__ inline void quantize(const float (&v)[8], bool there, uint32_t (&c)[8], _Float16& scale, _Float16& least) {
+  float lo = __builtin_inff(), hi = -__builtin_inff(), bad = 0.f;
+  float u[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    u[i] = __builtin_amdgcn_fmed3f(v[i], -kKV4Most, kKV4Most);
+    if (there) {
+      lo = fminf(lo, u[i]);
+      hi = fmaxf(hi, u[i]);
+      if (!(fabsf(v[i]) <= 3.4028234e38f)) bad = 1.f;
+    }
+  }
+  lo = lanes_reduce<LANES>(lo, [](float a, float b) { return fminf(a, b); });
+  hi = lanes_reduce<LANES>(hi, [](float a, float b) { return fmaxf(a, b); });
+  bad = lanes_reduce<LANES>(bad, [](float a, float b) { return fmaxf(a, b); });
+  least = (_Float16)lo;
+  const double l = (double)(float)least;
+  const float range = (float)(((double)hi - l) / 15.0);   // rounded to float32, then to fp16
+  scale = (_Float16)fmaxf(range, 0.f);
+  const float s = (float)scale;
+  const float inverse = s > 0.f ? 1.f / s : 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const double d = (double)u[i] - l;
+    const float n = floorf(fminf(fmaxf((float)d * inverse, 0.f), 15.f));
+    const double over = d - (double)s * ((double)n + 0.5);
+    const int k = (int)n;
+    c[i] = s > 0.f ? (uint32_t)min(k + ((over > 0.0) | ((over == 0.0) & (k & 1)) ? 1 : 0), 15) : 0u;
+  }
+  if (bad != 0.f) {
+    scale = least = (_Float16)__builtin_nanf("");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = 0;
+  }
+}
+
+// A workgroup of 256 threads takes 256 / LANES consecutive tokens of one head; blockIdx.y
+// counts query heads, then key heads, then value heads.
+template <class D, int DIM>
+__global__ void __launch_bounds__(256)
+kv4_append_kernel(KV4 cache, Heads<typename D::T> q, Heads<typename D::T> k, Heads<typename D::T> v, int64_t tokens,
+                  int q_heads, const int64_t* __restrict__ slots, Angles angles, typename D::T* __restrict__ q_out) {
+  constexpr int LANES = kLanes<DIM>, TOKENS = 256 / LANES;
+  const int lane = threadIdx.x % LANES;
+  const int64_t token = (int64_t)blockIdx.x * TOKENS + threadIdx.x / LANES;
+  const bool there = token < tokens && 8 * lane < DIM;
+  int head = blockIdx.y;
+  const int kind = head < q_heads ? 0 : head < q_heads + cache.heads ? 1 : 2;
+  head -= kind == 0 ? 0 : kind == 1 ? q_heads : q_heads + cache.heads;
+  const int64_t row = token < tokens ? token : 0;
+
+  Place p = {8 * lane, 8 * lane + 4, false};
+  if (kind < 2) p = place_of(lane, angles);
+  float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (there) {
+    const typename D::T* src = (kind == 0 ? q : kind == 1 ? k : v).at(row, head);
+    load_values<D, 4>(src + p.at, x);
+    load_values<D, 4>(src + p.more, x + 4);
+    if (p.turned) {
+      const int64_t pos = angles.positions[row];
+      const bool known = pos >= 0 && pos < angles.rows;
+      const int first = angles.interleaved ? 4 * lane : p.at;   // the first pair's angle
+      float c[4], s[4];
+      load_values<F32T, 4>(angles.cos_ + (known ? pos : 0) * (angles.rot / 2) + first, c);
+      load_values<F32T, 4>(angles.sin_ + (known ? pos : 0) * (angles.rot / 2) + first, s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (!known) c[i] = __builtin_nanf("");
+        if (angles.interleaved) turn(x[2 * i], x[2 * i + 1], c[i], s[i]);
+        else turn(x[i], x[4 + i], c[i], s[i]);
+      }
+    }
+  }
+  if (kind == 0) {
+    if (there) {
+      typename D::T out[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out[i] = D::from_f(x[i]);
+      typename D::T* to = q_out + (token * q_heads + head) * DIM;
+      __builtin_memcpy(to + p.at, out, 4 * sizeof(out[0]));
+      __builtin_memcpy(to + p.more, out + 4, 4 * sizeof(out[0]));
+    }
+    return;
+  }
+
+  uint32_t c[8];
+  _Float16 scale, least;
+  quantize<LANES>(x, there, c, scale, least);
+  const int64_t slot = slots[row];
+  if (!there || slot < 0 || slot >= cache.slots()) return;
+  const int64_t page = slot >> cache.shift;
+  const int place = (int)(slot & ((1 << cache.shift) - 1));
+  if (kind == 1) {
+    uint8_t* to = cache.key(page, head, place, DIM);
+    const uint16_t a = (uint16_t)(c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12);
+    const uint16_t b = (uint16_t)(c[4] | c[5] << 4 | c[6] << 8 | c[7] << 12);
+    *reinterpret_cast<uint16_t*>(to + p.at / 2) = a;
+    *reinterpret_cast<uint16_t*>(to + p.more / 2) = b;
+  } else {
+    uint8_t* to = cache.value_tile(page, head, place, DIM) + (place & 15);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[(4 * lane + i) * 16] = (uint8_t)(c[2 * i] | c[2 * i + 1] << 4);
+  }
+  if (lane == 0) {
+    _Float16* to = cache.param_tile(page, kind - 1, head, place) + (place & 15);
+    to[0] = scale;
+    to[16] = least;
+  }
+}
+
+// A thread reads eight values of a vector; blockIdx.y counts key heads, then value heads.
+template <class D, int DIM>
+__global__ void __launch_bounds__(256)
+kv4_read_kernel(KV4 cache, const int64_t* __restrict__ slots, int64_t tokens, typename D::T* __restrict__ k_out,
+                typename D::T* __restrict__ v_out) {
+  constexpr int LANES = kLanes<DIM>, TOKENS = 256 / LANES;
+  const int lane = threadIdx.x % LANES;
+  const int64_t token = (int64_t)blockIdx.x * TOKENS + threadIdx.x / LANES;
+  if (token >= tokens || 8 * lane >= DIM) return;
+  const bool values = blockIdx.y >= (unsigned)cache.heads;
+  const int head = values ? blockIdx.y - cache.heads : blockIdx.y;
+  const int64_t slot = slots[token];
+  typename D::T out[8] = {};
+  if (slot >= 0 && slot < cache.slots()) {
+    const int64_t page = slot >> cache.shift;
+    const int place = (int)(slot & ((1 << cache.shift) - 1));
+    uint32_t w = 0;
+    if (values) {
+      const uint8_t* from = cache.value_tile(page, head, place, DIM) + (place & 15) + 4 * lane * 16;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w |= (uint32_t)from[16 * i] << (8 * i);
+    } else {
+      w = *reinterpret_cast<const uint32_t*>(cache.key(page, head, place, DIM) + 4 * lane);
+    }
+    const _Float16* par = cache.param_tile(page, values, head, place) + (place & 15);
+    const float s = (float)par[0], lo = (float)par[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = fmaf(s, (float)(w >> (4 * i) & 15u), lo);
+      // the largest code may stand for half a step more than fp16 holds
+      out[i] = D::from_f(D::code == QO_DTYPE_F16 && fabsf(x) > kKV4Most ? copysignf(kKV4Most, x) : x);
+    }
+  }
+  __builtin_memcpy((values ? v_out : k_out) + (token * cache.heads + head) * DIM + 8 * lane, out, sizeof(out));
+}
+
+template <class F>
+bool with_dtype(int code, F&& f) {
+  if (code == QO_DTYPE_F32) f(F32T{});
+  else if (code == QO_DTYPE_F16) f(F16T{});
+  else if (code == QO_DTYPE_BF16) f(BF16T{});
+  else return false;
+  return true;
+}
+template <class F>
+void with_dim(int dim, F&& f) {
+  if (dim == 64) f(std::integral_constant<int, 64>{});
+  else if (dim == 96) f(std::integral_constant<int, 96>{});
+  else if (dim == 128) f(std::integral_constant<int, 128>{});
+  else if (dim == 192) f(std::integral_constant<int, 192>{});
+  else f(std::integral_constant<int, 256>{});
+}
+
+int check_tokens(const char* fn, int64_t tokens, int dtype) {
+  if (tokens < 0 || tokens > QO_KV4_MAX_TOKENS) {
+    qo_set_error("%s: invalid number of tokens %lld", fn, (long long)tokens);
+    return QO_ERR_SHAPE;
+  }
+  if (dtype != QO_DTYPE_F32 && dtype != QO_DTYPE_F16 && dtype != QO_DTYPE_BF16) {
+    qo_set_error("%s: unsupported dtype code %d", fn, dtype);
+    return QO_ERR_DTYPE;
+  }
+  return QO_OK;
+}
+
+int null_pointer(const char* fn) {
+  qo_set_error("%s: NULL pointer argument", fn);
+  return QO_ERR_NULL_POINTER;
+}
+
+}  // namespace
+
+}  // namespace qo
+
+extern "C" int qo_kv4_append(const qo_kv4_cache* cache, const qo_heads* q, const qo_heads* k, const qo_heads* v,
+                             int dtype, int64_t tokens, int q_heads, const int64_t* slots, const int64_t* positions,
+                             const float* cos_, const float* sin_, int64_t table_rows, int rot, int interleaved,
+                             void* q_out, void* stream) {
+  using namespace qo;
+  const char* fn = "qo_kv4_append";
+  KV4 c;
+  int st = kv4_cache(fn, cache, &c);
+  if (st == QO_OK) st = check_tokens(fn, tokens, dtype);
+  if (st != QO_OK) return st;
+  if (rot < 0 || rot > cache->head_dim || rot % 8 != 0 || table_rows < 0) {
+    qo_set_error("%s: rot must be a multiple of 8 from 0 to head_dim (%d), got %d", fn, (int)cache->head_dim, rot);
+    return QO_ERR_SHAPE;
+  }
+  if (q && (rot == 0 || q_heads < 1 || q_heads > 16384)) {
+    qo_set_error("%s: q needs a rotation and from 1 to 16384 heads, got rot %d and %d heads", fn, rot, q_heads);
+    return QO_ERR_SHAPE;
+  }
+  if (tokens == 0) return QO_OK;
+  if (!k || !v || !k->data || !v->data || !slots || (q && (!q->data || !q_out))) return null_pointer(fn);
+  if (rot && (!positions || (table_rows && (!cos_ || !sin_)))) return null_pointer(fn);
+  if (table_rows == 0 && rot) {
+    qo_set_error("%s: the table of angles is empty", fn);
+    return QO_ERR_SHAPE;
+  }
+  if (!q) q_heads = 0;
+  launch_begin();
+  with_dtype(dtype, [&](auto d) {
+    using D = decltype(d);
+    using T = typename D::T;
+    with_dim(cache->head_dim, [&](auto dim) {
+      constexpr int DIM = decltype(dim)::value, TOKENS = 256 / kLanes<DIM>;
+      auto heads = [](const qo_heads* h) {
+        return h ? Heads<T>{reinterpret_cast<const T*>(h->data), h->token_stride, h->head_stride} : Heads<T>{};
+      };
+      const dim3 grid((unsigned)((tokens + TOKENS - 1) / TOKENS), (unsigned)(q_heads + 2 * c.heads));
+      launch(kv4_append_kernel<D, DIM>, grid, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), c, heads(q), heads(k),
+             heads(v), tokens, q_heads, slots, Angles{positions, cos_, sin_, table_rows, rot, interleaved != 0},
+             reinterpret_cast<T*>(q_out));
+    });
+  });
+  return launch_result(fn);
+}
+
+extern "C" int qo_kv4_read(const qo_kv4_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out,
+                           int out_dtype, void* stream) {
+  using namespace qo;
+  const char* fn = "qo_kv4_read";
+  KV4 c;
+  int st = kv4_cache(fn, cache, &c);
+  if (st == QO_OK) st = check_tokens(fn, tokens, out_dtype);
+  if (st != QO_OK) return st;
+  if (tokens == 0) return QO_OK;
+  if (!slots || !k_out || !v_out) return null_pointer(fn);
+  launch_begin();
+  with_dtype(out_dtype, [&](auto d) {
+    using D = decltype(d);
+    using T = typename D::T;
+    with_dim(cache->head_dim, [&](auto dim) {
+      constexpr int DIM = decltype(dim)::value, TOKENS = 256 / kLanes<DIM>;
+      launch(kv4_read_kernel<D, DIM>, dim3((unsigned)((tokens + TOKENS - 1) / TOKENS), (unsigned)(2 * c.heads)), dim3(256),
+             0, reinterpret_cast<hipStream_t>(stream), c, slots, tokens, reinterpret_cast<T*>(k_out),
+             reinterpret_cast<T*>(v_out));
+    });
+  });
+  return launch_result(fn);
+}

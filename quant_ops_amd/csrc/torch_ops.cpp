@@ -7,8 +7,8 @@
 // are additions of this build: int4_matmul_ex (output dtype choice),
 // int4_matmul_bias (bias in the epilogue), w4a4_linear (the linear layer's
 // quantize + GEMM as one operator), dequantize_int4 (a device kernel
-// for the reference's Python function) and the microscaled operators (mx_*,
-// *_mx_quantize).
+// for the reference's Python function), the microscaled operators (mx_*,
+// *_mx_quantize) and those of the 4-bit key/value cache (kv4_*).
 //
 // Unlike the reference, kernels go to the caller's current HIP stream and the
 // host is never synchronised (cuda_quant_kernel.cu:379-385 synchronised the
@@ -430,6 +430,144 @@ at::Tensor mx_matmul(const at::Tensor& a, const at::Tensor& a_scales, const at::
   return out;
 }
 
+// ---------------------------------------------------------------------------
+// The 4-bit key/value cache: k_codes [pages, heads, P, D/2] and v_codes [pages,
+// heads, P/16, D/2, 16] (uint8), params [pages, 2, heads, P/16, 2, 16] (float16).
+// ---------------------------------------------------------------------------
+qo_kv4_cache kv4_of(const at::Tensor& k, const at::Tensor& v, const at::Tensor& params, const at::Tensor& on, const char* op) {
+  TORCH_CHECK(on.is_cuda() && k.device() == on.device() && v.device() == on.device() && params.device() == on.device(), op,
+              ": the cache and the other tensors must be on one GPU");
+  TORCH_CHECK(k.scalar_type() == at::kByte && v.scalar_type() == at::kByte && params.scalar_type() == at::kHalf, op,
+              ": the cache's codes must be uint8 and its params float16");
+  TORCH_CHECK(k.dim() == 4 && v.dim() == 5 && params.dim() == 6, op, ": not a cache: ", k.sizes(), ", ", v.sizes(), ", ",
+              params.sizes());
+  const int64_t pages = k.size(0), heads = k.size(1), P = k.size(2), half = k.size(3);
+  TORCH_CHECK(P % 16 == 0 && v.sizes() == at::IntArrayRef({pages, heads, P / 16, half, 16}) &&
+                  params.sizes() == at::IntArrayRef({pages, 2, heads, P / 16, 2, 16}),
+              op, ": the parts of the cache do not match: ", k.sizes(), ", ", v.sizes(), ", ", params.sizes());
+  TORCH_CHECK(k.is_contiguous() && v.is_contiguous() && params.is_contiguous(), op, ": the cache must be contiguous");
+  TORCH_CHECK(P <= QO_KV4_MAX_PAGE && heads <= INT32_MAX && half <= INT32_MAX, op, ": the cache's sizes are too large");
+  return {k.data_ptr(), v.data_ptr(), params.data_ptr(), pages, (int32_t)P, (int32_t)heads, (int32_t)(2 * half)};
+}
+
+// x [T, heads, D] of the cache's head_dim, or a copy of it, with unit inner stride.
+at::Tensor kv4_heads(const at::Tensor& x, const qo_kv4_cache& c, const at::Tensor& like, const char* op, const char* name) {
+  TORCH_CHECK(x.dim() == 3 && x.size(2) == c.head_dim, op, ": ", name, " must be [tokens, heads, ", c.head_dim, "], got ",
+              x.sizes());
+  TORCH_CHECK(x.scalar_type() == like.scalar_type() && x.device() == like.device() && x.size(0) == like.size(0), op, ": ",
+              name, " must have the others' tokens, dtype and device");
+  return x.stride(2) == 1 ? x : x.contiguous();
+}
+qo_heads kv4_view(const at::Tensor& x) { return {x.data_ptr(), x.stride(0), x.stride(1)}; }
+
+at::Tensor kv4_index(const at::Tensor& x, at::ScalarType type, const at::Tensor& on, const char* op, const char* name) {
+  TORCH_CHECK(x.scalar_type() == type && x.device() == on.device(), op, ": ", name, " must be ",
+              type == at::kLong ? "int64" : "int32", " on the others' device, got ", x.scalar_type());
+  return x.contiguous();
+}
+
+at::Tensor kv4_append(at::Tensor k_codes, at::Tensor v_codes, at::Tensor params, const at::Tensor& k, const at::Tensor& v,
+                      const at::Tensor& slots, const std::optional<at::Tensor>& positions,
+                      const std::optional<at::Tensor>& cos, const std::optional<at::Tensor>& sin,
+                      const std::optional<at::Tensor>& q, bool interleaved) {
+  const char* op = "kv4_append";
+  const qo_kv4_cache c = kv4_of(k_codes, v_codes, params, k, op);
+  TORCH_CHECK(dtype_code(k.scalar_type()) >= 0, op, ": k dtype must be float32, float16 or bfloat16, got ", k.scalar_type());
+  c10::DeviceGuard guard(k.device());
+  const at::Tensor K = kv4_heads(k, c, k, op, "k"), V = kv4_heads(v, c, k, op, "v");
+  const int64_t T = k.size(0);
+  TORCH_CHECK(k.size(1) == c.kv_heads && v.size(1) == c.kv_heads, op, ": k and v must have the cache's ", c.kv_heads, " heads");
+  TORCH_CHECK(slots.dim() == 1 && slots.size(0) == T, op, ": slots must hold one slot per token (", T, "), got ", slots.sizes());
+  const at::Tensor S = kv4_index(slots, at::kLong, k, op, "slots");
+  at::Tensor P, C, N, Q, out;
+  int64_t rows = 0, rot = 0;
+  TORCH_CHECK(cos.has_value() == sin.has_value() && cos.has_value() == positions.has_value(), op,
+              ": positions, cos and sin are given together or not at all");
+  if (cos.has_value()) {
+    TORCH_CHECK(positions->dim() == 1 && positions->size(0) == T, op, ": positions must hold one position per token (", T,
+                "), got ", positions->sizes());
+    P = kv4_index(*positions, at::kLong, k, op, "positions");
+    TORCH_CHECK(cos->dim() == 2 && cos->sizes() == sin->sizes() && cos->scalar_type() == at::kFloat &&
+                    sin->scalar_type() == at::kFloat && cos->device() == k.device() && sin->device() == k.device(),
+                op, ": cos and sin must be float32 [positions, rot / 2] on the others' device");
+    C = cos->contiguous();
+    N = sin->contiguous();
+    rows = C.size(0);
+    rot = 2 * C.size(1);
+    TORCH_CHECK(rows > 0 && rot > 0 && rot <= c.head_dim && rot % 8 == 0, op, ": cos and sin ", cos->sizes(),
+                " must have rows of a multiple of 4 angles, ", c.head_dim / 2, " at most");
+  }
+  if (q.has_value()) {
+    TORCH_CHECK(rot > 0, op, ": q is only rotated: it needs positions, cos and sin");
+    Q = kv4_heads(*q, c, k, op, "q");
+    out = at::detail::empty_cuda(Q.sizes(), Q.scalar_type(), Q.device(), std::nullopt);
+  } else {
+    out = mx_empty(0, 0, k.scalar_type(), k.device());
+  }
+  const qo_heads hk = kv4_view(K), hv = kv4_view(V), hq = Q.defined() ? kv4_view(Q) : qo_heads{};
+  const bool turn = Q.defined() && Q.size(1) > 0;
+  check_status(qo_kv4_append(&c, turn ? &hq : nullptr, &hk, &hv, dtype_code(k.scalar_type()), T,
+                             turn ? (int)Q.size(1) : 0, S.data_ptr<int64_t>(), P.defined() ? P.data_ptr<int64_t>() : nullptr,
+                             C.defined() ? C.data_ptr<float>() : nullptr, N.defined() ? N.data_ptr<float>() : nullptr, rows,
+                             (int)rot, interleaved, turn ? out.data_ptr() : nullptr, current_stream(k)),
+               op);
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> kv4_read(const at::Tensor& k_codes, const at::Tensor& v_codes, const at::Tensor& params,
+                                            const at::Tensor& slots, std::optional<at::ScalarType> out_dtype) {
+  const char* op = "kv4_read";
+  const qo_kv4_cache c = kv4_of(k_codes, v_codes, params, slots, op);
+  const at::ScalarType dtype = out_dtype.value_or(at::kFloat);
+  TORCH_CHECK(dtype_code(dtype) >= 0, op, ": out_dtype must be float32, float16 or bfloat16");
+  TORCH_CHECK(slots.dim() == 1, op, ": slots must be 1-D, got ", slots.sizes());
+  c10::DeviceGuard guard(slots.device());
+  const at::Tensor S = kv4_index(slots, at::kLong, slots, op, "slots");
+  const int64_t T = S.size(0);
+  auto empty = [&] { return at::detail::empty_cuda({T, c.kv_heads, c.head_dim}, dtype, slots.device(), std::nullopt); };
+  at::Tensor k = empty(), v = empty();
+  check_status(qo_kv4_read(&c, S.data_ptr<int64_t>(), T, k.data_ptr(), v.data_ptr(), dtype_code(dtype), current_stream(slots)),
+               op);
+  return {k, v};
+}
+
+at::Tensor kv4_attention(const at::Tensor& q, const at::Tensor& k_codes, const at::Tensor& v_codes, const at::Tensor& params,
+                         const at::Tensor& page_table, const at::Tensor& lengths, double scale,
+                         const std::optional<at::Tensor>& q_starts, int64_t window) {
+  const char* op = "kv4_attention";
+  const qo_kv4_cache c = kv4_of(k_codes, v_codes, params, q, op);
+  TORCH_CHECK(dtype_code(q.scalar_type()) >= 0, op, ": q dtype must be float32, float16 or bfloat16, got ", q.scalar_type());
+  c10::DeviceGuard guard(q.device());
+  const at::Tensor Q = kv4_heads(q, c, q, op, "q");
+  const int64_t T = Q.size(0), H = Q.size(1), B = page_table.dim() == 2 ? page_table.size(0) : -1;
+  TORCH_CHECK(H > 0 && H <= INT32_MAX && H % c.kv_heads == 0, op, ": q's heads (", H, ") must be a multiple of the cache's ",
+              c.kv_heads);
+  TORCH_CHECK(B >= 0 && lengths.dim() == 1 && lengths.size(0) == B, op,
+              ": page_table must be [sequences, pages] and lengths [sequences], got ", page_table.sizes(), " and ", lengths.sizes());
+  TORCH_CHECK(page_table.scalar_type() == at::kInt && page_table.device() == q.device(), op,
+              ": page_table must be int32 on the others' device, got ", page_table.scalar_type());
+  const int64_t W = page_table.size(1);
+  const at::Tensor table = (W <= 1 || page_table.stride(1) == 1) && (B <= 1 || page_table.stride(0) >= W) ? page_table
+                                                                                                    : page_table.contiguous();
+  const at::Tensor L = kv4_index(lengths, at::kInt, q, op, "lengths");
+  at::Tensor starts;
+  if (q_starts.has_value()) {
+    TORCH_CHECK(q_starts->dim() == 1 && q_starts->size(0) == B + 1, op, ": q_starts must hold sequences + 1 (", B + 1,
+                ") entries, got ", q_starts->sizes());
+    starts = kv4_index(*q_starts, at::kInt, q, op, "q_starts");
+  }
+  at::Tensor out = at::detail::empty_cuda({T, H, c.head_dim}, q.scalar_type(), q.device(), std::nullopt);
+  const int64_t ws_bytes = qo_kv4_attention_workspace_size(&c, T, (int)H, W, B, starts.defined(), window);
+  at::Tensor ws = gemm_workspace(ws_bytes, q);
+  const qo_heads hq = kv4_view(Q);
+  check_status(qo_kv4_attention(&c, &hq, dtype_code(q.scalar_type()), T, (int)H, table.data_ptr<int32_t>(),
+                                B > 1 ? table.stride(0) : W, W, L.data_ptr<int32_t>(),
+                                starts.defined() ? starts.data_ptr<int32_t>() : nullptr, B, (float)scale, window,
+                                out.data_ptr(), ws.defined() ? ws.data_ptr() : nullptr, ws_bytes, current_stream(q)),
+               op);
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(quant_ops, m) {
@@ -455,6 +593,15 @@ TORCH_LIBRARY(quant_ops, m) {
   m.def(
       "mx_matmul(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, Tensor? bias=None, "
       "ScalarType? out_dtype=None) -> Tensor");
+  m.def(
+      "kv4_append(Tensor(a!) k_codes, Tensor(b!) v_codes, Tensor(c!) params, Tensor k, Tensor v, Tensor slots, "
+      "Tensor? positions=None, Tensor? cos=None, Tensor? sin=None, Tensor? q=None, bool interleaved=False) -> Tensor");
+  m.def(
+      "kv4_read(Tensor k_codes, Tensor v_codes, Tensor params, Tensor slots, ScalarType? out_dtype=None) -> "
+      "(Tensor, Tensor)");
+  m.def(
+      "kv4_attention(Tensor q, Tensor k_codes, Tensor v_codes, Tensor params, Tensor page_table, Tensor lengths, "
+      "float scale, Tensor? q_starts=None, int window=0) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(quant_ops, CUDA, m) {
@@ -470,4 +617,7 @@ TORCH_LIBRARY_IMPL(quant_ops, CUDA, m) {
   m.impl("add_rms_norm_mx_quantize", &add_rms_norm_mx_quantize);
   m.impl("swiglu_mx_quantize", &swiglu_mx_quantize);
   m.impl("mx_matmul", &mx_matmul);
+  m.impl("kv4_append", &kv4_append);
+  m.impl("kv4_read", &kv4_read);
+  m.impl("kv4_attention", &kv4_attention);
 }

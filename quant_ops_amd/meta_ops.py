@@ -79,3 +79,20 @@ if _loader.KERNELS_AVAILABLE:
         @torch.library.register_fake("quant_ops::mx_matmul")
         def _mx_matmul_fake(a, a_scales, b, b_scales, bias=None, out_dtype=None):
             return a.new_empty((a.size(0), b.size(0)), dtype=out_dtype or torch.bfloat16)
+
+    if hasattr(torch.ops.quant_ops, "kv4_append"):
+
+        @torch.library.register_fake("quant_ops::kv4_append")
+        def _kv4_append_fake(k_codes, v_codes, params, k, v, slots, positions=None, cos=None, sin=None, q=None,
+                             interleaved=False):
+            return k.new_empty((0, 0) if q is None else tuple(q.shape))
+
+        @torch.library.register_fake("quant_ops::kv4_read")
+        def _kv4_read_fake(k_codes, v_codes, params, slots, out_dtype=None):
+            shape = (slots.size(0), k_codes.size(1), 2 * k_codes.size(3))
+            dtype = out_dtype or torch.float32
+            return params.new_empty(shape, dtype=dtype), params.new_empty(shape, dtype=dtype)
+
+        @torch.library.register_fake("quant_ops::kv4_attention")
+        def _kv4_attention_fake(q, k_codes, v_codes, params, page_table, lengths, scale, q_starts=None, window=0):
+            return q.new_empty(tuple(q.shape))
