@@ -60,7 +60,8 @@ def put(cache, which, slot, c, s, lo):
 
 
 def values(cache, which, slots):
-    """float64 values [T, H, D] of slots (a list), and their parts s c + |lo|."""
+    """float64 values [T, H, D] of slots (a list), and the size of their parts: of lo + s c or of (lo + 8 s) +
+    s (c - 8), whichever is larger."""
     k, v, params = (t.cpu() for t in cache)
     at = torch.tensor(slots, dtype=torch.int64)
     page, place = at // k.shape[2], at % k.shape[2]
@@ -68,7 +69,7 @@ def values(cache, which, slots):
     c = torch.stack((b % 16, b // 16), 3).flatten(2).double()
     par = params[page, which, :, place // 16, :, place % 16].double()
     s, lo = par[..., :1], par[..., 1:]
-    return lo + s * c, lo.abs() + s * c
+    return lo + s * c, torch.maximum(lo.abs() + s * c, (lo + 8 * s).abs() + s * (c - 8).abs())
 
 
 def read(cache, which, slot, dtype):
@@ -78,8 +79,8 @@ def read(cache, which, slot, dtype):
 
 
 def attention(q, cache, page_table, lengths, scale, q_starts=None, window=0):
-    """On the CPU, float64 [T, H, D]: outputs, sum_t p (s c + |lo|) of the values, and the largest of the scores'
-    magnitudes scale * sum |q| (s c + |lo|) [T, H]."""
+    """On the CPU, float64 [T, H, D]: outputs, sum_t p (size of the values' parts), and the largest of the scores'
+    magnitudes scale * sum |q| (size of the key's parts) [T, H]."""
     q, page_table, lengths = q.cpu().double(), page_table.cpu(), lengths.cpu()
     cache = tuple(t.cpu() for t in cache)
     pages, heads, size, _ = cache[0].shape

@@ -1,7 +1,8 @@
 // Causal attention over the 4-bit cache of kv4_common.h, on its codes: with k = lo + s c,
-// q . k = s (q . c) + lo sum(q), and with v the same, sum_t p v = sum_t (p s) c + sum_t p lo,
-// so both products run on the codes, which fp16 holds exactly, and the parameters are applied
-// to scores, in float32.
+// q . k = s (q . c) + lo sum(q), and with v = mid + s (c - 8), mid = lo + 8 s, sum_t p v =
+// sum_t (p s) (c - 8) + sum_t p mid: both products run on the codes, which fp16 holds exactly,
+// and the parameters are applied to scores, in float32. Values are taken from their middle so
+// that the sums hold no large terms that cancel.
 //
 // A wave takes 64 tokens a step (four tiles of 16) and 16 NB rows (a row: one query of one of
 // the heads that share a KV head). v_mfma_f32_16x16x32_f16 computes S^T = K Q^T (A: codes of 16
@@ -14,18 +15,21 @@
 //   * values of a vector (k of the first product) and tokens (of the second) come in the order
 //     in which masks take codes out of a word, and the queries and weights are put in it.
 //
-// A code is made fp16 by masking alone: its four bits at the bottom of an fp16 are the subnormal
-// c 2^-24, at bits 4 .. 7 c 2^-20. The matrix core keeps subnormals, but what it drops of a sum
-// of products (probed) goes by an exponent that a subnormal's leading zeros do not lower: with
-// bits 0 .. 3 the sums are off by 1e-7 of their terms' magnitudes, with bits 4 .. 7 by 2e-9.
-// 16-bit queries take both places (five instructions for eight codes), float32 the second alone
-// (seven).
+// For 16-bit queries a key's code is made fp16 by masking alone: its four bits at the bottom of an fp16
+// are the subnormal c 2^-24, at bits 4 .. 7 c 2^-20 (five instructions for eight codes). The matrix
+// core keeps subnormals, but what it drops of a sum of products (probed) goes by an exponent that a
+// subnormal's leading zeros do not lower: sums are off by 1e-7 of their terms' magnitudes. Values
+// meet weights of very different sizes, where that costs much more (2e-6 of the terms, all of one
+// sign, at 33210 tokens), so their codes less 8 are normal numbers (nine instructions for eight),
+// and float32 queries have keys' codes as those too.
 //
 // Queries: brought by a power of two for each row to a largest magnitude in [2^14, 2^15), 16-bit
 // values are exact in fp16 (those below 2^-28 of the largest lose bits); float32 takes two fp16
-// parts (22 bits). Weights: p s 2^15 / S, where S is a power of two that no scale of the tokens so
-// far exceeds, is at most 2^15, and rounded to fp16 (half a step 2^-12, beside bf16's 2^-9 of
-// the output) or, for fp16 and float32, to two parts. Maximum, sums and outputs are float32.
+// parts (22 bits). Weights: p s 2^15 / S, where p is 1 at the row's largest score so far and S a
+// power of two that no scale of the tokens so far exceeds, is at most 2^15, and rounded to fp16 (half
+// a step 2^-12, beside bf16's 2^-9 of the output) or, for fp16 and float32, to two parts. In
+// float32 the second parts have sums of their own: added to the first parts' they would lose what is
+// below 2^-24 of those. Maximum, sums and outputs are float32.
 #include "dispatch_rules.h"
 #include "kv4_common.h"
 
@@ -76,27 +80,35 @@ __device__ inline float groups_sum(float v) {
   return groups_reduce(v, [](float a, float b) { return a + b; });
 }
 
-// Eight codes of a word as fp16: even ones times kEven, odd ones times kOdd, in the order
-// 0, 4, 1, 5, 2, 6, 3, 7.
+// Codes less 8 as fp16 (those at bits 4 .. 7 times 16): with the exponent of 1024 in front, an
+// fp16's lowest bits count in ones.
 constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;
+__device__ inline uint32_t less(uint32_t two, _Float16 n) {
+  const v2h v = __builtin_bit_cast(v2h, two | 0x64006400u) - (v2h){n, n};
+  return __builtin_bit_cast(uint32_t, v);
+}
+__device__ inline uint32_t less_low(uint32_t w) { return less(w & kLow, (_Float16)1032.f); }
+__device__ inline uint32_t less_high(uint32_t w) { return less(w & kHigh, (_Float16)1152.f); }
+
+// The eight codes of a key's word in the order 0, 4, 1, 5, 2, 6, 3, 7: even ones times kEven, odd ones
+// times kOdd, all less kLess.
 template <bool FINE>
 struct Codes {
-  static constexpr float kEven = FINE ? 0x1p-20f : 0x1p-24f, kOdd = 0x1p-20f;
+  static constexpr float kEven = FINE ? 1.f : 0x1p-24f, kOdd = 16.f * kEven, kLess = FINE ? 8.f : 0.f;
   __device__ static inline v8h of(uint32_t w) {
     const uint32_t h = w >> 8;
-    if constexpr (FINE) return __builtin_bit_cast(v8h, (v4u){(w << 4) & kHigh, w & kHigh, (w >> 4) & kHigh, h & kHigh});
+    if constexpr (FINE) return __builtin_bit_cast(v8h, (v4u){less_low(w), less_high(w), less_low(h), less_high(h)});
     else return __builtin_bit_cast(v8h, (v4u){w & kLow, w & kHigh, h & kLow, h & kHigh});
   }
-  // The low (odd: high) halves of eight bytes, in the order 0, 2, 1, 3, 4, 6, 5, 7.
-  __device__ static inline v8h even(uint32_t a, uint32_t b) {
-    if constexpr (FINE)
-      return __builtin_bit_cast(v8h, (v4u){(a << 4) & kHigh, (a >> 4) & kHigh, (b << 4) & kHigh, (b >> 4) & kHigh});
-    else return __builtin_bit_cast(v8h, (v4u){a & kLow, (a >> 8) & kLow, b & kLow, (b >> 8) & kLow});
-  }
-  __device__ static inline v8h odd(uint32_t a, uint32_t b) {
-    return __builtin_bit_cast(v8h, (v4u){a & kHigh, (a >> 8) & kHigh, b & kHigh, (b >> 8) & kHigh});
-  }
 };
+
+// The low (odd: high) halves of eight bytes of values, in the order 0, 2, 1, 3, 4, 6, 5, 7.
+__device__ inline v8h values_even(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(v8h, (v4u){less_low(a), less_low(a >> 8), less_low(b), less_low(b >> 8)});
+}
+__device__ inline v8h values_odd(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(v8h, (v4u){less_high(a), less_high(a >> 8), less_high(b), less_high(b >> 8)});
+}
 
 __device__ inline uint32_t pk_max_u16(uint32_t a, uint32_t b) {
   typedef unsigned short v2u16 __attribute__((ext_vector_type(2)));
@@ -127,6 +139,7 @@ kv4_attention_kernel(Attention a) {
   constexpr int NS = DIM / 32;        // k-steps of a score, words of a key's codes in a lane
   constexpr int NF = DIM / 32;        // blocks of 16 pairs of values
   constexpr int ROWS = 16 * NB, TILE = 4 * ROWS;
+  constexpr int APART = FINE;         // second parts of weights have sums of their own
   using C = Codes<FINE>;
   using T = typename D::T;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
@@ -224,22 +237,23 @@ kv4_attention_kernel(Attention a) {
       for (int i = 0; i < 8; ++i) {
         const float v = ldexpf(x[s][kOrder[i]], e);
         sum += v;
-        const float w = kOrder[i] & 1 ? v * (C::kEven / C::kOdd) : v;
+        const float w = opaque(kOrder[i] & 1 ? v * (C::kEven / C::kOdd) : v);
         qf[0][n][s][i] = (_Float16)w;
-        if constexpr (NQ > 1) qf[1][n][s][i] = (_Float16)(w - (float)(_Float16)w);
+        if constexpr (NQ > 1) qf[1][n][s][i] = (_Float16)(w - (float)qf[0][n][s][i]);
       }
     qsum[n] = most < kInf ? groups_sum(sum) * C::kEven : __builtin_nanf("");   // an infinity's scores are NaN
     factor[n] = fmaxf(ldexpf(a.scale * kLog2e, -e) * (1.f / C::kEven), 0x1p-126f);   // 0 times a masked score: no number
   }
 
-  v4f o[NB][NF][2];
-  float most[NB], at[NB], total[NB], least[NB];   // largest score; exponent of weight 1; sums of weights, and times minima
+  v4f o[APART + 1][NB][NF][2];
+  float most[NB], at[NB], total[NB], middles[NB];   // largest score, as an exponent; sums of weights, and times middles
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     most[n] = -kInf;
-    at[n] = total[n] = least[n] = 0.f;
+    at[n] = total[n] = middles[n] = 0.f;
 #pragma unroll
-    for (int f = 0; f < NF; ++f) o[n][f][0] = o[n][f][1] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int f = 0; f < NF; ++f)
+      for (int h = 0; h <= APART; ++h) o[h][n][f][0] = o[h][n][f][1] = v4f{0.f, 0.f, 0.f, 0.f};
   }
   int scale_exp = -14;
 
@@ -296,19 +310,32 @@ kv4_attention_kernel(Attention a) {
     const uint32_t field = (uint32_t)groups_max((float)(max(big & 0xFFFFu, big >> 16) >> 10));
     const int exp_now = max(scale_exp, __builtin_amdgcn_readfirstlane((int)field) - 14);
 
-    v4f sc[NB][4];
+    float key_base[16], middle[16], scale[16];   // what codes kLess (of a key) and 8 stand for; s 2^15 / S
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      key_base[i] = fmaf(C::kLess, (float)ks[i], (float)kl[i]);
+      middle[i] = fmaf(8.f, (float)vs[i], (float)vl[i]);
+      scale[i] = (float)vs[i] * bits_float((uint32_t)(127 + 15 - exp_now) << 23);
+    }
+    v4f sc[NB][4], rest[NB];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
 #pragma unroll
-      for (int n = 0; n < NB; ++n) sc[n][u] = v4f{0.f, 0.f, 0.f, 0.f};
+      for (int n = 0; n < NB; ++n) sc[n][u] = rest[n] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         const v8h c = C::of(kw[u][s]);
 #pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          sc[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, qf[0][n][s], sc[n][u], 0, 0, 0);
+          if constexpr (NQ > 1) rest[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, qf[1][n][s], rest[n], 0, 0, 0);
+        }
+      }
+      if constexpr (NQ > 1) {
+#pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
-          for (int h = 0; h < NQ; ++h)
-            sc[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, qf[h][n][s], sc[n][u], 0, 0, 0);
+          for (int i = 0; i < 4; ++i) sc[n][u][i] += rest[n][i];
       }
     }
     v8h ph[NB][2], pl[NB][2];
@@ -319,7 +346,7 @@ kv4_attention_kernel(Attention a) {
       for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float y = fmaf((float)ks[4 * u + i], sc[n][u][i], (float)kl[4 * u + i] * qsum[n]);
+          float y = fmaf((float)ks[4 * u + i], sc[n][u][i], key_base[4 * u + i] * qsum[n]);
           if (!whole) {
             const int64_t t = t0 + 16 * g + 4 * u + i;
             if (t >= see[n].last || t < see[n].first) y = -kInf;
@@ -329,19 +356,22 @@ kv4_attention_kernel(Attention a) {
         }
       now = groups_max(now);
       if (__any(now > most[n]) || exp_now > scale_exp) {
-        const float next = now == -kInf ? 0.f : fmaf(factor[n], now, (float)(exp_now - 15));
+        const float next = now == -kInf ? 0.f : factor[n] * now;
         const float shrink = most[n] == -kInf ? 1.f : __builtin_amdgcn_exp2f(at[n] - next);   // before: all sums 0
+        const float shrink_o = shrink * bits_float((uint32_t)(127 + scale_exp - exp_now) << 23);
         most[n] = now;
         at[n] = next;
         total[n] *= shrink;
-        least[n] *= shrink;
+        middles[n] *= shrink;
 #pragma unroll
         for (int f = 0; f < NF; ++f)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            o[n][f][0][i] *= shrink;
-            o[n][f][1][i] *= shrink;
-          }
+          for (int h = 0; h <= APART; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              o[h][n][f][0][i] *= shrink_o;
+              o[h][n][f][1][i] *= shrink_o;
+            }
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u)
@@ -351,13 +381,18 @@ kv4_attention_kernel(Attention a) {
           constexpr int kSlot[4] = {0, 2, 1, 3};
           const int z = u >> 1, j = 4 * (u & 1) + kSlot[i];
           const float p = __builtin_amdgcn_exp2f(fmaf(factor[n], sc[n][u][i], -at[n]));
-          float s = (float)vs[4 * u + i], lo = (float)vl[4 * u + i];
-          if (!whole && sc[n][u][i] == -kInf) s = lo = 0.f;   // a masked token's NaN stays out
+          float s = scale[4 * u + i], mid = middle[4 * u + i];
+          if (!whole && sc[n][u][i] == -kInf) s = mid = 0.f;   // a masked token's NaN stays out
           total[n] += p;
-          least[n] = fmaf(p, lo, least[n]);
-          const _Float16 h = (_Float16)(p * s);
+          middles[n] = fmaf(p, mid, middles[n]);
+          _Float16 h = (_Float16)(p * s);
+          if constexpr (NP > 1) {
+            // one and the same rounding in both parts: the product rounded twice (to float32 first)
+            // or once differ by a step of h where it is next to a tie
+            asm("" : "+v"(h));
+            pl[n][z][j] = (_Float16)fmaf(p, s, -(float)h);
+          }
           ph[n][z][j] = h;
-          if constexpr (NP > 1) pl[n][z][j] = (_Float16)fmaf(p, s, -(float)h);
         }
     }
     scale_exp = exp_now;
@@ -365,33 +400,36 @@ kv4_attention_kernel(Attention a) {
     for (int f = 0; f < NF; ++f)
 #pragma unroll
       for (int z = 0; z < 2; ++z) {
-        const v8h even = C::even(vw[f][2 * z], vw[f][2 * z + 1]), odd = C::odd(vw[f][2 * z], vw[f][2 * z + 1]);
+        const v8h even = values_even(vw[f][2 * z], vw[f][2 * z + 1]), odd = values_odd(vw[f][2 * z], vw[f][2 * z + 1]);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          o[n][f][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, ph[n][z], o[n][f][0], 0, 0, 0);
-          o[n][f][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, ph[n][z], o[n][f][1], 0, 0, 0);
+          v4f(&hi)[2] = o[0][n][f], (&lo)[2] = o[APART][n][f];
+          hi[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, ph[n][z], hi[0], 0, 0, 0);
+          hi[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, ph[n][z], hi[1], 0, 0, 0);
           if constexpr (NP > 1) {
-            o[n][f][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, pl[n][z], o[n][f][0], 0, 0, 0);
-            o[n][f][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, pl[n][z], o[n][f][1], 0, 0, 0);
+            lo[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, pl[n][z], lo[0], 0, 0, 0);
+            lo[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, pl[n][z], lo[1], 0, 0, 0);
           }
         }
       }
   }
 
+  const float unit = bits_float((uint32_t)(127 - 15 + scale_exp) << 23);
   // Outputs in units of the weights, and the sums of all lanes. A wave that saw nothing has
   // the exponent -inf, so that it counts for nothing beside another.
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     total[n] = groups_sum(total[n]);
-    least[n] = groups_sum(least[n]);
+    middles[n] = groups_sum(middles[n]);
     if (most[n] == -kInf && total[n] == 0.f) at[n] = -kInf;
     if (poison) total[n] = __builtin_nanf(""), at[n] = 0.f;
 #pragma unroll
     for (int f = 0; f < NF; ++f)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        o[n][f][0][i] = fmaf(o[n][f][0][i], 1.f / C::kEven, least[n]);
-        o[n][f][1][i] = fmaf(o[n][f][1][i], 1.f / C::kOdd, least[n]);
+        if constexpr (APART) o[0][n][f][0][i] += o[1][n][f][0][i], o[0][n][f][1][i] += o[1][n][f][1][i];
+        o[0][n][f][0][i] = fmaf(o[0][n][f][0][i], unit, middles[n]);
+        o[0][n][f][1][i] = fmaf(o[0][n][f][1][i], 0.0625f * unit, middles[n]);
       }
   }
   // Waves that shared rows: half of them hand theirs to the others, twice for four.
@@ -408,7 +446,7 @@ kv4_attention_kernel(Attention a) {
 #pragma unroll
         for (int f = 0; f < NF; ++f)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) box[2 * NB + (n * NF + f) * 8 + i] = o[n][f][i >> 2][i & 3];
+          for (int i = 0; i < 8; ++i) box[2 * NB + (n * NF + f) * 8 + i] = o[0][n][f][i >> 2][i & 3];
       }
     }
     __syncthreads();
@@ -424,7 +462,7 @@ kv4_attention_kernel(Attention a) {
         for (int f = 0; f < NF; ++f)
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            o[n][f][i >> 2][i & 3] = o[n][f][i >> 2][i & 3] * x + box[2 * NB + (n * NF + f) * 8 + i] * y;
+            o[0][n][f][i >> 2][i & 3] = o[0][n][f][i >> 2][i & 3] * x + box[2 * NB + (n * NF + f) * 8 + i] * y;
       }
     }
     __syncthreads();
@@ -443,7 +481,7 @@ kv4_attention_kernel(Attention a) {
       for (int f = 0; f < NF; ++f) {
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = o[n][f][i & 1][i >> 1];
+        for (int i = 0; i < 8; ++i) v[i] = o[0][n][f][i & 1][i >> 1];
         __builtin_memcpy(to_o + 32 * f + 8 * g, v, sizeof(v));
       }
       if (g == 0) {
@@ -457,7 +495,7 @@ kv4_attention_kernel(Attention a) {
       for (int f = 0; f < NF; ++f) {
         T v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = D::from_f(total[n] == 0.f ? 0.f : o[n][f][i & 1][i >> 1] / total[n]);
+        for (int i = 0; i < 8; ++i) v[i] = D::from_f(total[n] == 0.f ? 0.f : o[0][n][f][i & 1][i >> 1] / total[n]);
         __builtin_memcpy(to_o + 32 * f + 8 * g, v, sizeof(v));
       }
     }

@@ -53,18 +53,18 @@ def bound(q, out, mag, big, lengths):
     """What the kernel's roundings may add up to, from the oracle's outputs, the magnitudes of their terms
     and of their scores'.
 
-    A matrix product of codes is off by 2^-20 of its terms' magnitudes at most for 16-bit queries and
-    2^-22 for float32 (the largest measured on random operands is 7.5e-7 and 1.9e-7), a float32 query by
-    2^-22 in its two fp16 parts; a score takes two more float32 roundings and the exponent's argument (the
-    score and 31 at most) two, the exponential one. d, of a weight, counts in numerator and denominator.
+    A matrix product of codes is off by 2^-20 of its terms' magnitudes at most where they are subnormal
+    (keys, 16-bit queries) and 2^-22 elsewhere (the largest measured on random operands is 7.5e-7 and
+    1.9e-7), a float32 query by 2^-22 in its two fp16 parts; a score takes two more float32 roundings and
+    the exponent's argument two, the exponential one. d, of a weight, counts in numerator and denominator.
     A weight's rounding to fp16 is half a step, 2^-11 (2^-22 in two parts). Sums over a lane's 16 tokens a
     step, over steps, waves and parts: a float32 rounding each. The division and the output's rounding."""
     few = q.dtype != torch.float32
     product = 2.0 ** -20 if few else 2.0 ** -22
-    d = big * (product + (0 if few else 2.0 ** -22) + 2 * U) + (2 * big + 31) * 2 * U + 2 * U
+    d = big * (product + (0 if few else 2.0 ** -22) + 2 * U) + 2 * big * 2 * U + 2 * U
     steps = max(lengths) / 64 + 16 + 70
     weight = 2.0 ** -11 if q.dtype == torch.bfloat16 else 2.0 ** -22
-    rel = 2 * d[..., None] + weight + product + 2 * steps * U
+    rel = 2 * d[..., None] + weight + 2.0 ** -22 + 2 * steps * U
     tiny = 2.0 ** -25 if q.dtype == torch.float16 else 0.0   # half a subnormal step
     return (HALF_STEP[q.dtype] + 2 * U) * (out.abs() + rel * mag) + rel * mag + tiny
 
