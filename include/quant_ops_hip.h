@@ -597,8 +597,8 @@ int qo_kv4_attention(const qo_kv4_cache* cache, const qo_heads* q, int dtype, in
                      const int32_t* page_table, int64_t table_ld, int64_t table_width, const int32_t* lengths,
                      const int32_t* q_starts, int64_t sequences, float scale, int64_t window, void* out,
                      void* workspace, int64_t workspace_bytes, void* stream);
-int64_t qo_kv4_attention_workspace_size(const qo_kv4_cache* cache, int64_t tokens, int q_heads, int64_t table_width,
-                                        int64_t sequences, int has_starts, int64_t window);
+int64_t qo_kv4_attention_workspace_size(const qo_kv4_cache* cache, int dtype, int64_t tokens, int q_heads,
+                                        int64_t table_width, int64_t sequences, int has_starts, int64_t window);
 
 #ifdef __cplusplus
 }

@@ -149,7 +149,7 @@ def lib():
     L.qo_kv4_attention.argtypes = [c_cache, c_heads, c_int, c_i64, c_int, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_f, c_i64,
                                    c_vp, c_vp, c_i64, c_vp]
     L.qo_kv4_attention_workspace_size.restype = c_i64
-    L.qo_kv4_attention_workspace_size.argtypes = [c_cache, c_i64, c_int, c_i64, c_i64, c_int, c_i64]
+    L.qo_kv4_attention_workspace_size.argtypes = [c_cache, c_int, c_i64, c_int, c_i64, c_i64, c_int, c_i64]
     _lib = L
     return L
 
@@ -609,9 +609,9 @@ def kv4_read(cache, slots, out_dtype=torch.float32, stream=None):
     return k, v
 
 
-def kv4_attention_workspace_size(cache, tokens, q_heads, table_width, sequences, has_starts=False, window=0):
+def kv4_attention_workspace_size(cache, dtype, tokens, q_heads, table_width, sequences, has_starts=False, window=0):
     """``qo_kv4_attention_workspace_size``."""
-    return int(lib().qo_kv4_attention_workspace_size(ctypes.byref(kv4_struct(cache)), tokens, q_heads, table_width, sequences,
+    return int(lib().qo_kv4_attention_workspace_size(ctypes.byref(kv4_struct(cache)), _TORCH_CODE[dtype], tokens, q_heads, table_width, sequences,
                                                      int(has_starts), window))
 
 
@@ -620,7 +620,7 @@ def kv4_attention(q, cache, page_table, lengths, scale, q_starts=None, window=0,
     q, page_table, lengths = _unit_rows(q), _unit_rows(page_table), lengths.contiguous()
     batch, width = page_table.shape
     if workspace is True:
-        need = kv4_attention_workspace_size(cache, q.shape[0], q.shape[1], width, batch, q_starts is not None, window)
+        need = kv4_attention_workspace_size(cache, q.dtype, q.shape[0], q.shape[1], width, batch, q_starts is not None, window)
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     if out is None:
         out = torch.empty(tuple(q.shape), dtype=q.dtype, device=q.device)

@@ -165,10 +165,10 @@ struct Kv4Plan {
   int splits;
 };
 inline Kv4Plan kv4_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t capacity,
-                        int64_t sequences, bool ragged, int64_t window, int64_t cus) {
+                        int64_t sequences, bool ragged, int64_t window, bool f32, int64_t cus) {
   const int64_t group = q_heads / kv_heads, rows = tokens * group;
   const int64_t each = sequences > 0 ? (rows + sequences - 1) / sequences : 0;
-  Kv4Plan p = {head_dim <= 128 && each > 16 ? 2 : 1, 0, 1};
+  Kv4Plan p = {head_dim <= 128 && !f32 && each > 16 ? 2 : 1, 0, 1};
   const int64_t tile = 64 * p.row_blocks;
   p.tiles = ragged ? rows / tile + sequences + 1 : sequences * ((each + tile - 1) / tile);
   // a split's share of the longest sequence is 256 tokens at least

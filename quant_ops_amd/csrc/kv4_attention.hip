@@ -42,6 +42,7 @@ typedef unsigned v2u __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.44269504f;
 constexpr float kInf = __builtin_inff();
+constexpr int kMostTokens = 0x7FFFFF00;   // of a sequence: positions and steps take 32 bits
 
 struct Attention {
   KV4 cache;
@@ -62,52 +63,58 @@ struct Attention {
   float* part;                // [splits][tokens * q_heads][DIM], then [splits][tokens * q_heads][2]
 };
 
-// Reductions over the four lane groups (lanes r, r + 16, r + 32, r + 48).
 __device__ inline float bits_float(uint32_t u) { return __builtin_bit_cast(float, u); }
+__device__ inline uint32_t float_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
+
+// Reductions over the four lane groups (lanes r, r + 16, r + 32, r + 48).
 template <class F>
-__device__ inline float groups_reduce(float v, F&& f) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+__device__ inline uint32_t groups_reduce(uint32_t u, F&& f) {
   const v2u a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  const float w = f(bits_float(a[0]), bits_float(a[1]));
-  const uint32_t x = __builtin_bit_cast(uint32_t, w);
-  const v2u b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-  return f(bits_float(b[0]), bits_float(b[1]));
+  const uint32_t w = f(a[0], a[1]);
+  const v2u b = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+  return f(b[0], b[1]);
 }
 __device__ inline float groups_max(float v) {
-  return groups_reduce(v, [](float a, float b) { return fmaxf(a, b); });
+  return bits_float(groups_reduce(float_bits(v), [](uint32_t a, uint32_t b) { return float_bits(fmaxf(bits_float(a), bits_float(b))); }));
 }
 __device__ inline float groups_sum(float v) {
-  return groups_reduce(v, [](float a, float b) { return a + b; });
+  return bits_float(groups_reduce(float_bits(v), [](uint32_t a, uint32_t b) { return float_bits(bits_float(a) + bits_float(b)); }));
 }
 
 // Codes less 8 as fp16 (those at bits 4 .. 7 times 16): with the exponent of 1024 in front, an
 // fp16's lowest bits count in ones.
 constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;
-__device__ inline uint32_t less(uint32_t two, _Float16 n) {
-  const v2h v = __builtin_bit_cast(v2h, two | 0x64006400u) - (v2h){n, n};
+__device__ inline uint32_t less(uint32_t w, uint32_t mask, uint32_t exponents, _Float16 n) {
+  const v2h v = __builtin_bit_cast(v2h, (w & mask) | exponents) - (v2h){n, n};
   return __builtin_bit_cast(uint32_t, v);
 }
-__device__ inline uint32_t less_low(uint32_t w) { return less(w & kLow, (_Float16)1032.f); }
-__device__ inline uint32_t less_high(uint32_t w) { return less(w & kHigh, (_Float16)1152.f); }
+// The exponents in a vector register: a mask and they are then one instruction's operands.
+__device__ inline uint32_t exponents_of_1024() {
+  uint32_t e = 0x64006400u;
+  asm("" : "+v"(e));
+  return e;
+}
+__device__ inline uint32_t less_low(uint32_t w, uint32_t e) { return less(w, kLow, e, (_Float16)1032.f); }
+__device__ inline uint32_t less_high(uint32_t w, uint32_t e) { return less(w, kHigh, e, (_Float16)1152.f); }
 
 // The eight codes of a key's word in the order 0, 4, 1, 5, 2, 6, 3, 7: even ones times kEven, odd ones
 // times kOdd, all less kLess.
 template <bool FINE>
 struct Codes {
   static constexpr float kEven = FINE ? 1.f : 0x1p-24f, kOdd = 16.f * kEven, kLess = FINE ? 8.f : 0.f;
-  __device__ static inline v8h of(uint32_t w) {
+  __device__ static inline v8h of(uint32_t w, uint32_t e) {
     const uint32_t h = w >> 8;
-    if constexpr (FINE) return __builtin_bit_cast(v8h, (v4u){less_low(w), less_high(w), less_low(h), less_high(h)});
+    if constexpr (FINE) return __builtin_bit_cast(v8h, (v4u){less_low(w, e), less_high(w, e), less_low(h, e), less_high(h, e)});
     else return __builtin_bit_cast(v8h, (v4u){w & kLow, w & kHigh, h & kLow, h & kHigh});
   }
 };
 
 // The low (odd: high) halves of eight bytes of values, in the order 0, 2, 1, 3, 4, 6, 5, 7.
-__device__ inline v8h values_even(uint32_t a, uint32_t b) {
-  return __builtin_bit_cast(v8h, (v4u){less_low(a), less_low(a >> 8), less_low(b), less_low(b >> 8)});
+__device__ inline v8h values_even(uint32_t a, uint32_t b, uint32_t e) {
+  return __builtin_bit_cast(v8h, (v4u){less_low(a, e), less_low(a >> 8, e), less_low(b, e), less_low(b >> 8, e)});
 }
-__device__ inline v8h values_odd(uint32_t a, uint32_t b) {
-  return __builtin_bit_cast(v8h, (v4u){less_high(a), less_high(a >> 8), less_high(b), less_high(b >> 8)});
+__device__ inline v8h values_odd(uint32_t a, uint32_t b, uint32_t e) {
+  return __builtin_bit_cast(v8h, (v4u){less_high(a, e), less_high(a >> 8, e), less_high(b, e), less_high(b >> 8, e)});
 }
 
 __device__ inline uint32_t pk_max_u16(uint32_t a, uint32_t b) {
@@ -115,26 +122,33 @@ __device__ inline uint32_t pk_max_u16(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2u16, a), __builtin_bit_cast(v2u16, b)));
 }
 
+// A page of one head: where it starts, and the bytes from page to page (below 2^32: the host's check).
+struct Pages {
+  const uint8_t* k;
+  const uint8_t* v;
+  const uint8_t* params;   // of keys; those of values stand param_values further
+  uint32_t codes, param_bytes, param_values;
+};
+
 // Where a tile of 16 tokens stands: its page (0 for one outside the cache) and the place of its first token.
 struct Tile {
-  int64_t page;
-  int place;
+  int page, place;
   bool bad;
 };
-__device__ inline Tile tile_at(const Attention& a, const int32_t* table, int64_t t) {
-  const int64_t at = t >> a.cache.shift;
-  const int64_t page = at < a.width ? table[at] : 0;   // beyond: past the tokens, masked
-  const bool bad = page < 0 || page >= a.cache.pages;
-  return {bad ? 0 : page, (int)(t & ((1 << a.cache.shift) - 1)), bad};
+__device__ inline Tile tile_at(const Attention& a, const int32_t* table, int t) {
+  const int at = t >> a.cache.shift;
+  const int page = at < (int)a.width ? table[at] : 0;   // beyond: past the tokens, masked
+  const bool bad = page < 0 || page >= (int)a.cache.pages;
+  return {bad ? 0 : page, t & ((1 << a.cache.shift) - 1), bad};
 }
 
-// One row's end: the token after the last that it sees, and the first.
+// The first token that a row sees and the one after the last.
 struct Sees {
-  int64_t first, last;
+  int first, last;
 };
 
 template <class D, int DIM, int NB, int NQ, int NP, bool FINE>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, DIM <= 128 && NB == 1 && !FINE ? 2 : 1)
 kv4_attention_kernel(Attention a) {
   constexpr int NS = DIM / 32;        // k-steps of a score, words of a key's codes in a lane
   constexpr int NF = DIM / 32;        // blocks of 16 pairs of values
@@ -143,48 +157,44 @@ kv4_attention_kernel(Attention a) {
   using C = Codes<FINE>;
   using T = typename D::T;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const int heads = a.cache.heads;
-  int64_t block = blockIdx.x;
-  const int head = (int)(block % heads);
-  block /= heads;
-  const int64_t tile = block % a.tiles;
-  const int split = (int)(block / a.tiles);
+  const int heads = a.cache.heads, tokens = (int)a.tokens, sequences = (int)a.sequences;
+  const int head = blockIdx.x % heads, tile = blockIdx.x / heads % (int)a.tiles, split = blockIdx.x / heads / (int)a.tiles;
 
   // The tile's sequence, its queries and the tile's first row. Tiles of ragged sequences are
   // counted from q_starts[b] * group / TILE + b on, which leaves room for every one's last.
-  int64_t b, start, count, row0;
-  auto begin_of = [&](int64_t i) {   // i >= 0; sequence 0 starts at 0, the rows behind the last are one more
-    const int64_t s = i == 0 ? 0 : (int64_t)a.q_starts[i];
-    return s < 0 ? 0 : s > a.tokens ? a.tokens : s;
+  int b, start, count, row0;
+  auto begin_of = [&](int i) {   // sequence 0 starts at 0, the rows behind the last are one more
+    const int s = i == 0 ? 0 : a.q_starts[i];
+    return s < 0 ? 0 : s > tokens ? tokens : s;
   };
   if (a.q_starts) {
-    int64_t n = 0;
-    for (int64_t base = 0; base <= a.sequences; base += 64) {
-      const int64_t i = base + lane;
-      const bool before = i <= a.sequences && begin_of(i) * a.group / TILE + i <= tile;
+    int n = 0;
+    for (int base = 0; base <= sequences; base += 64) {
+      const int i = base + lane;
+      const bool before = i <= sequences && begin_of(i) * a.group / TILE + i <= tile;
       const int got = __popcll(__ballot(before));
       n += got;
       if (got < 64) break;
     }
     b = n - 1;
     start = begin_of(b);
-    const int64_t end = b < a.sequences ? begin_of(b + 1) : a.tokens;
+    const int end = b < sequences ? begin_of(b + 1) : tokens;
     count = end > start ? end - start : 0;
     row0 = (tile - (start * a.group / TILE + b)) * TILE;
   } else {
-    const int64_t per = (a.each * a.group + TILE - 1) / TILE;
+    const int per = ((int)a.each * a.group + TILE - 1) / TILE;
     b = tile / per;
-    start = b * a.each;
-    count = a.each;
-    row0 = (tile % per) * TILE;
+    start = b * (int)a.each;
+    count = (int)a.each;
+    row0 = tile % per * TILE;
   }
-  const int64_t all = count * a.group;
+  const int all = count * a.group;
   if (row0 < 0 || row0 >= all) return;   // below 0: q_starts that do not ascend
-  const int rows = (int)(all - row0 < TILE ? all - row0 : TILE);
+  const int rows = all - row0 < TILE ? all - row0 : TILE;
 
-  const int64_t capacity = a.width << a.cache.shift;
-  int64_t length = b < a.sequences ? a.lengths[b] : 0;
-  const bool poison = length > capacity;
+  int length = b < sequences ? a.lengths[b] : 0;
+  const bool poison = length > kMostTokens || (length >> a.cache.shift) > a.width ||
+                      ((length >> a.cache.shift) == a.width && (length & ((1 << a.cache.shift) - 1)));
   if (length < 0 || poison) length = 0;
 
   // The waves' rows; waves with the same rows take turns at their tokens.
@@ -192,29 +202,29 @@ kv4_attention_kernel(Attention a) {
   const int sharing = blocks == 1 ? 4 : blocks == 2 ? 2 : 1;
   const int mine = wave / sharing, turn_of = wave % sharing;
   const bool active = mine < blocks;
-  const int64_t first_row = row0 + (active ? mine : 0) * ROWS;
-  const int64_t last_row = first_row + ROWS < row0 + rows ? first_row + ROWS - 1 : row0 + rows - 1;
-  auto sees = [&](int64_t row) {
-    const int64_t p = length - count + row / a.group;
-    const int64_t first = a.window && p + 1 > a.window ? p + 1 - a.window : 0;
-    return Sees{first, length ? (p + 1 > 0 ? p + 1 : 0) : 0};
+  const int first_row = row0 + (active ? mine : 0) * ROWS;
+  const int last_row = first_row + ROWS < row0 + rows ? first_row + ROWS - 1 : row0 + rows - 1;
+  const int window = a.window && a.window < kMostTokens ? (int)a.window : 0;
+  auto sees = [&](int row) {
+    const int p = length - count + row / a.group;
+    return Sees{window && p + 1 > window ? p + 1 - window : 0, length && p >= 0 ? p + 1 : 0};
   };
   const Sees top = sees(first_row), bottom = sees(last_row);
-
-  const int64_t row_of_lane[2] = {first_row + r <= last_row ? first_row + r : last_row,
-                                  first_row + 16 + r <= last_row ? first_row + 16 + r : last_row};
+  int row_of[NB];
   Sees see[NB];
 #pragma unroll
-  for (int n = 0; n < NB; ++n) see[n] = sees(row_of_lane[n]);
+  for (int n = 0; n < NB; ++n) {
+    row_of[n] = first_row + 16 * n + r <= last_row ? first_row + 16 * n + r : last_row;
+    see[n] = sees(row_of[n]);
+  }
 
   // Queries as fp16 parts in the order of Codes::of, the odd codes' factor taken out.
   v8h qf[NQ][NB][NS];
   float factor[NB], qsum[NB];   // of the exponent of two; sum of a query, in units of its scores
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    const int64_t row = row_of_lane[n];
-    const T* q = reinterpret_cast<const T*>(a.q) + (start + row / a.group) * a.q_token +
-                 (head * a.group + row % a.group) * a.q_head;
+    const T* q = reinterpret_cast<const T*>(a.q) + (start + row_of[n] / a.group) * a.q_token +
+                 (head * a.group + row_of[n] % a.group) * a.q_head;
     float x[NS][8], most = 0.f;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
@@ -257,74 +267,78 @@ kv4_attention_kernel(Attention a) {
   }
   int scale_exp = -14;
 
-  const int64_t begin = top.first & ~(int64_t)63;
-  const int64_t steps = bottom.last > begin ? (bottom.last - begin + 63) / 64 : 0;
-  const int64_t per_split = (steps + a.splits - 1) / a.splits;
-  const int64_t to = (split + 1) * per_split < steps ? (split + 1) * per_split : steps;
-  const int32_t* table = a.table + (b < a.sequences ? b : 0) * a.table_ld;
-  for (int64_t step = split * per_split + turn_of; active && step < to; step += sharing) {
-    const int64_t t0 = begin + 64 * step;
+  const int begin = top.first & ~63;
+  const int steps = bottom.last > begin ? (bottom.last - begin + 63) / 64 : 0;
+  const int per_split = (steps + a.splits - 1) / a.splits;
+  const int to = (split + 1) * per_split < steps ? (split + 1) * per_split : steps;
+  const int32_t* table = a.table + (b < sequences ? b : 0) * a.table_ld;
+  Pages pages;
+  {
+    const int shift = a.cache.shift;
+    pages.codes = (uint32_t)(heads << shift) * (DIM / 2);
+    pages.param_values = (uint32_t)(heads << (shift - 4)) * 64;
+    pages.param_bytes = 2 * pages.param_values;
+    pages.k = a.cache.k + ((int64_t)head << shift) * (DIM / 2);
+    pages.v = a.cache.v + ((int64_t)head << shift) * (DIM / 2);
+    pages.params = reinterpret_cast<const uint8_t*>(a.cache.params) + ((int64_t)head << (shift - 4)) * 64;
+  }
+
+  // A step's loads go out a step ahead: its pages two, its keys as soon as the scores of the step
+  // before are made, its values after that step's second product.
+  uint32_t kw[4][NS];
+  v4u vw[NF], kpar[4], vpar[4];   // codes; scales (two words of eight) and minima
+  Tile kt, vt;
+  bool bad = false;               // the lane's tokens (16 g ..) stand on a page outside the cache
+  auto find = [&](int step) {
     // keys: lane row r reads token 16 (r / 4) + 4 u + r % 4 of tile u, its words of group g
-    const Tile kt = tile_at(a, table, t0 + 16 * (r >> 2)), vt = tile_at(a, table, t0 + 16 * g);
-    const uint8_t* kp = a.cache.key(kt.page, head, kt.place + (r & 3), DIM) + g * (4 * NS);
-    const uint8_t* vp = a.cache.value_tile(vt.page, head, vt.place, DIM) + r * 16;
-    uint32_t kw[4][NS];
-    v4u vw[NF];
-    v4u kpar[4], vpar[4];   // scales (two words of eight), minima
+    kt = tile_at(a, table, begin + 64 * step + 16 * (r >> 2));
+    vt = tile_at(a, table, begin + 64 * step + 16 * g);
+  };
+  auto load_keys = [&] {
+    const uint8_t* p = pages.k + (uint64_t)(uint32_t)kt.page * pages.codes + ((kt.place + (r & 3)) * (DIM / 2) + g * (4 * NS));
+    const v4u* par = reinterpret_cast<const v4u*>(pages.params + (uint64_t)(uint32_t)vt.page * pages.param_bytes + vt.place * 4);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) __builtin_memcpy(kw[u], kp + u * 4 * (DIM / 2), sizeof(kw[u]));
-    const v4u* pk = reinterpret_cast<const v4u*>(a.cache.param_tile(vt.page, 0, head, vt.place));
-    const v4u* pv = reinterpret_cast<const v4u*>(a.cache.param_tile(vt.page, 1, head, vt.place));
+    for (int u = 0; u < 4; ++u) __builtin_memcpy(kw[u], p + u * 4 * (DIM / 2), sizeof(kw[u]));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) kpar[i] = pk[i], vpar[i] = pv[i];
+    for (int i = 0; i < 4; ++i) kpar[i] = par[i];
+  };
+  auto load_values = [&] {
+    const uint8_t* p = pages.v + (uint64_t)(uint32_t)vt.page * pages.codes + (vt.place * (DIM / 2) + r * 16);
+    const v4u* par = reinterpret_cast<const v4u*>(pages.params + (uint64_t)(uint32_t)vt.page * pages.param_bytes + pages.param_values +
+                                                  vt.place * 4);
 #pragma unroll
-    for (int f = 0; f < NF; ++f) vw[f] = *reinterpret_cast<const v4u*>(vp + f * 256);
+    for (int i = 0; i < 4; ++i) vpar[i] = par[i];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) vw[f] = *reinterpret_cast<const v4u*>(p + f * 256);
+  };
+  auto half_of = [](const v4u* par, int t) {   // t of 16 scales (from word 4 on: minima)
+    const uint32_t w = par[t / 8][t % 8 / 2];
+    return (float)__builtin_bit_cast(v2h, w)[t & 1];
+  };
+  const uint32_t exponents = exponents_of_1024();
 
-    const bool whole = t0 + 64 <= top.last && t0 >= bottom.first && !__any(vt.bad);
-    _Float16 ks[16], kl[16], vs[16], vl[16];
-    __builtin_memcpy(ks, kpar, 32);
-    __builtin_memcpy(kl, kpar + 2, 32);
-    __builtin_memcpy(vs, vpar, 32);
-    __builtin_memcpy(vl, vpar + 2, 32);
-    if (!whole) {
-      // tokens that no row sees may hold anything; those on a bad page are NaN
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int64_t t = t0 + 16 * g + i;
-        const bool seen = t >= top.first && t < bottom.last;
-        const _Float16 nan = (_Float16)__builtin_nanf(""), zero = (_Float16)0.f;
-        ks[i] = !seen ? zero : vt.bad ? nan : ks[i];
-        kl[i] = !seen ? zero : vt.bad ? nan : kl[i];
-        vs[i] = !seen ? zero : vt.bad ? nan : vs[i];
-        vl[i] = !seen ? zero : vt.bad ? nan : vl[i];
-      }
-    }
-    uint32_t big = 0;
-#pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-      uint32_t two;
-      __builtin_memcpy(&two, vs + i, 4);
-      big = pk_max_u16(big, two & 0x7FFF7FFFu);
-    }
-    // the exponent of the largest scale, over the step's tokens (as bits, which order like it)
-    const uint32_t field = (uint32_t)groups_max((float)(max(big & 0xFFFFu, big >> 16) >> 10));
-    const int exp_now = max(scale_exp, __builtin_amdgcn_readfirstlane((int)field) - 14);
-
-    float key_base[16], middle[16], scale[16];   // what codes kLess (of a key) and 8 stand for; s 2^15 / S
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      key_base[i] = fmaf(C::kLess, (float)ks[i], (float)kl[i]);
-      middle[i] = fmaf(8.f, (float)vs[i], (float)vl[i]);
-      scale[i] = (float)vs[i] * bits_float((uint32_t)(127 + 15 - exp_now) << 23);
-    }
-    v4f sc[NB][4], rest[NB];
+  const int first_step = split * per_split + turn_of;
+  if (active && first_step < to) {
+    find(first_step);
+    bad = vt.bad;
+    load_keys();
+    load_values();
+    find(first_step + sharing);
+  }
+  for (int step = first_step; active && step < to; step += sharing) {
+    const int t0 = begin + 64 * step;
+    const bool more = step + sharing < to;
+    const bool whole = t0 + 64 <= top.last && t0 >= bottom.first && !__any(bad);
+    // scores
+    v4f sc[NB][4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
+      v4f rest[NB];
 #pragma unroll
       for (int n = 0; n < NB; ++n) sc[n][u] = rest[n] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        const v8h c = C::of(kw[u][s]);
+        const v8h c = C::of(kw[u][s], exponents);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           sc[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, qf[0][n][s], sc[n][u], 0, 0, 0);
@@ -338,22 +352,53 @@ kv4_attention_kernel(Attention a) {
           for (int i = 0; i < 4; ++i) sc[n][u][i] += rest[n][i];
       }
     }
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int t = 0; t < 16; ++t) {
+        const float ks = half_of(kpar, t), kl = half_of(kpar + 2, t);
+        sc[n][t / 4][t % 4] = fmaf(ks, sc[n][t / 4][t % 4], fmaf(C::kLess, ks, kl) * qsum[n]);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    const bool bad_now = bad;
+    if (more) {
+      bad = vt.bad;
+      load_keys();
+    }
+    if (!whole) {
+      // Tokens that a row does not see get no weight, whatever stands there. A NaN (or a page outside the
+      // cache) that it sees makes its sum NaN; a value's parameters are then 0, for the rows that do not.
+#pragma unroll
+      for (int t = 0; t < 16; ++t) {
+        const int at_t = t0 + 16 * g + t;
+        const float vs = half_of(vpar, t), vl = half_of(vpar + 2, t);
+        const bool finite = fabsf(vs) < kInf && fabsf(vl) < kInf && !bad_now, any = at_t >= top.first && at_t < bottom.last;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          const bool seen = at_t >= see[n].first && at_t < see[n].last;
+          sc[n][t / 4][t % 4] = seen ? sc[n][t / 4][t % 4] : -kInf;
+          if (seen && !finite) total[n] = __builtin_nanf("");
+        }
+        if (!finite || !any) {
+          const uint32_t keep = t & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+          vpar[t / 8][t % 8 / 2] &= keep;
+          vpar[2 + t / 8][t % 8 / 2] &= keep;
+        }
+      }
+    }
+    // the exponent of the largest scale, over the step's tokens (as bits, which order like it)
+    uint32_t big = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) big = pk_max_u16(big, vpar[i / 4][i % 4] & 0x7FFF7FFFu);
+    const uint32_t field = groups_reduce(max(big & 0xFFFFu, big >> 16) >> 10, [](uint32_t x, uint32_t y) { return max(x, y); });
+    const int exp_now = max(scale_exp, __builtin_amdgcn_readfirstlane((int)field) - 14);
+    const float to_scale = bits_float((uint32_t)(127 + 15 - exp_now) << 23);
     v8h ph[NB][2], pl[NB][2];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
       float now = most[n];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float y = fmaf((float)ks[4 * u + i], sc[n][u][i], key_base[4 * u + i] * qsum[n]);
-          if (!whole) {
-            const int64_t t = t0 + 16 * g + 4 * u + i;
-            if (t >= see[n].last || t < see[n].first) y = -kInf;
-          }
-          sc[n][u][i] = y;
-          now = fmaxf(now, y);
-        }
+      for (int t = 0; t < 16; ++t) now = fmaxf(now, sc[n][t / 4][t % 4]);
       now = groups_max(now);
       if (__any(now > most[n]) || exp_now > scale_exp) {
         const float next = now == -kInf ? 0.f : factor[n] * now;
@@ -374,33 +419,32 @@ kv4_attention_kernel(Attention a) {
             }
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // tokens 8 z .. 8 z + 7 of the lane in the order of Codes::even
-          constexpr int kSlot[4] = {0, 2, 1, 3};
-          const int z = u >> 1, j = 4 * (u & 1) + kSlot[i];
-          const float p = __builtin_amdgcn_exp2f(fmaf(factor[n], sc[n][u][i], -at[n]));
-          float s = scale[4 * u + i], mid = middle[4 * u + i];
-          if (!whole && sc[n][u][i] == -kInf) s = mid = 0.f;   // a masked token's NaN stays out
-          total[n] += p;
-          middles[n] = fmaf(p, mid, middles[n]);
-          _Float16 h = (_Float16)(p * s);
-          if constexpr (NP > 1) {
-            // one and the same rounding in both parts: the product rounded twice (to float32 first)
-            // or once differ by a step of h where it is next to a tie
-            asm("" : "+v"(h));
-            pl[n][z][j] = (_Float16)fmaf(p, s, -(float)h);
-          }
-          ph[n][z][j] = h;
+      for (int t = 0; t < 16; ++t) {
+        // tokens 8 z .. 8 z + 7 of the lane in the order of values_even
+        constexpr int kSlot[4] = {0, 2, 1, 3};
+        const int z = t / 8, j = 4 * (t / 4 & 1) + kSlot[t % 4];
+        const float vs = half_of(vpar, t), vl = half_of(vpar + 2, t);
+        const float p = __builtin_amdgcn_exp2f(fmaf(factor[n], sc[n][t / 4][t % 4], -at[n]));
+        const float s = vs * to_scale;   // s 2^15 / S
+        total[n] += p;
+        middles[n] = fmaf(p, fmaf(8.f, vs, vl), middles[n]);
+        _Float16 h = (_Float16)(p * s);
+        if constexpr (NP > 1) {
+          // one and the same rounding in both parts: the product rounded twice (to float32 first)
+          // or once differ by a step of h where it is next to a tie
+          asm("" : "+v"(h));
+          pl[n][z][j] = (_Float16)fmaf(p, s, -(float)h);
         }
+        ph[n][z][j] = h;
+      }
     }
     scale_exp = exp_now;
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int f = 0; f < NF; ++f)
 #pragma unroll
       for (int z = 0; z < 2; ++z) {
-        const v8h even = values_even(vw[f][2 * z], vw[f][2 * z + 1]), odd = values_odd(vw[f][2 * z], vw[f][2 * z + 1]);
+        const v8h even = values_even(vw[f][2 * z], vw[f][2 * z + 1], exponents), odd = values_odd(vw[f][2 * z], vw[f][2 * z + 1], exponents);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           v4f(&hi)[2] = o[0][n][f], (&lo)[2] = o[APART][n][f];
@@ -412,6 +456,11 @@ kv4_attention_kernel(Attention a) {
           }
         }
       }
+    __builtin_amdgcn_sched_barrier(0);
+    if (more) {
+      load_values();
+      find(step + 2 * sharing);
+    }
   }
 
   const float unit = bits_float((uint32_t)(127 - 15 + scale_exp) << 23);
@@ -468,12 +517,12 @@ kv4_attention_kernel(Attention a) {
     __syncthreads();
   }
   if (!active || turn_of) return;
-  const int64_t total_rows = a.tokens * a.q_heads;
+  const int64_t total_rows = a.tokens * a.q_heads;   // of all heads
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    const int64_t row = first_row + 16 * n + r;
+    const int row = first_row + 16 * n + r;
     if (row > last_row) continue;
-    const int64_t at_row = (start + row / a.group) * a.q_heads + head * a.group + row % a.group;
+    const int64_t at_row = (int64_t)(start + row / a.group) * a.q_heads + head * a.group + row % a.group;
     if (a.splits > 1) {
       const int64_t slot = split * total_rows + at_row;
       float* to_o = a.part + slot * DIM;
@@ -542,13 +591,13 @@ void with_dim(int dim, F&& f) {
 
 }  // namespace qo
 
-extern "C" int64_t qo_kv4_attention_workspace_size(const qo_kv4_cache* cache, int64_t tokens, int q_heads,
+extern "C" int64_t qo_kv4_attention_workspace_size(const qo_kv4_cache* cache, int dtype, int64_t tokens, int q_heads,
                                                    int64_t table_width, int64_t sequences, int has_starts,
                                                    int64_t window) {
   using namespace qo;
   if (!cache || cache->kv_heads < 1 || tokens < 1 || q_heads < cache->kv_heads || sequences < 1) return 0;
   const Kv4Plan p = kv4_plan(tokens, q_heads, cache->kv_heads, cache->head_dim, table_width * cache->page_size,
-                             sequences, has_starts != 0, window, device_cu_count());
+                             sequences, has_starts != 0, window, dtype == QO_DTYPE_F32, device_cu_count());
   return p.splits > 1 ? p.splits * tokens * q_heads * (cache->head_dim + 2) * 4 : 0;
 }
 
@@ -594,13 +643,18 @@ extern "C" int qo_kv4_attention(const qo_kv4_cache* cache, const qo_heads* q, in
     return QO_ERR_ALIGNMENT;
   }
   Kv4Plan plan = kv4_plan(tokens, q_heads, c.heads, cache->head_dim, table_width * cache->page_size, sequences,
-                          q_starts != nullptr, window, device_cu_count());
+                          q_starts != nullptr, window, dtype == QO_DTYPE_F32, device_cu_count());
   if (plan.splits > 1 &&
       (!workspace || workspace_bytes < plan.splits * tokens * q_heads * (cache->head_dim + 2) * 4))
     plan.splits = 1;
   const int64_t grid = plan.tiles * c.heads * plan.splits;
-  if (grid > (1 << 24) - 1) {   // 256 threads each
-    qo_set_error("%s: too many rows for one call (%lld workgroups)", fn, (long long)grid);
+  // rows of a KV head, workgroups (256 threads each) and a page's bytes take 32 bits
+  if (tokens * (q_heads / c.heads) > (1 << 30) || grid > (1 << 24) - 1) {
+    qo_set_error("%s: too many rows for one call (%lld queries of %d heads)", fn, (long long)tokens, q_heads);
+    return QO_ERR_SHAPE;
+  }
+  if ((int64_t)c.heads * cache->page_size * cache->head_dim > INT32_MAX) {
+    qo_set_error("%s: pages of %d tokens of %d heads are too large", fn, (int)cache->page_size, c.heads);
     return QO_ERR_SHAPE;
   }
   Attention a = {c, q->data, q->token_stride, q->head_stride, out, page_table, table_ld, table_width, lengths, q_starts,
@@ -616,7 +670,7 @@ extern "C" int qo_kv4_attention(const qo_kv4_cache* cache, const qo_heads* q, in
       constexpr int DIM = decltype(dim)::value;
       hipStream_t s = reinterpret_cast<hipStream_t>(stream);
       if (plan.row_blocks == 1) launch(kv4_attention_kernel<D, DIM, 1, NQ, NP, FINE>, dim3((unsigned)grid), dim3(256), 0, s, a);
-      else if constexpr (DIM <= 128) launch(kv4_attention_kernel<D, DIM, 2, NQ, NP, FINE>, dim3((unsigned)grid), dim3(256), 0, s, a);
+      else if constexpr (DIM <= 128 && !FINE) launch(kv4_attention_kernel<D, DIM, 2, NQ, NP, FINE>, dim3((unsigned)grid), dim3(256), 0, s, a);
       if (plan.splits > 1) {
         const int64_t rows = tokens * q_heads;
         launch(kv4_attention_join<D, DIM>, dim3((unsigned)((rows * (DIM / 4) + 255) / 256)), dim3(256), 0, s,

@@ -557,7 +557,7 @@ at::Tensor kv4_attention(const at::Tensor& q, const at::Tensor& k_codes, const a
     starts = kv4_index(*q_starts, at::kInt, q, op, "q_starts");
   }
   at::Tensor out = at::detail::empty_cuda({T, H, c.head_dim}, q.scalar_type(), q.device(), std::nullopt);
-  const int64_t ws_bytes = qo_kv4_attention_workspace_size(&c, T, (int)H, W, B, starts.defined(), window);
+  const int64_t ws_bytes = qo_kv4_attention_workspace_size(&c, dtype_code(q.scalar_type()), T, (int)H, W, B, starts.defined(), window);
   at::Tensor ws = gemm_workspace(ws_bytes, q);
   const qo_heads hq = kv4_view(Q);
   check_status(qo_kv4_attention(&c, &hq, dtype_code(q.scalar_type()), T, (int)H, table.data_ptr<int32_t>(),

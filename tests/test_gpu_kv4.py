@@ -303,7 +303,7 @@ def test_split_and_whole_agree(gpu):
     for case in (([5000], 4, 1, 128, 64, 1, 0), ([3000, 10], 2, 2, 64, 16, [3, 1], 0)):
         q, cache, table, lengths, starts, window = (t.to(gpu) if torch.is_tensor(t) else t for t in make(case, torch.float32))
         cache = _to(cache, gpu)
-        need = capi.kv4_attention_workspace_size(cache, q.shape[0], q.shape[1], table.shape[1], table.shape[0], starts is not None)
+        need = capi.kv4_attention_workspace_size(cache, q.dtype, q.shape[0], q.shape[1], table.shape[1], table.shape[0], starts is not None)
         assert need > 0
         ws = torch.full((need,), 255, dtype=torch.uint8, device=gpu)
         a = capi.kv4_attention(q, cache, table, lengths, 0.1, q_starts=starts, workspace=ws)
