@@ -156,20 +156,20 @@ inline MxPlan mx_plan(int64_t M, int64_t N, int64_t blocks, bool fp8, int64_t cu
   return best;
 }
 
-// Rows and workgroups of attention over the 4-bit cache. A workgroup has four waves of 16
-// `row_blocks` rows (a row: a query of one of the heads that share a KV head); waves without rows
-// of their own share others' tokens, and `splits` workgroups do.
+// Rows and workgroups of attention over the 4-bit cache. A workgroup has four waves of `rows`
+// rows (a row: a query of one of the heads that share a KV head); waves without rows of their own
+// share others' tokens, and `splits` workgroups do.
 struct Kv4Plan {
-  int row_blocks;
-  int64_t tiles;   // of 64 row_blocks rows, of all sequences
+  int rows;        // 4, 8, 16 or 32
+  int64_t tiles;   // of 4 rows, of all sequences
   int splits;
 };
 inline Kv4Plan kv4_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t capacity,
                         int64_t sequences, bool ragged, int64_t window, bool f32, int64_t cus) {
   const int64_t group = q_heads / kv_heads, rows = tokens * group;
   const int64_t each = sequences > 0 ? (rows + sequences - 1) / sequences : 0;
-  Kv4Plan p = {head_dim <= 128 && !f32 && each > 16 ? 2 : 1, 0, 1};
-  const int64_t tile = 64 * p.row_blocks;
+  Kv4Plan p = {each <= 4 ? 4 : each <= 8 ? 8 : head_dim > 128 || f32 || each <= 16 ? 16 : 32, 0, 1};
+  const int64_t tile = 4 * p.rows;
   p.tiles = ragged ? rows / tile + sequences + 1 : sequences * ((each + tile - 1) / tile);
   // a split's share of the longest sequence is 256 tokens at least
   const int64_t queries = sequences > 0 ? (tokens + sequences - 1) / sequences : 0;

@@ -23,10 +23,14 @@
 // sign, at 33210 tokens), so their codes less 8 are normal numbers (nine instructions for eight),
 // and float32 queries have keys' codes as those too.
 //
+// Rows that are few (FOLD times 16 / FOLD of them) stand in every 16 / FOLD columns again, and the lanes
+// of those columns share a row's scores: each takes 16 / FOLD of its group's tokens from the scores
+// to the weights, which then go back to the first columns.
+//
 // Queries: brought by a power of two for each row to a largest magnitude in [2^14, 2^15), 16-bit
 // values are exact in fp16 (those below 2^-28 of the largest lose bits); float32 takes two fp16
-// parts (22 bits). Weights: p s 2^15 / S, where p is 1 at the row's largest score so far and S a
-// power of two that no scale of the tokens so far exceeds, is at most 2^15, and rounded to fp16 (half
+// parts (22 bits). Weights: p s 2^14 / S, where p is 1 at the row's largest score so far and S a
+// power of two that no scale of the tokens so far exceeds, is at most 2^14, and rounded to fp16 (half
 // a step 2^-12, beside bf16's 2^-9 of the output) or, for fp16 and float32, to two parts. In
 // float32 the second parts have sums of their own: added to the first parts' they would lose what is
 // below 2^-24 of those. Maximum, sums and outputs are float32.
@@ -73,6 +77,32 @@ __device__ inline uint32_t groups_reduce(uint32_t u, F&& f) {
   const uint32_t w = f(a[0], a[1]);
   const v2u b = __builtin_amdgcn_permlane16_swap(w, w, false, false);
   return f(b[0], b[1]);
+}
+// And over lanes r, r + CW, .. of a row of 16.
+template <int CW, class F>
+__device__ inline uint32_t row_reduce(uint32_t u, F&& f) {
+  if constexpr (CW <= 4) u = f(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x124, 0xF, 0xF, false));   // row_ror:4
+  if constexpr (CW <= 8) u = f(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x128, 0xF, 0xF, false));   // row_ror:8
+  return u;
+}
+template <int CW>
+__device__ inline float group_row_max(float v) {
+  auto f = [](uint32_t a, uint32_t b) { return float_bits(fmaxf(bits_float(a), bits_float(b))); };
+  return bits_float(groups_reduce(row_reduce<CW>(float_bits(v), f), f));
+}
+template <int CW>
+__device__ inline float group_row_sum(float v) {
+  auto f = [](uint32_t a, uint32_t b) { return float_bits(bits_float(a) + bits_float(b)); };
+  return bits_float(groups_reduce(row_reduce<CW>(float_bits(v), f), f));
+}
+// In lanes Q CW .. of a row of 16 the value that lane r - Q CW has, elsewhere old; and back.
+template <int CW, int Q>
+__device__ inline uint32_t to_lanes(uint32_t old, uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, 0x110 + CW * Q, 0xF, CW == 8 ? 0xC : 1 << Q, false);   // row_shr
+}
+template <int CW, int Q>
+__device__ inline uint32_t from_lanes(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x100 + CW * Q, 0xF, 0xF, true);   // row_shl
 }
 __device__ inline float groups_max(float v) {
   return bits_float(groups_reduce(float_bits(v), [](uint32_t a, uint32_t b) { return float_bits(fmaxf(bits_float(a), bits_float(b))); }));
@@ -147,12 +177,14 @@ struct Sees {
   int first, last;
 };
 
-template <class D, int DIM, int NB, int NQ, int NP, bool FINE>
+template <class D, int DIM, int NB, int FOLD, int NQ, int NP, bool FINE>
 __global__ void __launch_bounds__(256, DIM <= 128 && NB == 1 && !FINE ? 2 : 1)
 kv4_attention_kernel(Attention a) {
   constexpr int NS = DIM / 32;        // k-steps of a score, words of a key's codes in a lane
   constexpr int NF = DIM / 32;        // blocks of 16 pairs of values
-  constexpr int ROWS = 16 * NB, TILE = 4 * ROWS;
+  constexpr int CW = 16 / FOLD;       // columns with rows of their own, and tokens of a step for a lane's softmax
+  constexpr int ROWS = CW * NB, TILE = 4 * ROWS;
+  static_assert(NB == 1 || FOLD == 1, "more than 16 rows");
   constexpr int APART = FINE;         // second parts of weights have sums of their own
   using C = Codes<FINE>;
   using T = typename D::T;
@@ -214,7 +246,7 @@ kv4_attention_kernel(Attention a) {
   Sees see[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    row_of[n] = first_row + 16 * n + r <= last_row ? first_row + 16 * n + r : last_row;
+    row_of[n] = first_row + 16 * n + r % CW <= last_row ? first_row + 16 * n + r % CW : last_row;
     see[n] = sees(row_of[n]);
   }
 
@@ -285,10 +317,12 @@ kv4_attention_kernel(Attention a) {
 
   // A step's loads go out a step ahead: its pages two, its keys as soon as the scores of the step
   // before are made, its values after that step's second product.
-  uint32_t kw[4][NS];
-  v4u vw[NF], kpar[4], vpar[4];   // codes; scales (two words of eight) and minima
+  // The lane's tokens of a step, from the scores to the weights: 16 g + own ..; their parameters in pairs.
+  const int own = r / CW * CW;
+  uint32_t kw[4][NS], ks[CW / 2], kl[CW / 2], vs[CW / 2], vl[CW / 2];
+  v4u vw[NF];
   Tile kt, vt;
-  bool bad = false;               // the lane's tokens (16 g ..) stand on a page outside the cache
+  bool bad = false;               // the lane's tokens stand on a page outside the cache
   auto find = [&](int step) {
     // keys: lane row r reads token 16 (r / 4) + 4 u + r % 4 of tile u, its words of group g
     kt = tile_at(a, table, begin + 64 * step + 16 * (r >> 2));
@@ -296,23 +330,22 @@ kv4_attention_kernel(Attention a) {
   };
   auto load_keys = [&] {
     const uint8_t* p = pages.k + (uint64_t)(uint32_t)kt.page * pages.codes + ((kt.place + (r & 3)) * (DIM / 2) + g * (4 * NS));
-    const v4u* par = reinterpret_cast<const v4u*>(pages.params + (uint64_t)(uint32_t)vt.page * pages.param_bytes + vt.place * 4);
+    const uint8_t* par = pages.params + (uint64_t)(uint32_t)vt.page * pages.param_bytes + (vt.place * 4 + own * 2);
 #pragma unroll
     for (int u = 0; u < 4; ++u) __builtin_memcpy(kw[u], p + u * 4 * (DIM / 2), sizeof(kw[u]));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) kpar[i] = par[i];
+    __builtin_memcpy(ks, par, sizeof(ks));
+    __builtin_memcpy(kl, par + 32, sizeof(kl));
   };
   auto load_values = [&] {
     const uint8_t* p = pages.v + (uint64_t)(uint32_t)vt.page * pages.codes + (vt.place * (DIM / 2) + r * 16);
-    const v4u* par = reinterpret_cast<const v4u*>(pages.params + (uint64_t)(uint32_t)vt.page * pages.param_bytes + pages.param_values +
-                                                  vt.place * 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) vpar[i] = par[i];
+    const uint8_t* par = pages.params + (uint64_t)(uint32_t)vt.page * pages.param_bytes + pages.param_values + (vt.place * 4 + own * 2);
+    __builtin_memcpy(vs, par, sizeof(vs));
+    __builtin_memcpy(vl, par + 32, sizeof(vl));
 #pragma unroll
     for (int f = 0; f < NF; ++f) vw[f] = *reinterpret_cast<const v4u*>(p + f * 256);
   };
-  auto half_of = [](const v4u* par, int t) {   // t of 16 scales (from word 4 on: minima)
-    const uint32_t w = par[t / 8][t % 8 / 2];
+  auto half_of = [](const uint32_t* pairs, int t) {
+    const uint32_t w = pairs[t / 2];
     return (float)__builtin_bit_cast(v2h, w)[t & 1];
   };
   const uint32_t exponents = exponents_of_1024();
@@ -352,12 +385,21 @@ kv4_attention_kernel(Attention a) {
           for (int i = 0; i < 4; ++i) sc[n][u][i] += rest[n][i];
       }
     }
+    float x[NB][CW];   // of the lane's tokens
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int t = 0; t < 16; ++t) {
-        const float ks = half_of(kpar, t), kl = half_of(kpar + 2, t);
-        sc[n][t / 4][t % 4] = fmaf(ks, sc[n][t / 4][t % 4], fmaf(C::kLess, ks, kl) * qsum[n]);
+      for (int t = 0; t < CW; ++t) {
+        auto at_token = [&](int i) { return float_bits(sc[n][i / 4][i % 4]); };
+        uint32_t y = at_token(t);
+        if constexpr (FOLD == 2) y = to_lanes<CW, 1>(y, at_token(CW + t));
+        if constexpr (FOLD == 4) {
+          y = to_lanes<CW, 1>(y, at_token(CW + t));
+          y = to_lanes<CW, 2>(y, at_token(2 * CW + t));
+          y = to_lanes<CW, 3>(y, at_token(3 * CW + t));
+        }
+        const float s = half_of(ks, t), lo = half_of(kl, t);
+        x[n][t] = fmaf(s, bits_float(y), fmaf(C::kLess, s, lo) * qsum[n]);
       }
     __builtin_amdgcn_sched_barrier(0);
     const bool bad_now = bad;
@@ -369,37 +411,47 @@ kv4_attention_kernel(Attention a) {
       // Tokens that a row does not see get no weight, whatever stands there. A NaN (or a page outside the
       // cache) that it sees makes its sum NaN; a value's parameters are then 0, for the rows that do not.
 #pragma unroll
-      for (int t = 0; t < 16; ++t) {
-        const int at_t = t0 + 16 * g + t;
-        const float vs = half_of(vpar, t), vl = half_of(vpar + 2, t);
-        const bool finite = fabsf(vs) < kInf && fabsf(vl) < kInf && !bad_now, any = at_t >= top.first && at_t < bottom.last;
+      for (int t = 0; t < CW; ++t) {
+        const int at_t = t0 + 16 * g + own + t;
+        const bool finite = fabsf(half_of(vs, t)) < kInf && fabsf(half_of(vl, t)) < kInf && !bad_now;
+        const bool any = at_t >= top.first && at_t < bottom.last;
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           const bool seen = at_t >= see[n].first && at_t < see[n].last;
-          sc[n][t / 4][t % 4] = seen ? sc[n][t / 4][t % 4] : -kInf;
+          x[n][t] = seen ? x[n][t] : -kInf;
           if (seen && !finite) total[n] = __builtin_nanf("");
         }
         if (!finite || !any) {
           const uint32_t keep = t & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-          vpar[t / 8][t % 8 / 2] &= keep;
-          vpar[2 + t / 8][t % 8 / 2] &= keep;
+          vs[t / 2] &= keep;
+          vl[t / 2] &= keep;
         }
       }
     }
     // the exponent of the largest scale, over the step's tokens (as bits, which order like it)
     uint32_t big = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) big = pk_max_u16(big, vpar[i / 4][i % 4] & 0x7FFF7FFFu);
-    const uint32_t field = groups_reduce(max(big & 0xFFFFu, big >> 16) >> 10, [](uint32_t x, uint32_t y) { return max(x, y); });
+    for (int i = 0; i < CW / 2; ++i) big = pk_max_u16(big, vs[i] & 0x7FFF7FFFu);
+    auto larger = [](uint32_t p, uint32_t q) { return max(p, q); };
+    const uint32_t field = groups_reduce(row_reduce<CW>(max(big & 0xFFFFu, big >> 16) >> 10, larger), larger);
     const int exp_now = max(scale_exp, __builtin_amdgcn_readfirstlane((int)field) - 14);
-    const float to_scale = bits_float((uint32_t)(127 + 15 - exp_now) << 23);
-    v8h ph[NB][2], pl[NB][2];
+    // s becomes s 2^14 / S, exactly, in one packed product or (scales below 1/4) two
+    const int up = 14 - exp_now;
+    auto by_power = [&](int e) {
+      const _Float16 f = (_Float16)bits_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+      for (int i = 0; i < CW / 2; ++i) vs[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, vs[i]) * (v2h){f, f});
+    };
+    by_power(min(up, 15));
+    if (up > 15) by_power(up - 15);
+    const float eight = bits_float((uint32_t)(127 + 3 - up) << 23);   // 8 of the scale as it was
+    uint32_t wh[NB][CW / 2], wl[NB][CW / 2];   // weights, in the order of values_even
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
       float now = most[n];
 #pragma unroll
-      for (int t = 0; t < 16; ++t) now = fmaxf(now, sc[n][t / 4][t % 4]);
-      now = groups_max(now);
+      for (int t = 0; t < CW; ++t) now = fmaxf(now, x[n][t]);
+      now = group_row_max<CW>(now);
       if (__any(now > most[n]) || exp_now > scale_exp) {
         const float next = now == -kInf ? 0.f : factor[n] * now;
         const float shrink = most[n] == -kInf ? 1.f : __builtin_amdgcn_exp2f(at[n] - next);   // before: all sums 0
@@ -418,28 +470,48 @@ kv4_attention_kernel(Attention a) {
               o[h][n][f][1][i] *= shrink_o;
             }
       }
+      _Float16 hi[CW], lo[CW];
 #pragma unroll
-      for (int t = 0; t < 16; ++t) {
-        // tokens 8 z .. 8 z + 7 of the lane in the order of values_even
+      for (int t = 0; t < CW; ++t) {
         constexpr int kSlot[4] = {0, 2, 1, 3};
-        const int z = t / 8, j = 4 * (t / 4 & 1) + kSlot[t % 4];
-        const float vs = half_of(vpar, t), vl = half_of(vpar + 2, t);
-        const float p = __builtin_amdgcn_exp2f(fmaf(factor[n], sc[n][t / 4][t % 4], -at[n]));
-        const float s = vs * to_scale;   // s 2^15 / S
+        const int j = t / 4 * 4 + kSlot[t % 4];
+        const float p = __builtin_amdgcn_exp2f(fmaf(factor[n], x[n][t], -at[n]));
+        const float s = half_of(vs, t);
         total[n] += p;
-        middles[n] = fmaf(p, fmaf(8.f, vs, vl), middles[n]);
-        _Float16 h = (_Float16)(p * s);
+        middles[n] = fmaf(p, fmaf(eight, s, half_of(vl, t)), middles[n]);   // what code 8 stands for
+        hi[j] = (_Float16)fmaf(p, s, 0.f);
         if constexpr (NP > 1) {
           // one and the same rounding in both parts: the product rounded twice (to float32 first)
           // or once differ by a step of h where it is next to a tie
-          asm("" : "+v"(h));
-          pl[n][z][j] = (_Float16)fmaf(p, s, -(float)h);
+          asm("" : "+v"(hi[j]));
+          lo[j] = (_Float16)fmaf(p, s, -(float)hi[j]);
         }
-        ph[n][z][j] = h;
       }
+      __builtin_memcpy(wh[n], hi, sizeof(wh[n]));
+      if constexpr (NP > 1) __builtin_memcpy(wl[n], lo, sizeof(wl[n]));
     }
     scale_exp = exp_now;
     __builtin_amdgcn_sched_barrier(0);
+    // tokens 8 z .. 8 z + 7 of the group
+    auto weights = [&](const uint32_t* w, int z) {
+      v4u v;
+      if constexpr (FOLD == 1) v = (v4u){w[4 * z], w[4 * z + 1], w[4 * z + 2], w[4 * z + 3]};
+      if constexpr (FOLD == 2)
+        v = z == 0 ? (v4u){w[0], w[1], w[2], w[3]}
+                   : (v4u){from_lanes<CW, 1>(w[0]), from_lanes<CW, 1>(w[1]), from_lanes<CW, 1>(w[2]), from_lanes<CW, 1>(w[3])};
+      if constexpr (FOLD == 4)
+        v = z == 0 ? (v4u){w[0], w[1], from_lanes<CW, 1>(w[0]), from_lanes<CW, 1>(w[1])}
+                   : (v4u){from_lanes<CW, 2>(w[0]), from_lanes<CW, 2>(w[1]), from_lanes<CW, 3>(w[0]), from_lanes<CW, 3>(w[1])};
+      return __builtin_bit_cast(v8h, v);
+    };
+    v8h ph[NB][2], pl[NB][2];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        ph[n][z] = weights(wh[n], z);
+        if constexpr (NP > 1) pl[n][z] = weights(wl[n], z);
+      }
 #pragma unroll
     for (int f = 0; f < NF; ++f)
 #pragma unroll
@@ -463,13 +535,13 @@ kv4_attention_kernel(Attention a) {
     }
   }
 
-  const float unit = bits_float((uint32_t)(127 - 15 + scale_exp) << 23);
+  const float unit = bits_float((uint32_t)(127 - 14 + scale_exp) << 23);
   // Outputs in units of the weights, and the sums of all lanes. A wave that saw nothing has
   // the exponent -inf, so that it counts for nothing beside another.
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    total[n] = groups_sum(total[n]);
-    middles[n] = groups_sum(middles[n]);
+    total[n] = group_row_sum<CW>(total[n]);
+    middles[n] = group_row_sum<CW>(middles[n]);
     if (most[n] == -kInf && total[n] == 0.f) at[n] = -kInf;
     if (poison) total[n] = __builtin_nanf(""), at[n] = 0.f;
 #pragma unroll
@@ -521,7 +593,7 @@ kv4_attention_kernel(Attention a) {
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     const int row = first_row + 16 * n + r;
-    if (row > last_row) continue;
+    if (row > last_row || r >= CW) continue;
     const int64_t at_row = (int64_t)(start + row / a.group) * a.q_heads + head * a.group + row % a.group;
     if (a.splits > 1) {
       const int64_t slot = split * total_rows + at_row;
@@ -551,31 +623,61 @@ kv4_attention_kernel(Attention a) {
   }
 }
 
-// Parts of a row's tokens to its output. A thread takes four values.
-template <class D, int DIM>
-__global__ void __launch_bounds__(256)
+// Parts of a row's tokens to its output, a row to a workgroup: a lane of the first wave weighs a part,
+// then DIM / 4 lanes (four values each) take a part's values, in GROUPS whose sums meet in LDS.
+constexpr int kMostSplits = 64;
+template <class D, int DIM, int GROUPS>
+__global__ void __launch_bounds__((GROUPS * DIM / 4 + 63) / 64 * 64)
 kv4_attention_join(const float* __restrict__ part, int splits, int64_t rows, typename D::T* __restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = i / (DIM / 4);
-  if (row >= rows) return;
-  const float* ml = part + splits * rows * DIM + row * 2;
-  float most = -kInf;
-  for (int s = 0; s < splits; ++s) most = fmaxf(most, ml[s * rows * 2]);
-  float total = 0.f;
-  v4f sum = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < splits; ++s) {
-    const float at = ml[s * rows * 2];
-    if (at == -kInf) continue;
-    const float w = __builtin_amdgcn_exp2f(at - most);
-    const v4f v = *reinterpret_cast<const v4f*>(part + (s * rows + row) * DIM + (i % (DIM / 4)) * 4);
-    total = fmaf(w, ml[s * rows * 2 + 1], total);
+  constexpr int LANES = DIM / 4;
+  __shared__ float weight[kMostSplits], box[GROUPS][4][LANES], sum_of_weights;
+  const int64_t row = blockIdx.x;
+  const int d = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  v4f v[2];   // under way while the weights are made
+  auto load = [&](int s) { return *reinterpret_cast<const v4f*>(part + (s * rows + row) * DIM + d * 4); };
+  const bool mine = group < GROUPS;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum[j] = fmaf(w, v[j], sum[j]);
+  for (int i = 0; i < 2; ++i) v[i] = mine && group + i * GROUPS < splits ? load(group + i * GROUPS) : v4f{0.f, 0.f, 0.f, 0.f};
+  if (threadIdx.x < 64) {
+    const int s = threadIdx.x;
+    const float* ml = part + splits * rows * DIM + (s * rows + row) * 2;
+    const float at = s < splits ? ml[0] : -kInf, total = s < splits ? ml[1] : 0.f;
+    const float most = wave_max(at);
+    const float w = at == -kInf ? 0.f : __builtin_amdgcn_exp2f(at - most);
+    float sum = w * total;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    weight[s] = w;
+    if (s == 0) sum_of_weights = sum;
   }
+  __syncthreads();
+  v4f sum = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](int s, const v4f& x) {
+    const float w = weight[s];
+    if (w == 0.f) return;   // a part without tokens holds nothing
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] = fmaf(w, x[j], sum[j]);
+  };
+  if (mine) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (group + i * GROUPS < splits) add(group + i * GROUPS, v[i]);
+#pragma unroll 4
+    for (int s = group + 2 * GROUPS; s < splits; s += GROUPS) add(s, load(s));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) box[group][j][d] = sum[j];
+  }
+  __syncthreads();
+  if (group) return;
+#pragma unroll
+  for (int i = 1; i < GROUPS; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] += box[i][j][d];
+  const float total = sum_of_weights;
   typename D::T t[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) t[j] = D::from_f(total == 0.f ? 0.f : sum[j] / total);
-  __builtin_memcpy(out + row * DIM + (i % (DIM / 4)) * 4, t, sizeof(t));
+  __builtin_memcpy(out + row * DIM + d * 4, t, sizeof(t));
 }
 
 template <class F>
@@ -669,12 +771,20 @@ extern "C" int qo_kv4_attention(const qo_kv4_cache* cache, const qo_heads* q, in
     with_dim(cache->head_dim, [&](auto dim) {
       constexpr int DIM = decltype(dim)::value;
       hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-      if (plan.row_blocks == 1) launch(kv4_attention_kernel<D, DIM, 1, NQ, NP, FINE>, dim3((unsigned)grid), dim3(256), 0, s, a);
-      else if constexpr (DIM <= 128 && !FINE) launch(kv4_attention_kernel<D, DIM, 2, NQ, NP, FINE>, dim3((unsigned)grid), dim3(256), 0, s, a);
+      auto attend = [&](auto kernel) { launch(kernel, dim3((unsigned)grid), dim3(256), 0, s, a); };
+      if (plan.rows == 4) attend(kv4_attention_kernel<D, DIM, 1, 4, NQ, NP, FINE>);
+      else if (plan.rows == 8) attend(kv4_attention_kernel<D, DIM, 1, 2, NQ, NP, FINE>);
+      else if (plan.rows == 16) attend(kv4_attention_kernel<D, DIM, 1, 1, NQ, NP, FINE>);
+      else if constexpr (DIM <= 128 && !FINE) attend(kv4_attention_kernel<D, DIM, 2, 1, NQ, NP, FINE>);
       if (plan.splits > 1) {
         const int64_t rows = tokens * q_heads;
-        launch(kv4_attention_join<D, DIM>, dim3((unsigned)((rows * (DIM / 4) + 255) / 256)), dim3(256), 0, s,
-               reinterpret_cast<const float*>(workspace), plan.splits, rows, reinterpret_cast<typename D::T*>(out));
+        auto join = [&](auto groups) {
+          constexpr int GROUPS = decltype(groups)::value;
+          launch(kv4_attention_join<D, DIM, GROUPS>, dim3((unsigned)rows), dim3((GROUPS * DIM / 4 + 63) / 64 * 64), 0, s,
+                 reinterpret_cast<const float*>(workspace), plan.splits, rows, reinterpret_cast<typename D::T*>(out));
+        };
+        if (plan.splits <= 4) join(std::integral_constant<int, 2>{});
+        else join(std::integral_constant<int, 8>{});
       }
     });
   };
