@@ -28,7 +28,7 @@ OBJ = os.path.join(HERE, "_obj")
 
 HIP_SOURCES = ["capi.hip", "flatquant_quant.hip", "flatquant_tile_f16.hip", "flatquant_tile_bf16.hip",
                "flatquant_f32.hip", "int4_gemm.hip", "int4_gemm_f6.hip", "dequant.hip", "layout.hip", "w4a4_linear.hip",
-               "mx_quantize.hip", "mx_gemm.hip", "kv4_cache.hip", "kv4_attention.hip"]
+               "mx_quantize.hip", "mx_gemm.hip", "kv4_cache.hip", "kv4_attention.hip", "kv4_prefill.hip"]
 LIB_NAME = "libquant_ops_hip.so"
 TORCH_LIB_NAME = "_quant_ops_torch.so"
 # microbenchmarks of the hardware ceilings (bench.py --ceilings), a library of its own

@@ -4,8 +4,7 @@
 // and the parameters are applied to scores, in float32. Values are taken from their middle so
 // that the sums hold no large terms that cancel.
 //
-// A wave takes 64 tokens a step (four tiles of 16) and 16 NB rows (a row: one query of one of
-// the heads that share a KV head). v_mfma_f32_16x16x32_f16 computes S^T = K Q^T (A: codes of 16
+// A wave takes 64 tokens a step (four tiles of 16) and up to 16 rows. v_mfma_f32_16x16x32_f16 computes S^T = K Q^T (A: codes of 16
 // tokens, B: queries) and O^T += V^T P^T (A: codes of 16 pairs' values, B: weights). Lane
 // l = r + 16 g of an operand holds eight consecutive k of row r, a lane of the result rows
 // 4 g .. 4 g + 3 of column r; the order of k is free as long as both operands have it. So
@@ -35,65 +34,18 @@
 // float32 the second parts have sums of their own: added to the first parts' they would lose what is
 // below 2^-24 of those. Maximum, sums and outputs are float32.
 #include "dispatch_rules.h"
-#include "kv4_common.h"
+#include "kv4_attention.h"
 
 namespace qo {
 
 namespace {
 
-typedef unsigned v4u __attribute__((ext_vector_type(4)));
-typedef unsigned v2u __attribute__((ext_vector_type(2)));
-
-constexpr float kLog2e = 1.44269504f;
-constexpr float kInf = __builtin_inff();
-constexpr int kMostTokens = 0x7FFFFF00;   // of a sequence: positions and steps take 32 bits
-
-struct Attention {
-  KV4 cache;
-  const void* q;
-  int64_t q_token, q_head;
-  void* out;
-  const int32_t* table;
-  int64_t table_ld;
-  int64_t width;              // pages of a row of the table
-  const int32_t* lengths;
-  const int32_t* q_starts;    // or null: `each` queries a sequence
-  int64_t tokens, sequences, each;
-  int q_heads, group;
-  float scale;
-  int64_t window;             // 0: none
-  int64_t tiles;              // row tiles of all sequences
-  int splits;
-  float* part;                // [splits][tokens * q_heads][DIM], then [splits][tokens * q_heads][2]
-};
-
-__device__ inline float bits_float(uint32_t u) { return __builtin_bit_cast(float, u); }
-__device__ inline uint32_t float_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
-
-// Reductions over the four lane groups (lanes r, r + 16, r + 32, r + 48).
-template <class F>
-__device__ inline uint32_t groups_reduce(uint32_t u, F&& f) {
-  const v2u a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  const uint32_t w = f(a[0], a[1]);
-  const v2u b = __builtin_amdgcn_permlane16_swap(w, w, false, false);
-  return f(b[0], b[1]);
-}
 // And over lanes r, r + CW, .. of a row of 16.
 template <int CW, class F>
-__device__ inline uint32_t row_reduce(uint32_t u, F&& f) {
+__device__ inline uint32_t row_reduce(uint32_t u, F f) {
   if constexpr (CW <= 4) u = f(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x124, 0xF, 0xF, false));   // row_ror:4
   if constexpr (CW <= 8) u = f(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x128, 0xF, 0xF, false));   // row_ror:8
-  return u;
-}
-template <int CW>
-__device__ inline float group_row_max(float v) {
-  auto f = [](uint32_t a, uint32_t b) { return float_bits(fmaxf(bits_float(a), bits_float(b))); };
-  return bits_float(groups_reduce(row_reduce<CW>(float_bits(v), f), f));
-}
-template <int CW>
-__device__ inline float group_row_sum(float v) {
-  auto f = [](uint32_t a, uint32_t b) { return float_bits(bits_float(a) + bits_float(b)); };
-  return bits_float(groups_reduce(row_reduce<CW>(float_bits(v), f), f));
+  return groups_reduce(u, f);
 }
 // In lanes Q CW .. of a row of 16 the value that lane r - Q CW has, elsewhere old; and back.
 template <int CW, int Q>
@@ -104,31 +56,9 @@ template <int CW, int Q>
 __device__ inline uint32_t from_lanes(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x100 + CW * Q, 0xF, 0xF, true);   // row_shl
 }
-__device__ inline float groups_max(float v) {
-  return bits_float(groups_reduce(float_bits(v), [](uint32_t a, uint32_t b) { return float_bits(fmaxf(bits_float(a), bits_float(b))); }));
-}
-__device__ inline float groups_sum(float v) {
-  return bits_float(groups_reduce(float_bits(v), [](uint32_t a, uint32_t b) { return float_bits(bits_float(a) + bits_float(b)); }));
-}
 
-// Codes less 8 as fp16 (those at bits 4 .. 7 times 16): with the exponent of 1024 in front, an
-// fp16's lowest bits count in ones.
-constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;
-__device__ inline uint32_t less(uint32_t w, uint32_t mask, uint32_t exponents, _Float16 n) {
-  const v2h v = __builtin_bit_cast(v2h, (w & mask) | exponents) - (v2h){n, n};
-  return __builtin_bit_cast(uint32_t, v);
-}
-// The exponents in a vector register: a mask and they are then one instruction's operands.
-__device__ inline uint32_t exponents_of_1024() {
-  uint32_t e = 0x64006400u;
-  asm("" : "+v"(e));
-  return e;
-}
-__device__ inline uint32_t less_low(uint32_t w, uint32_t e) { return less(w, kLow, e, (_Float16)1032.f); }
-__device__ inline uint32_t less_high(uint32_t w, uint32_t e) { return less(w, kHigh, e, (_Float16)1152.f); }
-
-// The eight codes of a key's word in the order 0, 4, 1, 5, 2, 6, 3, 7: even ones times kEven, odd ones
-// times kOdd, all less kLess.
+// The eight codes of a key's word in the order of kCodeOrder: even ones times kEven, odd ones times
+// kOdd, all less kLess.
 template <bool FINE>
 struct Codes {
   static constexpr float kEven = FINE ? 1.f : 0x1p-24f, kOdd = 16.f * kEven, kLess = FINE ? 8.f : 0.f;
@@ -147,116 +77,37 @@ __device__ inline v8h values_odd(uint32_t a, uint32_t b, uint32_t e) {
   return __builtin_bit_cast(v8h, (v4u){less_high(a, e), less_high(a >> 8, e), less_high(b, e), less_high(b >> 8, e)});
 }
 
-__device__ inline uint32_t pk_max_u16(uint32_t a, uint32_t b) {
-  typedef unsigned short v2u16 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2u16, a), __builtin_bit_cast(v2u16, b)));
-}
-
-// A page of one head: where it starts, and the bytes from page to page (below 2^32: the host's check).
-struct Pages {
-  const uint8_t* k;
-  const uint8_t* v;
-  const uint8_t* params;   // of keys; those of values stand param_values further
-  uint32_t codes, param_bytes, param_values;
-};
-
-// Where a tile of 16 tokens stands: its page (0 for one outside the cache) and the place of its first token.
-struct Tile {
-  int page, place;
-  bool bad;
-};
-__device__ inline Tile tile_at(const Attention& a, const int32_t* table, int t) {
-  const int at = t >> a.cache.shift;
-  const int page = at < (int)a.width ? table[at] : 0;   // beyond: past the tokens, masked
-  const bool bad = page < 0 || page >= (int)a.cache.pages;
-  return {bad ? 0 : page, t & ((1 << a.cache.shift) - 1), bad};
-}
-
-// The first token that a row sees and the one after the last.
-struct Sees {
-  int first, last;
-};
-
-template <class D, int DIM, int NB, int FOLD, int NQ, int NP, bool FINE>
-__global__ void __launch_bounds__(256, DIM <= 128 && NB == 1 && !FINE ? 2 : 1)
+template <class D, int DIM, int FOLD, int NQ, int NP, bool FINE>
+__global__ void __launch_bounds__(256, DIM <= 128 && !FINE ? 2 : 1)
 kv4_attention_kernel(Attention a) {
   constexpr int NS = DIM / 32;        // k-steps of a score, words of a key's codes in a lane
   constexpr int NF = DIM / 32;        // blocks of 16 pairs of values
   constexpr int CW = 16 / FOLD;       // columns with rows of their own, and tokens of a step for a lane's softmax
-  constexpr int ROWS = CW * NB, TILE = 4 * ROWS;
-  static_assert(NB == 1 || FOLD == 1, "more than 16 rows");
+  constexpr int TILE = 4 * CW;
   constexpr int APART = FINE;         // second parts of weights have sums of their own
   using C = Codes<FINE>;
   using T = typename D::T;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const int heads = a.cache.heads, tokens = (int)a.tokens, sequences = (int)a.sequences;
-  const int head = blockIdx.x % heads, tile = blockIdx.x / heads % (int)a.tiles, split = blockIdx.x / heads / (int)a.tiles;
-
-  // The tile's sequence, its queries and the tile's first row. Tiles of ragged sequences are
-  // counted from q_starts[b] * group / TILE + b on, which leaves room for every one's last.
-  int b, start, count, row0;
-  auto begin_of = [&](int i) {   // sequence 0 starts at 0, the rows behind the last are one more
-    const int s = i == 0 ? 0 : a.q_starts[i];
-    return s < 0 ? 0 : s > tokens ? tokens : s;
-  };
-  if (a.q_starts) {
-    int n = 0;
-    for (int base = 0; base <= sequences; base += 64) {
-      const int i = base + lane;
-      const bool before = i <= sequences && begin_of(i) * a.group / TILE + i <= tile;
-      const int got = __popcll(__ballot(before));
-      n += got;
-      if (got < 64) break;
-    }
-    b = n - 1;
-    start = begin_of(b);
-    const int end = b < sequences ? begin_of(b + 1) : tokens;
-    count = end > start ? end - start : 0;
-    row0 = (tile - (start * a.group / TILE + b)) * TILE;
-  } else {
-    const int per = ((int)a.each * a.group + TILE - 1) / TILE;
-    b = tile / per;
-    start = b * (int)a.each;
-    count = (int)a.each;
-    row0 = tile % per * TILE;
-  }
-  const int all = count * a.group;
-  if (row0 < 0 || row0 >= all) return;   // below 0: q_starts that do not ascend
-  const int rows = all - row0 < TILE ? all - row0 : TILE;
-
-  int length = b < sequences ? a.lengths[b] : 0;
-  const bool poison = length > kMostTokens || (length >> a.cache.shift) > a.width ||
-                      ((length >> a.cache.shift) == a.width && (length & ((1 << a.cache.shift) - 1)));
-  if (length < 0 || poison) length = 0;
+  const int heads = a.cache.heads;
+  const int head = blockIdx.x % heads, split = blockIdx.x / heads / a.tiles;
+  const Rows w = find_rows<TILE>(a, blockIdx.x / heads % a.tiles);
+  if (!w.rows) return;
 
   // The waves' rows; waves with the same rows take turns at their tokens.
-  const int blocks = (rows + ROWS - 1) / ROWS;
+  const int blocks = (w.rows + CW - 1) / CW;
   const int sharing = blocks == 1 ? 4 : blocks == 2 ? 2 : 1;
   const int mine = wave / sharing, turn_of = wave % sharing;
   const bool active = mine < blocks;
-  const int first_row = row0 + (active ? mine : 0) * ROWS;
-  const int last_row = first_row + ROWS < row0 + rows ? first_row + ROWS - 1 : row0 + rows - 1;
-  const int window = a.window && a.window < kMostTokens ? (int)a.window : 0;
-  auto sees = [&](int row) {
-    const int p = length - count + row / a.group;
-    return Sees{window && p + 1 > window ? p + 1 - window : 0, length && p >= 0 ? p + 1 : 0};
-  };
-  const Sees top = sees(first_row), bottom = sees(last_row);
-  int row_of[NB];
-  Sees see[NB];
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    row_of[n] = first_row + 16 * n + r % CW <= last_row ? first_row + 16 * n + r % CW : last_row;
-    see[n] = sees(row_of[n]);
-  }
+  const int first_row = w.row0 + (active ? mine : 0) * CW;
+  const int last_row = min(first_row + CW, w.row0 + w.rows) - 1;
+  const int row = min(first_row + r % CW, last_row);
+  const Sees top = sees(a, w, first_row), bottom = sees(a, w, last_row), see = sees(a, w, row);
 
-  // Queries as fp16 parts in the order of Codes::of, the odd codes' factor taken out.
-  v8h qf[NQ][NB][NS];
-  float factor[NB], qsum[NB];   // of the exponent of two; sum of a query, in units of its scores
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    const T* q = reinterpret_cast<const T*>(a.q) + (start + row_of[n] / a.group) * a.q_token +
-                 (head * a.group + row_of[n] % a.group) * a.q_head;
+  // The query as fp16 parts in the order of Codes::of, the odd codes' factor taken out.
+  v8h qf[NQ][NS];
+  float factor, qsum;   // of the exponent of two; sum of the query, in units of its scores
+  {
+    const T* q = reinterpret_cast<const T*>(a.q) + (w.start + row / a.group) * a.q_token + (head * a.group + row % a.group) * a.q_head;
     float x[NS][8], most = 0.f;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
@@ -268,52 +119,38 @@ kv4_attention_kernel(Attention a) {
         most = fmaxf(most, fabsf(x[s][i]));
       }
     }
-    most = groups_max(most);
-    int e = 15 - __builtin_amdgcn_frexp_expf(most);   // 2^14 <= most 2^e < 2^15
-    e = most > 0.f && most < kInf ? min(max(e, -100), 60) : 0;
+    most = bits_float(groups_reduce(float_bits(most), FMax{}));
+    const int e = query_exponent(most);
     float sum = 0.f;
-    constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float v = ldexpf(x[s][kOrder[i]], e);
+        const float v = ldexpf(x[s][kCodeOrder[i]], e);
         sum += v;
-        const float w = opaque(kOrder[i] & 1 ? v * (C::kEven / C::kOdd) : v);
-        qf[0][n][s][i] = (_Float16)w;
-        if constexpr (NQ > 1) qf[1][n][s][i] = (_Float16)(w - (float)qf[0][n][s][i]);
+        const float part = opaque(kCodeOrder[i] & 1 ? v * (C::kEven / C::kOdd) : v);
+        qf[0][s][i] = (_Float16)part;
+        if constexpr (NQ > 1) qf[1][s][i] = (_Float16)(part - (float)qf[0][s][i]);
       }
-    qsum[n] = most < kInf ? groups_sum(sum) * C::kEven : __builtin_nanf("");   // an infinity's scores are NaN
-    factor[n] = fmaxf(ldexpf(a.scale * kLog2e, -e) * (1.f / C::kEven), 0x1p-126f);   // 0 times a masked score: no number
+    sum = bits_float(groups_reduce(float_bits(sum), FAdd{}));
+    qsum = most < kInf ? sum * C::kEven : __builtin_nanf("");   // an infinity's scores are NaN
+    factor = fmaxf(ldexpf(a.scale * kLog2e, -e) * (1.f / C::kEven), 0x1p-126f);   // 0 times a masked score: no number
   }
 
-  v4f o[APART + 1][NB][NF][2];
-  float most[NB], at[NB], total[NB], middles[NB];   // largest score, as an exponent; sums of weights, and times middles
+  v4f o[APART + 1][NF][2];
+  float most = -kInf, at = 0.f, total = 0.f, middles = 0.f;   // largest score, as an exponent; sums of weights, and times middles
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    most[n] = -kInf;
-    at[n] = total[n] = middles[n] = 0.f;
+  for (int h = 0; h <= APART; ++h)
 #pragma unroll
-    for (int f = 0; f < NF; ++f)
-      for (int h = 0; h <= APART; ++h) o[h][n][f][0] = o[h][n][f][1] = v4f{0.f, 0.f, 0.f, 0.f};
-  }
+    for (int f = 0; f < NF; ++f) o[h][f][0] = o[h][f][1] = v4f{0.f, 0.f, 0.f, 0.f};
   int scale_exp = -14;
 
   const int begin = top.first & ~63;
   const int steps = bottom.last > begin ? (bottom.last - begin + 63) / 64 : 0;
   const int per_split = (steps + a.splits - 1) / a.splits;
   const int to = (split + 1) * per_split < steps ? (split + 1) * per_split : steps;
-  const int32_t* table = a.table + (b < sequences ? b : 0) * a.table_ld;
-  Pages pages;
-  {
-    const int shift = a.cache.shift;
-    pages.codes = (uint32_t)(heads << shift) * (DIM / 2);
-    pages.param_values = (uint32_t)(heads << (shift - 4)) * 64;
-    pages.param_bytes = 2 * pages.param_values;
-    pages.k = a.cache.k + ((int64_t)head << shift) * (DIM / 2);
-    pages.v = a.cache.v + ((int64_t)head << shift) * (DIM / 2);
-    pages.params = reinterpret_cast<const uint8_t*>(a.cache.params) + ((int64_t)head << (shift - 4)) * 64;
-  }
+  const int32_t* table = a.table + (w.b < a.sequences ? w.b : 0) * a.table_ld;
+  const Pages pages(a.cache, head, DIM);
 
   // A step's loads go out a step ahead: its pages two, its keys as soon as the scores of the step
   // before are made, its values after that step's second product.
@@ -344,10 +181,6 @@ kv4_attention_kernel(Attention a) {
 #pragma unroll
     for (int f = 0; f < NF; ++f) vw[f] = *reinterpret_cast<const v4u*>(p + f * 256);
   };
-  auto half_of = [](const uint32_t* pairs, int t) {
-    const uint32_t w = pairs[t / 2];
-    return (float)__builtin_bit_cast(v2h, w)[t & 1];
-  };
   const uint32_t exponents = exponents_of_1024();
 
   const int first_step = split * per_split + turn_of;
@@ -363,34 +196,26 @@ kv4_attention_kernel(Attention a) {
     const bool more = step + sharing < to;
     const bool whole = t0 + 64 <= top.last && t0 >= bottom.first && !__any(bad);
     // scores
-    v4f sc[NB][4];
+    v4f sc[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      v4f rest[NB];
-#pragma unroll
-      for (int n = 0; n < NB; ++n) sc[n][u] = rest[n] = v4f{0.f, 0.f, 0.f, 0.f};
+      v4f rest = {0.f, 0.f, 0.f, 0.f};
+      sc[u] = rest;
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         const v8h c = C::of(kw[u][s], exponents);
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          sc[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, qf[0][n][s], sc[n][u], 0, 0, 0);
-          if constexpr (NQ > 1) rest[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, qf[1][n][s], rest[n], 0, 0, 0);
-        }
+        sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, qf[0][s], sc[u], 0, 0, 0);
+        if constexpr (NQ > 1) rest = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, qf[1][s], rest, 0, 0, 0);
       }
       if constexpr (NQ > 1) {
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sc[n][u][i] += rest[n][i];
+        for (int i = 0; i < 4; ++i) sc[u][i] += rest[i];
       }
     }
-    float x[NB][CW];   // of the lane's tokens
+    float x[CW];   // of the lane's tokens
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int t = 0; t < CW; ++t) {
-        auto at_token = [&](int i) { return float_bits(sc[n][i / 4][i % 4]); };
+    for (int t = 0; t < CW; ++t) {
+        auto at_token = [&](int i) { return float_bits(sc[i / 4][i % 4]); };
         uint32_t y = at_token(t);
         if constexpr (FOLD == 2) y = to_lanes<CW, 1>(y, at_token(CW + t));
         if constexpr (FOLD == 4) {
@@ -399,7 +224,7 @@ kv4_attention_kernel(Attention a) {
           y = to_lanes<CW, 3>(y, at_token(3 * CW + t));
         }
         const float s = half_of(ks, t), lo = half_of(kl, t);
-        x[n][t] = fmaf(s, bits_float(y), fmaf(C::kLess, s, lo) * qsum[n]);
+        x[t] = fmaf(s, bits_float(y), fmaf(C::kLess, s, lo) * qsum);
       }
     __builtin_amdgcn_sched_barrier(0);
     const bool bad_now = bad;
@@ -408,19 +233,15 @@ kv4_attention_kernel(Attention a) {
       load_keys();
     }
     if (!whole) {
-      // Tokens that a row does not see get no weight, whatever stands there. A NaN (or a page outside the
+      // Tokens that the row does not see get no weight, whatever stands there. A NaN (or a page outside the
       // cache) that it sees makes its sum NaN; a value's parameters are then 0, for the rows that do not.
 #pragma unroll
       for (int t = 0; t < CW; ++t) {
         const int at_t = t0 + 16 * g + own + t;
         const bool finite = fabsf(half_of(vs, t)) < kInf && fabsf(half_of(vl, t)) < kInf && !bad_now;
-        const bool any = at_t >= top.first && at_t < bottom.last;
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          const bool seen = at_t >= see[n].first && at_t < see[n].last;
-          x[n][t] = seen ? x[n][t] : -kInf;
-          if (seen && !finite) total[n] = __builtin_nanf("");
-        }
+        const bool any = at_t >= top.first && at_t < bottom.last, seen = at_t >= see.first && at_t < see.last;
+        x[t] = seen ? x[t] : -kInf;
+        if (seen && !finite) total = __builtin_nanf("");
         if (!finite || !any) {
           const uint32_t keep = t & 1 ? 0x0000FFFFu : 0xFFFF0000u;
           vs[t / 2] &= keep;
@@ -432,53 +253,49 @@ kv4_attention_kernel(Attention a) {
     uint32_t big = 0;
 #pragma unroll
     for (int i = 0; i < CW / 2; ++i) big = pk_max_u16(big, vs[i] & 0x7FFF7FFFu);
-    auto larger = [](uint32_t p, uint32_t q) { return max(p, q); };
-    const uint32_t field = groups_reduce(row_reduce<CW>(max(big & 0xFFFFu, big >> 16) >> 10, larger), larger);
+    const uint32_t field = row_reduce<CW>(max(big & 0xFFFFu, big >> 16) >> 10, UMax{});
     const int exp_now = max(scale_exp, __builtin_amdgcn_readfirstlane((int)field) - 14);
     // s becomes s 2^14 / S, exactly, in one packed product or (scales below 1/4) two
     const int up = 14 - exp_now;
     auto by_power = [&](int e) {
-      const _Float16 f = (_Float16)bits_float((uint32_t)(127 + e) << 23);
+      const _Float16 f = (_Float16)power_of_two(e);
 #pragma unroll
       for (int i = 0; i < CW / 2; ++i) vs[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, vs[i]) * (v2h){f, f});
     };
     by_power(min(up, 15));
     if (up > 15) by_power(up - 15);
-    const float eight = bits_float((uint32_t)(127 + 3 - up) << 23);   // 8 of the scale as it was
-    uint32_t wh[NB][CW / 2], wl[NB][CW / 2];   // weights, in the order of values_even
+    const float eight = power_of_two(3 - up);   // 8 of the scale as it was
+    float now = most;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      float now = most[n];
+    for (int t = 0; t < CW; ++t) now = fmaxf(now, x[t]);
+    now = bits_float(row_reduce<CW>(float_bits(now), FMax{}));
+    if (__any(now > most) || exp_now > scale_exp) {
+      const float next = now == -kInf ? 0.f : factor * now;
+      const float shrink = most == -kInf ? 1.f : __builtin_amdgcn_exp2f(at - next);   // before: all sums 0
+      const float shrink_o = shrink * power_of_two(scale_exp - exp_now);
+      most = now;
+      at = next;
+      total *= shrink;
+      middles *= shrink;
 #pragma unroll
-      for (int t = 0; t < CW; ++t) now = fmaxf(now, x[n][t]);
-      now = group_row_max<CW>(now);
-      if (__any(now > most[n]) || exp_now > scale_exp) {
-        const float next = now == -kInf ? 0.f : factor[n] * now;
-        const float shrink = most[n] == -kInf ? 1.f : __builtin_amdgcn_exp2f(at[n] - next);   // before: all sums 0
-        const float shrink_o = shrink * bits_float((uint32_t)(127 + scale_exp - exp_now) << 23);
-        most[n] = now;
-        at[n] = next;
-        total[n] *= shrink;
-        middles[n] *= shrink;
+      for (int h = 0; h <= APART; ++h)
 #pragma unroll
-        for (int f = 0; f < NF; ++f)
-#pragma unroll
-          for (int h = 0; h <= APART; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              o[h][n][f][0][i] *= shrink_o;
-              o[h][n][f][1][i] *= shrink_o;
-            }
-      }
+        for (int f = 0; f < NF; ++f) {
+          o[h][f][0] *= shrink_o;
+          o[h][f][1] *= shrink_o;
+        }
+    }
+    uint32_t wh[CW / 2], wl[CW / 2];   // weights, in the order of values_even
+    {
       _Float16 hi[CW], lo[CW];
 #pragma unroll
       for (int t = 0; t < CW; ++t) {
         constexpr int kSlot[4] = {0, 2, 1, 3};
         const int j = t / 4 * 4 + kSlot[t % 4];
-        const float p = __builtin_amdgcn_exp2f(fmaf(factor[n], x[n][t], -at[n]));
+        const float p = __builtin_amdgcn_exp2f(fmaf(factor, x[t], -at));
         const float s = half_of(vs, t);
-        total[n] += p;
-        middles[n] = fmaf(p, fmaf(eight, s, half_of(vl, t)), middles[n]);   // what code 8 stands for
+        total += p;
+        middles = fmaf(p, fmaf(eight, s, half_of(vl, t)), middles);   // what code 8 stands for
         hi[j] = (_Float16)fmaf(p, s, 0.f);
         if constexpr (NP > 1) {
           // one and the same rounding in both parts: the product rounded twice (to float32 first)
@@ -487,45 +304,40 @@ kv4_attention_kernel(Attention a) {
           lo[j] = (_Float16)fmaf(p, s, -(float)hi[j]);
         }
       }
-      __builtin_memcpy(wh[n], hi, sizeof(wh[n]));
-      if constexpr (NP > 1) __builtin_memcpy(wl[n], lo, sizeof(wl[n]));
+      __builtin_memcpy(wh, hi, sizeof(wh));
+      if constexpr (NP > 1) __builtin_memcpy(wl, lo, sizeof(wl));
     }
     scale_exp = exp_now;
     __builtin_amdgcn_sched_barrier(0);
     // tokens 8 z .. 8 z + 7 of the group
-    auto weights = [&](const uint32_t* w, int z) {
+    auto weights = [&](const uint32_t* x, int z) {
       v4u v;
-      if constexpr (FOLD == 1) v = (v4u){w[4 * z], w[4 * z + 1], w[4 * z + 2], w[4 * z + 3]};
+      if constexpr (FOLD == 1) v = (v4u){x[4 * z], x[4 * z + 1], x[4 * z + 2], x[4 * z + 3]};
       if constexpr (FOLD == 2)
-        v = z == 0 ? (v4u){w[0], w[1], w[2], w[3]}
-                   : (v4u){from_lanes<CW, 1>(w[0]), from_lanes<CW, 1>(w[1]), from_lanes<CW, 1>(w[2]), from_lanes<CW, 1>(w[3])};
+        v = z == 0 ? (v4u){x[0], x[1], x[2], x[3]}
+                   : (v4u){from_lanes<CW, 1>(x[0]), from_lanes<CW, 1>(x[1]), from_lanes<CW, 1>(x[2]), from_lanes<CW, 1>(x[3])};
       if constexpr (FOLD == 4)
-        v = z == 0 ? (v4u){w[0], w[1], from_lanes<CW, 1>(w[0]), from_lanes<CW, 1>(w[1])}
-                   : (v4u){from_lanes<CW, 2>(w[0]), from_lanes<CW, 2>(w[1]), from_lanes<CW, 3>(w[0]), from_lanes<CW, 3>(w[1])};
+        v = z == 0 ? (v4u){x[0], x[1], from_lanes<CW, 1>(x[0]), from_lanes<CW, 1>(x[1])}
+                   : (v4u){from_lanes<CW, 2>(x[0]), from_lanes<CW, 2>(x[1]), from_lanes<CW, 3>(x[0]), from_lanes<CW, 3>(x[1])};
       return __builtin_bit_cast(v8h, v);
     };
-    v8h ph[NB][2], pl[NB][2];
+    v8h ph[2], pl[2];
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        ph[n][z] = weights(wh[n], z);
-        if constexpr (NP > 1) pl[n][z] = weights(wl[n], z);
-      }
+    for (int z = 0; z < 2; ++z) {
+      ph[z] = weights(wh, z);
+      if constexpr (NP > 1) pl[z] = weights(wl, z);
+    }
 #pragma unroll
     for (int f = 0; f < NF; ++f)
 #pragma unroll
       for (int z = 0; z < 2; ++z) {
         const v8h even = values_even(vw[f][2 * z], vw[f][2 * z + 1], exponents), odd = values_odd(vw[f][2 * z], vw[f][2 * z + 1], exponents);
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          v4f(&hi)[2] = o[0][n][f], (&lo)[2] = o[APART][n][f];
-          hi[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, ph[n][z], hi[0], 0, 0, 0);
-          hi[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, ph[n][z], hi[1], 0, 0, 0);
-          if constexpr (NP > 1) {
-            lo[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, pl[n][z], lo[0], 0, 0, 0);
-            lo[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, pl[n][z], lo[1], 0, 0, 0);
-          }
+        v4f(&hi)[2] = o[0][f], (&lo)[2] = o[APART][f];
+        hi[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, ph[z], hi[0], 0, 0, 0);
+        hi[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, ph[z], hi[1], 0, 0, 0);
+        if constexpr (NP > 1) {
+          lo[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, pl[z], lo[0], 0, 0, 0);
+          lo[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, pl[z], lo[1], 0, 0, 0);
         }
       }
     __builtin_amdgcn_sched_barrier(0);
@@ -535,90 +347,74 @@ kv4_attention_kernel(Attention a) {
     }
   }
 
-  const float unit = bits_float((uint32_t)(127 - 14 + scale_exp) << 23);
   // Outputs in units of the weights, and the sums of all lanes. A wave that saw nothing has
   // the exponent -inf, so that it counts for nothing beside another.
+  const float unit = power_of_two(scale_exp - 14);
+  total = bits_float(row_reduce<CW>(float_bits(total), FAdd{}));
+  middles = bits_float(row_reduce<CW>(float_bits(middles), FAdd{}));
+  if (most == -kInf && total == 0.f) at = -kInf;
+  if (w.poison) total = __builtin_nanf(""), at = 0.f;
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    total[n] = group_row_sum<CW>(total[n]);
-    middles[n] = group_row_sum<CW>(middles[n]);
-    if (most[n] == -kInf && total[n] == 0.f) at[n] = -kInf;
-    if (poison) total[n] = __builtin_nanf(""), at[n] = 0.f;
+  for (int f = 0; f < NF; ++f)
 #pragma unroll
-    for (int f = 0; f < NF; ++f)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (APART) o[0][n][f][0][i] += o[1][n][f][0][i], o[0][n][f][1][i] += o[1][n][f][1][i];
-        o[0][n][f][0][i] = fmaf(o[0][n][f][0][i], unit, middles[n]);
-        o[0][n][f][1][i] = fmaf(o[0][n][f][1][i], 0.0625f * unit, middles[n]);
-      }
-  }
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (APART) o[0][f][0][i] += o[1][f][0][i], o[0][f][1][i] += o[1][f][1][i];
+      o[0][f][0][i] = fmaf(o[0][f][0][i], unit, middles);
+      o[0][f][1][i] = fmaf(o[0][f][1][i], 0.0625f * unit, middles);
+    }
   // Waves that shared rows: half of them hand theirs to the others, twice for four.
-  __shared__ float join[2][64][NB * NF * 8 + 2 * NB + 1];   // one float more: lanes in different banks
+  __shared__ float join[2][64][NF * 8 + 3];   // an odd number: lanes in different banks
   for (int step = sharing / 2; step > 0; step /= 2) {
     // of two waves that share rows and stand `step` turns apart the later gives
     const int slot = sharing == 4 ? (turn_of % step) : mine;
     float* box = join[slot & 1][lane];
     if (active && turn_of >= step && turn_of < 2 * step) {
+      box[0] = at;
+      box[1] = total;
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        box[2 * n] = at[n];
-        box[2 * n + 1] = total[n];
+      for (int f = 0; f < NF; ++f)
 #pragma unroll
-        for (int f = 0; f < NF; ++f)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) box[2 * NB + (n * NF + f) * 8 + i] = o[0][n][f][i >> 2][i & 3];
-      }
+        for (int i = 0; i < 8; ++i) box[2 + f * 8 + i] = o[0][f][i >> 2][i & 3];
     }
     __syncthreads();
     if (active && turn_of < step) {
+      const float other = box[0], both = fmaxf(at, other);
+      const float x = at == -kInf ? 0.f : __builtin_amdgcn_exp2f(at - both);
+      const float y = other == -kInf ? 0.f : __builtin_amdgcn_exp2f(other - both);
+      at = both;
+      total = total * x + box[1] * y;
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const float other = box[2 * n], both = fmaxf(at[n], other);
-        const float x = at[n] == -kInf ? 0.f : __builtin_amdgcn_exp2f(at[n] - both);
-        const float y = other == -kInf ? 0.f : __builtin_amdgcn_exp2f(other - both);
-        at[n] = both;
-        total[n] = total[n] * x + box[2 * n + 1] * y;
+      for (int f = 0; f < NF; ++f)
 #pragma unroll
-        for (int f = 0; f < NF; ++f)
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            o[0][n][f][i >> 2][i & 3] = o[0][n][f][i >> 2][i & 3] * x + box[2 * NB + (n * NF + f) * 8 + i] * y;
-      }
+        for (int i = 0; i < 8; ++i) o[0][f][i >> 2][i & 3] = o[0][f][i >> 2][i & 3] * x + box[2 + f * 8 + i] * y;
     }
     __syncthreads();
   }
-  if (!active || turn_of) return;
-  const int64_t total_rows = a.tokens * a.q_heads;   // of all heads
+  if (!active || turn_of || r >= CW || first_row + r > last_row) return;
+  const int64_t total_rows = (int64_t)a.tokens * a.q_heads;   // of all heads
+  const int64_t at_row = (int64_t)(w.start + row / a.group) * a.q_heads + head * a.group + row % a.group;
+  float v[NF][8];
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    const int row = first_row + 16 * n + r;
-    if (row > last_row || r >= CW) continue;
-    const int64_t at_row = (int64_t)(start + row / a.group) * a.q_heads + head * a.group + row % a.group;
-    if (a.splits > 1) {
-      const int64_t slot = split * total_rows + at_row;
-      float* to_o = a.part + slot * DIM;
+  for (int f = 0; f < NF; ++f)
 #pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        float v[8];
+    for (int i = 0; i < 8; ++i) v[f][i] = o[0][f][i & 1][i >> 1];
+  if (a.splits > 1) {
+    const int64_t slot = split * total_rows + at_row;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = o[0][n][f][i & 1][i >> 1];
-        __builtin_memcpy(to_o + 32 * f + 8 * g, v, sizeof(v));
-      }
-      if (g == 0) {
-        float* ml = a.part + a.splits * total_rows * DIM + slot * 2;
-        ml[0] = at[n];
-        ml[1] = total[n];
-      }
-    } else {
-      T* to_o = reinterpret_cast<T*>(a.out) + at_row * DIM;
+    for (int f = 0; f < NF; ++f) __builtin_memcpy(a.part + slot * DIM + 32 * f + 8 * g, v[f], sizeof(v[f]));
+    if (g == 0) {
+      float* ml = a.part + a.splits * total_rows * DIM + slot * 2;
+      ml[0] = at;
+      ml[1] = total;
+    }
+  } else {
+    T* to_o = reinterpret_cast<T*>(a.out) + at_row * DIM;
 #pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        T v[8];
+    for (int f = 0; f < NF; ++f) {
+      T out[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = D::from_f(total[n] == 0.f ? 0.f : o[0][n][f][i & 1][i >> 1] / total[n]);
-        __builtin_memcpy(to_o + 32 * f + 8 * g, v, sizeof(v));
-      }
+      for (int i = 0; i < 8; ++i) out[i] = D::from_f(total == 0.f ? 0.f : v[f][i] / total);
+      __builtin_memcpy(to_o + 32 * f + 8 * g, out, sizeof(out));
     }
   }
 }
@@ -759,10 +555,11 @@ extern "C" int qo_kv4_attention(const qo_kv4_cache* cache, const qo_heads* q, in
     qo_set_error("%s: pages of %d tokens of %d heads are too large", fn, (int)cache->page_size, c.heads);
     return QO_ERR_SHAPE;
   }
-  Attention a = {c, q->data, q->token_stride, q->head_stride, out, page_table, table_ld, table_width, lengths, q_starts,
-                 tokens, sequences, sequences ? tokens / sequences : 0, q_heads, q_heads / c.heads, scale, window,
-                 plan.tiles, plan.splits, reinterpret_cast<float*>(workspace)};
-  if (c.pages == 0) a.width = 0;   // nothing to read
+  const Attention a = {c, q->data, q->token_stride, q->head_stride, out, page_table, table_ld,
+                       c.pages ? (int)table_width : 0,   // without pages there is nothing to read
+                       lengths, q_starts, (int)tokens, (int)sequences, sequences ? (int)(tokens / sequences) : 0, q_heads,
+                       q_heads / c.heads, scale, window < kMostTokens ? (int)window : 0, (int)plan.tiles, plan.splits,
+                       reinterpret_cast<float*>(workspace)};
   launch_begin();
   auto go = [&](auto d, auto parts_q, auto parts_p, auto fine) {
     using D = decltype(d);
@@ -772,10 +569,10 @@ extern "C" int qo_kv4_attention(const qo_kv4_cache* cache, const qo_heads* q, in
       constexpr int DIM = decltype(dim)::value;
       hipStream_t s = reinterpret_cast<hipStream_t>(stream);
       auto attend = [&](auto kernel) { launch(kernel, dim3((unsigned)grid), dim3(256), 0, s, a); };
-      if (plan.rows == 4) attend(kv4_attention_kernel<D, DIM, 1, 4, NQ, NP, FINE>);
-      else if (plan.rows == 8) attend(kv4_attention_kernel<D, DIM, 1, 2, NQ, NP, FINE>);
-      else if (plan.rows == 16) attend(kv4_attention_kernel<D, DIM, 1, 1, NQ, NP, FINE>);
-      else if constexpr (DIM <= 128 && !FINE) attend(kv4_attention_kernel<D, DIM, 2, 1, NQ, NP, FINE>);
+      if (plan.rows == 4) attend(kv4_attention_kernel<D, DIM, 4, NQ, NP, FINE>);
+      else if (plan.rows == 8) attend(kv4_attention_kernel<D, DIM, 2, NQ, NP, FINE>);
+      else if (plan.rows == 16) attend(kv4_attention_kernel<D, DIM, 1, NQ, NP, FINE>);
+      else kv4_prefill(a, dtype, DIM, grid, s);
       if (plan.splits > 1) {
         const int64_t rows = tokens * q_heads;
         auto join = [&](auto groups) {

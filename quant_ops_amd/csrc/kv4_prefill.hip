@@ -1,0 +1,367 @@
+// Attention over the 4-bit cache for sequences of many rows (prompts and their chunks), 16-bit types:
+// the mathematics of kv4_attention.hip with the codes unpacked once for a workgroup.
+//
+// Four waves of 32 rows share tiles of 64 tokens: while they multiply one, each unpacks a quarter of
+// the next (its codes on their way to registers since a tile before) into the other half of LDS, as
+// fragments of v_mfma_f32_32x32x16_f16 that a wave reads with consecutive 16-byte reads. Fragments: lane
+// l = r + 32 g of an operand holds eight consecutive k of row r, a lane of the result rows 8 m + 4 g + i
+// (register 4 m + i) of column r. S^T = K Q^T (rows: 32 tokens), O^T += V^T P^T (rows: the even and then
+// the odd values of 16 pairs): lane half g has tokens 8 m + 4 g + i of a tile's weights, in the order in which
+// the values' fragments hold them, so that weights stay in their lanes.
+//
+// bf16 (EXACT false): keys and values are unpacked to what they stand for, halved (15 steps of a scale may
+// pass fp16's range), rounded to fp16: half a step of 2^-11, beside 2^-8 of the output. That takes the
+// parameters out of the softmax, whose instructions bound the kernel. fp16 (EXACT): codes less 8, the parameters
+// applied to scores in float32 and weights in two parts, as in kv4_attention.hip.
+#include "kv4_attention.h"
+
+namespace qo {
+
+namespace {
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+__device__ inline uint32_t pk(v2h v) { return __builtin_bit_cast(uint32_t, v); }
+__device__ inline v2h unpk(uint32_t u) { return __builtin_bit_cast(v2h, u); }
+// Codes as they are (EXACT: less 8), two to a word, from the low and the high halves of bytes. High codes less 8 are times 16.
+template <bool EXACT>
+__device__ inline v2h low_codes(uint32_t w, uint32_t e) {
+  return EXACT ? unpk(less_low(w, e)) : unpk((w & kLow) | e) - (v2h){(_Float16)1024.f, (_Float16)1024.f};
+}
+template <bool EXACT>
+__device__ inline v2h high_codes(uint32_t w, uint32_t e) {
+  if constexpr (EXACT) return unpk(less_high(w, e));
+  const v2h sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f}, off = {(_Float16)-64.f, (_Float16)-64.f};
+  return __builtin_elementwise_fma(unpk((w & kHigh) | e), sixteenth, off);
+}
+
+template <class D, int DIM, int NP, bool EXACT>
+__global__ void __launch_bounds__(256, DIM <= 128 ? 2 : 1)
+kv4_prefill_kernel(Attention a) {
+  constexpr int NS = DIM / 16;        // k-steps of a score
+  constexpr int NF = DIM / 32;        // blocks of 32 values
+  constexpr int NW = DIM / 32;        // words of a key's codes that a lane unpacks
+  constexpr int NV = (DIM / 2 + 63) / 64;   // pairs of values (16 tokens of each) that a lane unpacks
+  constexpr int TILE = 128;
+  using T = typename D::T;
+  struct Stage {
+    v4u k[2][NS][64];      // fragments: 32 tokens, k-step
+    v4u v[NF][4][64];      // block of values, 16 tokens
+    v4u params[4][2][4];   // EXACT: keys' s, lo, values' s, lo; lane half g; its 32 tokens, 8 to a piece
+  };
+  __shared__ Stage stage[2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, g = lane >> 5;
+  const int heads = a.cache.heads;
+  const int head = blockIdx.x % heads, split = blockIdx.x / heads / a.tiles;
+  const Rows w = find_rows<TILE>(a, blockIdx.x / heads % a.tiles);
+  if (!w.rows) return;
+
+  const int first_row = min(w.row0 + 32 * wave, w.row0 + w.rows - 1), last_row = min(first_row + 31, w.row0 + w.rows - 1);
+  const bool active = 32 * wave < w.rows;
+  const int row = min(first_row + r, last_row);
+  const Sees top = sees(a, w, first_row), bottom = sees(a, w, last_row), see = sees(a, w, row);
+  const Sees all_top = sees(a, w, w.row0), all_bottom = sees(a, w, w.row0 + w.rows - 1);
+
+  // The query in fp16, brought to 2^14 .. 2^15, in the order in which a word gives a key's codes.
+  v8h qf[NS];
+  float factor, qsum;
+  {
+    const T* q = reinterpret_cast<const T*>(a.q) + (w.start + row / a.group) * a.q_token + (head * a.group + row % a.group) * a.q_head;
+    T t[NS][8];
+    float most = 0.f;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      __builtin_memcpy(t[s], q + (2 * s + g) * 8, sizeof(t[s]));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(D::to_f(t[s][i])));
+    }
+    most = bits_float(halves_reduce(float_bits(most), FMax{}));
+    const int e = query_exponent(most);
+    float sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = ldexpf(D::to_f(t[s][kCodeOrder[i]]), e);
+        sum += v;
+        qf[s][i] = (_Float16)(EXACT && (kCodeOrder[i] & 1) ? v * 0.0625f : v);
+      }
+    sum = bits_float(halves_reduce(float_bits(sum), FAdd{}));
+    qsum = most < kInf ? sum : __builtin_nanf("");   // an infinity's scores are NaN
+    factor = fmaxf(ldexpf(a.scale * kLog2e, -e) * (EXACT ? 1.f : 2.f), 0x1p-126f);   // 0 times a masked score: no number
+  }
+
+  v16f o[NF];
+#pragma unroll
+  for (int f = 0; f < NF; ++f)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[f][i] = 0.f;
+  float most = -kInf, at = 0.f, middles = 0.f;
+  float total = qsum != qsum && see.last > see.first ? qsum : 0.f;   // infinite queries: NaN, also where all scores are -inf
+  int scale_exp = -14;
+
+  const int begin = all_top.first & ~63;
+  const int steps = all_bottom.last > begin ? (all_bottom.last - begin + 63) / 64 : 0;
+  const int per_split = (steps + a.splits - 1) / a.splits;
+  const int from = split * per_split, to = min(from + per_split, steps);
+  const int32_t* table = a.table + (w.b < a.sequences ? w.b : 0) * a.table_ld;
+  const Pages pages(a.cache, head, DIM);
+  const uint32_t exponents = exponents_of_1024();
+
+  // Unpacking: wave i takes tile i of a step's four tiles of 16 tokens. Keys: lane c + 16 d token c, words NW d ..;
+  // values: a lane the 16 tokens of pair `lane` (+ 64).
+  const int c = lane & 15, d = lane >> 4;
+  uint32_t kw[NW], key_s, key_lo, value_s, value_lo;   // the lane's token's parameters (16 bits)
+  uint32_t vs[8], vl[8];                               // those of the tile's 16 values
+  v4u vw[NV];
+  Tile tile;
+  bool bad = false;
+  auto find = [&](int step) { tile = tile_at(a, table, begin + 64 * step + 16 * wave); };
+  auto load = [&] {
+    bad = tile.bad;
+    const uint8_t* kp = pages.k + (uint64_t)(uint32_t)tile.page * pages.codes + ((tile.place + c) * (DIM / 2) + d * (4 * NW));
+    const uint8_t* vp = pages.v + (uint64_t)(uint32_t)tile.page * pages.codes + (tile.place * (DIM / 2) + lane * 16);
+    const uint8_t* par = pages.params + (uint64_t)(uint32_t)tile.page * pages.param_bytes + tile.place * 4;
+    __builtin_memcpy(kw, kp, sizeof(kw));
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (64 * i + lane < DIM / 2) vw[i] = *reinterpret_cast<const v4u*>(vp + 1024 * i);
+    const uint16_t* ks = reinterpret_cast<const uint16_t*>(par) + c;
+    const uint16_t* vss = reinterpret_cast<const uint16_t*>(par + pages.param_values) + c;
+    key_s = ks[0], key_lo = ks[16], value_s = vss[0], value_lo = vss[16];
+    if constexpr (!EXACT) {
+      __builtin_memcpy(vs, par + pages.param_values, sizeof(vs));
+      __builtin_memcpy(vl, par + pages.param_values + 32, sizeof(vl));
+    }
+  };
+  auto unpack = [&](Stage& st, int step) {
+    // A value that is no number (or on a page outside the cache) becomes 0 and its key NaN: the rows that see the
+    // token are NaN then, and the others are not.
+    const bool finite = (value_s & 0x7C00u) != 0x7C00u && (value_lo & 0x7C00u) != 0x7C00u && !bad;
+    if (!finite) key_s = key_lo = 0x7E00u;
+    const int t = begin + 64 * step + 16 * wave + c;
+    if (!finite || t < all_top.first || t >= all_bottom.last) value_s = value_lo = 0u;   // unseen ones have no say in S
+    if constexpr (!EXACT) {
+      if (__any(!finite)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t keep = __builtin_amdgcn_readlane((int)finite, i) ? 0xFFFFFFFFu : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+          vs[i / 2] &= keep;
+          vl[i / 2] &= keep;
+        }
+      }
+    }
+    const v2h half = {(_Float16)0.5f, (_Float16)0.5f};
+    v2h s2 = unpk(key_s | key_s << 16), lo2 = unpk(key_lo | key_lo << 16);
+    if constexpr (!EXACT) s2 *= half, lo2 *= half;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      const int word = d * NW + i;   // of the token's row: dims 8 word ..
+      const uint32_t x = kw[i], h = x >> 8;
+      v2h f[4] = {low_codes<EXACT>(x, exponents), high_codes<EXACT>(x, exponents), low_codes<EXACT>(h, exponents), high_codes<EXACT>(h, exponents)};
+      if constexpr (!EXACT) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = __builtin_elementwise_fma(f[j], s2, lo2);
+      }
+      st.k[wave >> 1][word >> 1][(wave & 1) * 16 + c + 32 * (word & 1)] = (v4u){pk(f[0]), pk(f[1]), pk(f[2]), pk(f[3])};
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (64 * i + lane < DIM / 2) {
+        const int pair = 64 * i + lane;
+        v4u even[2], odd[2];   // of lane half g: tokens 4 g .. and 8 + 4 g ..
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {   // tokens 4 q + 2 h, and the next
+            const uint32_t two = __builtin_amdgcn_perm(0, vw[i][q], h ? 0x0C030C02u : 0x0C010C00u);
+            v2h x = low_codes<EXACT>(two, exponents), y = high_codes<EXACT>(two, exponents);
+            if constexpr (!EXACT) {
+              const v2h s = unpk(vs[2 * q + h]) * half, lo = unpk(vl[2 * q + h]) * half;
+              x = __builtin_elementwise_fma(x, s, lo);
+              y = __builtin_elementwise_fma(y, s, lo);
+            }
+            even[q & 1][2 * (q >> 1) + h] = pk(x);
+            odd[q & 1][2 * (q >> 1) + h] = pk(y);
+          }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          st.v[pair >> 4][wave][(pair & 15) + 32 * h] = even[h];
+          st.v[pair >> 4][wave][(pair & 15) + 16 + 32 * h] = odd[h];
+        }
+      }
+    if constexpr (EXACT) {
+      // token 16 wave + c of the step: of lane half (c / 4) % 2, its token 8 wave + 4 (c / 8) + c % 4
+      if (d == 0) {
+        const int half_of_c = c >> 2 & 1, place = 8 * wave + 4 * (c >> 3) + (c & 3);
+        auto put = [&](int which, uint32_t x) { reinterpret_cast<uint16_t*>(&st.params[which][half_of_c][0])[place] = (uint16_t)x; };
+        put(0, key_s), put(1, key_lo), put(2, value_s), put(3, value_lo);
+      }
+    }
+  };
+
+  if (from < to) {
+    find(from);
+    load();
+    find(from + 1);
+    unpack(stage[0], from);
+    if (from + 1 < to) {
+      load();
+      find(from + 2);
+    }
+    lds_barrier();
+  }
+  for (int step = from; step < to; ++step) {
+    const Stage& st = stage[(step - from) & 1];
+    if (step + 1 < to) {
+      unpack(stage[(step - from + 1) & 1], step + 1);
+      if (step + 2 < to) {
+        load();
+        find(step + 3);
+      }
+    }
+    const int t0 = begin + 64 * step;
+    if (active && t0 < bottom.last && t0 + 64 > top.first) {
+      v16f sc[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[u][i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, st.k[u][s][lane]), qf[s], sc[u], 0, 0, 0);
+      }
+      uint32_t vs[16], vl[16];   // EXACT: of the lane's 32 tokens
+      int exp_now = scale_exp;
+      float eight = 0.f;
+      if constexpr (EXACT) {
+        uint32_t ks[16], kl[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const v4u x = st.params[0][g][i], y = st.params[1][g][i], z = st.params[2][g][i], t = st.params[3][g][i];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) ks[4 * i + j] = x[j], kl[4 * i + j] = y[j], vs[4 * i + j] = z[j], vl[4 * i + j] = t[j];
+        }
+#pragma unroll
+        for (int t = 0; t < 32; ++t) {
+          const float s = half_of(ks, t);
+          sc[t / 16][t % 16] = fmaf(s, sc[t / 16][t % 16], fmaf(8.f, s, half_of(kl, t)) * qsum);
+        }
+        uint32_t big = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) big = pk_max_u16(big, vs[i]);
+        const uint32_t field = halves_reduce(max(big & 0xFFFFu, big >> 16) >> 10, UMax{});
+        exp_now = max(scale_exp, __builtin_amdgcn_readfirstlane((int)field) - 14);
+        const int up = 14 - exp_now;
+        auto by_power = [&](int e) {
+          const _Float16 f = (_Float16)power_of_two(e);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) vs[i] = pk(unpk(vs[i]) * (v2h){f, f});
+        };
+        by_power(min(up, 15));
+        if (up > 15) by_power(up - 15);
+        eight = power_of_two(3 - up);
+      }
+      if (!(t0 + 64 <= top.last && t0 >= bottom.first)) {   // some row does not see some token
+#pragma unroll
+        for (int t = 0; t < 32; ++t) {
+          const int at_t = t0 + t / 16 * 32 + t % 16 / 4 * 8 + 4 * g + t % 4;
+          if (at_t < see.first || at_t >= see.last) sc[t / 16][t % 16] = -kInf;
+        }
+      }
+      float now = most;
+#pragma unroll
+      for (int t = 0; t < 32; ++t) now = fmaxf(now, sc[t / 16][t % 16]);
+      now = bits_float(halves_reduce(float_bits(now), FMax{}));
+      if (__any(now > most) || exp_now > scale_exp) {
+        const float next = now == -kInf ? 0.f : factor * now - (EXACT ? 0.f : 14.f);   // weights up to 1 (not EXACT: 2^14)
+        const float shrink = most == -kInf ? 1.f : __builtin_amdgcn_exp2f(at - next);   // before: all sums 0
+        const float shrink_o = shrink * power_of_two(scale_exp - exp_now);
+        most = now;
+        at = next;
+        total *= shrink;
+        middles *= shrink;
+        scale_exp = exp_now;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) o[f] *= shrink_o;
+      }
+      v8h ph[4], pl[4];
+#pragma unroll
+      for (int t = 0; t < 32; ++t) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(factor, sc[t / 16][t % 16], -at));
+        total += p;
+        if constexpr (EXACT) {
+          const float s = half_of(vs, t);
+          middles = fmaf(p, fmaf(eight, s, half_of(vl, t)), middles);
+          _Float16 h = (_Float16)fmaf(p, s, 0.f);
+          if constexpr (NP > 1) {
+            asm("" : "+v"(h));   // one and the same rounding in both parts
+            pl[t / 8][t % 8] = (_Float16)fmaf(p, s, -(float)h);
+          }
+          ph[t / 8][t % 8] = h;
+        } else {
+          ph[t / 8][t % 8] = (_Float16)p;
+        }
+      }
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const v8h v = __builtin_bit_cast(v8h, st.v[f][i][lane]);
+          o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[i], o[f], 0, 0, 0);
+          if constexpr (NP > 1) o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[i], o[f], 0, 0, 0);
+        }
+    }
+    lds_barrier();
+  }
+  if (!active) return;
+
+  total = bits_float(halves_reduce(float_bits(total), FAdd{}));
+  middles = bits_float(halves_reduce(float_bits(middles), FAdd{}));
+  if (most == -kInf && total == 0.f) at = -kInf;
+  if (w.poison) total = __builtin_nanf(""), at = 0.f;
+  if (first_row + r > last_row) return;
+  const float unit = EXACT ? power_of_two(scale_exp - 14) : 2.f;
+  const int64_t total_rows = (int64_t)a.tokens * a.q_heads;   // of all heads
+  const int64_t at_row = (int64_t)(w.start + row / a.group) * a.q_heads + head * a.group + row % a.group;
+#pragma unroll
+  for (int f = 0; f < NF; ++f)
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {   // values 32 f + 16 m + 8 g ..: pairs 16 f + 8 m + 4 g + i
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = fmaf(o[f][4 * m + i], unit, middles);
+        v[2 * i + 1] = fmaf(o[f][8 + 4 * m + i], EXACT ? unit * 0.0625f : unit, middles);
+      }
+      if (a.splits > 1) {
+        __builtin_memcpy(a.part + (split * total_rows + at_row) * DIM + 32 * f + 16 * m + 8 * g, v, sizeof(v));
+      } else {
+        T out[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) out[i] = D::from_f(total == 0.f ? 0.f : v[i] / total);
+        __builtin_memcpy(reinterpret_cast<T*>(a.out) + at_row * DIM + 32 * f + 16 * m + 8 * g, out, sizeof(out));
+      }
+    }
+  if (a.splits > 1 && g == 0) {
+    float* ml = a.part + a.splits * total_rows * DIM + (split * total_rows + at_row) * 2;
+    ml[0] = at;
+    ml[1] = total;
+  }
+}
+
+}  // namespace
+
+void kv4_prefill(const Attention& a, int dtype, int dim, int64_t grid, hipStream_t stream) {
+  auto go = [&](auto n) {
+    constexpr int DIM = decltype(n)::value;
+    if (dtype == QO_DTYPE_BF16) launch(kv4_prefill_kernel<BF16T, DIM, 1, false>, dim3((unsigned)grid), dim3(256), 0, stream, a);
+    else launch(kv4_prefill_kernel<F16T, DIM, 2, true>, dim3((unsigned)grid), dim3(256), 0, stream, a);
+  };
+  if (dim == 64) go(std::integral_constant<int, 64>{});
+  else if (dim == 96) go(std::integral_constant<int, 96>{});
+  else if (dim == 128) go(std::integral_constant<int, 128>{});
+  else if (dim == 192) go(std::integral_constant<int, 192>{});
+  else go(std::integral_constant<int, 256>{});
+}
+
+}  // namespace qo

@@ -181,6 +181,13 @@ GPU_CASES = [
     ([300, 5], 16, 1, 96, 256, [100, 1], 40),
     ([400], 7, 1, 128, 16, 90, 0),
     ([140] * 70, 2, 1, 64, 16, [1] * 35 + [0] * 20 + [2] * 15, 0),   # more sequences than a wave has lanes
+    ([200, 330], 4, 2, 128, 16, 50, 0),            # more than 64 rows a sequence
+    ([500], 8, 1, 64, 64, 40, 0),
+    ([257, 64, 1], 6, 2, 96, 32, [130, 64, 1], 0),
+    ([300], 3, 1, 192, 16, 100, 130),
+    ([150, 90], 5, 1, 256, 16, 30, 0),
+    ([100], 2, 1, 128, 16, 150, 0),
+    ([700, 20], 2, 2, 128, 32, [300, 20], 200),
     ([3], 1, 1, 256, 16, 3, 0),
     ([2], 2, 1, 128, 16, 40, 0),       # queries before the first token
 ]
@@ -211,6 +218,28 @@ def test_masked_values_only(gpu):
     got = _run(gpu, q, cache, table, lengths)
     assert not torch.isnan(got[:4]).any() and torch.isnan(got[4:]).all()
     check(q, got, cache, table, lengths, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_masked_places_in_prompts(gpu, dtype):
+    """The same for sequences of many rows: garbage behind the last token and before the window, a token whose
+    value is NaN, one whose key is, a page outside the cache, and NaN and infinite queries."""
+    q, cache, table, lengths, _, _ = make(([230, 150], 2, 1, 128, 16, 100, 60), dtype)   # queries from 130 and 50 on
+    for b, t in ((0, 170), (1, 100)):
+        cache.params[int(table[b, t // 16]), 1 - b, :, t % 16 // 16, 0, t % 16] = float("nan")
+    for t in list(range(0, 70)) + list(range(230, 240)):
+        cache.params[int(table[0, t // 16]), :, :, 0, :, t % 16] = float("inf")
+    table[1, 9] = -1                                        # tokens 144 ..
+    q[20, 1, 7], q[30, 0, 100] = float("nan"), -float("inf")
+    got = _run(gpu, q, cache, table, lengths, window=60)
+    i = torch.arange(200)
+    p = torch.where(i < 100, 130 + i, i - 50)
+    bad = torch.where(i < 100, (p >= 170) & (p < 230), (p >= 100) & (p < 160))[:, None].repeat(1, 2)
+    bad[20, 1] = bad[30, 0] = True
+    assert torch.equal(torch.isnan(got).any(2).cpu(), bad) and torch.equal(torch.isnan(got).all(2).cpu(), bad)
+    q[20, 1, 7] = q[30, 0, 100] = 0.0
+    got = _run(gpu, q, cache, table, lengths, window=60)
+    check(q, got, cache, table, lengths, 128 ** -0.5, None, 60)
 
 
 def test_bad_pages_and_lengths(gpu):
