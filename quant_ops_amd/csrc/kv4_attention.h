@@ -32,6 +32,7 @@ struct Attention {
   int window;                 // 0: none
   int tiles;                  // row tiles of all sequences
   int splits;
+  bool paired;                // all workgroups run at once
   float* part;                // [splits][tokens * q_heads][DIM], then [splits][tokens * q_heads][2]
 };
 
@@ -119,7 +120,11 @@ __device__ inline Rows find_rows(const Attention& a, int tile) {
     w.b = tile / per;
     w.start = w.b * a.each;
     w.count = a.each;
-    w.row0 = (per - 1 - tile % per) * TILE;   // those that see most tokens first
+    // those that see most tokens first; where all workgroups run at once, two to a CU, the second half from the
+    // other end: a CU's two are the longest and the shortest, and so on
+    const int k = tile % per;
+    const int first = a.paired ? (per + 1) / 2 : per;
+    w.row0 = (k < first ? per - 1 - k : k - first) * TILE;
   }
   const int all = w.count * a.group;
   w.rows = w.row0 < 0 || w.row0 >= all ? 0 : all - w.row0 < TILE ? all - w.row0 : TILE;   // below 0: q_starts that do not ascend

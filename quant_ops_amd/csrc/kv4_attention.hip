@@ -559,6 +559,7 @@ extern "C" int qo_kv4_attention(const qo_kv4_cache* cache, const qo_heads* q, in
                        c.pages ? (int)table_width : 0,   // without pages there is nothing to read
                        lengths, q_starts, (int)tokens, (int)sequences, sequences ? (int)(tokens / sequences) : 0, q_heads,
                        q_heads / c.heads, scale, window < kMostTokens ? (int)window : 0, (int)plan.tiles, plan.splits,
+                       sequences == 1 && grid <= 2 * device_cu_count(),
                        reinterpret_cast<float*>(workspace)};
   launch_begin();
   auto go = [&](auto d, auto parts_q, auto parts_p, auto fine) {

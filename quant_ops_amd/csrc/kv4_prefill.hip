@@ -222,13 +222,28 @@ kv4_prefill_kernel(Attention a) {
     }
     const int t0 = begin + 64 * step;
     if (active && t0 < bottom.last && t0 + 64 > top.first) {
+      // Fragments come from LDS four ahead of the products: 128 cycles, about what a read takes.
+      v8h frag[2][4];
+      auto fetch = [&](const v4u(*from)[64], int group) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) frag[group & 1][i] = __builtin_bit_cast(v8h, from[4 * group + i][lane]);
+        __builtin_amdgcn_sched_barrier(0);
+      };
       v16f sc[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[u][i] = 0.f;
+      fetch(&st.k[0][0], 0);
 #pragma unroll
-        for (int s = 0; s < NS; ++s) sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, st.k[u][s][lane]), qf[s], sc[u], 0, 0, 0);
+      for (int group = 0; group < NS / 2; ++group) {
+        if (group + 1 < NS / 2) fetch(&st.k[0][0], group + 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int u = (4 * group + i) / NS, k = (4 * group + i) % NS;
+          sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(frag[group & 1][i], qf[k], sc[u], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
       uint32_t vs[16], vl[16];   // EXACT: of the lane's 32 tokens
       int exp_now = scale_exp;
@@ -284,6 +299,7 @@ kv4_prefill_kernel(Attention a) {
 #pragma unroll
         for (int f = 0; f < NF; ++f) o[f] *= shrink_o;
       }
+      fetch(&st.v[0][0], 0);
       v8h ph[4], pl[4];
 #pragma unroll
       for (int t = 0; t < 32; ++t) {
@@ -303,13 +319,15 @@ kv4_prefill_kernel(Attention a) {
         }
       }
 #pragma unroll
-      for (int f = 0; f < NF; ++f)
+      for (int f = 0; f < NF; ++f) {
+        if (f + 1 < NF) fetch(&st.v[0][0], f + 1);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const v8h v = __builtin_bit_cast(v8h, st.v[f][i][lane]);
-          o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[i], o[f], 0, 0, 0);
-          if constexpr (NP > 1) o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[i], o[f], 0, 0, 0);
+          o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(frag[f & 1][i], ph[i], o[f], 0, 0, 0);
+          if constexpr (NP > 1) o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(frag[f & 1][i], pl[i], o[f], 0, 0, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     lds_barrier();
   }
