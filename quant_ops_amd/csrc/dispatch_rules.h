@@ -158,10 +158,10 @@ inline MxPlan mx_plan(int64_t M, int64_t N, int64_t blocks, bool fp8, int64_t cu
 
 // Rows and workgroups of attention over the 4-bit cache (a row: a query of one of the heads that
 // share a KV head). A workgroup has four waves of `rows` rows; up to 16 they read the cache each for
-// itself and waves without rows of their own share others' tokens; with 32 they share the tiles that they
-// read (kv4_prefill, 16-bit types). `splits` workgroups share a tile's tokens.
+// itself and waves without rows of their own share others' tokens; with 32 (and 64: eight waves of 32)
+// they share the tiles that they read (kv4_prefill, 16-bit types). `splits` workgroups share a tile's tokens.
 struct Kv4Plan {
-  int rows;        // 4, 8, 16 or 32
+  int rows;        // 4, 8, 16, 32 or 64
   int64_t tiles;   // of 4 rows, of all sequences
   int splits;
 };
@@ -169,13 +169,13 @@ inline Kv4Plan kv4_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64
                         int64_t sequences, bool ragged, int64_t window, bool f32, int64_t cus) {
   const int64_t group = q_heads / kv_heads, rows = tokens * group;
   const int64_t each = sequences > 0 ? (rows + sequences - 1) / sequences : 0;
-  Kv4Plan p = {each <= 4 ? 4 : each <= 8 ? 8 : f32 || each <= 64 ? 16 : 32, 0, 1};
+  Kv4Plan p = {each <= 4 ? 4 : each <= 8 ? 8 : f32 || each <= 64 ? 16 : each <= 128 || head_dim > 128 ? 32 : 64, 0, 1};
   const int64_t tile = 4 * p.rows;
   p.tiles = ragged ? rows / tile + sequences + 1 : sequences * ((each + tile - 1) / tile);
   // a split's share of the longest sequence is 256 tokens at least
   const int64_t queries = sequences > 0 ? (tokens + sequences - 1) / sequences : 0;
   const int64_t longest = window > 0 && window + queries < capacity ? window + queries : capacity;
-  const int64_t groups = p.tiles * kv_heads, want = ((p.rows == 32 ? 1 : 4) * cus + groups - 1) / groups, most = longest / 256;
+  const int64_t groups = p.tiles * kv_heads, want = ((p.rows >= 32 ? 1 : 4) * cus + groups - 1) / groups, most = longest / 256;
   const int64_t n = want < most ? want : most;
   p.splits = n < 1 ? 1 : n > 64 ? 64 : (int)n;
   return p;

@@ -32,7 +32,6 @@ struct Attention {
   int window;                 // 0: none
   int tiles;                  // row tiles of all sequences
   int splits;
-  bool paired;                // all workgroups run at once
   float* part;                // [splits][tokens * q_heads][DIM], then [splits][tokens * q_heads][2]
 };
 
@@ -87,12 +86,12 @@ __device__ inline uint32_t exponents_of_1024() {
 }
 constexpr int kCodeOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};   // of a word's codes, as masks and shifts by 8 take them out
 
-// A workgroup's rows: of sequence b (or, b = sequences, behind the last), queries start .. start + count - 1, rows
-// row0 .. row0 + rows - 1 of the sequence's. Tiles of ragged sequences are counted from q_starts[b] * group /
-// TILE + b on, which leaves room for every one's last.
+// Where a workgroup's rows are: sequence b (or, b = sequences, behind the last), whose queries are start .. start +
+// count - 1, and the number `index` of its tiles of TILE rows (below 0 or past the last: nothing). Tiles of ragged
+// sequences are counted from q_starts[b] * group / TILE + b on, which leaves room for every one's last.
 struct Rows {
-  int b, start, count, row0, rows, length;
-  bool poison;   // the sequence is longer than its row of the table
+  int b, start, count, index, all, length;   // all: rows of the sequence
+  bool poison;                               // the sequence is longer than its row of the table
 };
 template <int TILE>
 __device__ inline Rows find_rows(const Attention& a, int tile) {
@@ -114,21 +113,17 @@ __device__ inline Rows find_rows(const Attention& a, int tile) {
     w.start = begin_of(w.b);
     const int end = w.b < a.sequences ? begin_of(w.b + 1) : a.tokens;
     w.count = end > w.start ? end - w.start : 0;
-    w.row0 = (tile - (w.start * a.group / TILE + w.b)) * TILE;
+    w.index = tile - (w.start * a.group / TILE + w.b);   // below 0: q_starts that do not ascend
   } else {
     const int per = (a.each * a.group + TILE - 1) / TILE;
     w.b = tile / per;
     w.start = w.b * a.each;
     w.count = a.each;
-    // those that see most tokens first; where all workgroups run at once, two to a CU, the second half from the
-    // other end: a CU's two are the longest and the shortest, and so on
-    const int k = tile % per;
-    const int first = a.paired ? (per + 1) / 2 : per;
-    w.row0 = (k < first ? per - 1 - k : k - first) * TILE;
+    w.index = tile % per;
   }
-  const int all = w.count * a.group;
-  w.rows = w.row0 < 0 || w.row0 >= all ? 0 : all - w.row0 < TILE ? all - w.row0 : TILE;   // below 0: q_starts that do not ascend
-  w.length = w.rows && w.b < a.sequences ? a.lengths[w.b] : 0;
+  w.all = w.count * a.group;
+  if (w.index < 0 || (int64_t)w.index * TILE >= w.all) w.all = 0;
+  w.length = w.all && w.b < a.sequences ? a.lengths[w.b] : 0;
   const int shift = a.cache.shift, pages = w.length >> shift;
   w.poison = w.length > kMostTokens || pages > a.width || (pages == a.width && (w.length & ((1 << shift) - 1)));
   if (w.length < 0 || w.poison) w.length = 0;
@@ -177,7 +172,7 @@ __device__ inline int query_exponent(float most) {
   return most > 0.f && most < kInf ? min(max(15 - __builtin_amdgcn_frexp_expf(most), -100), 60) : 0;
 }
 
-// Starts the kernel for more than 64 rows a sequence (16-bit types); the grid is that of kv4_plan.
-void kv4_prefill(const Attention& a, int dtype, int dim, int64_t grid, hipStream_t stream);
+// Starts the kernel for many rows a sequence (16-bit types), in tiles of 128 or 256; the grid is that of kv4_plan.
+void kv4_prefill(const Attention& a, int dtype, int dim, int tile, int64_t grid, hipStream_t stream);
 
 }  // namespace qo

@@ -91,15 +91,16 @@ kv4_attention_kernel(Attention a) {
   const int heads = a.cache.heads;
   const int head = blockIdx.x % heads, split = blockIdx.x / heads / a.tiles;
   const Rows w = find_rows<TILE>(a, blockIdx.x / heads % a.tiles);
-  if (!w.rows) return;
+  if (!w.all) return;
+  const int row0 = w.index * TILE, rows = min(w.all - row0, TILE);
 
   // The waves' rows; waves with the same rows take turns at their tokens.
-  const int blocks = (w.rows + CW - 1) / CW;
+  const int blocks = (rows + CW - 1) / CW;
   const int sharing = blocks == 1 ? 4 : blocks == 2 ? 2 : 1;
   const int mine = wave / sharing, turn_of = wave % sharing;
   const bool active = mine < blocks;
-  const int first_row = w.row0 + (active ? mine : 0) * CW;
-  const int last_row = min(first_row + CW, w.row0 + w.rows) - 1;
+  const int first_row = row0 + (active ? mine : 0) * CW;
+  const int last_row = min(first_row + CW, row0 + rows) - 1;
   const int row = min(first_row + r % CW, last_row);
   const Sees top = sees(a, w, first_row), bottom = sees(a, w, last_row), see = sees(a, w, row);
 
@@ -559,7 +560,6 @@ extern "C" int qo_kv4_attention(const qo_kv4_cache* cache, const qo_heads* q, in
                        c.pages ? (int)table_width : 0,   // without pages there is nothing to read
                        lengths, q_starts, (int)tokens, (int)sequences, sequences ? (int)(tokens / sequences) : 0, q_heads,
                        q_heads / c.heads, scale, window < kMostTokens ? (int)window : 0, (int)plan.tiles, plan.splits,
-                       sequences == 1 && grid <= 2 * device_cu_count(),
                        reinterpret_cast<float*>(workspace)};
   launch_begin();
   auto go = [&](auto d, auto parts_q, auto parts_p, auto fine) {
@@ -573,7 +573,7 @@ extern "C" int qo_kv4_attention(const qo_kv4_cache* cache, const qo_heads* q, in
       if (plan.rows == 4) attend(kv4_attention_kernel<D, DIM, 4, NQ, NP, FINE>);
       else if (plan.rows == 8) attend(kv4_attention_kernel<D, DIM, 2, NQ, NP, FINE>);
       else if (plan.rows == 16) attend(kv4_attention_kernel<D, DIM, 1, NQ, NP, FINE>);
-      else kv4_prefill(a, dtype, DIM, grid, s);
+      else kv4_prefill(a, dtype, DIM, 4 * plan.rows, grid, s);
       if (plan.splits > 1) {
         const int64_t rows = tokens * q_heads;
         auto join = [&](auto groups) {

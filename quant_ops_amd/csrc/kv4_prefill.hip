@@ -19,6 +19,15 @@ namespace qo {
 
 namespace {
 
+#ifndef KV4_V1
+#define KV4_V1 3
+#define KV4_V2 3
+#endif
+// A weight at the row's reference, in fp16, and how far (exponents) a larger score may pass the reference before
+// sums and outputs move to it: each row's maximum grows now and then, some row's of 32 nearly every step.
+constexpr int kAtRest = 6;
+constexpr float kSlack = 8.f;
+
 typedef float v16f __attribute__((ext_vector_type(16)));
 
 __device__ inline uint32_t pk(v2h v) { return __builtin_bit_cast(uint32_t, v); }
@@ -35,14 +44,14 @@ __device__ inline v2h high_codes(uint32_t w, uint32_t e) {
   return __builtin_elementwise_fma(unpk((w & kHigh) | e), sixteenth, off);
 }
 
-template <class D, int DIM, int NP, bool EXACT>
-__global__ void __launch_bounds__(256, DIM <= 128 ? 2 : 1)
+template <class D, int DIM, int NP, bool EXACT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, DIM <= 128 ? 2 : 1)
 kv4_prefill_kernel(Attention a) {
   constexpr int NS = DIM / 16;        // k-steps of a score
   constexpr int NF = DIM / 32;        // blocks of 32 values
   constexpr int NW = DIM / 32;        // words of a key's codes that a lane unpacks
   constexpr int NV = (DIM / 2 + 63) / 64;   // pairs of values (16 tokens of each) that a lane unpacks
-  constexpr int TILE = 128;
+  constexpr int TILE = 32 * WAVES;
   using T = typename D::T;
   struct Stage {
     v4u k[2][NS][64];      // fragments: 32 tokens, k-step
@@ -54,13 +63,23 @@ kv4_prefill_kernel(Attention a) {
   const int heads = a.cache.heads;
   const int head = blockIdx.x % heads, split = blockIdx.x / heads / a.tiles;
   const Rows w = find_rows<TILE>(a, blockIdx.x / heads % a.tiles);
-  if (!w.rows) return;
+  if (!w.all) return;
 
-  const int first_row = min(w.row0 + 32 * wave, w.row0 + w.rows - 1), last_row = min(first_row + 31, w.row0 + w.rows - 1);
-  const bool active = 32 * wave < w.rows;
+  // Waves 0 .. 3 have one tile of 128 rows, 4 .. 7 another: its mirror image from the sequence's end, so that all
+  // workgroups have the same work (with a window the next one, which sees the same tokens).
+  const int tiles = (w.all + 127) / 128;
+  int mine = w.index, other = w.index;
+  if constexpr (WAVES == 8) {
+    const int a_tile = a.window ? 2 * w.index : w.index, b_tile = a.window ? 2 * w.index + 1 : tiles - 1 - w.index;
+    mine = wave < 4 ? b_tile : a_tile;
+    other = wave < 4 ? a_tile : b_tile;
+  }
+  const bool active = mine * 128 + 32 * (wave & 3) < w.all && (wave < 4 || mine != other);
+  const int first_row = min(mine * 128 + 32 * (wave & 3), w.all - 1), last_row = min(first_row + 31, w.all - 1);
   const int row = min(first_row + r, last_row);
   const Sees top = sees(a, w, first_row), bottom = sees(a, w, last_row), see = sees(a, w, row);
-  const Sees all_top = sees(a, w, w.row0), all_bottom = sees(a, w, w.row0 + w.rows - 1);
+  const Sees all_top = sees(a, w, min(min(mine, other) * 128, w.all - 1));
+  const Sees all_bottom = sees(a, w, min(max(mine, other) * 128 + 127, w.all - 1));
 
   // The query in fp16, brought to 2^14 .. 2^15, in the order in which a word gives a key's codes.
   v8h qf[NS];
@@ -108,28 +127,30 @@ kv4_prefill_kernel(Attention a) {
   const Pages pages(a.cache, head, DIM);
   const uint32_t exponents = exponents_of_1024();
 
-  // Unpacking: wave i takes tile i of a step's four tiles of 16 tokens. Keys: lane c + 16 d token c, words NW d ..;
+  // Unpacking: wave i takes tile i % 4 of a step's four tiles of 16 tokens, of eight waves the first its keys and
+  // the others its values. Keys: lane c + 16 d token c, words NW d ..;
   // values: a lane the 16 tokens of pair `lane` (+ 64).
-  const int c = lane & 15, d = lane >> 4;
+  const int c = lane & 15, d = lane >> 4, part = wave & 3;
+  const bool keys = WAVES == 4 || wave < 4, values_too = WAVES == 4 || wave >= 4;
   uint32_t kw[NW], key_s, key_lo, value_s, value_lo;   // the lane's token's parameters (16 bits)
   uint32_t vs[8], vl[8];                               // those of the tile's 16 values
   v4u vw[NV];
   Tile tile;
   bool bad = false;
-  auto find = [&](int step) { tile = tile_at(a, table, begin + 64 * step + 16 * wave); };
+  auto find = [&](int step) { tile = tile_at(a, table, begin + 64 * step + 16 * part); };
   auto load = [&] {
     bad = tile.bad;
     const uint8_t* kp = pages.k + (uint64_t)(uint32_t)tile.page * pages.codes + ((tile.place + c) * (DIM / 2) + d * (4 * NW));
     const uint8_t* vp = pages.v + (uint64_t)(uint32_t)tile.page * pages.codes + (tile.place * (DIM / 2) + lane * 16);
     const uint8_t* par = pages.params + (uint64_t)(uint32_t)tile.page * pages.param_bytes + tile.place * 4;
-    __builtin_memcpy(kw, kp, sizeof(kw));
+    if (keys) __builtin_memcpy(kw, kp, sizeof(kw));
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (64 * i + lane < DIM / 2) vw[i] = *reinterpret_cast<const v4u*>(vp + 1024 * i);
+      if (values_too && 64 * i + lane < DIM / 2) vw[i] = *reinterpret_cast<const v4u*>(vp + 1024 * i);
     const uint16_t* ks = reinterpret_cast<const uint16_t*>(par) + c;
     const uint16_t* vss = reinterpret_cast<const uint16_t*>(par + pages.param_values) + c;
     key_s = ks[0], key_lo = ks[16], value_s = vss[0], value_lo = vss[16];
-    if constexpr (!EXACT) {
+    if (!EXACT && values_too) {
       __builtin_memcpy(vs, par + pages.param_values, sizeof(vs));
       __builtin_memcpy(vl, par + pages.param_values + 32, sizeof(vl));
     }
@@ -139,9 +160,9 @@ kv4_prefill_kernel(Attention a) {
     // token are NaN then, and the others are not.
     const bool finite = (value_s & 0x7C00u) != 0x7C00u && (value_lo & 0x7C00u) != 0x7C00u && !bad;
     if (!finite) key_s = key_lo = 0x7E00u;
-    const int t = begin + 64 * step + 16 * wave + c;
+    const int t = begin + 64 * step + 16 * part + c;
     if (!finite || t < all_top.first || t >= all_bottom.last) value_s = value_lo = 0u;   // unseen ones have no say in S
-    if constexpr (!EXACT) {
+    if (!EXACT && values_too) {
       if (__any(!finite)) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -154,6 +175,7 @@ kv4_prefill_kernel(Attention a) {
     const v2h half = {(_Float16)0.5f, (_Float16)0.5f};
     v2h s2 = unpk(key_s | key_s << 16), lo2 = unpk(key_lo | key_lo << 16);
     if constexpr (!EXACT) s2 *= half, lo2 *= half;
+    if (keys) {
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
       const int word = d * NW + i;   // of the token's row: dims 8 word ..
@@ -163,11 +185,12 @@ kv4_prefill_kernel(Attention a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[j] = __builtin_elementwise_fma(f[j], s2, lo2);
       }
-      st.k[wave >> 1][word >> 1][(wave & 1) * 16 + c + 32 * (word & 1)] = (v4u){pk(f[0]), pk(f[1]), pk(f[2]), pk(f[3])};
+      st.k[part >> 1][word >> 1][(part & 1) * 16 + c + 32 * (word & 1)] = (v4u){pk(f[0]), pk(f[1]), pk(f[2]), pk(f[3])};
+    }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (64 * i + lane < DIM / 2) {
+      if (values_too && 64 * i + lane < DIM / 2) {
         const int pair = 64 * i + lane;
         v4u even[2], odd[2];   // of lane half g: tokens 4 g .. and 8 + 4 g ..
 #pragma unroll
@@ -186,14 +209,14 @@ kv4_prefill_kernel(Attention a) {
           }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          st.v[pair >> 4][wave][(pair & 15) + 32 * h] = even[h];
-          st.v[pair >> 4][wave][(pair & 15) + 16 + 32 * h] = odd[h];
+          st.v[pair >> 4][part][(pair & 15) + 32 * h] = even[h];
+          st.v[pair >> 4][part][(pair & 15) + 16 + 32 * h] = odd[h];
         }
       }
     if constexpr (EXACT) {
-      // token 16 wave + c of the step: of lane half (c / 4) % 2, its token 8 wave + 4 (c / 8) + c % 4
-      if (d == 0) {
-        const int half_of_c = c >> 2 & 1, place = 8 * wave + 4 * (c >> 3) + (c & 3);
+      // token 16 part + c of the step: of lane half (c / 4) % 2, its token 8 part + 4 (c / 8) + c % 4
+      if (keys && d == 0) {
+        const int half_of_c = c >> 2 & 1, place = 8 * part + 4 * (c >> 3) + (c & 3);
         auto put = [&](int which, uint32_t x) { reinterpret_cast<uint16_t*>(&st.params[which][half_of_c][0])[place] = (uint16_t)x; };
         put(0, key_s), put(1, key_lo), put(2, value_s), put(3, value_lo);
       }
@@ -222,112 +245,150 @@ kv4_prefill_kernel(Attention a) {
     }
     const int t0 = begin + 64 * step;
     if (active && t0 < bottom.last && t0 + 64 > top.first) {
-      // Fragments come from LDS four ahead of the products: 128 cycles, about what a read takes.
-      v8h frag[2][4];
-      auto fetch = [&](const v4u(*from)[64], int group) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) frag[group & 1][i] = __builtin_bit_cast(v8h, from[4 * group + i][lane]);
-        __builtin_amdgcn_sched_barrier(0);
-      };
       v16f sc[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
+      v8h ph[4], pl[4];
+      // The scores of 32 tokens.
+      auto scores = [&](int u) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[u][i] = 0.f;
-      fetch(&st.k[0][0], 0);
 #pragma unroll
-      for (int group = 0; group < NS / 2; ++group) {
-        if (group + 1 < NS / 2) fetch(&st.k[0][0], group + 1);
+        for (int k = 0; k < NS; ++k)
+          sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, st.k[u][k][lane]), qf[k], sc[u], 0, 0, 0);
+      };
+      // Their weights' product with the values.
+      auto values = [&](int u) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int u = (4 * group + i) / NS, k = (4 * group + i) % NS;
-          sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(frag[group & 1][i], qf[k], sc[u], 0, 0, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      uint32_t vs[16], vl[16];   // EXACT: of the lane's 32 tokens
-      int exp_now = scale_exp;
-      float eight = 0.f;
-      if constexpr (EXACT) {
-        uint32_t ks[16], kl[16];
+        for (int f = 0; f < NF; ++f)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const v4u x = st.params[0][g][i], y = st.params[1][g][i], z = st.params[2][g][i], t = st.params[3][g][i];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) ks[4 * i + j] = x[j], kl[4 * i + j] = y[j], vs[4 * i + j] = z[j], vl[4 * i + j] = t[j];
-        }
-#pragma unroll
-        for (int t = 0; t < 32; ++t) {
-          const float s = half_of(ks, t);
-          sc[t / 16][t % 16] = fmaf(s, sc[t / 16][t % 16], fmaf(8.f, s, half_of(kl, t)) * qsum);
-        }
-        uint32_t big = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) big = pk_max_u16(big, vs[i]);
-        const uint32_t field = halves_reduce(max(big & 0xFFFFu, big >> 16) >> 10, UMax{});
-        exp_now = max(scale_exp, __builtin_amdgcn_readfirstlane((int)field) - 14);
-        const int up = 14 - exp_now;
-        auto by_power = [&](int e) {
-          const _Float16 f = (_Float16)power_of_two(e);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) vs[i] = pk(unpk(vs[i]) * (v2h){f, f});
-        };
-        by_power(min(up, 15));
-        if (up > 15) by_power(up - 15);
-        eight = power_of_two(3 - up);
-      }
-      if (!(t0 + 64 <= top.last && t0 >= bottom.first)) {   // some row does not see some token
-#pragma unroll
-        for (int t = 0; t < 32; ++t) {
-          const int at_t = t0 + t / 16 * 32 + t % 16 / 4 * 8 + 4 * g + t % 4;
-          if (at_t < see.first || at_t >= see.last) sc[t / 16][t % 16] = -kInf;
-        }
-      }
-      float now = most;
-#pragma unroll
-      for (int t = 0; t < 32; ++t) now = fmaxf(now, sc[t / 16][t % 16]);
-      now = bits_float(halves_reduce(float_bits(now), FMax{}));
-      if (__any(now > most) || exp_now > scale_exp) {
-        const float next = now == -kInf ? 0.f : factor * now - (EXACT ? 0.f : 14.f);   // weights up to 1 (not EXACT: 2^14)
-        const float shrink = most == -kInf ? 1.f : __builtin_amdgcn_exp2f(at - next);   // before: all sums 0
-        const float shrink_o = shrink * power_of_two(scale_exp - exp_now);
-        most = now;
-        at = next;
-        total *= shrink;
-        middles *= shrink;
-        scale_exp = exp_now;
-#pragma unroll
-        for (int f = 0; f < NF; ++f) o[f] *= shrink_o;
-      }
-      fetch(&st.v[0][0], 0);
-      v8h ph[4], pl[4];
-#pragma unroll
-      for (int t = 0; t < 32; ++t) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(factor, sc[t / 16][t % 16], -at));
-        total += p;
-        if constexpr (EXACT) {
-          const float s = half_of(vs, t);
-          middles = fmaf(p, fmaf(eight, s, half_of(vl, t)), middles);
-          _Float16 h = (_Float16)fmaf(p, s, 0.f);
-          if constexpr (NP > 1) {
-            asm("" : "+v"(h));   // one and the same rounding in both parts
-            pl[t / 8][t % 8] = (_Float16)fmaf(p, s, -(float)h);
+          for (int i = 2 * u; i < 2 * u + 2; ++i) {
+            const v8h v = __builtin_bit_cast(v8h, st.v[f][i][lane]);
+            o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[i], o[f], 0, 0, 0);
+            if constexpr (NP > 1) o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[i], o[f], 0, 0, 0);
           }
-          ph[t / 8][t % 8] = h;
-        } else {
-          ph[t / 8][t % 8] = (_Float16)p;
+      };
+      uint32_t vs[8], vl[8];   // EXACT: of the lane's 16 tokens
+      float eight = 0.f;
+      float shrink_o = 1.f;
+      // Parameters, masks and the largest score; sums follow a larger one, and outputs do in rescale(), once the
+      // weights made before it are in them.
+      auto largest = [&](int u) {
+        int exp_now = scale_exp;
+        if constexpr (EXACT) {
+          uint32_t ks[8], kl[8];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const v4u x = st.params[0][g][2 * u + i], y = st.params[1][g][2 * u + i], z = st.params[2][g][2 * u + i], t = st.params[3][g][2 * u + i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) ks[4 * i + j] = x[j], kl[4 * i + j] = y[j], vs[4 * i + j] = z[j], vl[4 * i + j] = t[j];
+          }
+#pragma unroll
+          for (int t = 0; t < 16; ++t) {
+            const float s = half_of(ks, t);
+            sc[u][t] = fmaf(s, sc[u][t], fmaf(8.f, s, half_of(kl, t)) * qsum);
+          }
+          uint32_t big = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) big = pk_max_u16(big, vs[i]);
+          const uint32_t field = halves_reduce(max(big & 0xFFFFu, big >> 16) >> 10, UMax{});
+          exp_now = max(scale_exp, __builtin_amdgcn_readfirstlane((int)field) - 14);
+          const int up = kAtRest - exp_now;
+          auto by_power = [&](int e) {
+            const _Float16 f = (_Float16)power_of_two(e);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) vs[i] = pk(unpk(vs[i]) * (v2h){f, f});
+          };
+          by_power(min(up, 15));
+          if (up > 15) by_power(up - 15);
+          eight = power_of_two(3 - up);
         }
-      }
+        if (!(t0 + 32 * u + 32 <= top.last && t0 + 32 * u >= bottom.first)) {   // some row does not see some token
 #pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        if (f + 1 < NF) fetch(&st.v[0][0], f + 1);
+          for (int t = 0; t < 16; ++t) {
+            const int at_t = t0 + 32 * u + t / 4 * 8 + 4 * g + t % 4;
+            if (at_t < see.first || at_t >= see.last) sc[u][t] = -kInf;
+          }
+        }
+        float now = -kInf;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(frag[f & 1][i], ph[i], o[f], 0, 0, 0);
-          if constexpr (NP > 1) o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(frag[f & 1][i], pl[i], o[f], 0, 0, 0);
+        for (int t = 0; t < 16; ++t) now = fmaxf(now, sc[u][t]);
+        now = bits_float(halves_reduce(float_bits(now), FMax{}));
+        if (__any(factor * (now - most) > kSlack) || exp_now > scale_exp) {
+          now = fmaxf(now, most);
+          const float next = now == -kInf ? 0.f : factor * now - (EXACT ? 0 : kAtRest);
+          const float shrink = most == -kInf ? 1.f : __builtin_amdgcn_exp2f(at - next);   // before: all sums 0
+          shrink_o = shrink * power_of_two(scale_exp - exp_now);
+          most = now;
+          at = next;
+          total *= shrink;
+          middles *= shrink;
+          scale_exp = exp_now;
+          return true;
+        }
+        return false;
+      };
+      auto rescale = [&](bool larger) {
+        if (larger) {
+#pragma unroll
+          for (int f = 0; f < NF; ++f) o[f] *= shrink_o;
         }
         __builtin_amdgcn_sched_barrier(0);
-      }
+      };
+      auto weights = [&](int u) {
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(factor, sc[u][t], -at));
+          total += p;
+          if constexpr (EXACT) {
+            const float s = half_of(vs, t);
+            middles = fmaf(p, fmaf(eight, s, half_of(vl, t)), middles);
+            _Float16 h = (_Float16)fmaf(p, s, 0.f);
+            if constexpr (NP > 1) {
+              asm("" : "+v"(h));   // one and the same rounding in both parts
+              pl[2 * u + t / 8][t % 8] = (_Float16)fmaf(p, s, -(float)h);
+            }
+            ph[2 * u + t / 8][t % 8] = h;
+          } else {
+            ph[2 * u + t / 8][t % 8] = (_Float16)p;
+          }
+        }
+        // here and not where the product takes them
+#pragma unroll
+        for (int i = 2 * u; i < 2 * u + 2; ++i) {
+          asm volatile("" : "+v"(ph[i]));
+          if constexpr (NP > 1) asm volatile("" : "+v"(pl[i]));
+        }
+      };
+      // Products of one half beside the softmax of the other: reads of four fragments, then a product, a read and
+      // some VALU instructions in turn.
+      auto beside = [&](auto products, auto valu) {
+        constexpr int N = decltype(products)::value, V = decltype(valu)::value;
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          if (V) {
+            __builtin_amdgcn_sched_group_barrier(0x002, V, 0);
+            __builtin_amdgcn_sched_group_barrier(0x400, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, V, 0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      scores(0);
+      beside(std::integral_constant<int, NS>{}, std::integral_constant<int, 0>{});
+      rescale(largest(0));
+      scores(1);
+      weights(0);
+      beside(std::integral_constant<int, NS>{}, std::integral_constant<int, KV4_V1>{});
+      const bool larger = largest(1);
+      __builtin_amdgcn_sched_barrier(0);
+      values(0);
+      weights(1);
+      beside(std::integral_constant<int, 2 * NF * NP>{}, std::integral_constant<int, KV4_V2>{});
+      rescale(larger);
+      values(1);
+      beside(std::integral_constant<int, 2 * NF * NP>{}, std::integral_constant<int, 0>{});
     }
     lds_barrier();
   }
@@ -338,7 +399,7 @@ kv4_prefill_kernel(Attention a) {
   if (most == -kInf && total == 0.f) at = -kInf;
   if (w.poison) total = __builtin_nanf(""), at = 0.f;
   if (first_row + r > last_row) return;
-  const float unit = EXACT ? power_of_two(scale_exp - 14) : 2.f;
+  const float unit = EXACT ? power_of_two(scale_exp - kAtRest) : 2.f;
   const int64_t total_rows = (int64_t)a.tokens * a.q_heads;   // of all heads
   const int64_t at_row = (int64_t)(w.start + row / a.group) * a.q_heads + head * a.group + row % a.group;
 #pragma unroll
@@ -369,11 +430,16 @@ kv4_prefill_kernel(Attention a) {
 
 }  // namespace
 
-void kv4_prefill(const Attention& a, int dtype, int dim, int64_t grid, hipStream_t stream) {
+void kv4_prefill(const Attention& a, int dtype, int dim, int tile, int64_t grid, hipStream_t stream) {
   auto go = [&](auto n) {
     constexpr int DIM = decltype(n)::value;
-    if (dtype == QO_DTYPE_BF16) launch(kv4_prefill_kernel<BF16T, DIM, 1, false>, dim3((unsigned)grid), dim3(256), 0, stream, a);
-    else launch(kv4_prefill_kernel<F16T, DIM, 2, true>, dim3((unsigned)grid), dim3(256), 0, stream, a);
+    auto attend = [&](auto kernel) { launch(kernel, dim3((unsigned)grid), dim3(2 * tile), 0, stream, a); };
+    const bool bf16 = dtype == QO_DTYPE_BF16;
+    if constexpr (DIM <= 128) {
+      if (tile == 256) return bf16 ? attend(kv4_prefill_kernel<BF16T, DIM, 1, false, 8>) : attend(kv4_prefill_kernel<F16T, DIM, 2, true, 8>);
+    }
+    if (bf16) attend(kv4_prefill_kernel<BF16T, DIM, 1, false, 4>);
+    else attend(kv4_prefill_kernel<F16T, DIM, 2, true, 4>);
   };
   if (dim == 64) go(std::integral_constant<int, 64>{});
   else if (dim == 96) go(std::integral_constant<int, 96>{});

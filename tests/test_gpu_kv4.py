@@ -188,6 +188,9 @@ GPU_CASES = [
     ([150, 90], 5, 1, 256, 16, 30, 0),
     ([100], 2, 1, 128, 16, 150, 0),
     ([700, 20], 2, 2, 128, 32, [300, 20], 200),
+    ([900], 4, 1, 128, 64, 200, 0),                # seven tiles of 128 rows
+    ([640], 2, 1, 64, 32, 320, 100),
+    ([500, 450, 333], 3, 1, 128, 16, [300, 129, 43], 0),
     ([3], 1, 1, 256, 16, 3, 0),
     ([2], 2, 1, 128, 16, 40, 0),       # queries before the first token
 ]
