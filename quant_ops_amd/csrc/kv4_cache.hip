@@ -52,10 +52,15 @@ __device__ inline void load_values(const typename D::T* p, float* v) {
   for (int i = 0; i < N; ++i) v[i] = D::to_f(t[i]);
 }
 
+// Over the LANES lanes of a vector.
 template <int LANES, class F>
 __device__ inline float lanes_reduce(float v, F&& f) {
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) v = f(v, __shfl_xor(v, o, LANES));
+  auto with = [&](int other) { v = f(v, __builtin_bit_cast(float, other)); };
+  with(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, false));    // quad_perm 1,0,3,2
+  with(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, false));    // quad_perm 2,3,0,1
+  with(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xF, 0xF, false));   // row_half_mirror
+  if constexpr (LANES > 8) with(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xF, 0xF, false));   // row_mirror
+  if constexpr (LANES > 16) with(__builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F));   // lanes 16 apart
   return v;
 }
 
@@ -82,124 +87,182 @@ __device__ inline Place place_of(int lane, const Angles& a) {
 // (a, b) -> (a cos - b sin, b cos + a sin). A product of two float32 is exact in 64 bits, so
 // the results are the formula's, rounded to 64 bits and then to 32: whoever computes it in
 // 64 bits gets the same codes.
-__device__ inline void turn(float& a, float& b, float c, float s) {
+__device__ inline void turn(float& a, float& b, double c, double s) {
   const double x = (double)a * c - (double)b * s, y = (double)b * c + (double)a * s;
   a = (float)x;
   b = (float)y;
 }
 
-// Codes of a vector's eight values and its parameters. Borders between codes are decided in
-// 64 bits: n = floor of an estimate of (v - lo) / s is the quotient's floor, or beside it
-// where the quotient is next to a whole number, and either way v - lo against s (n + 1/2),
-// which is exact, says whether the nearest code is n or n + 1.
+// Codes (as floats) of a vector's eight values and its parameters. The quotient's estimate is off by 2^-18 at most
+// (of 15, its difference, the scale's reciprocal and their product 2^-23 each), so its nearest whole number is the
+// code unless it lies next to a border. There (one value in 10^5, or a tie) 64 bits decide: with n the
+// whole number below the border, v - lo against s (n + 1/2), which is exact.
 template <int LANES>
-__device__ inline void quantize(const float (&v)[8], bool there, uint32_t (&c)[8], _Float16& scale, _Float16& least) {
-  float lo = __builtin_inff(), hi = -__builtin_inff(), bad = 0.f;
+__device__ inline void quantize(const float (&v)[8], bool there, float (&c)[8], _Float16& scale, _Float16& least) {
+  float lo = __builtin_inff(), hi = -__builtin_inff(), size = 0.f;
   float u[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     u[i] = __builtin_amdgcn_fmed3f(v[i], -kKV4Most, kKV4Most);
-    if (there) {
-      lo = fminf(lo, u[i]);
-      hi = fmaxf(hi, u[i]);
-      if (!(fabsf(v[i]) <= 3.4028234e38f)) bad = 1.f;
-    }
+    lo = fminf(lo, u[i]);
+    hi = fmaxf(hi, u[i]);
+    size = fmaf(v[i], 0.f, size);   // NaN for a NaN or an infinity
   }
+  if (!there) lo = __builtin_inff(), hi = -__builtin_inff(), size = 0.f;
   lo = lanes_reduce<LANES>(lo, [](float a, float b) { return fminf(a, b); });
   hi = lanes_reduce<LANES>(hi, [](float a, float b) { return fmaxf(a, b); });
-  bad = lanes_reduce<LANES>(bad, [](float a, float b) { return fmaxf(a, b); });
   least = (_Float16)lo;
-  const double l = (double)(float)least;
-  const float range = (float)(((double)hi - l) / 15.0);   // rounded to float32, then to fp16
+  const float l = (float)least;
+  const double d = (double)hi - (double)l, q = d * (1.0 / 15.0);
+  const float range = (float)fma(fma(-15.0, q, d), 1.0 / 15.0, q);   // the quotient, rounded to float32, then to fp16
   scale = (_Float16)fmaxf(range, 0.f);
   const float s = (float)scale;
-  const float inverse = s > 0.f ? 1.f / s : 0.f;
+  const float inverse = s > 0.f ? __builtin_amdgcn_rcpf(s) : 0.f;
+  float near = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const double d = (double)u[i] - l;
-    const float n = floorf(fminf(fmaxf((float)d * inverse, 0.f), 15.f));
-    const double over = d - (double)s * ((double)n + 0.5);
-    const int k = (int)n;
-    c[i] = s > 0.f ? (uint32_t)min(k + ((over > 0.0) | ((over == 0.0) & (k & 1)) ? 1 : 0), 15) : 0u;
+    const float r = (u[i] - l) * inverse, n = rintf(r);
+    near = fmaxf(near, fabsf(r - n));
+    c[i] = __builtin_amdgcn_fmed3f(n, 0.f, 15.f);
   }
-  if (bad != 0.f) {
-    scale = least = (_Float16)__builtin_nanf("");
+  if (__any(near > 0.5f - 0x1p-17f)) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = 0;
+    for (int i = 0; i < 8; ++i) {
+      const float n = floorf(__builtin_amdgcn_fmed3f((u[i] - l) * inverse, 0.f, 15.f));
+      const double over = ((double)u[i] - (double)l) - (double)s * ((double)n + 0.5);
+      const bool up = over > 0.0 || (over == 0.0 && ((int)n & 1));
+      c[i] = s > 0.f ? fminf(n + (up ? 1.f : 0.f), 15.f) : 0.f;
+    }
+  }
+  if (__any(size != 0.f)) {   // some vector has a NaN or an infinity
+    const float bad = lanes_reduce<LANES>(size != 0.f ? 1.f : 0.f, [](float a, float b) { return fmaxf(a, b); });
+    if (bad != 0.f) {
+      scale = least = (_Float16)__builtin_nanf("");
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = 0.f;
+    }
   }
 }
+// Two codes a byte, four and eight to a word: sums that float32 holds exactly.
+__device__ inline uint32_t bytes2(const float* c) { return (uint32_t)fmaf(c[3], 4096.f, fmaf(c[2], 256.f, fmaf(c[1], 16.f, c[0]))); }
 
-// A workgroup of 256 threads takes 256 / LANES consecutive tokens of one head; blockIdx.y
-// counts query heads, then key heads, then value heads.
+// A workgroup of 256 threads takes 256 / LANES consecutive tokens of `per` heads in turn, of the queries, the keys or the
+// values (blockIdx.y counts groups of heads); a token's angles are read once for them all. Values' codes
+// go through LDS, so that a thread has a byte of four tokens, one word where they stand beside each other.
 template <class D, int DIM>
 __global__ void __launch_bounds__(256)
 kv4_append_kernel(KV4 cache, Heads<typename D::T> q, Heads<typename D::T> k, Heads<typename D::T> v, int64_t tokens,
-                  int q_heads, const int64_t* __restrict__ slots, Angles angles, typename D::T* __restrict__ q_out) {
+                  int q_heads, int per, const int64_t* __restrict__ slots, Angles angles, typename D::T* __restrict__ q_out) {
   constexpr int LANES = kLanes<DIM>, TOKENS = 256 / LANES;
-  const int lane = threadIdx.x % LANES;
-  const int64_t token = (int64_t)blockIdx.x * TOKENS + threadIdx.x / LANES;
+  __shared__ uint8_t bytes[2][DIM / 2][TOKENS];
+  __shared__ int64_t token_slots[TOKENS];
+  const int lane = threadIdx.x % LANES, mine = threadIdx.x / LANES;
+  const int64_t token = (int64_t)blockIdx.x * TOKENS + mine;
   const bool there = token < tokens && 8 * lane < DIM;
-  int head = blockIdx.y;
-  const int kind = head < q_heads ? 0 : head < q_heads + cache.heads ? 1 : 2;
-  head -= kind == 0 ? 0 : kind == 1 ? q_heads : q_heads + cache.heads;
   const int64_t row = token < tokens ? token : 0;
+  const int q_groups = (q_heads + per - 1) / per, groups = (cache.heads + per - 1) / per;
+  int group = blockIdx.y;
+  const int kind = group < q_groups ? 0 : group < q_groups + groups ? 1 : 2;
+  group -= kind == 0 ? 0 : kind == 1 ? q_groups : q_groups + groups;
+  const int first = group * per, last = min(first + per, kind == 0 ? q_heads : cache.heads);
 
   Place p = {8 * lane, 8 * lane + 4, false};
   if (kind < 2) p = place_of(lane, angles);
-  float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (there) {
-    const typename D::T* src = (kind == 0 ? q : kind == 1 ? k : v).at(row, head);
-    load_values<D, 4>(src + p.at, x);
-    load_values<D, 4>(src + p.more, x + 4);
-    if (p.turned) {
-      const int64_t pos = angles.positions[row];
-      const bool known = pos >= 0 && pos < angles.rows;
-      const int first = angles.interleaved ? 4 * lane : p.at;   // the first pair's angle
-      float c[4], s[4];
-      load_values<F32T, 4>(angles.cos_ + (known ? pos : 0) * (angles.rot / 2) + first, c);
-      load_values<F32T, 4>(angles.sin_ + (known ? pos : 0) * (angles.rot / 2) + first, s);
+  double c[4], s[4];
+  if (p.turned && there) {
+    const int64_t pos = angles.positions[row];
+    const bool known = pos >= 0 && pos < angles.rows;
+    const int64_t at = (known ? pos : 0) * (angles.rot / 2) + (angles.interleaved ? 4 * lane : p.at);   // the first pair's angle
+    float a[4], b[4];
+    load_values<F32T, 4>(angles.cos_ + at, a);
+    load_values<F32T, 4>(angles.sin_ + at, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = known ? a[i] : __builtin_nanf(""), s[i] = b[i];
+  }
+  int64_t page = 0;
+  int place = 0;
+  bool kept = false;
+  if (kind > 0) {
+    const int64_t slot = token < tokens ? slots[row] : -1;
+    kept = slot >= 0 && slot < cache.slots();
+    page = slot >> cache.shift;
+    place = (int)(slot & ((1 << cache.shift) - 1));
+    if (kind == 2 && lane == 0) token_slots[mine] = kept ? slot : -1;
+  }
+  auto source = kind == 0 ? q : kind == 1 ? k : v;
+  float next[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  auto load = [&](int head) {
+    const typename D::T* src = source.at(row, head);
+    load_values<D, 4>(src + p.at, next);
+    load_values<D, 4>(src + p.more, next + 4);
+  };
+  if (there) load(first);
+  for (int head = first; head < last; ++head) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = next[i];
+    if (there && head + 1 < last) load(head + 1);
+    if (p.turned && there) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (!known) c[i] = __builtin_nanf("");
         if (angles.interleaved) turn(x[2 * i], x[2 * i + 1], c[i], s[i]);
         else turn(x[i], x[4 + i], c[i], s[i]);
       }
     }
-  }
-  if (kind == 0) {
-    if (there) {
-      typename D::T out[8];
+    if (kind == 0) {
+      if (there) {
+        typename D::T out[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out[i] = D::from_f(x[i]);
-      typename D::T* to = q_out + (token * q_heads + head) * DIM;
-      __builtin_memcpy(to + p.at, out, 4 * sizeof(out[0]));
-      __builtin_memcpy(to + p.more, out + 4, 4 * sizeof(out[0]));
+        for (int i = 0; i < 8; ++i) out[i] = D::from_f(x[i]);
+        typename D::T* to = q_out + (token * q_heads + head) * DIM;
+        __builtin_memcpy(to + p.at, out, 4 * sizeof(out[0]));
+        __builtin_memcpy(to + p.more, out + 4, 4 * sizeof(out[0]));
+      }
+      continue;
     }
-    return;
-  }
-
-  uint32_t c[8];
-  _Float16 scale, least;
-  quantize<LANES>(x, there, c, scale, least);
-  const int64_t slot = slots[row];
-  if (!there || slot < 0 || slot >= cache.slots()) return;
-  const int64_t page = slot >> cache.shift;
-  const int place = (int)(slot & ((1 << cache.shift) - 1));
-  if (kind == 1) {
-    uint8_t* to = cache.key(page, head, place, DIM);
-    const uint16_t a = (uint16_t)(c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12);
-    const uint16_t b = (uint16_t)(c[4] | c[5] << 4 | c[6] << 8 | c[7] << 12);
-    *reinterpret_cast<uint16_t*>(to + p.at / 2) = a;
-    *reinterpret_cast<uint16_t*>(to + p.more / 2) = b;
-  } else {
-    uint8_t* to = cache.value_tile(page, head, place, DIM) + (place & 15);
+    float codes[8];
+    _Float16 scale, least;
+    quantize<LANES>(x, there, codes, scale, least);
+    const uint32_t w0 = bytes2(codes), w1 = bytes2(codes + 4);
+    if (kind == 1 && there && kept) {
+      uint8_t* to = cache.key(page, head, place, DIM);
+      *reinterpret_cast<uint16_t*>(to + p.at / 2) = (uint16_t)w0;
+      *reinterpret_cast<uint16_t*>(to + p.more / 2) = (uint16_t)w1;
+    }
+    if (there && kept && lane == 0) {
+      _Float16* to = cache.param_tile(page, kind - 1, head, place) + (place & 15);
+      to[0] = scale;
+      to[16] = least;
+    }
+    if (kind == 2) {
+      uint8_t(*box)[TOKENS] = bytes[(head - first) & 1];
+      if (there) {
+        box[4 * lane][mine] = (uint8_t)w0;
+        box[4 * lane + 1][mine] = (uint8_t)(w0 >> 8);
+        box[4 * lane + 2][mine] = (uint8_t)w1;
+        box[4 * lane + 3][mine] = (uint8_t)(w1 >> 8);
+      }
+      __syncthreads();   // the other box is written next: one barrier a head
+      for (int i = threadIdx.x; i < DIM / 2 * (TOKENS / 4); i += 256) {
+        const int pair = i / (TOKENS / 4), t = 4 * (i % (TOKENS / 4));
+        const uint32_t four = *reinterpret_cast<const uint32_t*>(&box[pair][t]);
+        const int64_t slot = token_slots[t];
+        auto at = [&](int64_t sl) {
+          const int in_page = (int)(sl & ((1 << cache.shift) - 1));
+          return cache.value_tile(sl >> cache.shift, head, in_page, DIM) + pair * 16 + (in_page & 15);
+        };
+        bool beside = slot >= 0 && (slot & 3) == 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) to[(4 * lane + i) * 16] = (uint8_t)(c[2 * i] | c[2 * i + 1] << 4);
-  }
-  if (lane == 0) {
-    _Float16* to = cache.param_tile(page, kind - 1, head, place) + (place & 15);
-    to[0] = scale;
-    to[16] = least;
+        for (int n = 1; n < 4; ++n) beside = beside && token_slots[t + n] == slot + n;
+        if (beside) {
+          *reinterpret_cast<uint32_t*>(at(slot)) = four;
+        } else {
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+            if (token_slots[t + n] >= 0) *at(token_slots[t + n]) = (uint8_t)(four >> (8 * n));
+        }
+      }
+    }
   }
 }
 
@@ -312,9 +375,12 @@ extern "C" int qo_kv4_append(const qo_kv4_cache* cache, const qo_heads* q, const
       auto heads = [](const qo_heads* h) {
         return h ? Heads<T>{reinterpret_cast<const T*>(h->data), h->token_stride, h->head_stride} : Heads<T>{};
       };
-      const dim3 grid((unsigned)((tokens + TOKENS - 1) / TOKENS), (unsigned)(q_heads + 2 * c.heads));
+      // heads to a workgroup: as many as leave four workgroups for each CU, eight at most
+      const int64_t blocks = (tokens + TOKENS - 1) / TOKENS, all = blocks * (q_heads + 2 * c.heads) / (4 * device_cu_count());
+      const int per = all < 1 ? 1 : all > 8 ? 8 : (int)all;
+      const dim3 grid((unsigned)blocks, (unsigned)((q_heads + per - 1) / per + 2 * ((c.heads + per - 1) / per)));
       launch(kv4_append_kernel<D, DIM>, grid, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), c, heads(q), heads(k),
-             heads(v), tokens, q_heads, slots, Angles{positions, cos_, sin_, table_rows, rot, interleaved != 0},
+             heads(v), tokens, q_heads, per, slots, Angles{positions, cos_, sin_, table_rows, rot, interleaved != 0},
              reinterpret_cast<T*>(q_out));
     });
   });
