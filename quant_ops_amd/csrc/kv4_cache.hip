@@ -70,7 +70,7 @@ struct Angles {
   const float* cos_;
   const float* sin_;
   int64_t rows;
-  int rot, interleaved;
+  int rot;
 };
 
 // Eight values of a vector and where they stand: `at` the first four, `more` the others. In
@@ -79,9 +79,10 @@ struct Place {
   int at, more;
   bool turned;
 };
-__device__ inline Place place_of(int lane, const Angles& a) {
-  if (8 * lane >= a.rot || a.interleaved) return {8 * lane, 8 * lane + 4, 8 * lane < a.rot};
-  return {4 * lane, a.rot / 2 + 4 * lane, true};
+template <bool PAIRS>
+__device__ inline Place place_of(int lane, int rot) {
+  if (8 * lane >= rot || PAIRS) return {8 * lane, 8 * lane + 4, 8 * lane < rot};
+  return {4 * lane, rot / 2 + 4 * lane, true};
 }
 
 // (a, b) -> (a cos - b sin, b cos + a sin). A product of two float32 is exact in 64 bits, so
@@ -93,68 +94,110 @@ __device__ inline void turn(float& a, float& b, double c, double s) {
   b = (float)y;
 }
 
-// Codes (as floats) of a vector's eight values and its parameters. The quotient's estimate is off by 2^-18 at most
-// (of 15, its difference, the scale's reciprocal and their product 2^-23 each), so its nearest whole number is the
-// code unless it lies next to a border. There (one value in 10^5, or a tie) 64 bits decide: with n the
-// whole number below the border, v - lo against s (n + 1/2), which is exact.
+// Codes of a vector's eight values (in the low bytes of words: two by two) and its parameters. A code is the whole number
+// nearest to an estimate (v - lo) / s, which is off by 2^-19 at most (of 15, the difference and the scale's reciprocal
+// 2^-24 and 2^-23), unless that lies next to a border between codes or outside them. There (one value in 10^5, exact ties,
+// vectors whose size is far above their range) 64 bits decide: with n the whole number below the border, v - lo
+// against s (n + 1/2), which is exact.
 template <int LANES>
-__device__ inline void quantize(const float (&v)[8], bool there, float (&c)[8], _Float16& scale, _Float16& least) {
-  float lo = __builtin_inff(), hi = -__builtin_inff(), size = 0.f;
-  float u[8];
+__device__ inline void quantize(const float (&v)[8], bool there, uint32_t (&two)[4], _Float16& scale, _Float16& least) {
+  float lo = v[0], hi = v[0];   // hi: NaN for a NaN
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    u[i] = __builtin_amdgcn_fmed3f(v[i], -kKV4Most, kKV4Most);
-    lo = fminf(lo, u[i]);
-    hi = fmaxf(hi, u[i]);
-    size = fmaf(v[i], 0.f, size);   // NaN for a NaN or an infinity
+  for (int i = 1; i < 8; ++i) {
+    lo = fminf(lo, v[i]);
+    hi = __builtin_elementwise_maximum(hi, v[i]);
   }
-  if (!there) lo = __builtin_inff(), hi = -__builtin_inff(), size = 0.f;
+  if (!there) lo = __builtin_inff(), hi = -__builtin_inff();
   lo = lanes_reduce<LANES>(lo, [](float a, float b) { return fminf(a, b); });
-  hi = lanes_reduce<LANES>(hi, [](float a, float b) { return fmaxf(a, b); });
-  least = (_Float16)lo;
+  hi = lanes_reduce<LANES>(hi, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+  const bool finite = lo > -__builtin_inff() && hi < __builtin_inff();
+  lo = fmaxf(lo, -kKV4Most);
+  hi = fminf(hi, kKV4Most);
+  least = (_Float16)fminf(lo, kKV4Most);
   const float l = (float)least;
-  const double d = (double)hi - (double)l, q = d * (1.0 / 15.0);
+  const double d = (double)fmaxf(hi, -kKV4Most) - (double)l, q = d * (1.0 / 15.0);
   const float range = (float)fma(fma(-15.0, q, d), 1.0 / 15.0, q);   // the quotient, rounded to float32, then to fp16
   scale = (_Float16)fmaxf(range, 0.f);
   const float s = (float)scale;
   const float inverse = s > 0.f ? __builtin_amdgcn_rcpf(s) : 0.f;
-  float near = 0.f;
+  constexpr float kRound = 12582912.f;   // 1.5 2^23: a sum with it is a whole number, in its low bits
+  float near = 0.f, m[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float r = (u[i] - l) * inverse, n = rintf(r);
-    near = fmaxf(near, fabsf(r - n));
-    c[i] = __builtin_amdgcn_fmed3f(n, 0.f, 15.f);
+    const float x = v[i] - l;
+    m[i] = fmaf(x, inverse, kRound);
+    near = fmaxf(near, fabsf(fmaf(x, inverse, -(m[i] - kRound))));
   }
-  if (__any(near > 0.5f - 0x1p-17f)) {
+  // beyond a border lies what is above 15 1/2 or below -1/2, values past fp16 among them
+  const float high = fmaxf((hi - l) * inverse - 15.f, (l - lo) * inverse);
+  if (__any(!(fmaxf(near, high) < 0.5f - 0x1p-17f) || !finite || s == 0.f || hi == kKV4Most || lo == -kKV4Most)) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float n = floorf(__builtin_amdgcn_fmed3f((u[i] - l) * inverse, 0.f, 15.f));
-      const double over = ((double)u[i] - (double)l) - (double)s * ((double)n + 0.5);
+      const float u = __builtin_amdgcn_fmed3f(v[i], -kKV4Most, kKV4Most);
+      const float n = floorf(__builtin_amdgcn_fmed3f((u - l) * inverse, 0.f, 15.f));
+      const double over = ((double)u - (double)l) - (double)s * ((double)n + 0.5);
       const bool up = over > 0.0 || (over == 0.0 && ((int)n & 1));
-      c[i] = s > 0.f ? fminf(n + (up ? 1.f : 0.f), 15.f) : 0.f;
+      m[i] = (s > 0.f && finite ? fminf(n + (up ? 1.f : 0.f), 15.f) : 0.f) + kRound;
     }
+    if (!finite) scale = least = (_Float16)__builtin_nanf("");
   }
-  if (__any(size != 0.f)) {   // some vector has a NaN or an infinity
-    const float bad = lanes_reduce<LANES>(size != 0.f ? 1.f : 0.f, [](float a, float b) { return fmaxf(a, b); });
-    if (bad != 0.f) {
-      scale = least = (_Float16)__builtin_nanf("");
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = 0.f;
+  for (int i = 0; i < 4; ++i)
+    two[i] = __builtin_bit_cast(uint32_t, m[2 * i + 1]) << 4 | __builtin_bit_cast(uint32_t, m[2 * i]);
+}
+
+// Where values' bytes of TOKENS tokens go from a box in LDS: a thread has a byte (a pair of values) of four
+// tokens, which share a word of the cache where their slots do; four threads have 16 tokens of a pair, so that
+// single bytes too go to whole lines. A head's bytes stand head_bytes behind those of the head before.
+template <int DIM, int TOKENS>
+struct ValueBytes {
+  uint8_t* at[4];   // null: no such token
+  bool beside, there;
+  int pair, t;
+  int64_t head_bytes;
+
+  __device__ ValueBytes(const KV4& cache, int head, const int64_t* token_slots) {
+    pair = threadIdx.x / (TOKENS / 4), t = 4 * (threadIdx.x % (TOKENS / 4));
+    there = pair < DIM / 2;
+    head_bytes = (int64_t)DIM / 2 << cache.shift;
+    const int64_t first = token_slots[t];
+    beside = there && first >= 0 && (first & 3) == 0;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int64_t slot = token_slots[t + n];
+      const int place = (int)(slot & ((1 << cache.shift) - 1));
+      at[n] = there && slot >= 0 ? cache.value_tile(slot >> cache.shift, head, place, DIM) + pair * 16 + (place & 15) : nullptr;
+      beside = beside && slot == first + n;
     }
   }
-}
-// Two codes a byte, four and eight to a word: sums that float32 holds exactly.
-__device__ inline uint32_t bytes2(const float* c) { return (uint32_t)fmaf(c[3], 4096.f, fmaf(c[2], 256.f, fmaf(c[1], 16.f, c[0]))); }
+  __device__ inline void next_head() {
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      if (at[n]) at[n] += head_bytes;
+  }
+  __device__ inline void put(uint32_t four) const {
+    if (beside) {
+      *reinterpret_cast<uint32_t*>(at[0]) = four;
+    } else {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        if (at[n]) *at[n] = (uint8_t)(four >> (8 * n));
+    }
+  }
+};
 
 // A workgroup of 256 threads takes 256 / LANES consecutive tokens of `per` heads in turn, of the queries, the keys or the
-// values (blockIdx.y counts groups of heads); a token's angles are read once for them all. Values' codes
-// go through LDS, so that a thread has a byte of four tokens, one word where they stand beside each other.
-template <class D, int DIM>
+// values (blockIdx.y counts groups of heads); a token's angles are read once for them all, and a head's values are on
+// their way while those of the head before are worked on. 8192 tokens of 32 + 8 + 8 heads of 128, bf16: 44 us, of them
+// 22 for the 16 heads with codes, as long as copying the queries alone takes (67 MB in and out, 19 us). The codes' part is
+// bound by its arithmetic, 230 vector instructions for eight values, half of them in the way through 64 bits.
+template <class D, int DIM, bool PAIRS>
 __global__ void __launch_bounds__(256)
 kv4_append_kernel(KV4 cache, Heads<typename D::T> q, Heads<typename D::T> k, Heads<typename D::T> v, int64_t tokens,
                   int q_heads, int per, const int64_t* __restrict__ slots, Angles angles, typename D::T* __restrict__ q_out) {
+  using T = typename D::T;
   constexpr int LANES = kLanes<DIM>, TOKENS = 256 / LANES;
-  __shared__ uint8_t bytes[2][DIM / 2][TOKENS];
+  __shared__ __align__(4) uint8_t bytes[2][DIM / 2][TOKENS];
   __shared__ int64_t token_slots[TOKENS];
   const int lane = threadIdx.x % LANES, mine = threadIdx.x / LANES;
   const int64_t token = (int64_t)blockIdx.x * TOKENS + mine;
@@ -167,106 +210,108 @@ kv4_append_kernel(KV4 cache, Heads<typename D::T> q, Heads<typename D::T> k, Hea
   const int first = group * per, last = min(first + per, kind == 0 ? q_heads : cache.heads);
 
   Place p = {8 * lane, 8 * lane + 4, false};
-  if (kind < 2) p = place_of(lane, angles);
+  if (kind < 2) p = place_of<PAIRS>(lane, angles.rot);
+  const Heads<T> source = kind == 0 ? q : kind == 1 ? k : v;
+  const T* src = source.at(row, first);
+  T raw[8];
+  auto load = [&] {
+    if (there) {
+      __builtin_memcpy(raw, src + p.at, 4 * sizeof(T));
+      __builtin_memcpy(raw + 4, src + p.more, 4 * sizeof(T));
+    }
+    src += source.head;
+  };
+  load();
   double c[4], s[4];
   if (p.turned && there) {
     const int64_t pos = angles.positions[row];
     const bool known = pos >= 0 && pos < angles.rows;
-    const int64_t at = (known ? pos : 0) * (angles.rot / 2) + (angles.interleaved ? 4 * lane : p.at);   // the first pair's angle
+    const int64_t at = (known ? pos : 0) * (angles.rot / 2) + 4 * lane;   // the first pair's angle
     float a[4], b[4];
-    load_values<F32T, 4>(angles.cos_ + at, a);
-    load_values<F32T, 4>(angles.sin_ + at, b);
+    __builtin_memcpy(a, angles.cos_ + at, sizeof(a));
+    __builtin_memcpy(b, angles.sin_ + at, sizeof(b));
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[i] = known ? a[i] : __builtin_nanf(""), s[i] = b[i];
   }
-  int64_t page = 0;
-  int place = 0;
-  bool kept = false;
-  if (kind > 0) {
-    const int64_t slot = token < tokens ? slots[row] : -1;
-    kept = slot >= 0 && slot < cache.slots();
-    page = slot >> cache.shift;
-    place = (int)(slot & ((1 << cache.shift) - 1));
-    if (kind == 2 && lane == 0) token_slots[mine] = kept ? slot : -1;
-  }
-  auto source = kind == 0 ? q : kind == 1 ? k : v;
-  float next[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  auto load = [&](int head) {
-    const typename D::T* src = source.at(row, head);
-    load_values<D, 4>(src + p.at, next);
-    load_values<D, 4>(src + p.more, next + 4);
-  };
-  if (there) load(first);
-  for (int head = first; head < last; ++head) {
-    float x[8];
+  // The lane's vector x of the next head, turned where it is.
+  auto take = [&](bool more, float(&x)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = next[i];
-    if (there && head + 1 < last) load(head + 1);
+    for (int i = 0; i < 8; ++i) x[i] = there ? D::to_f(raw[i]) : 0.f;
+    if (more) load();
     if (p.turned && there) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (angles.interleaved) turn(x[2 * i], x[2 * i + 1], c[i], s[i]);
+        if constexpr (PAIRS) turn(x[2 * i], x[2 * i + 1], c[i], s[i]);
         else turn(x[i], x[4 + i], c[i], s[i]);
       }
     }
-    if (kind == 0) {
-      if (there) {
-        typename D::T out[8];
+  };
+  if (kind == 0) {
+    T* to = q_out + (token * q_heads + first) * DIM;
+    for (int head = first; head < last; ++head, to += DIM) {
+      float x[8];
+      take(head + 1 < last, x);
+      if (!there) continue;
+      T out[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) out[i] = D::from_f(x[i]);
-        typename D::T* to = q_out + (token * q_heads + head) * DIM;
-        __builtin_memcpy(to + p.at, out, 4 * sizeof(out[0]));
-        __builtin_memcpy(to + p.more, out + 4, 4 * sizeof(out[0]));
-      }
-      continue;
+      for (int i = 0; i < 8; ++i) out[i] = D::from_f(x[i]);
+      __builtin_memcpy(to + p.at, out, 4 * sizeof(T));
+      __builtin_memcpy(to + p.more, out + 4, 4 * sizeof(T));
     }
-    float codes[8];
+    return;
+  }
+
+  const int64_t slot = token < tokens ? slots[row] : -1;
+  const bool known = slot >= 0 && slot < cache.slots(), kept = there && known;
+  const int64_t page = known ? slot >> cache.shift : 0;
+  const int place = known ? (int)(slot & ((1 << cache.shift) - 1)) : 0;
+  _Float16* par = cache.param_tile(page, kind - 1, first, place) + (place & 15);
+  const int64_t head_params = (int64_t)2 << cache.shift;
+  auto parameters = [&](_Float16 scale, _Float16 least) {
+    if (kept && lane == 0) par[0] = scale, par[16] = least;
+    par += head_params;
+  };
+  if (kind == 1) {
+    uint8_t* to = cache.key(page, first, place, DIM);
+    for (int head = first; head < last; ++head, to += (int64_t)DIM / 2 << cache.shift) {
+      float x[8];
+      take(head + 1 < last, x);
+      uint32_t two[4];
+      _Float16 scale, least;
+      quantize<LANES>(x, there, two, scale, least);
+      if (kept) {
+        *reinterpret_cast<uint16_t*>(to + p.at / 2) = (uint16_t)__builtin_amdgcn_perm(two[1], two[0], 0x0C0C0400u);
+        *reinterpret_cast<uint16_t*>(to + p.more / 2) = (uint16_t)__builtin_amdgcn_perm(two[3], two[2], 0x0C0C0400u);
+      }
+      parameters(scale, least);
+    }
+    return;
+  }
+  if (lane == 0) token_slots[mine] = known ? slot : -1;
+  __syncthreads();
+  ValueBytes<DIM, TOKENS> to(cache, first, token_slots);
+  for (int head = first; head < last; ++head) {
+    float x[8];
+    take(head + 1 < last, x);
+    uint32_t two[4];
     _Float16 scale, least;
-    quantize<LANES>(x, there, codes, scale, least);
-    const uint32_t w0 = bytes2(codes), w1 = bytes2(codes + 4);
-    if (kind == 1 && there && kept) {
-      uint8_t* to = cache.key(page, head, place, DIM);
-      *reinterpret_cast<uint16_t*>(to + p.at / 2) = (uint16_t)w0;
-      *reinterpret_cast<uint16_t*>(to + p.more / 2) = (uint16_t)w1;
-    }
-    if (there && kept && lane == 0) {
-      _Float16* to = cache.param_tile(page, kind - 1, head, place) + (place & 15);
-      to[0] = scale;
-      to[16] = least;
-    }
-    if (kind == 2) {
-      uint8_t(*box)[TOKENS] = bytes[(head - first) & 1];
-      if (there) {
-        box[4 * lane][mine] = (uint8_t)w0;
-        box[4 * lane + 1][mine] = (uint8_t)(w0 >> 8);
-        box[4 * lane + 2][mine] = (uint8_t)w1;
-        box[4 * lane + 3][mine] = (uint8_t)(w1 >> 8);
-      }
-      __syncthreads();   // the other box is written next: one barrier a head
-      for (int i = threadIdx.x; i < DIM / 2 * (TOKENS / 4); i += 256) {
-        const int pair = i / (TOKENS / 4), t = 4 * (i % (TOKENS / 4));
-        const uint32_t four = *reinterpret_cast<const uint32_t*>(&box[pair][t]);
-        const int64_t slot = token_slots[t];
-        auto at = [&](int64_t sl) {
-          const int in_page = (int)(sl & ((1 << cache.shift) - 1));
-          return cache.value_tile(sl >> cache.shift, head, in_page, DIM) + pair * 16 + (in_page & 15);
-        };
-        bool beside = slot >= 0 && (slot & 3) == 0;
+    quantize<LANES>(x, there, two, scale, least);
+    uint8_t(*box)[TOKENS] = bytes[(head - first) & 1];
+    if (there) {
 #pragma unroll
-        for (int n = 1; n < 4; ++n) beside = beside && token_slots[t + n] == slot + n;
-        if (beside) {
-          *reinterpret_cast<uint32_t*>(at(slot)) = four;
-        } else {
-#pragma unroll
-          for (int n = 0; n < 4; ++n)
-            if (token_slots[t + n] >= 0) *at(token_slots[t + n]) = (uint8_t)(four >> (8 * n));
-        }
-      }
+      for (int i = 0; i < 4; ++i) box[4 * lane + i][mine] = (uint8_t)two[i];
     }
+    lds_barrier();   // the other box is written next: one barrier a head
+    if (to.there) to.put(*reinterpret_cast<const uint32_t*>(&box[to.pair][to.t]));
+    to.next_head();
+    parameters(scale, least);
   }
 }
 
-// A thread reads eight values of a vector; blockIdx.y counts key heads, then value heads.
+// A thread reads eight values of a vector; blockIdx.y counts key heads, then value heads. What bounds it is the
+// writing of the values, four times the codes' bytes in 16 bits (8192 tokens, 8 heads of 128 to bf16: 15.4 us for 43 MB,
+// 2.8 TB/s; at random slots 18.7). A lane's four bytes of a value's codes are loads of their own: the lanes of 16
+// tokens share their lines, and the same through words and LDS, as they were written, took 19 us (22).
 template <class D, int DIM>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(KV4 cache, const int64_t* __restrict__ slots, int64_t tokens, typename D::T* __restrict__ k_out,
@@ -331,6 +376,13 @@ int check_tokens(const char* fn, int64_t tokens, int dtype) {
   return QO_OK;
 }
 
+// Heads that a workgroup takes in turn: as many as leave four workgroups for each CU, eight at most (8192 tokens of 48
+// heads of 128, bf16: one 74 us, two 60, four and eight 44 to 54).
+int heads_per_group(int64_t blocks, int heads) {
+  const int64_t n = blocks * heads / (4 * device_cu_count());
+  return n < 1 ? 1 : n > 8 ? 8 : (int)n;
+}
+
 int null_pointer(const char* fn) {
   qo_set_error("%s: NULL pointer argument", fn);
   return QO_ERR_NULL_POINTER;
@@ -375,13 +427,12 @@ extern "C" int qo_kv4_append(const qo_kv4_cache* cache, const qo_heads* q, const
       auto heads = [](const qo_heads* h) {
         return h ? Heads<T>{reinterpret_cast<const T*>(h->data), h->token_stride, h->head_stride} : Heads<T>{};
       };
-      // heads to a workgroup: as many as leave four workgroups for each CU, eight at most
-      const int64_t blocks = (tokens + TOKENS - 1) / TOKENS, all = blocks * (q_heads + 2 * c.heads) / (4 * device_cu_count());
-      const int per = all < 1 ? 1 : all > 8 ? 8 : (int)all;
+      const int64_t blocks = (tokens + TOKENS - 1) / TOKENS;
+      const int per = heads_per_group(blocks, q_heads + 2 * c.heads);
       const dim3 grid((unsigned)blocks, (unsigned)((q_heads + per - 1) / per + 2 * ((c.heads + per - 1) / per)));
-      launch(kv4_append_kernel<D, DIM>, grid, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), c, heads(q), heads(k),
-             heads(v), tokens, q_heads, per, slots, Angles{positions, cos_, sin_, table_rows, rot, interleaved != 0},
-             reinterpret_cast<T*>(q_out));
+      launch(interleaved ? kv4_append_kernel<D, DIM, true> : kv4_append_kernel<D, DIM, false>, grid, dim3(256), 0,
+             reinterpret_cast<hipStream_t>(stream), c, heads(q), heads(k), heads(v), tokens, q_heads, per, slots,
+             Angles{positions, cos_, sin_, table_rows, rot}, reinterpret_cast<T*>(q_out));
     });
   });
   return launch_result(fn);
