@@ -172,12 +172,26 @@ inline Kv4Plan kv4_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64
   Kv4Plan p = {each <= 4 ? 4 : each <= 8 ? 8 : f32 || each <= 64 ? 16 : each <= 128 || head_dim > 128 ? 32 : 64, 0, 1};
   const int64_t tile = 4 * p.rows;
   p.tiles = ragged ? rows / tile + sequences + 1 : sequences * ((each + tile - 1) / tile);
-  // a split's share of the longest sequence is 256 tokens at least
+  // Splits that leave the fewest tokens one after the other: rounds of workgroups (of ragged sequences those that can be
+  // expected to have rows) times a split's tokens. To begin and end costs a workgroup as much as two of a wave's steps
+  // of 64 tokens (waves without rows of their own share others' tokens), to join the parts as much again, and a split has no
+  // fewer. With w workgroups of the `resident` that fit a CU a round takes (resident + w) / 2 resident of a full one's time.
+  // 24 sequences of up to 1024 tokens, float32 of 256, 192 workgroups: in one 32 us, in two 42, in four 50; 119 workgroups of
+  // 2558 tokens, float32 of 192: in two 31 us, in three 44, in four 49; 8 workgroups of 131072 tokens: in 32 37 us, in 64 33;
+  // 2 workgroups of 64 rows on 800 tokens: in one 37 us, in six 18.
   const int64_t queries = sequences > 0 ? (tokens + sequences - 1) / sequences : 0;
   const int64_t longest = window > 0 && window + queries < capacity ? window + queries : capacity;
-  const int64_t groups = p.tiles * kv_heads, want = ((p.rows >= 32 ? 1 : 4) * cus + groups - 1) / groups, most = longest / 256;
-  const int64_t n = want < most ? want : most;
-  p.splits = n < 1 ? 1 : n > 64 ? 64 : (int)n;
+  const int64_t filled = ragged ? (rows / tile > sequences ? rows / tile : sequences) : p.tiles;
+  const int64_t groups = filled * kv_heads;
+  const int64_t resident = p.rows == 64 || head_dim > (f32 ? 64 : 128) ? 1 : f32 || p.rows > 16 || head_dim > 64 ? 2 : 4;
+  const int64_t cost = p.rows >= 32 ? 256 : 128 * (each <= p.rows ? 4 : each <= 2 * p.rows ? 2 : 1);
+  int64_t least = INT64_MAX;
+  for (int n = 1; n <= 64 && (n == 1 || n * cost <= longest); ++n) {
+    const int64_t all = n * groups, share = (longest + n - 1) / n + cost;
+    const int64_t full = all / (resident * cus), rest = all % (resident * cus);
+    const int64_t time = 2 * resident * (full * share + (n > 1 ? cost : 0)) + (rest ? resident + (rest + cus - 1) / cus : 0) * share;
+    if (time < least) least = time, p.splits = n;
+  }
   return p;
 }
 
