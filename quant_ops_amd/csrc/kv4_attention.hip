@@ -477,6 +477,43 @@ kv4_attention_join(const float* __restrict__ part, int splits, int64_t rows, typ
   __builtin_memcpy(out + row * DIM + d * 4, t, sizeof(t));
 }
 
+// The same of a few parts: DIM / 4 lanes have a row and weigh its parts themselves, 256 / (DIM / 4) rows to a workgroup.
+constexpr int kFewSplits = 4;
+template <class D, int DIM>
+__global__ void __launch_bounds__(256)
+kv4_attention_join_few(const float* __restrict__ part, int splits, int64_t rows, typename D::T* __restrict__ out) {
+  constexpr int LANES = DIM / 4, ROWS = 256 / LANES;
+  const int d = threadIdx.x % LANES;
+  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
+  if ((int)threadIdx.x >= ROWS * LANES || row >= rows) return;
+  float at[kFewSplits], total[kFewSplits], most = -kInf;
+  v4f v[kFewSplits];
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    const bool there = s < splits;
+    const int64_t slot = there ? s * rows + row : row;
+    const float* ml = part + splits * rows * DIM + slot * 2;
+    at[s] = there ? ml[0] : -kInf;
+    total[s] = ml[1];
+    v[s] = *reinterpret_cast<const v4f*>(part + slot * DIM + d * 4);
+    most = fmaxf(most, at[s]);
+  }
+  float all = 0.f;
+  v4f sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    if (at[s] == -kInf) continue;   // a part without tokens holds nothing
+    const float w = __builtin_amdgcn_exp2f(at[s] - most);
+    all = fmaf(w, total[s], all);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] = fmaf(w, v[s][j], sum[j]);
+  }
+  typename D::T t[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) t[j] = D::from_f(all == 0.f ? 0.f : sum[j] / all);
+  __builtin_memcpy(out + row * DIM + d * 4, t, sizeof(t));
+}
+
 template <class F>
 void with_dim(int dim, F&& f) {
   if (dim == 64) f(std::integral_constant<int, 64>{});
@@ -576,13 +613,15 @@ extern "C" int qo_kv4_attention(const qo_kv4_cache* cache, const qo_heads* q, in
       else kv4_prefill(a, dtype, DIM, 4 * plan.rows, grid, s);
       if (plan.splits > 1) {
         const int64_t rows = tokens * q_heads;
-        auto join = [&](auto groups) {
-          constexpr int GROUPS = decltype(groups)::value;
-          launch(kv4_attention_join<D, DIM, GROUPS>, dim3((unsigned)rows), dim3((GROUPS * DIM / 4 + 63) / 64 * 64), 0, s,
-                 reinterpret_cast<const float*>(workspace), plan.splits, rows, reinterpret_cast<typename D::T*>(out));
-        };
-        if (plan.splits <= 4) join(std::integral_constant<int, 2>{});
-        else join(std::integral_constant<int, 8>{});
+        const float* parts = reinterpret_cast<const float*>(workspace);
+        auto* to = reinterpret_cast<typename D::T*>(out);
+        constexpr int GROUPS = 8, ROWS = 256 / (DIM / 4);
+        if (plan.splits <= kFewSplits)
+          launch(kv4_attention_join_few<D, DIM>, dim3((unsigned)((rows + ROWS - 1) / ROWS)), dim3(256), 0, s, parts, plan.splits,
+                 rows, to);
+        else
+          launch(kv4_attention_join<D, DIM, GROUPS>, dim3((unsigned)rows), dim3((GROUPS * DIM / 4 + 63) / 64 * 64), 0, s, parts,
+                 plan.splits, rows, to);
       }
     });
   };

@@ -19,10 +19,6 @@ namespace qo {
 
 namespace {
 
-#ifndef KV4_V1
-#define KV4_V1 3
-#define KV4_V2 3
-#endif
 // A weight at the row's reference, in fp16, and how far (exponents) a larger score may pass the reference before
 // sums and outputs move to it: each row's maximum grows now and then, some row's of 32 nearly every step.
 constexpr int kAtRest = 6;
@@ -56,7 +52,8 @@ kv4_prefill_kernel(Attention a) {
   struct Stage {
     v4u k[2][NS][64];      // fragments: 32 tokens, k-step
     v4u v[NF][4][64];      // block of values, 16 tokens
-    v4u params[4][2][4];   // EXACT: keys' s, lo, values' s, lo; lane half g; its 32 tokens, 8 to a piece
+    v4f params[4][2][8];   // EXACT: keys' scale and middle, values' middle and scale; lane half g; its 32 tokens
+    int largest[4];        // EXACT: of 16 values' scales, the exponent's bits
   };
   __shared__ Stage stage[2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, g = lane >> 5;
@@ -117,7 +114,7 @@ kv4_prefill_kernel(Attention a) {
     for (int i = 0; i < 16; ++i) o[f][i] = 0.f;
   float most = -kInf, at = 0.f, middles = 0.f;
   float total = qsum != qsum && see.last > see.first ? qsum : 0.f;   // infinite queries: NaN, also where all scores are -inf
-  int scale_exp = -14;
+  int scale_exp = -14;   // EXACT: every scale so far is below two to it
 
   const int begin = all_top.first & ~63;
   const int steps = all_bottom.last > begin ? (all_bottom.last - begin + 63) / 64 : 0;
@@ -217,8 +214,19 @@ kv4_prefill_kernel(Attention a) {
       // token 16 part + c of the step: of lane half (c / 4) % 2, its token 8 part + 4 (c / 8) + c % 4
       if (keys && d == 0) {
         const int half_of_c = c >> 2 & 1, place = 8 * part + 4 * (c >> 3) + (c & 3);
-        auto put = [&](int which, uint32_t x) { reinterpret_cast<uint16_t*>(&st.params[which][half_of_c][0])[place] = (uint16_t)x; };
-        put(0, key_s), put(1, key_lo), put(2, value_s), put(3, value_lo);
+        auto put = [&](int which, float x) { reinterpret_cast<float*>(&st.params[which][half_of_c][0])[place] = x; };
+        const float ks = half_of(&key_s, 0), vs = half_of(&value_s, 0);
+        put(0, ks);
+        put(1, fmaf(8.f, ks, half_of(&key_lo, 0)));
+        put(2, fmaf(8.f, vs, half_of(&value_lo, 0)));
+        put(3, vs);
+        uint32_t top_of = value_s & 0x7FFFu;
+        auto with = [&](int other) { top_of = max(top_of, (uint32_t)other); };
+        with(__builtin_amdgcn_update_dpp(0, (int)top_of, 0xB1, 0xF, 0xF, false));    // quad_perm 1,0,3,2
+        with(__builtin_amdgcn_update_dpp(0, (int)top_of, 0x4E, 0xF, 0xF, false));    // quad_perm 2,3,0,1
+        with(__builtin_amdgcn_update_dpp(0, (int)top_of, 0x141, 0xF, 0xF, false));   // row_half_mirror
+        with(__builtin_amdgcn_update_dpp(0, (int)top_of, 0x140, 0xF, 0xF, false));   // row_mirror
+        if (c == 0) st.largest[part] = (int)(top_of >> 10);
       }
     }
   };
@@ -266,40 +274,28 @@ kv4_prefill_kernel(Attention a) {
             if constexpr (NP > 1) o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[i], o[f], 0, 0, 0);
           }
       };
-      uint32_t vs[8], vl[8];   // EXACT: of the lane's 16 tokens
-      float eight = 0.f;
       float shrink_o = 1.f;
+      // EXACT: a parameter of the lane's 16 tokens of a half.
+      auto params = [&](int which, int u, float(&x)[16]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const v4f four = st.params[which][g][4 * u + i];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[4 * i + j] = four[j];
+        }
+      };
       // Parameters, masks and the largest score; sums follow a larger one, and outputs do in rescale(), once the
       // weights made before it are in them.
       auto largest = [&](int u) {
         int exp_now = scale_exp;
         if constexpr (EXACT) {
-          uint32_t ks[8], kl[8];
+          float ks[16], middle[16];
+          params(0, u, ks);
+          params(1, u, middle);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const v4u x = st.params[0][g][2 * u + i], y = st.params[1][g][2 * u + i], z = st.params[2][g][2 * u + i], t = st.params[3][g][2 * u + i];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) ks[4 * i + j] = x[j], kl[4 * i + j] = y[j], vs[4 * i + j] = z[j], vl[4 * i + j] = t[j];
-          }
-#pragma unroll
-          for (int t = 0; t < 16; ++t) {
-            const float s = half_of(ks, t);
-            sc[u][t] = fmaf(s, sc[u][t], fmaf(8.f, s, half_of(kl, t)) * qsum);
-          }
-          uint32_t big = 0;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) big = pk_max_u16(big, vs[i]);
-          const uint32_t field = halves_reduce(max(big & 0xFFFFu, big >> 16) >> 10, UMax{});
-          exp_now = max(scale_exp, __builtin_amdgcn_readfirstlane((int)field) - 14);
-          const int up = kAtRest - exp_now;
-          auto by_power = [&](int e) {
-            const _Float16 f = (_Float16)power_of_two(e);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) vs[i] = pk(unpk(vs[i]) * (v2h){f, f});
-          };
-          by_power(min(up, 15));
-          if (up > 15) by_power(up - 15);
-          eight = power_of_two(3 - up);
+          for (int t = 0; t < 16; ++t) sc[u][t] = fmaf(ks[t], sc[u][t], middle[t] * qsum);
+          const int field = max(st.largest[2 * u], st.largest[2 * u + 1]);
+          exp_now = max(scale_exp, __builtin_amdgcn_readfirstlane(field) - 14);
         }
         if (!(t0 + 32 * u + 32 <= top.last && t0 + 32 * u >= bottom.first)) {   // some row does not see some token
 #pragma unroll
@@ -314,13 +310,12 @@ kv4_prefill_kernel(Attention a) {
         now = bits_float(halves_reduce(float_bits(now), FMax{}));
         if (__any(factor * (now - most) > kSlack) || exp_now > scale_exp) {
           now = fmaxf(now, most);
-          const float next = now == -kInf ? 0.f : factor * now - (EXACT ? 0 : kAtRest);
-          const float shrink = most == -kInf ? 1.f : __builtin_amdgcn_exp2f(at - next);   // before: all sums 0
-          shrink_o = shrink * power_of_two(scale_exp - exp_now);
+          const float next = (now == -kInf ? 0.f : factor * now) - (float)(kAtRest - (EXACT ? exp_now : 0));
+          shrink_o = most == -kInf ? 1.f : __builtin_amdgcn_exp2f(at - next);   // before: all sums 0
           most = now;
           at = next;
-          total *= shrink;
-          middles *= shrink;
+          total *= shrink_o;
+          middles *= shrink_o;
           scale_exp = exp_now;
           return true;
         }
@@ -334,17 +329,21 @@ kv4_prefill_kernel(Attention a) {
         __builtin_amdgcn_sched_barrier(0);
       };
       auto weights = [&](int u) {
+        float middle[16], vs[16];
+        if constexpr (EXACT) {
+          params(2, u, middle);
+          params(3, u, vs);
+        }
 #pragma unroll
         for (int t = 0; t < 16; ++t) {
           const float p = __builtin_amdgcn_exp2f(fmaf(factor, sc[u][t], -at));
           total += p;
           if constexpr (EXACT) {
-            const float s = half_of(vs, t);
-            middles = fmaf(p, fmaf(eight, s, half_of(vl, t)), middles);
-            _Float16 h = (_Float16)fmaf(p, s, 0.f);
+            middles = fmaf(p, middle[t], middles);
+            _Float16 h = (_Float16)fmaf(p, vs[t], 0.f);
             if constexpr (NP > 1) {
               asm("" : "+v"(h));   // one and the same rounding in both parts
-              pl[2 * u + t / 8][t % 8] = (_Float16)fmaf(p, s, -(float)h);
+              pl[2 * u + t / 8][t % 8] = (_Float16)fmaf(p, vs[t], -(float)h);
             }
             ph[2 * u + t / 8][t % 8] = h;
           } else {
@@ -380,12 +379,12 @@ kv4_prefill_kernel(Attention a) {
       rescale(largest(0));
       scores(1);
       weights(0);
-      beside(std::integral_constant<int, NS>{}, std::integral_constant<int, KV4_V1>{});
+      beside(std::integral_constant<int, NS>{}, std::integral_constant<int, 3>{});
       const bool larger = largest(1);
       __builtin_amdgcn_sched_barrier(0);
       values(0);
       weights(1);
-      beside(std::integral_constant<int, 2 * NF * NP>{}, std::integral_constant<int, KV4_V2>{});
+      beside(std::integral_constant<int, 2 * NF * NP>{}, std::integral_constant<int, 3>{});
       rescale(larger);
       values(1);
       beside(std::integral_constant<int, 2 * NF * NP>{}, std::integral_constant<int, 0>{});
@@ -399,7 +398,7 @@ kv4_prefill_kernel(Attention a) {
   if (most == -kInf && total == 0.f) at = -kInf;
   if (w.poison) total = __builtin_nanf(""), at = 0.f;
   if (first_row + r > last_row) return;
-  const float unit = EXACT ? power_of_two(scale_exp - kAtRest) : 2.f;
+  const float unit = EXACT ? 1.f : 2.f;
   const int64_t total_rows = (int64_t)a.tokens * a.q_heads;   // of all heads
   const int64_t at_row = (int64_t)(w.start + row / a.group) * a.q_heads + head * a.group + row % a.group;
 #pragma unroll
