@@ -128,6 +128,23 @@ def test_large_prefill_equals_the_host(gpu):
     assert torch.equal(a, b.cpu()) and _same(host, [t.cpu() for t in dev])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,heads,kv,interleaved,first", [(64, 19, 7, False, 33), (128, 19, 7, True, 65), (192, 11, 9, False, 2), (96, 40, 4, True, 64)])
+def test_many_heads_equal_the_host(gpu, dim, heads, kv, interleaved, first, dtype):
+    """Several heads to a workgroup, the last groups not full; a run of slots that starts inside a word, with holes; values
+    of few bits, so that many lie on a border between codes."""
+    _say(f"many heads {dim} {heads} {kv} {first} {dtype}")
+    g = torch.Generator().manual_seed(dim + heads)
+    tokens = 2100
+    x = (torch.randint(-60, 61, (tokens, heads + 2 * kv, dim), generator=g) / 8).to(dtype)
+    slots = torch.arange(tokens) + first
+    slots[::97] = -1
+    cos, sin = angles(tokens, dim)
+    host, dev, a, b = _both(gpu, x[:, heads:heads + kv], x[:, heads + kv:], slots, page=64, pages=40, positions=torch.arange(tokens),
+                            cos=cos, sin=sin, q=x[:, :heads], interleaved=interleaved)
+    assert torch.equal(a, b.cpu()) and _same(host, [t.cpu() for t in dev])
+
+
 def test_other_strides(gpu):
     """Heads before tokens, values at a stride of two, one row for all tokens, offsets of one element."""
     g = torch.Generator().manual_seed(12)
@@ -193,11 +210,22 @@ GPU_CASES = [
     ([500, 450, 333], 3, 1, 128, 16, [300, 129, 43], 0),
     ([3], 1, 1, 256, 16, 3, 0),
     ([2], 2, 1, 128, 16, 40, 0),       # queries before the first token
+    ([4000, 70], 4, 1, 64, 64, 1, 0),  # many parts
 ]
 
 
+# Every kernel of every head size: waves of 4, 8 and 16 rows, prompts in tiles of 128 and 256.
+EVERY_KERNEL = [c for dim in (64, 96, 128, 192, 256) for c in (
+    ([150, 21], 6, 2, dim, 16, 1, 0),
+    ([99, 140], 6, 1, dim, 32, 1, 70),
+    ([77, 200, 31], 6, 1, dim, 16, [9, 4, 3], 0),
+    ([200, 65], 3, 1, dim, 64, 33, 0),
+    ([190, 260], 3, 1, dim, 16, [110, 90], 0),
+)]
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("case", GPU_CASES)
+@pytest.mark.parametrize("case", GPU_CASES + EVERY_KERNEL)
 def test_attention_more(gpu, case, dtype):
     _say(f"attention {case} {dtype}")
     _check(gpu, *make(case, dtype))
