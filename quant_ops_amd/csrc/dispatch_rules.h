@@ -184,7 +184,8 @@ inline Kv4Plan kv4_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64
   const int64_t longest = window > 0 && window + queries < capacity ? window + queries : capacity;
   const int64_t filled = ragged ? (rows / tile > sequences ? rows / tile : sequences) : p.tiles;
   const int64_t groups = filled * kv_heads;
-  const int64_t resident = p.rows == 64 || head_dim > (f32 ? 64 : 128) ? 1 : f32 || p.rows > 16 || head_dim > 64 ? 2 : 4;
+  const int64_t most = p.rows <= 8 ? 256 : p.rows == 16 ? (f32 ? 96 : 192) : p.rows == 32 ? 128 : 0;   // head_dim of two
+  const int64_t resident = head_dim > most ? 1 : head_dim > 64 || p.rows > (f32 ? 8 : 16) ? 2 : 4;
   const int64_t cost = p.rows >= 32 ? 256 : 128 * (each <= p.rows ? 4 : each <= 2 * p.rows ? 2 : 1);
   int64_t least = INT64_MAX;
   for (int n = 1; n <= 64 && (n == 1 || n * cost <= longest); ++n) {

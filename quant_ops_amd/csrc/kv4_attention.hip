@@ -24,15 +24,23 @@
 //
 // Rows that are few (FOLD times 16 / FOLD of them) stand in every 16 / FOLD columns again, and the lanes
 // of those columns share a row's scores: each takes 16 / FOLD of its group's tokens from the scores
-// to the weights, which then go back to the first columns.
+// to the weights, which then go back to the first columns. Second parts (of float32 queries, of weights) then
+// stand in columns 8 .. 15: one product makes the sums of both parts, in half the instructions and registers, and the two
+// meet by a rotation of lanes (24 sequences of 1024 tokens, float32 of 256: 32 -> 26 us;
+// 16 x 2048 tokens of 32 heads, fp16: 25 -> 24).
 //
 // Queries: brought by a power of two for each row to a largest magnitude in [2^14, 2^15), 16-bit
 // values are exact in fp16 (those below 2^-28 of the largest lose bits); float32 takes two fp16
 // parts (22 bits). Weights: p s 2^14 / S, where p is 1 at the row's largest score so far and S a
 // power of two that no scale of the tokens so far exceeds, is at most 2^14, and rounded to fp16 (half
-// a step 2^-12, beside bf16's 2^-9 of the output) or, for fp16 and float32, to two parts. In
+// a step 2^-11, beside bf16's 2^-8 of the output) or, for fp16 and float32, to two parts. In
 // float32 the second parts have sums of their own: added to the first parts' they would lose what is
 // below 2^-24 of those. Maximum, sums and outputs are float32.
+//
+// What bounds it: one sequence of 131072 tokens (64 heads on 8 of 128, bf16, 142 MB) takes 32 us, 4.4 TB/s, and
+// 262144 tokens come at the 5.0 TB/s of a copy; 64 sequences of 100 to 4096 tokens (32 on 8 heads, 146 MB) take 41 us, 3.5
+// TB/s, for which unpacking and softmax take as long as the bytes. Loads a step ahead were worth 100 -> 55 us there, lanes
+// that share scores 55 -> 46.
 #include "dispatch_rules.h"
 #include "kv4_attention.h"
 
@@ -47,15 +55,18 @@ __device__ inline uint32_t row_reduce(uint32_t u, F f) {
   if constexpr (CW <= 8) u = f(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x128, 0xF, 0xF, false));   // row_ror:8
   return groups_reduce(u, f);
 }
-// In lanes Q CW .. of a row of 16 the value that lane r - Q CW has, elsewhere old; and back.
-template <int CW, int Q>
-__device__ inline uint32_t to_lanes(uint32_t old, uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, 0x110 + CW * Q, 0xF, CW == 8 ? 0xC : 1 << Q, false);   // row_shr
-}
+// The value of lane r + Q CW of a row of 16 (0 beyond).
 template <int CW, int Q>
 __device__ inline uint32_t from_lanes(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x100 + CW * Q, 0xF, 0xF, true);   // row_shl
 }
+
+// v from another lane of the row of 16 (CTRL) in lanes of the banks of four of BANKS, elsewhere old.
+template <int CTRL, int BANKS>
+__device__ inline uint32_t merge(uint32_t old, uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, 0xF, BANKS, false);
+}
+constexpr int kStay = 0xE4, kRor8 = 0x128, kShl4 = 0x104, kShl12 = 0x10C, kShr4 = 0x114;   // quad_perm, row_ror, row_shl, row_shr
 
 // The eight codes of a key's word in the order of kCodeOrder: even ones times kEven, odd ones times
 // kOdd, all less kLess.
@@ -78,13 +89,15 @@ __device__ inline v8h values_odd(uint32_t a, uint32_t b, uint32_t e) {
 }
 
 template <class D, int DIM, int FOLD, int NQ, int NP, bool FINE>
-__global__ void __launch_bounds__(256, DIM <= 128 && !FINE ? 2 : 1)
+__global__ void __launch_bounds__(256, DIM <= (FOLD > 1 ? 256 : FINE ? 96 : 192) ? 2 : 1)
 kv4_attention_kernel(Attention a) {
+  constexpr bool PACK = NP > 1 && FOLD > 1;   // second parts in columns 8 .. 15
+  constexpr int NQF = PACK ? 1 : NQ;
   constexpr int NS = DIM / 32;        // k-steps of a score, words of a key's codes in a lane
   constexpr int NF = DIM / 32;        // blocks of 16 pairs of values
   constexpr int CW = 16 / FOLD;       // columns with rows of their own, and tokens of a step for a lane's softmax
   constexpr int TILE = 4 * CW;
-  constexpr int APART = FINE;         // second parts of weights have sums of their own
+  constexpr int APART = FINE && !PACK;   // second parts of weights have sums of their own
   using C = Codes<FINE>;
   using T = typename D::T;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
@@ -105,7 +118,7 @@ kv4_attention_kernel(Attention a) {
   const Sees top = sees(a, w, first_row), bottom = sees(a, w, last_row), see = sees(a, w, row);
 
   // The query as fp16 parts in the order of Codes::of, the odd codes' factor taken out.
-  v8h qf[NQ][NS];
+  v8h qf[NQF][NS];
   float factor, qsum;   // of the exponent of two; sum of the query, in units of its scores
   {
     const T* q = reinterpret_cast<const T*>(a.q) + (w.start + row / a.group) * a.q_token + (head * a.group + row % a.group) * a.q_head;
@@ -130,8 +143,13 @@ kv4_attention_kernel(Attention a) {
         const float v = ldexpf(x[s][kCodeOrder[i]], e);
         sum += v;
         const float part = opaque(kCodeOrder[i] & 1 ? v * (C::kEven / C::kOdd) : v);
-        qf[0][s][i] = (_Float16)part;
-        if constexpr (NQ > 1) qf[1][s][i] = (_Float16)(part - (float)qf[0][s][i]);
+        const _Float16 hi = (_Float16)part;
+        qf[0][s][i] = hi;
+        if constexpr (NQ > 1) {
+          const _Float16 lo = (_Float16)(part - (float)hi);
+          if constexpr (PACK) qf[0][s][i] = r & 8 ? lo : hi;
+          else qf[1][s][i] = lo;
+        }
       }
     sum = bits_float(groups_reduce(float_bits(sum), FAdd{}));
     qsum = most < kInf ? sum * C::kEven : __builtin_nanf("");   // an infinity's scores are NaN
@@ -206,9 +224,9 @@ kv4_attention_kernel(Attention a) {
       for (int s = 0; s < NS; ++s) {
         const v8h c = C::of(kw[u][s], exponents);
         sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, qf[0][s], sc[u], 0, 0, 0);
-        if constexpr (NQ > 1) rest = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, qf[1][s], rest, 0, 0, 0);
+        if constexpr (NQF > 1) rest = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, qf[1][s], rest, 0, 0, 0);
       }
-      if constexpr (NQ > 1) {
+      if constexpr (NQF > 1) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) sc[u][i] += rest[i];
       }
@@ -216,17 +234,24 @@ kv4_attention_kernel(Attention a) {
     float x[CW];   // of the lane's tokens
 #pragma unroll
     for (int t = 0; t < CW; ++t) {
-        auto at_token = [&](int i) { return float_bits(sc[i / 4][i % 4]); };
-        uint32_t y = at_token(t);
-        if constexpr (FOLD == 2) y = to_lanes<CW, 1>(y, at_token(CW + t));
+      auto at_token = [&](int i) { return float_bits(sc[i / 4][i % 4]); };
+      auto pick = [&](int first) {   // token first + t of the lane's own, of columns with the same values
+        const int n = FOLD - 1;
+        uint32_t y = at_token(first + t);
+        if constexpr (FOLD == 2) y = merge<kStay, 0xC>(y, at_token((first + CW & n * CW) + t));
         if constexpr (FOLD == 4) {
-          y = to_lanes<CW, 1>(y, at_token(CW + t));
-          y = to_lanes<CW, 2>(y, at_token(2 * CW + t));
-          y = to_lanes<CW, 3>(y, at_token(3 * CW + t));
+          y = merge<kStay, 2>(y, at_token((first + CW & n * CW) + t));
+          y = merge<kStay, 4>(y, at_token((first + 2 * CW & n * CW) + t));
+          y = merge<kStay, 8>(y, at_token((first + 3 * CW & n * CW) + t));
         }
-        const float s = half_of(ks, t), lo = half_of(kl, t);
-        x[t] = fmaf(s, bits_float(y), fmaf(C::kLess, s, lo) * qsum);
-      }
+        return y;
+      };
+      uint32_t y = pick(0);
+      // the other part's share comes from the column 8 apart
+      if constexpr (PACK && NQ > 1) y = float_bits(bits_float(y) + bits_float(merge<kRor8, 0xF>(0, pick(8))));
+      const float s = half_of(ks, t), lo = half_of(kl, t);
+      x[t] = fmaf(s, bits_float(y), fmaf(C::kLess, s, lo) * qsum);
+    }
     __builtin_amdgcn_sched_barrier(0);
     const bool bad_now = bad;
     if (more) {
@@ -322,11 +347,32 @@ kv4_attention_kernel(Attention a) {
                    : (v4u){from_lanes<CW, 2>(x[0]), from_lanes<CW, 2>(x[1]), from_lanes<CW, 3>(x[0]), from_lanes<CW, 3>(x[1])};
       return __builtin_bit_cast(v8h, v);
     };
+    // the same with the second parts, in columns 8 ..
+    auto both = [&](int z) {
+      v4u v;
+      if constexpr (PACK && FOLD == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = z == 0 ? merge<kRor8, 0xC>(wh[i], wl[i]) : merge<kRor8, 0x3>(wl[i], wh[i]);
+      }
+      if constexpr (PACK && FOLD == 4) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          v[i] = z == 0 ? merge<kRor8, 0x4>(wh[i], wl[i]) : merge<kRor8, 0x1>(wl[i], wh[i]);
+          v[2 + i] = z == 0 ? merge<kShr4, 0x4>(merge<kShl4, 0xF>(0, wh[i]), wl[i])
+                            : merge<kShl12, 0x1>(merge<kShl4, 0xF>(0, wl[i]), wh[i]);
+        }
+      }
+      return __builtin_bit_cast(v8h, v);
+    };
     v8h ph[2], pl[2];
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
-      ph[z] = weights(wh, z);
-      if constexpr (NP > 1) pl[z] = weights(wl, z);
+      if constexpr (PACK) {
+        ph[z] = both(z);
+      } else {
+        ph[z] = weights(wh, z);
+        if constexpr (NP > 1) pl[z] = weights(wl, z);
+      }
     }
 #pragma unroll
     for (int f = 0; f < NF; ++f)
@@ -336,7 +382,7 @@ kv4_attention_kernel(Attention a) {
         v4f(&hi)[2] = o[0][f], (&lo)[2] = o[APART][f];
         hi[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, ph[z], hi[0], 0, 0, 0);
         hi[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, ph[z], hi[1], 0, 0, 0);
-        if constexpr (NP > 1) {
+        if constexpr (NP > 1 && !PACK) {
           lo[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, pl[z], lo[0], 0, 0, 0);
           lo[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, pl[z], lo[1], 0, 0, 0);
         }
@@ -359,6 +405,12 @@ kv4_attention_kernel(Attention a) {
   for (int f = 0; f < NF; ++f)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      if constexpr (PACK) {
+        for (int h = 0; h < 2; ++h) {
+          const float first = o[0][f][h][i];
+          o[0][f][h][i] = first + bits_float(merge<kRor8, 0xF>(0, float_bits(first)));
+        }
+      }
       if constexpr (APART) o[0][f][0][i] += o[1][f][0][i], o[0][f][1][i] += o[1][f][1][i];
       o[0][f][0][i] = fmaf(o[0][f][0][i], unit, middles);
       o[0][f][1][i] = fmaf(o[0][f][1][i], 0.0625f * unit, middles);
