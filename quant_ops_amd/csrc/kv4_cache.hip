@@ -43,15 +43,6 @@ namespace {
 template <int DIM>
 constexpr int kLanes = DIM <= 64 ? 8 : DIM <= 128 ? 16 : 32;
 
-// N elements at p (16 bytes at most, at any alignment).
-template <class D, int N>
-__device__ inline void load_values(const typename D::T* p, float* v) {
-  typename D::T t[N];
-  __builtin_memcpy(t, p, sizeof(t));
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = D::to_f(t[i]);
-}
-
 // Over the LANES lanes of a vector.
 template <int LANES, class F>
 __device__ inline float lanes_reduce(float v, F&& f) {

@@ -1,9 +1,12 @@
 // Attention over the 4-bit cache for sequences of many rows (prompts and their chunks), 16-bit types:
 // the mathematics of kv4_attention.hip with the codes unpacked once for a workgroup.
 //
-// Four waves of 32 rows share tiles of 64 tokens: while they multiply one, each unpacks a quarter of
-// the next (its codes on their way to registers since a tile before) into the other half of LDS, as
-// fragments of v_mfma_f32_32x32x16_f16 that a wave reads with consecutive 16-byte reads. Fragments: lane
+// Waves of 32 rows share tiles of 64 tokens: while they multiply one, each unpacks a part of the next (its
+// codes on their way to registers since a tile before) into the other half of LDS, as fragments of
+// v_mfma_f32_32x32x16_f16 that a wave reads with consecutive 16-byte reads. Eight waves have two tiles of 128 rows:
+// the first four one tile and the keys' unpacking, the others the tile that mirrors it from the sequence's end and
+// the values' (half the unpacking a row, and under a causal mask every workgroup the same work); fewer rows, and head
+// sizes whose outputs leave no room for two waves on a SIMD, have four. Fragments: lane
 // l = r + 32 g of an operand holds eight consecutive k of row r, a lane of the result rows 8 m + 4 g + i
 // (register 4 m + i) of column r. S^T = K Q^T (rows: 32 tokens), O^T += V^T P^T (rows: the even and then
 // the odd values of 16 pairs): lane half g has tokens 8 m + 4 g + i of a tile's weights, in the order in which
@@ -12,7 +15,14 @@
 // bf16 (EXACT false): keys and values are unpacked to what they stand for, halved (15 steps of a scale may
 // pass fp16's range), rounded to fp16: half a step of 2^-11, beside 2^-8 of the output. That takes the
 // parameters out of the softmax, whose instructions bound the kernel. fp16 (EXACT): codes less 8, the parameters
-// applied to scores in float32 and weights in two parts, as in kv4_attention.hip.
+// applied to scores in float32 and weights in two parts, as in kv4_attention.hip; they come from LDS as float32,
+// and the power of two that brings weights times scales into fp16 stands in the exponent's argument.
+//
+// A wave's 32 x 64 scores take about 500 vector instructions and 32 exponentials beside 32 products (128 values,
+// bf16), on the same SIMD: products run beside the other half's softmax, but the two overlap in part only. 2048
+// queries of 32 heads on 4096 tokens (8 heads): of 128 136 us in bf16 (758 TFLOP/s of the pairs that a causal mask
+// leaves, 63% of a large product's rate) and 199 in fp16, of 64 103 and 157. On the way: one product after
+// the other 152 us, fragments four reads ahead 149, eight waves and products beside the softmax 136.
 #include "kv4_attention.h"
 
 namespace qo {

@@ -219,6 +219,7 @@ EVERY_KERNEL = [c for dim in (64, 96, 128, 192, 256) for c in (
     ([150, 21], 6, 2, dim, 16, 1, 0),
     ([99, 140], 6, 1, dim, 32, 1, 70),
     ([77, 200, 31], 6, 1, dim, 16, [9, 4, 3], 0),
+    ([90, 333], 8, 1, dim, 32, 3, 0),
     ([200, 65], 3, 1, dim, 64, 33, 0),
     ([190, 260], 3, 1, dim, 16, [110, 90], 0),
 )]
