@@ -531,7 +531,7 @@ typedef struct qo_kv4_cache {
   int32_t head_dim;
 } qo_kv4_cache;
 #define QO_KV4_MAX_PAGE 4096
-#define QO_KV4_MAX_TOKENS (1LL << 27)
+#define QO_KV4_MAX_TOKENS (1LL << 26)
 
 /* Vectors of [tokens, heads, head_dim] at any strides (in elements), unit inner stride. */
 typedef struct qo_heads {
@@ -577,7 +577,7 @@ int qo_kv4_read(const qo_kv4_cache* cache, const int64_t* slots, int64_t tokens,
  *   page_table  int32 [sequences, table_width], row stride table_ld: pages of each sequence in
  *               order. A visible token on a page outside the cache makes its queries NaN
  *   lengths     int32 [sequences]: cached tokens, those of the queries included (negative: 0).
- *               One above table_width * page_size makes the sequence's queries NaN
+ *               One above table_width * page_size or 2^31 - 4096 makes the sequence's queries NaN
  *   q_starts    int32 [sequences + 1], ascending from 0: sequence b has the queries
  *               q_starts[b] .. q_starts[b + 1] - 1, or NULL: tokens / sequences each. Rows from
  *               the last entry on are zeros

@@ -184,9 +184,10 @@ inline Kv4Plan kv4_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64
   // 2 workgroups of 64 rows on 800 tokens: in one 37 us, in six 18; 8 ragged sequences of 300 to 2000 tokens, half of them
   // prompts: in one 89 us, in two 80, in three 73, in four 78.
   const int64_t queries = sequences > 0 ? (tokens + sequences - 1) / sequences : 0;
-  const int64_t longest = window > 0 && window + queries < capacity ? window + queries : capacity;
+  const int64_t seen = window > 0 && window < (int64_t)1 << 31 && window + queries < capacity ? window + queries : capacity;
+  const int64_t longest = seen < (int64_t)1 << 31 ? seen : (int64_t)1 << 31;
   const int64_t filled = ragged ? (rows / tile > sequences ? rows / tile : sequences) : p.tiles;
-  const int64_t groups = filled * kv_heads;
+  const int64_t groups = filled * kv_heads < 1 << 24 ? filled * kv_heads : 1 << 24;
   const int64_t most = p.rows <= 8 ? 256 : p.rows == 16 ? (f32 ? 96 : 192) : p.rows == 32 ? 128 : 0;   // head_dim of two
   const int64_t resident = head_dim > most ? 1 : head_dim > 64 || p.rows > (f32 ? 8 : 16) ? 2 : 4;
   const int64_t cost = p.rows >= 32 ? 256 : 128 * (each <= p.rows ? 4 : each <= 2 * p.rows ? 2 : 1);

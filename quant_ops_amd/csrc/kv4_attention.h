@@ -14,7 +14,7 @@ typedef unsigned v2u __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.44269504f;
 constexpr float kInf = __builtin_inff();
-constexpr int kMostTokens = 0x7FFFFF00;   // of a sequence: positions and steps take 32 bits
+constexpr int kMostTokens = 0x7FFFF000;   // of a sequence: positions take 32 bits, those a few steps ahead too
 
 struct Attention {
   KV4 cache;

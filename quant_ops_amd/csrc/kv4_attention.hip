@@ -636,8 +636,8 @@ extern "C" int qo_kv4_attention(const qo_kv4_cache* cache, const qo_heads* q, in
       (!workspace || workspace_bytes < plan.splits * tokens * q_heads * (cache->head_dim + 2) * 4))
     plan.splits = 1;
   const int64_t grid = plan.tiles * c.heads * plan.splits;
-  // rows of a KV head, workgroups (256 threads each) and a page's bytes take 32 bits
-  if (tokens * (q_heads / c.heads) > (1 << 30) || grid > (1 << 24) - 1) {
+  // rows of a KV head, threads (512 a workgroup at most) and a page's bytes take 32 bits
+  if (tokens * (q_heads / c.heads) > (1 << 30) || grid > (1 << 23) - 1) {
     qo_set_error("%s: too many rows for one call (%lld queries of %d heads)", fn, (long long)tokens, q_heads);
     return QO_ERR_SHAPE;
   }

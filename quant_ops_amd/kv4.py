@@ -264,7 +264,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, le
     scale (positive) defaults to 1 / sqrt(D).
 
     A query that sees a token on a page outside the cache gives NaN, and so do those of a sequence
-    longer than its row of page_table (entries past a sequence's tokens are not used). A narrower
+    longer than its row of page_table or than 2^31 - 4096 tokens (entries past a sequence's tokens are not used). A narrower
     view of page_table tells the operator that no sequence is longer.
     """
     if scale is None:

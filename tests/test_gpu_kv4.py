@@ -447,6 +447,20 @@ def _step(inputs, cache, heads=8, kv=2):
     return qo.kv4_attention(q, cache, table, lengths)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries", [1, 60])
+def test_positions_next_to_31_bits(gpu, queries, dtype):
+    """The longest sequence there may be, over one page, and one that is longer."""
+    g = torch.Generator().manual_seed(8)
+    cache = random_cache(g, 2, 4096, 1, 64)
+    q = torch.randn(queries, 3, 64, generator=g).to(dtype)
+    most = 0x7FFFF000
+    table = torch.ones(1, most // 4096 + 2, dtype=torch.int32)
+    got = _run(gpu, q, cache, table, torch.tensor([most], dtype=torch.int32), window=100)
+    check(q, got, cache, torch.ones(1, 1, dtype=torch.int32), torch.tensor([4096], dtype=torch.int32), 0.125, None, 100)
+    assert torch.isnan(_run(gpu, q, cache, table, torch.tensor([most + 1], dtype=torch.int32), window=100)).all()
+
+
 def test_a_step_of_all(gpu):
     """Appended, read and attended to, as a decode step runs them."""
     inputs, cache = _step_inputs(gpu, 1)
