@@ -347,8 +347,8 @@ kv4_prefill_kernel(Attention a) {
 #pragma unroll
         for (int t = 0; t < 16; ++t) {
           const float p = __builtin_amdgcn_exp2f(fmaf(factor, sc[u][t], -at));
-          total += p;
           if constexpr (EXACT) {
+            total += p;
             middles = fmaf(p, middle[t], middles);
             _Float16 h = (_Float16)fmaf(p, vs[t], 0.f);
             if constexpr (NP > 1) {
@@ -358,6 +358,8 @@ kv4_prefill_kernel(Attention a) {
             ph[2 * u + t / 8][t % 8] = h;
           } else {
             ph[2 * u + t / 8][t % 8] = (_Float16)p;
+            // the sum of the weights as they are rounded, two an instruction
+            if (t & 1) total = __builtin_amdgcn_fdot2((v2h){ph[2 * u + t / 8][t % 8 - 1], ph[2 * u + t / 8][t % 8]}, (v2h){(_Float16)1.f, (_Float16)1.f}, total, false);
           }
         }
         // here and not where the product takes them
