@@ -66,7 +66,7 @@ kv4_prefill_kernel(Attention a) {
     int largest[4];        // EXACT: of 16 values' scales, the exponent's bits
   };
   __shared__ Stage stage[2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, g = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, g = lane >> 5;
   const int heads = a.cache.heads;
   const int head = blockIdx.x % heads, split = blockIdx.x / heads / a.tiles;
   const Rows w = find_rows<TILE>(a, blockIdx.x / heads % a.tiles);
