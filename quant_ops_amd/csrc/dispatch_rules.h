@@ -162,7 +162,7 @@ inline MxPlan mx_plan(int64_t M, int64_t N, int64_t blocks, bool fp8, int64_t cu
 // they share the tiles that they read (kv4_prefill, 16-bit types). `splits` workgroups share a tile's tokens.
 // 16 sequences of 2048 tokens on 4 heads of 128, bf16, in waves of 16, 32, 32 x 8: of 32 rows 21, 22, 22 us, of 48 29, 28, 24,
 // of 96 38, 31, 30, of 192 60, 41, 37 (fp16: 22, 25, 29; 30, 31, 31; 40, 35, 36; 62, 49, 45); one sequence of 4096 tokens:
-// of 128 rows 18, 20, 20, of 200 22, 20, 23, and 8192 rows on 8 heads 149 and 136 us in waves of 32 and 32 x 8.
+// of 128 rows 18, 20, 20, of 200 22, 20, 23; heads of 192, bf16, in 16 and 32: of 48 rows 32, 35, of 64 36, 37, of 96 46, 39; and 8192 rows on 8 heads 149 and 136 us in waves of 32 and 32 x 8.
 struct Kv4Plan {
   int rows;        // 4, 8, 16, 32 or 64
   int64_t tiles;   // of 4 rows, of all sequences
@@ -172,7 +172,7 @@ inline Kv4Plan kv4_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64
                         int64_t sequences, bool ragged, int64_t window, bool f32, int64_t cus) {
   const int64_t group = q_heads / kv_heads, rows = tokens * group;
   const int64_t each = sequences > 0 ? (rows + sequences - 1) / sequences : 0;
-  Kv4Plan p = {each <= 4 ? 4 : each <= 8 ? 8 : f32 || each <= 32 ? 16 : each <= 128 || head_dim > 128 ? 32 : 64, 0, 1};
+  Kv4Plan p = {each <= 4 ? 4 : each <= 8 ? 8 : f32 || each <= (head_dim > 128 ? 64 : 32) ? 16 : each <= 128 || head_dim > 128 ? 32 : 64, 0, 1};
   const int64_t tile = 4 * p.rows;
   p.tiles = ragged ? rows / tile + sequences + 1 : sequences * ((each + tile - 1) / tile);
   // Splits that leave the fewest tokens one after the other: rounds of workgroups (of ragged sequences those that can be

@@ -100,7 +100,7 @@ kv4_attention_kernel(Attention a) {
   constexpr int APART = FINE && !PACK;   // second parts of weights have sums of their own
   using C = Codes<FINE>;
   using T = typename D::T;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int heads = a.cache.heads;
   const int head = blockIdx.x % heads, split = blockIdx.x / heads / a.tiles;
   const Rows w = find_rows<TILE>(a, blockIdx.x / heads % a.tiles);
