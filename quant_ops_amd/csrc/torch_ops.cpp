@@ -442,7 +442,7 @@ qo_kv4_cache kv4_of(const at::Tensor& k, const at::Tensor& v, const at::Tensor& 
   TORCH_CHECK(k.dim() == 4 && v.dim() == 5 && params.dim() == 6, op, ": not a cache: ", k.sizes(), ", ", v.sizes(), ", ",
               params.sizes());
   const int64_t pages = k.size(0), heads = k.size(1), P = k.size(2), half = k.size(3);
-  TORCH_CHECK(P % 16 == 0 && v.sizes() == at::IntArrayRef({pages, heads, P / 16, half, 16}) &&
+  TORCH_CHECK(heads > 0 && P % 16 == 0 && v.sizes() == at::IntArrayRef({pages, heads, P / 16, half, 16}) &&
                   params.sizes() == at::IntArrayRef({pages, 2, heads, P / 16, 2, 16}),
               op, ": the parts of the cache do not match: ", k.sizes(), ", ", v.sizes(), ", ", params.sizes());
   TORCH_CHECK(k.is_contiguous() && v.is_contiguous() && params.is_contiguous(), op, ": the cache must be contiguous");

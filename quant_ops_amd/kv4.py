@@ -77,6 +77,7 @@ def _check_cache(cache, on):
     _check(k.dim() == 4, f"not a cache: {tuple(k.shape)}")
     pages, heads, size, half = k.shape
     _check_sizes(size, 2 * half)
+    _check(heads > 0, "the cache has no heads")
     _check(v.shape == (pages, heads, size // 16, half, 16) and p.shape == (pages, 2, heads, size // 16, 2, 16),
            f"the parts of the cache do not match: {tuple(k.shape)}, {tuple(v.shape)}, {tuple(p.shape)}")
     _check(all(t.is_contiguous() for t in cache), "the cache must be contiguous")

@@ -145,6 +145,7 @@ def refusals(device):
                        torch.zeros(2, 1, p // 16, d // 2, 16, dtype=torch.uint8, device=device),
                        torch.zeros(2, 2, 1, p // 16, 2, 16, dtype=torch.float16, device=device)) for p, d in ((48, 64), (16, 80), (16, 320), (8192, 64))]
     turn = dict(positions=pos, cos=cos, sin=cos)
+    headless = qo.KV4Cache(cache.k_codes[:, :0].contiguous(), cache.v_codes[:, :0].contiguous(), cache.params[:, :, :0].contiguous())
     return [
         lambda: qo.kv4_append(cache, x.double(), x.double(), slots),
         lambda: qo.kv4_append(cache, x, x.half(), slots),
@@ -198,6 +199,9 @@ def refusals(device):
         lambda: qo.kv4_attention(x, cache, table, lengths, window=-1),
         lambda: qo.kv4_attention(x, other, table, lengths),
         lambda: qo.kv4_attention(x, odd[1], table, lengths),
+        lambda: qo.kv4_attention(x, headless, table, lengths),
+        lambda: qo.kv4_append(headless, x[:, :0], x[:, :0], slots),
+        lambda: qo.kv4_read(headless, slots),
     ]
 
 
