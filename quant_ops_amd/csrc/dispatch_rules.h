@@ -179,7 +179,7 @@ inline Kv4Plan kv4_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64
   // expected to have rows) times a split's tokens. To begin and end costs a workgroup as much as two of a wave's steps
   // of 64 tokens (waves without rows of their own share others' tokens), to join the parts as much again, and a split has no
   // fewer. With w workgroups of the `resident` that fit a CU a round takes (resident + w) / 2 resident of a full one's time.
-  // 24 sequences of up to 1024 tokens, float32 of 256, 192 workgroups: in one 32 us, in two 42, in four 50; 119 workgroups of
+  // 24 sequences of up to 1024 tokens, float32 of 256, 192 workgroups: in one 27 us, in two 27, in four 37; 119 workgroups of
   // 2558 tokens, float32 of 192: in two 31 us, in three 44, in four 49; 8 workgroups of 131072 tokens: in 32 37 us, in 64 33;
   // 2 workgroups of 64 rows on 800 tokens: in one 37 us, in six 18; 8 ragged sequences of 300 to 2000 tokens, half of them
   // prompts: in one 89 us, in two 80, in three 73, in four 78.
