@@ -167,13 +167,15 @@ kv4_prefill_kernel(Attention a) {
     // token are NaN then, and the others are not.
     const bool finite = (value_s & 0x7C00u) != 0x7C00u && (value_lo & 0x7C00u) != 0x7C00u && !bad;
     if (!finite) key_s = key_lo = 0x7E00u;
+    // Values that no row sees are 0 too: they have no say in S, and one past fp16's range would be no number times 0.
     const int t = begin + 64 * step + 16 * part + c;
-    if (!finite || t < all_top.first || t >= all_bottom.last) value_s = value_lo = 0u;   // unseen ones have no say in S
+    const bool kept = finite && t >= all_top.first && t < all_bottom.last;
+    if (!kept) value_s = value_lo = 0u;
     if (!EXACT && values_too) {
-      if (__any(!finite)) {
+      if (__any(!kept)) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const uint32_t keep = __builtin_amdgcn_readlane((int)finite, i) ? 0xFFFFFFFFu : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+          const uint32_t keep = __builtin_amdgcn_readlane((int)kept, i) ? 0xFFFFFFFFu : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
           vs[i / 2] &= keep;
           vl[i / 2] &= keep;
         }
