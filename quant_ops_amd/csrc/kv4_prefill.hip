@@ -12,17 +12,18 @@
 // the odd values of 16 pairs): lane half g has tokens 8 m + 4 g + i of a tile's weights, in the order in which
 // the values' fragments hold them, so that weights stay in their lanes.
 //
-// bf16 (EXACT false): keys and values are unpacked to what they stand for, halved (15 steps of a scale may
-// pass fp16's range), rounded to fp16: half a step of 2^-11, beside 2^-8 of the output. That takes the
-// parameters out of the softmax, whose instructions bound the kernel. fp16 (EXACT): codes less 8, the parameters
-// applied to scores in float32 and weights in two parts, as in kv4_attention.hip; they come from LDS as float32,
-// and the power of two that brings weights times scales into fp16 stands in the exponent's argument.
+// Codes less 8 are multiplied as they are, whatever a key's offset or outliers and a value's size: the parameters are applied to
+// scores and weights in float32, as in kv4_attention.hip. They come from LDS as float32, and the power of two that brings weights
+// times scales into fp16 stands in the exponent's argument. A weight is rounded to fp16 once for bf16 (half a step 2^-11, beside
+// the output's 2^-8: 0.00167 of the outputs' norm where the output's rounding alone is 0.00166; a second part brings the two
+// together and takes 190 us where one takes 161) and has two parts for fp16.
 //
-// A wave's 32 x 64 scores take about 500 vector instructions and 32 exponentials beside 32 products (128 values,
+// A wave's 32 x 64 scores take 208 vector instructions and 32 exponentials beside 32 products (128 values,
 // bf16), on the same SIMD: products run beside the other half's softmax, but the two overlap in part only. 2048
-// queries of 32 heads on 4096 tokens (8 heads): of 128 136 us in bf16 (758 TFLOP/s of the pairs that a causal mask
-// leaves, 63% of a large product's rate) and 199 in fp16, of 64 103 and 157. On the way: one product after
-// the other 152 us, fragments four reads ahead 149, eight waves and products beside the softmax 136.
+// queries of 32 heads on 4096 tokens (8 heads): of 128 161 us in bf16 (640 TFLOP/s of the pairs that a causal mask
+// leaves, 53% of a large product's rate) and 191 in fp16, of 64 136 and 157. Keys and values unpacked to what they stand for
+// in fp16 take the parameters out of the softmax (131 us in bf16), but a key's rounding then counts with its offset and
+// outliers, in an exponent: twenty times the output's own for keys about 100.
 #include "kv4_attention.h"
 
 namespace qo {
@@ -36,21 +37,7 @@ constexpr float kSlack = 8.f;
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 
-__device__ inline uint32_t pk(v2h v) { return __builtin_bit_cast(uint32_t, v); }
-__device__ inline v2h unpk(uint32_t u) { return __builtin_bit_cast(v2h, u); }
-// Codes as they are (EXACT: less 8), two to a word, from the low and the high halves of bytes. High codes less 8 are times 16.
-template <bool EXACT>
-__device__ inline v2h low_codes(uint32_t w, uint32_t e) {
-  return EXACT ? unpk(less_low(w, e)) : unpk((w & kLow) | e) - (v2h){(_Float16)1024.f, (_Float16)1024.f};
-}
-template <bool EXACT>
-__device__ inline v2h high_codes(uint32_t w, uint32_t e) {
-  if constexpr (EXACT) return unpk(less_high(w, e));
-  const v2h sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f}, off = {(_Float16)-64.f, (_Float16)-64.f};
-  return __builtin_elementwise_fma(unpk((w & kHigh) | e), sixteenth, off);
-}
-
-template <class D, int DIM, int NP, bool EXACT, int WAVES>
+template <class D, int DIM, int NP, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, DIM <= 128 ? 2 : 1)
 kv4_prefill_kernel(Attention a) {
   constexpr int NS = DIM / 16;        // k-steps of a score
@@ -62,8 +49,8 @@ kv4_prefill_kernel(Attention a) {
   struct Stage {
     v4u k[2][NS][64];      // fragments: 32 tokens, k-step
     v4u v[NF][4][64];      // block of values, 16 tokens
-    v4f params[4][2][8];   // EXACT: keys' scale and middle, values' middle and scale; lane half g; its 32 tokens
-    int largest[4];        // EXACT: of 16 values' scales, the exponent's bits
+    v4f params[4][2][8];   // keys' scale and middle, values' middle and scale; lane half g; its 32 tokens
+    int largest[4];        // of 16 values' scales, the exponent's bits
   };
   __shared__ Stage stage[2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, g = lane >> 5;
@@ -110,11 +97,11 @@ kv4_prefill_kernel(Attention a) {
       for (int i = 0; i < 8; ++i) {
         const float v = ldexpf(D::to_f(t[s][kCodeOrder[i]]), e);
         sum += v;
-        qf[s][i] = (_Float16)(EXACT && (kCodeOrder[i] & 1) ? v * 0.0625f : v);
+        qf[s][i] = (_Float16)(kCodeOrder[i] & 1 ? v * 0.0625f : v);
       }
     sum = bits_float(halves_reduce(float_bits(sum), FAdd{}));
     qsum = most < kInf ? sum : __builtin_nanf("");   // an infinity's scores are NaN
-    factor = fmaxf(ldexpf(a.scale * kLog2e, -e) * (EXACT ? 1.f : 2.f), 0x1p-126f);   // 0 times a masked score: no number
+    factor = fmaxf(ldexpf(a.scale * kLog2e, -e), 0x1p-126f);   // 0 times a masked score: no number
   }
 
   v16f o[NF];
@@ -124,7 +111,7 @@ kv4_prefill_kernel(Attention a) {
     for (int i = 0; i < 16; ++i) o[f][i] = 0.f;
   float most = -kInf, at = 0.f, middles = 0.f;
   float total = qsum != qsum && see.last > see.first ? qsum : 0.f;   // infinite queries: NaN, also where all scores are -inf
-  int scale_exp = -14;   // EXACT: every scale so far is below two to it
+  int scale_exp = -14;   // every scale so far is below two to it
 
   const int begin = all_top.first & ~63;
   const int steps = all_bottom.last > begin ? (all_bottom.last - begin + 63) / 64 : 0;
@@ -140,7 +127,6 @@ kv4_prefill_kernel(Attention a) {
   const int c = lane & 15, d = lane >> 4, part = wave & 3;
   const bool keys = WAVES == 4 || wave < 4, values_too = WAVES == 4 || wave >= 4;
   uint32_t kw[NW], key_s, key_lo, value_s, value_lo;   // the lane's token's parameters (16 bits)
-  uint32_t vs[8], vl[8];                               // those of the tile's 16 values
   v4u vw[NV];
   Tile tile;
   bool bad = false;
@@ -154,48 +140,21 @@ kv4_prefill_kernel(Attention a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (values_too && 64 * i + lane < DIM / 2) vw[i] = *reinterpret_cast<const v4u*>(vp + 1024 * i);
-    const uint16_t* ks = reinterpret_cast<const uint16_t*>(par) + c;
-    const uint16_t* vss = reinterpret_cast<const uint16_t*>(par + pages.param_values) + c;
-    key_s = ks[0], key_lo = ks[16], value_s = vss[0], value_lo = vss[16];
-    if (!EXACT && values_too) {
-      __builtin_memcpy(vs, par + pages.param_values, sizeof(vs));
-      __builtin_memcpy(vl, par + pages.param_values + 32, sizeof(vl));
+    if (keys) {
+      const uint16_t* ks = reinterpret_cast<const uint16_t*>(par) + c;
+      const uint16_t* vs = reinterpret_cast<const uint16_t*>(par + pages.param_values) + c;
+      key_s = ks[0], key_lo = ks[16], value_s = vs[0], value_lo = vs[16];
     }
   };
   auto unpack = [&](Stage& st, int step) {
-    // A value that is no number (or on a page outside the cache) becomes 0 and its key NaN: the rows that see the
-    // token are NaN then, and the others are not.
-    const bool finite = (value_s & 0x7C00u) != 0x7C00u && (value_lo & 0x7C00u) != 0x7C00u && !bad;
-    if (!finite) key_s = key_lo = 0x7E00u;
-    // Values that no row sees are 0 too: they have no say in S, and one past fp16's range would be no number times 0.
-    const int t = begin + 64 * step + 16 * part + c;
-    const bool kept = finite && t >= all_top.first && t < all_bottom.last;
-    if (!kept) value_s = value_lo = 0u;
-    if (!EXACT && values_too) {
-      if (__any(!kept)) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t keep = __builtin_amdgcn_readlane((int)kept, i) ? 0xFFFFFFFFu : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-          vs[i / 2] &= keep;
-          vl[i / 2] &= keep;
-        }
-      }
-    }
-    const v2h half = {(_Float16)0.5f, (_Float16)0.5f};
-    v2h s2 = unpk(key_s | key_s << 16), lo2 = unpk(key_lo | key_lo << 16);
-    if constexpr (!EXACT) s2 *= half, lo2 *= half;
     if (keys) {
 #pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      const int word = d * NW + i;   // of the token's row: dims 8 word ..
-      const uint32_t x = kw[i], h = x >> 8;
-      v2h f[4] = {low_codes<EXACT>(x, exponents), high_codes<EXACT>(x, exponents), low_codes<EXACT>(h, exponents), high_codes<EXACT>(h, exponents)};
-      if constexpr (!EXACT) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = __builtin_elementwise_fma(f[j], s2, lo2);
+      for (int i = 0; i < NW; ++i) {
+        const int word = d * NW + i;   // of the token's row: dims 8 word ..
+        const uint32_t x = kw[i], h = x >> 8;
+        st.k[part >> 1][word >> 1][(part & 1) * 16 + c + 32 * (word & 1)] =
+            (v4u){less_low(x, exponents), less_high(x, exponents), less_low(h, exponents), less_high(h, exponents)};
       }
-      st.k[part >> 1][word >> 1][(part & 1) * 16 + c + 32 * (word & 1)] = (v4u){pk(f[0]), pk(f[1]), pk(f[2]), pk(f[3])};
-    }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -207,14 +166,8 @@ kv4_prefill_kernel(Attention a) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {   // tokens 4 q + 2 h, and the next
             const uint32_t two = __builtin_amdgcn_perm(0, vw[i][q], h ? 0x0C030C02u : 0x0C010C00u);
-            v2h x = low_codes<EXACT>(two, exponents), y = high_codes<EXACT>(two, exponents);
-            if constexpr (!EXACT) {
-              const v2h s = unpk(vs[2 * q + h]) * half, lo = unpk(vl[2 * q + h]) * half;
-              x = __builtin_elementwise_fma(x, s, lo);
-              y = __builtin_elementwise_fma(y, s, lo);
-            }
-            even[q & 1][2 * (q >> 1) + h] = pk(x);
-            odd[q & 1][2 * (q >> 1) + h] = pk(y);
+            even[q & 1][2 * (q >> 1) + h] = less_low(two, exponents);
+            odd[q & 1][2 * (q >> 1) + h] = less_high(two, exponents);
           }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -222,24 +175,28 @@ kv4_prefill_kernel(Attention a) {
           st.v[pair >> 4][part][(pair & 15) + 16 + 32 * h] = odd[h];
         }
       }
-    if constexpr (EXACT) {
-      // token 16 part + c of the step: of lane half (c / 4) % 2, its token 8 part + 4 (c / 8) + c % 4
-      if (keys && d == 0) {
-        const int half_of_c = c >> 2 & 1, place = 8 * part + 4 * (c >> 3) + (c & 3);
-        auto put = [&](int which, float x) { reinterpret_cast<float*>(&st.params[which][half_of_c][0])[place] = x; };
-        const float ks = half_of(&key_s, 0), vs = half_of(&value_s, 0);
-        put(0, ks);
-        put(1, fmaf(8.f, ks, half_of(&key_lo, 0)));
-        put(2, fmaf(8.f, vs, half_of(&value_lo, 0)));
-        put(3, vs);
-        uint32_t top_of = value_s & 0x7FFFu;
-        auto with = [&](int other) { top_of = max(top_of, (uint32_t)other); };
-        with(__builtin_amdgcn_update_dpp(0, (int)top_of, 0xB1, 0xF, 0xF, false));    // quad_perm 1,0,3,2
-        with(__builtin_amdgcn_update_dpp(0, (int)top_of, 0x4E, 0xF, 0xF, false));    // quad_perm 2,3,0,1
-        with(__builtin_amdgcn_update_dpp(0, (int)top_of, 0x141, 0xF, 0xF, false));   // row_half_mirror
-        with(__builtin_amdgcn_update_dpp(0, (int)top_of, 0x140, 0xF, 0xF, false));   // row_mirror
-        if (c == 0) st.largest[part] = (int)(top_of >> 10);
-      }
+    // The parameters, as float32: of token 16 part + c of the step, of lane half (c / 4) % 2 its token 8 part + 4 (c / 8) + c % 4.
+    if (keys && d == 0) {
+      // A value that is no number (or on a page outside the cache) becomes 0 and its key NaN: the rows that see the
+      // token are NaN then, and the others are not. Values that no row sees are 0 too: they have no say in S.
+      const bool finite = (value_s & 0x7C00u) != 0x7C00u && (value_lo & 0x7C00u) != 0x7C00u && !bad;
+      if (!finite) key_s = key_lo = 0x7E00u;
+      const int t = begin + 64 * step + 16 * part + c;
+      if (!(finite && t >= all_top.first && t < all_bottom.last)) value_s = value_lo = 0u;
+      const int half_of_c = c >> 2 & 1, place = 8 * part + 4 * (c >> 3) + (c & 3);
+      auto put = [&](int which, float x) { reinterpret_cast<float*>(&st.params[which][half_of_c][0])[place] = x; };
+      const float ks = half_of(&key_s, 0), vs = half_of(&value_s, 0);
+      put(0, ks);
+      put(1, fmaf(8.f, ks, half_of(&key_lo, 0)));
+      put(2, fmaf(8.f, vs, half_of(&value_lo, 0)));
+      put(3, vs);
+      uint32_t top_of = value_s & 0x7FFFu;
+      auto with = [&](int other) { top_of = max(top_of, (uint32_t)other); };
+      with(__builtin_amdgcn_update_dpp(0, (int)top_of, 0xB1, 0xF, 0xF, false));    // quad_perm 1,0,3,2
+      with(__builtin_amdgcn_update_dpp(0, (int)top_of, 0x4E, 0xF, 0xF, false));    // quad_perm 2,3,0,1
+      with(__builtin_amdgcn_update_dpp(0, (int)top_of, 0x141, 0xF, 0xF, false));   // row_half_mirror
+      with(__builtin_amdgcn_update_dpp(0, (int)top_of, 0x140, 0xF, 0xF, false));   // row_mirror
+      if (c == 0) st.largest[part] = (int)(top_of >> 10);
     }
   };
 
@@ -287,7 +244,7 @@ kv4_prefill_kernel(Attention a) {
           }
       };
       float shrink_o = 1.f;
-      // EXACT: a parameter of the lane's 16 tokens of a half.
+      // A parameter of the lane's 16 tokens of a half.
       auto params = [&](int which, int u, float(&x)[16]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -299,16 +256,13 @@ kv4_prefill_kernel(Attention a) {
       // Parameters, masks and the largest score; sums follow a larger one, and outputs do in rescale(), once the
       // weights made before it are in them.
       auto largest = [&](int u) {
-        int exp_now = scale_exp;
-        if constexpr (EXACT) {
-          float ks[16], middle[16];
-          params(0, u, ks);
-          params(1, u, middle);
+        float ks[16], middle[16];
+        params(0, u, ks);
+        params(1, u, middle);
 #pragma unroll
-          for (int t = 0; t < 16; ++t) sc[u][t] = fmaf(ks[t], sc[u][t], middle[t] * qsum);
-          const int field = max(st.largest[2 * u], st.largest[2 * u + 1]);
-          exp_now = max(scale_exp, __builtin_amdgcn_readfirstlane(field) - 14);
-        }
+        for (int t = 0; t < 16; ++t) sc[u][t] = fmaf(ks[t], sc[u][t], middle[t] * qsum);
+        const int field = max(st.largest[2 * u], st.largest[2 * u + 1]);
+        const int exp_now = max(scale_exp, __builtin_amdgcn_readfirstlane(field) - 14);
         if (!(t0 + 32 * u + 32 <= top.last && t0 + 32 * u >= bottom.first)) {   // some row does not see some token
 #pragma unroll
           for (int t = 0; t < 16; ++t) {
@@ -322,7 +276,7 @@ kv4_prefill_kernel(Attention a) {
         now = bits_float(halves_reduce(float_bits(now), FMax{}));
         if (__any(factor * (now - most) > kSlack) || exp_now > scale_exp) {
           now = fmaxf(now, most);
-          const float next = (now == -kInf ? 0.f : factor * now) - (float)(kAtRest - (EXACT ? exp_now : 0));
+          const float next = (now == -kInf ? 0.f : factor * now) - (float)(kAtRest - exp_now);
           shrink_o = most == -kInf ? 1.f : __builtin_amdgcn_exp2f(at - next);   // before: all sums 0
           most = now;
           at = next;
@@ -342,27 +296,19 @@ kv4_prefill_kernel(Attention a) {
       };
       auto weights = [&](int u) {
         float middle[16], vs[16];
-        if constexpr (EXACT) {
-          params(2, u, middle);
-          params(3, u, vs);
-        }
+        params(2, u, middle);
+        params(3, u, vs);
 #pragma unroll
         for (int t = 0; t < 16; ++t) {
           const float p = __builtin_amdgcn_exp2f(fmaf(factor, sc[u][t], -at));
-          if constexpr (EXACT) {
-            total += p;
-            middles = fmaf(p, middle[t], middles);
-            _Float16 h = (_Float16)fmaf(p, vs[t], 0.f);
-            if constexpr (NP > 1) {
-              asm("" : "+v"(h));   // one and the same rounding in both parts
-              pl[2 * u + t / 8][t % 8] = (_Float16)fmaf(p, vs[t], -(float)h);
-            }
-            ph[2 * u + t / 8][t % 8] = h;
-          } else {
-            ph[2 * u + t / 8][t % 8] = (_Float16)p;
-            // the sum of the weights as they are rounded, two an instruction
-            if (t & 1) total = __builtin_amdgcn_fdot2((v2h){ph[2 * u + t / 8][t % 8 - 1], ph[2 * u + t / 8][t % 8]}, (v2h){(_Float16)1.f, (_Float16)1.f}, total, false);
+          total += p;
+          middles = fmaf(p, middle[t], middles);
+          _Float16 h = (_Float16)fmaf(p, vs[t], 0.f);
+          if constexpr (NP > 1) {
+            asm("" : "+v"(h));   // one and the same rounding in both parts
+            pl[2 * u + t / 8][t % 8] = (_Float16)fmaf(p, vs[t], -(float)h);
           }
+          ph[2 * u + t / 8][t % 8] = h;
         }
         // here and not where the product takes them
 #pragma unroll
@@ -412,7 +358,6 @@ kv4_prefill_kernel(Attention a) {
   if (most == -kInf && total == 0.f) at = -kInf;
   if (w.poison) total = __builtin_nanf(""), at = 0.f;
   if (first_row + r > last_row) return;
-  const float unit = EXACT ? 1.f : 2.f;
   const int64_t total_rows = (int64_t)a.tokens * a.q_heads;   // of all heads
   const int64_t at_row = (int64_t)(w.start + row / a.group) * a.q_heads + head * a.group + row % a.group;
 #pragma unroll
@@ -422,8 +367,8 @@ kv4_prefill_kernel(Attention a) {
       float v[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        v[2 * i] = fmaf(o[f][4 * m + i], unit, middles);
-        v[2 * i + 1] = fmaf(o[f][8 + 4 * m + i], EXACT ? unit * 0.0625f : unit, middles);
+        v[2 * i] = o[f][4 * m + i] + middles;
+        v[2 * i + 1] = fmaf(o[f][8 + 4 * m + i], 0.0625f, middles);
       }
       if (a.splits > 1) {
         __builtin_memcpy(a.part + (split * total_rows + at_row) * DIM + 32 * f + 16 * m + 8 * g, v, sizeof(v));
@@ -449,10 +394,10 @@ void kv4_prefill(const Attention& a, int dtype, int dim, int tile, int64_t grid,
     auto attend = [&](auto kernel) { launch(kernel, dim3((unsigned)grid), dim3(2 * tile), 0, stream, a); };
     const bool bf16 = dtype == QO_DTYPE_BF16;
     if constexpr (DIM <= 128) {
-      if (tile == 256) return bf16 ? attend(kv4_prefill_kernel<BF16T, DIM, 1, false, 8>) : attend(kv4_prefill_kernel<F16T, DIM, 2, true, 8>);
+      if (tile == 256) return bf16 ? attend(kv4_prefill_kernel<BF16T, DIM, 1, 8>) : attend(kv4_prefill_kernel<F16T, DIM, 2, 8>);
     }
-    if (bf16) attend(kv4_prefill_kernel<BF16T, DIM, 1, false, 4>);
-    else attend(kv4_prefill_kernel<F16T, DIM, 2, true, 4>);
+    if (bf16) attend(kv4_prefill_kernel<BF16T, DIM, 1, 4>);
+    else attend(kv4_prefill_kernel<F16T, DIM, 2, 4>);
   };
   if (dim == 64) go(std::integral_constant<int, 64>{});
   else if (dim == 96) go(std::integral_constant<int, 96>{});
