@@ -32,10 +32,10 @@
 // Queries: brought by a power of two for each row to a largest magnitude in [2^14, 2^15), 16-bit
 // values are exact in fp16 (those below 2^-28 of the largest lose bits); float32 takes two fp16
 // parts (22 bits). Weights: p s 2^14 / S, where p is 1 at the row's largest score so far and S a
-// power of two that no scale of the tokens so far exceeds, is at most 2^14, and rounded to fp16 (half
-// a step 2^-11, beside bf16's 2^-8 of the output) or, for fp16 and float32, to two parts. In
-// float32 the second parts have sums of their own: added to the first parts' they would lose what is
-// below 2^-24 of those. Maximum, sums and outputs are float32.
+// power of two that no scale of the tokens so far exceeds, is at most 2^14, in two fp16 parts (22 bits; with one a
+// bf16 output in twenty is a step off, and the second costs 2 to 3 % up to eight rows a sequence, 3 to 7 % up to 32). In
+// float32 the second parts have sums of their own: added to the first parts' they would lose what is below 2^-24 of
+// those. Maximum, sums and outputs are float32.
 //
 // What bounds it: one sequence of 131072 tokens (64 heads on 8 of 128, bf16, 142 MB) takes 32 us, 4.4 TB/s, and
 // 262144 tokens come at the 5.0 TB/s of a copy; 64 sequences of 100 to 4096 tokens (32 on 8 heads, 146 MB) take 41 us, 3.5
@@ -54,11 +54,6 @@ __device__ inline uint32_t row_reduce(uint32_t u, F f) {
   if constexpr (CW <= 4) u = f(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x124, 0xF, 0xF, false));   // row_ror:4
   if constexpr (CW <= 8) u = f(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x128, 0xF, 0xF, false));   // row_ror:8
   return groups_reduce(u, f);
-}
-// The value of lane r + Q CW of a row of 16 (0 beyond).
-template <int CW, int Q>
-__device__ inline uint32_t from_lanes(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x100 + CW * Q, 0xF, 0xF, true);   // row_shl
 }
 
 // v from another lane of the row of 16 (CTRL) in lanes of the banks of four of BANKS, elsewhere old.
@@ -88,10 +83,10 @@ __device__ inline v8h values_odd(uint32_t a, uint32_t b, uint32_t e) {
   return __builtin_bit_cast(v8h, (v4u){less_high(a, e), less_high(a >> 8, e), less_high(b, e), less_high(b >> 8, e)});
 }
 
-template <class D, int DIM, int FOLD, int NQ, int NP, bool FINE>
+template <class D, int DIM, int FOLD, int NQ, bool FINE>
 __global__ void __launch_bounds__(256, DIM <= (FOLD > 1 ? 256 : FINE ? 96 : 192) ? 2 : 1)
 kv4_attention_kernel(Attention a) {
-  constexpr bool PACK = NP > 1 && FOLD > 1;   // second parts in columns 8 .. 15
+  constexpr bool PACK = FOLD > 1;     // second parts in columns 8 .. 15
   constexpr int NQF = PACK ? 1 : NQ;
   constexpr int NS = DIM / 32;        // k-steps of a score, words of a key's codes in a lane
   constexpr int NF = DIM / 32;        // blocks of 16 pairs of values
@@ -323,31 +318,21 @@ kv4_attention_kernel(Attention a) {
         total += p;
         middles = fmaf(p, fmaf(eight, s, half_of(vl, t)), middles);   // what code 8 stands for
         hi[j] = (_Float16)fmaf(p, s, 0.f);
-        if constexpr (NP > 1) {
-          // one and the same rounding in both parts: the product rounded twice (to float32 first)
-          // or once differ by a step of h where it is next to a tie
-          asm("" : "+v"(hi[j]));
-          lo[j] = (_Float16)fmaf(p, s, -(float)hi[j]);
-        }
+        // one and the same rounding in both parts: the product rounded twice (to float32 first)
+        // or once differ by a step of h where it is next to a tie
+        asm("" : "+v"(hi[j]));
+        lo[j] = (_Float16)fmaf(p, s, -(float)hi[j]);
       }
       __builtin_memcpy(wh, hi, sizeof(wh));
-      if constexpr (NP > 1) __builtin_memcpy(wl, lo, sizeof(wl));
+      __builtin_memcpy(wl, lo, sizeof(wl));
     }
     scale_exp = exp_now;
     __builtin_amdgcn_sched_barrier(0);
-    // tokens 8 z .. 8 z + 7 of the group
+    // Tokens 8 z .. 8 z + 7 of the group.
     auto weights = [&](const uint32_t* x, int z) {
-      v4u v;
-      if constexpr (FOLD == 1) v = (v4u){x[4 * z], x[4 * z + 1], x[4 * z + 2], x[4 * z + 3]};
-      if constexpr (FOLD == 2)
-        v = z == 0 ? (v4u){x[0], x[1], x[2], x[3]}
-                   : (v4u){from_lanes<CW, 1>(x[0]), from_lanes<CW, 1>(x[1]), from_lanes<CW, 1>(x[2]), from_lanes<CW, 1>(x[3])};
-      if constexpr (FOLD == 4)
-        v = z == 0 ? (v4u){x[0], x[1], from_lanes<CW, 1>(x[0]), from_lanes<CW, 1>(x[1])}
-                   : (v4u){from_lanes<CW, 2>(x[0]), from_lanes<CW, 2>(x[1]), from_lanes<CW, 3>(x[0]), from_lanes<CW, 3>(x[1])};
-      return __builtin_bit_cast(v8h, v);
+      return __builtin_bit_cast(v8h, (v4u){x[4 * z], x[4 * z + 1], x[4 * z + 2], x[4 * z + 3]});
     };
-    // the same with the second parts, in columns 8 ..
+    // The same of both parts, the second in columns 8 ..
     auto both = [&](int z) {
       v4u v;
       if constexpr (PACK && FOLD == 2) {
@@ -371,7 +356,7 @@ kv4_attention_kernel(Attention a) {
         ph[z] = both(z);
       } else {
         ph[z] = weights(wh, z);
-        if constexpr (NP > 1) pl[z] = weights(wl, z);
+        pl[z] = weights(wl, z);
       }
     }
 #pragma unroll
@@ -382,7 +367,7 @@ kv4_attention_kernel(Attention a) {
         v4f(&hi)[2] = o[0][f], (&lo)[2] = o[APART][f];
         hi[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, ph[z], hi[0], 0, 0, 0);
         hi[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, ph[z], hi[1], 0, 0, 0);
-        if constexpr (NP > 1 && !PACK) {
+        if constexpr (!PACK) {
           lo[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, pl[z], lo[0], 0, 0, 0);
           lo[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, pl[z], lo[1], 0, 0, 0);
         }
@@ -651,17 +636,17 @@ extern "C" int qo_kv4_attention(const qo_kv4_cache* cache, const qo_heads* q, in
                        q_heads / c.heads, scale, window < kMostTokens ? (int)window : 0, (int)plan.tiles, plan.splits,
                        reinterpret_cast<float*>(workspace)};
   launch_begin();
-  auto go = [&](auto d, auto parts_q, auto parts_p, auto fine) {
+  auto go = [&](auto d, auto parts_q, auto fine) {
     using D = decltype(d);
-    constexpr int NQ = decltype(parts_q)::value, NP = decltype(parts_p)::value;
+    constexpr int NQ = decltype(parts_q)::value;
     constexpr bool FINE = decltype(fine)::value;
     with_dim(cache->head_dim, [&](auto dim) {
       constexpr int DIM = decltype(dim)::value;
       hipStream_t s = reinterpret_cast<hipStream_t>(stream);
       auto attend = [&](auto kernel) { launch(kernel, dim3((unsigned)grid), dim3(256), 0, s, a); };
-      if (plan.rows == 4) attend(kv4_attention_kernel<D, DIM, 4, NQ, NP, FINE>);
-      else if (plan.rows == 8) attend(kv4_attention_kernel<D, DIM, 2, NQ, NP, FINE>);
-      else if (plan.rows == 16) attend(kv4_attention_kernel<D, DIM, 1, NQ, NP, FINE>);
+      if (plan.rows == 4) attend(kv4_attention_kernel<D, DIM, 4, NQ, FINE>);
+      else if (plan.rows == 8) attend(kv4_attention_kernel<D, DIM, 2, NQ, FINE>);
+      else if (plan.rows == 16) attend(kv4_attention_kernel<D, DIM, 1, NQ, FINE>);
       else kv4_prefill(a, dtype, DIM, 4 * plan.rows, grid, s);
       if (plan.splits > 1) {
         const int64_t rows = tokens * q_heads;
@@ -679,8 +664,8 @@ extern "C" int qo_kv4_attention(const qo_kv4_cache* cache, const qo_heads* q, in
   };
   using One = std::integral_constant<int, 1>;
   using Two = std::integral_constant<int, 2>;
-  if (dtype == QO_DTYPE_BF16) go(BF16T{}, One{}, One{}, std::false_type{});
-  else if (dtype == QO_DTYPE_F16) go(F16T{}, One{}, Two{}, std::false_type{});
-  else go(F32T{}, Two{}, Two{}, std::true_type{});
+  if (dtype == QO_DTYPE_BF16) go(BF16T{}, One{}, std::false_type{});
+  else if (dtype == QO_DTYPE_F16) go(F16T{}, One{}, std::false_type{});
+  else go(F32T{}, Two{}, std::true_type{});
   return launch_result(fn);
 }
