@@ -167,6 +167,11 @@ __device__ inline Tile tile_at(const Attention& a, const int32_t* table, int t) 
   return {bad ? 0 : page, t & ((1 << a.cache.shift) - 1), bad};
 }
 
+// A weight is 2^(factor x - at), at the rounded factor x of the row's largest score, by one fma. It is 1 for that score, up
+// to at's rounding, which is the same for all of a row's weights and at most 2^-3 below kFar. From there on the
+// products are rounded before the difference, as at is.
+constexpr float kFar = 0x1p22f;
+
 // The power of two that brings a row's largest magnitude into [2^14, 2^15).
 __device__ inline int query_exponent(float most) {
   return most > 0.f && most < kInf ? min(max(15 - __builtin_amdgcn_frexp_expf(most), -100), 60) : 0;

@@ -158,6 +158,7 @@ kv4_attention_kernel(Attention a) {
 #pragma unroll
     for (int f = 0; f < NF; ++f) o[h][f][0] = o[h][f][1] = v4f{0.f, 0.f, 0.f, 0.f};
   int scale_exp = -14;
+  bool far = false;   // some row's exponent is kFar or more
 
   const int begin = top.first & ~63;
   const int steps = bottom.last > begin ? (bottom.last - begin + 63) / 64 : 0;
@@ -296,6 +297,7 @@ kv4_attention_kernel(Attention a) {
       const float shrink_o = shrink * power_of_two(scale_exp - exp_now);
       most = now;
       at = next;
+      far = __any(fabsf(at) >= kFar);
       total *= shrink;
       middles *= shrink;
 #pragma unroll
@@ -306,6 +308,11 @@ kv4_attention_kernel(Attention a) {
           o[h][f][1] *= shrink_o;
         }
     }
+    if (far) {
+#pragma unroll
+      for (int t = 0; t < CW; ++t) x[t] *= factor;
+    }
+    const float slope = far ? 1.f : factor;
     uint32_t wh[CW / 2], wl[CW / 2];   // weights, in the order of values_even
     {
       _Float16 hi[CW], lo[CW];
@@ -313,7 +320,7 @@ kv4_attention_kernel(Attention a) {
       for (int t = 0; t < CW; ++t) {
         constexpr int kSlot[4] = {0, 2, 1, 3};
         const int j = t / 4 * 4 + kSlot[t % 4];
-        const float p = __builtin_amdgcn_exp2f(fmaf(factor, x[t], -at));
+        const float p = __builtin_amdgcn_exp2f(fmaf(slope, x[t], -at));
         const float s = half_of(vs, t);
         total += p;
         middles = fmaf(p, fmaf(eight, s, half_of(vl, t)), middles);   // what code 8 stands for

@@ -109,9 +109,12 @@ kv4_prefill_kernel(Attention a) {
   for (int f = 0; f < NF; ++f)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[f][i] = 0.f;
-  float most = -kInf, at = 0.f, middles = 0.f;
+  float most = -kInf, slope = factor, offset = 0.f, middles = 0.f;   // a weight is 2^(slope score + offset)
   float total = qsum != qsum && see.last > see.first ? qsum : 0.f;   // infinite queries: NaN, also where all scores are -inf
   int scale_exp = -14;   // every scale so far is below two to it
+  bool far = false;      // some row's exponent is kFar or more
+
+  auto exponent = [&](float score) { return score == -kInf ? 0.f : factor * score; };
 
   const int begin = all_top.first & ~63;
   const int steps = all_bottom.last > begin ? (all_bottom.last - begin + 63) / 64 : 0;
@@ -274,15 +277,23 @@ kv4_prefill_kernel(Attention a) {
 #pragma unroll
         for (int t = 0; t < 16; ++t) now = fmaxf(now, sc[u][t]);
         now = bits_float(halves_reduce(float_bits(now), FMax{}));
-        if (__any(factor * (now - most) > kSlack) || exp_now > scale_exp) {
+        if (__any(factor * (now - most) > kSlack) || exp_now > scale_exp || far) {
           now = fmaxf(now, most);
-          const float next = (now == -kInf ? 0.f : factor * now) - (float)(kAtRest - exp_now);
-          shrink_o = most == -kInf ? 1.f : __builtin_amdgcn_exp2f(at - next);   // before: all sums 0
+          const float at = exponent(most), next = exponent(now), rest = (float)(kAtRest - exp_now);
+          const bool now_far = __any(fabsf(next) >= kFar);
+          const float by = far || now_far ? (at - next) + (float)(scale_exp - exp_now) : (rest - next) - offset;
+          shrink_o = most == -kInf ? 1.f : __builtin_amdgcn_exp2f(by);   // before: all sums 0
           most = now;
-          at = next;
+          slope = now_far ? 1.f : factor;
+          offset = now_far ? rest : rest - next;
+          far = now_far;
           total *= shrink_o;
           middles *= shrink_o;
           scale_exp = exp_now;
+          if (far) {
+#pragma unroll
+            for (int t = 0; t < 16; ++t) sc[u][t] = factor * sc[u][t] - next;
+          }
           return true;
         }
         return false;
@@ -300,7 +311,7 @@ kv4_prefill_kernel(Attention a) {
         params(3, u, vs);
 #pragma unroll
         for (int t = 0; t < 16; ++t) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(factor, sc[u][t], -at));
+          const float p = __builtin_amdgcn_exp2f(fmaf(slope, sc[u][t], offset));
           total += p;
           middles = fmaf(p, middle[t], middles);
           _Float16 h = (_Float16)fmaf(p, vs[t], 0.f);
@@ -355,6 +366,9 @@ kv4_prefill_kernel(Attention a) {
 
   total = bits_float(halves_reduce(float_bits(total), FAdd{}));
   middles = bits_float(halves_reduce(float_bits(middles), FAdd{}));
+  // The sums are in units of 2^at, or else of 2^(at - offset).
+  float at = far ? exponent(most) : -offset;
+  const float unit = far ? power_of_two(scale_exp - kAtRest) : 1.f;
   if (most == -kInf && total == 0.f) at = -kInf;
   if (w.poison) total = __builtin_nanf(""), at = 0.f;
   if (first_row + r > last_row) return;
@@ -371,6 +385,8 @@ kv4_prefill_kernel(Attention a) {
         v[2 * i + 1] = fmaf(o[f][8 + 4 * m + i], 0.0625f, middles);
       }
       if (a.splits > 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= unit;
         __builtin_memcpy(a.part + (split * total_rows + at_row) * DIM + 32 * f + 16 * m + 8 * g, v, sizeof(v));
       } else {
         T out[8];
@@ -382,7 +398,7 @@ kv4_prefill_kernel(Attention a) {
   if (a.splits > 1 && g == 0) {
     float* ml = a.part + a.splits * total_rows * DIM + (split * total_rows + at_row) * 2;
     ml[0] = at;
-    ml[1] = total;
+    ml[1] = total * unit;
   }
 }
 
