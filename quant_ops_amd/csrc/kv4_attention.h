@@ -173,8 +173,13 @@ __device__ inline Tile tile_at(const Attention& a, const int32_t* table, int t) 
 constexpr float kFar = 0x1p22f;
 
 // The power of two that brings a row's largest magnitude into [2^14, 2^15).
-__device__ inline int query_exponent(float most) {
-  return most > 0.f && most < kInf ? min(max(15 - __builtin_amdgcn_frexp_expf(most), -100), 60) : 0;
+__device__ inline int query_exponent(float most) { return most > 0.f && most < kInf ? 15 - __builtin_amdgcn_frexp_expf(most) : 0; }
+
+// What brings such a row's scores, times `unit`, to exponents of two. 0 would make no number of a masked score, and
+// no exponent below 2^-80 differs from 0; an infinite one would make none of a score of 0, and at the largest
+// number any two scores that differ are as far apart as they need to be.
+__device__ inline float score_factor(float scale, int e, float unit) {
+  return fminf(fmaxf(ldexpf(scale, -e) * kLog2e * unit, 0x1p-126f), 0x1.fffffep127f);
 }
 
 // Starts the kernel for many rows a sequence (16-bit types), in tiles of 128 or 256; the grid is that of kv4_plan.

@@ -148,7 +148,7 @@ kv4_attention_kernel(Attention a) {
       }
     sum = bits_float(groups_reduce(float_bits(sum), FAdd{}));
     qsum = most < kInf ? sum * C::kEven : __builtin_nanf("");   // an infinity's scores are NaN
-    factor = fmaxf(ldexpf(a.scale * kLog2e, -e) * (1.f / C::kEven), 0x1p-126f);   // 0 times a masked score: no number
+    factor = score_factor(a.scale, e, 1.f / C::kEven);
   }
 
   v4f o[APART + 1][NF][2];

@@ -101,7 +101,7 @@ kv4_prefill_kernel(Attention a) {
       }
     sum = bits_float(halves_reduce(float_bits(sum), FAdd{}));
     qsum = most < kInf ? sum : __builtin_nanf("");   // an infinity's scores are NaN
-    factor = fmaxf(ldexpf(a.scale * kLog2e, -e), 0x1p-126f);   // 0 times a masked score: no number
+    factor = score_factor(a.scale, e, 1.f);
   }
 
   v16f o[NF];
