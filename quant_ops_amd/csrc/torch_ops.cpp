@@ -621,3 +621,9 @@ TORCH_LIBRARY_IMPL(quant_ops, CUDA, m) {
   m.impl("kv4_read", &kv4_read);
   m.impl("kv4_attention", &kv4_attention);
 }
+
+// The operators of the cache carry no gradient: without these, results and the cache's params get a graph from inputs that
+// require one, which a decode step's appends would lengthen one after the other.
+TORCH_LIBRARY_IMPL(quant_ops, AutogradCUDA, m) {
+  for (const char* op : {"kv4_append", "kv4_read", "kv4_attention"}) m.impl(op, torch::CppFunction::makeFallthrough());
+}

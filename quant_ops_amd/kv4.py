@@ -133,6 +133,7 @@ def _rotate_pytorch(x, cos, sin, interleaved):
     return torch.cat((turned, x[..., rot:]), 2).float()
 
 
+@torch.no_grad()
 def _values_pytorch(cache, page, place):
     """float32 keys and values [..., heads, D] at (page, place)."""
     def values(codes, which):
@@ -144,6 +145,31 @@ def _values_pytorch(cache, page, place):
             values(cache.v_codes[page, :, place // 16, :, place % 16], 1))
 
 
+@torch.no_grad()
+def _append_pytorch(cache, k, v, slots, positions, cos, sin, q, interleaved):
+    keys = k.float()
+    turned = None
+    if cos is not None:
+        known = (positions >= 0) & (positions < cos.shape[0])
+        at = torch.where(known, positions, 0)
+        c, s = torch.where(known[:, None], cos[at], float("nan")), sin[at]
+        keys = _rotate_pytorch(keys, c, s, interleaved)
+        turned = None if q is None else _rotate_pytorch(q, c, s, interleaved).to(q.dtype)
+    size = cache.page_size
+    keep = (slots >= 0) & (slots < cache.k_codes.shape[0] * size)
+    page, place = slots[keep] // size, slots[keep] % size
+    for which, x in enumerate((keys, v.float())):
+        c, par = _quantize_pytorch(x[keep])
+        codes = c[..., 0::2] | (c[..., 1::2] << 4)
+        if which == 0:
+            cache.k_codes[page, :, place] = codes
+        else:
+            cache.v_codes[page, :, place // 16, :, place % 16] = codes
+        cache.params[page, which, :, place // 16, :, place % 16] = par
+    return turned
+
+
+@torch.no_grad()
 def _attention_pytorch(q, cache, page_table, lengths, scale, q_starts, window):
     out = torch.zeros_like(q, memory_format=torch.contiguous_format)
     size, group = cache.page_size, q.shape[1] // cache.k_codes.shape[1]
@@ -206,31 +232,13 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.T
     _check_index(slots, torch.int64, (tokens,), k, "slots")
     _check((positions is None) == (cos is None) == (sin is None), "positions, cos and sin are given together or not at all")
     _check(q is None or cos is not None, "q is only rotated: it needs positions, cos and sin")
-    keys = k.float()
-    turned = None
     if cos is not None:
         _check_index(positions, torch.int64, (tokens,), k, "positions")
         _check(cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32 and cos.device == sin.device == k.device,
                "cos and sin must be float32 [positions, rot / 2] on the others' device")
         _check(cos.shape[0] > 0 and 0 < 2 * cos.shape[1] <= cache.head_dim and cos.shape[1] % 4 == 0,
                f"cos and sin {tuple(cos.shape)} must have rows of a multiple of 4 angles, {cache.head_dim // 2} at most")
-        known = (positions >= 0) & (positions < cos.shape[0])
-        at = torch.where(known, positions, 0)
-        c, s = torch.where(known[:, None], cos[at], float("nan")), sin[at]
-        keys = _rotate_pytorch(keys, c, s, interleaved)
-        turned = None if q is None else _rotate_pytorch(q, c, s, interleaved).to(q.dtype)
-    size = cache.page_size
-    keep = (slots >= 0) & (slots < cache.k_codes.shape[0] * size)
-    page, place = slots[keep] // size, slots[keep] % size
-    for which, x in enumerate((keys, v.float())):
-        c, par = _quantize_pytorch(x[keep])
-        codes = c[..., 0::2] | (c[..., 1::2] << 4)
-        if which == 0:
-            cache.k_codes[page, :, place] = codes
-        else:
-            cache.v_codes[page, :, place // 16, :, place % 16] = codes
-        cache.params[page, which, :, place // 16, :, place % 16] = par
-    return turned
+    return _append_pytorch(cache, k, v, slots, positions, cos, sin, q, interleaved)
 
 
 def kv4_read(cache: KV4Cache, slots: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
