@@ -28,6 +28,7 @@ from . import _loader
 
 HEAD_DIMS = (64, 96, 128, 192, 256)
 MAX_PAGE = 4096
+MAX_LENGTH = 2 ** 31 - 4096   # tokens of a sequence
 _MOST = 65504.0
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -179,7 +180,7 @@ def _attention_pytorch(q, cache, page_table, lengths, scale, q_starts, window):
         lo, hi = (min(max(i, 0), total) for i in (starts[b] if b else 0, starts[b + 1]))
         if hi <= lo:
             continue
-        if length > page_table.shape[1] * size:
+        if length > min(page_table.shape[1] * size, MAX_LENGTH):
             out[lo:hi] = float("nan")
             continue
         length = max(length, 0)
