@@ -160,9 +160,10 @@ inline MxPlan mx_plan(int64_t M, int64_t N, int64_t blocks, bool fp8, int64_t cu
 // share a KV head). A workgroup has four waves of `rows` rows; up to 16 they read the cache each for
 // itself and waves without rows of their own share others' tokens; with 32 (and 64: eight waves of 32)
 // they share the tiles that they read (kv4_prefill, 16-bit types). `splits` workgroups share a tile's tokens.
-// 16 sequences of 2048 tokens on 4 heads of 128, bf16, in waves of 16, 32, 32 x 8: of 32 rows 21, 22, 22 us, of 48 29, 28, 24,
-// of 96 38, 31, 30, of 192 60, 41, 37 (fp16: 22, 25, 29; 30, 31, 31; 40, 35, 36; 62, 49, 45); one sequence of 4096 tokens:
-// of 128 rows 18, 20, 20, of 200 22, 20, 23; heads of 192, bf16, in 16 and 32: of 48 rows 32, 35, of 64 36, 37, of 96 46, 39; and 8192 rows on 8 heads 149 and 136 us in waves of 32 and 32 x 8.
+// 16 sequences of 2048 tokens on 4 heads of 128, bf16, in waves of 16, 32, 32 x 8: of 32 rows 22, 24, 26 us, of 40 28, 28, 27,
+// of 96 40, 33, 32, of 192 62, 43, 40 (fp16: 22, 25, 28; 28, 30, 29; 39, 35, 34; 61, 48, 44); one sequence of 4096 tokens:
+// of 128 rows 18, 21, 22, of 200 24, 22, 26; heads of 192, bf16, in 16 and 32: of 48 rows 33, 40, of 64 38, 41, of 72 50, 42, of 96
+// 49, 44; and 8192 rows on 8 heads 189 and 164 us in waves of 32 and 32 x 8.
 struct Kv4Plan {
   int rows;        // 4, 8, 16, 32 or 64
   int64_t tiles;   // of 4 rows, of all sequences
@@ -180,8 +181,8 @@ inline Kv4Plan kv4_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64
   // of 64 tokens (waves without rows of their own share others' tokens), to join the parts as much again, and a split has no
   // fewer. With w workgroups of the `resident` that fit a CU a round takes (resident + w) / 2 resident of a full one's time.
   // 24 sequences of up to 1024 tokens, float32 of 256, 192 workgroups: in one 27 us, in two 27, in four 37; 119 workgroups of
-  // 2558 tokens, float32 of 192: in two 31 us, in three 44, in four 49; 8 workgroups of 131072 tokens: in 32 37 us, in 64 33;
-  // 2 workgroups of 64 rows on 800 tokens: in one 37 us, in six 18; 8 ragged sequences of 300 to 2000 tokens, half of them
+  // 2558 tokens, float32 of 192: in two 31 us, in three 44, in four 49; 8 workgroups of 131072 tokens: in 32 40 us, in 64 36;
+  // 2 workgroups of 64 rows on 800 tokens (bf16, of 128): in one 37 us, in three 20; 8 ragged sequences of 300 to 2000 tokens, half of them
   // prompts: in one 89 us, in two 80, in three 73, in four 78.
   const int64_t queries = sequences > 0 ? (tokens + sequences - 1) / sequences : 0;
   const int64_t seen = window > 0 && window < (int64_t)1 << 31 && window + queries < capacity ? window + queries : capacity;

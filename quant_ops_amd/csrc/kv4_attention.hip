@@ -35,12 +35,12 @@
 // power of two that no scale of the tokens so far exceeds, is at most 2^14, in two fp16 parts (22 bits; with one a
 // bf16 output in twenty is a step off, and the second costs 2 to 3 % up to eight rows a sequence, 3 to 7 % up to 32). In
 // float32 the second parts have sums of their own: added to the first parts' they would lose what is below 2^-24 of
-// those. Maximum, sums and outputs are float32.
+// those. Weights p s below 2^-28 of S lose bits (in kv4_prefill.hip below 2^-20). Maximum, sums and outputs are float32.
 //
-// What bounds it: one sequence of 131072 tokens (64 heads on 8 of 128, bf16, 142 MB) takes 32 us, 4.4 TB/s, and
-// 262144 tokens come at the 5.0 TB/s of a copy; 64 sequences of 100 to 4096 tokens (32 on 8 heads, 146 MB) take 41 us, 3.5
-// TB/s, for which unpacking and softmax take as long as the bytes. Loads a step ahead were worth 100 -> 55 us there, lanes
-// that share scores 55 -> 46.
+// What bounds it: one sequence of 131072 tokens (64 heads on 8 of 128, bf16, 142 MB) takes 33 us, 4.3 TB/s; 64 sequences of
+// 2098 tokens (32 on 8 heads, 146 MB) take 30 us, 4.9 TB/s, where a copy reaches 5.1. The same tokens in sequences of 100 to
+// 4096 take 43 us: a workgroup each, the longest twice an even share. Loads a step ahead were worth 100 -> 55 us there,
+// lanes that share scores 55 -> 46.
 #include "dispatch_rules.h"
 #include "kv4_attention.h"
 

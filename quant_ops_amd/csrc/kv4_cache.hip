@@ -86,10 +86,10 @@ __device__ inline void turn(float& a, float& b, double c, double s) {
 }
 
 // Codes of a vector's eight values (in the low bytes of words: two by two) and its parameters. A code is the whole number
-// nearest to an estimate (v - lo) / s, which is off by 2^-19 at most (of 15, the difference and the scale's reciprocal
-// 2^-24 and 2^-23), unless that lies next to a border between codes or outside them. There (one value in 10^5, exact ties,
-// vectors whose size is far above their range) 64 bits decide: with n the whole number below the border, v - lo
-// against s (n + 1/2), which is exact.
+// nearest to an estimate (v - lo) / s, which is off by 2^-18 at most (15 1/2 times the difference's 2^-24 and the scale's
+// reciprocal's 2^-23), unless that lies within 2^-17 of a border between codes or outside them. There (one value in 10^5,
+// exact ties, vectors whose size is far above their range) 64 bits decide: with n the whole number below the border,
+// v - lo against s (n + 1/2), which is exact but for the difference's rounding to 64 bits (where v is below 2^-29 of lo).
 template <int LANES>
 __device__ inline void quantize(const float (&v)[8], bool there, uint32_t (&two)[4], _Float16& scale, _Float16& least) {
   float lo = v[0], hi = v[0];   // hi: NaN for a NaN
@@ -179,9 +179,9 @@ struct ValueBytes {
 
 // A workgroup of 256 threads takes 256 / LANES consecutive tokens of `per` heads in turn, of the queries, the keys or the
 // values (blockIdx.y counts groups of heads); a token's angles are read once for them all, and a head's values are on
-// their way while those of the head before are worked on. 8192 tokens of 32 + 8 + 8 heads of 128, bf16: 44 us, of them
-// 22 for the 16 heads with codes, as long as copying the queries alone takes (67 MB in and out, 19 us). The codes' part is
-// bound by its arithmetic, 230 vector instructions for eight values, half of them in the way through 64 bits.
+// their way while those of the head before are worked on. 8192 tokens of 32 + 8 + 8 heads of 128, bf16 (178 MB from memory):
+// 46 us; the 16 heads with codes alone 22 (44 MB), a copy of the queries alone 25 (67 MB read and 67 written). The codes'
+// part is bound by its arithmetic, 230 vector instructions for eight values, half of them in the way through 64 bits.
 template <class D, int DIM, bool PAIRS>
 __global__ void __launch_bounds__(256)
 kv4_append_kernel(KV4 cache, Heads<typename D::T> q, Heads<typename D::T> k, Heads<typename D::T> v, int64_t tokens,
@@ -299,9 +299,9 @@ kv4_append_kernel(KV4 cache, Heads<typename D::T> q, Heads<typename D::T> k, Hea
   }
 }
 
-// A thread reads eight values of a vector; blockIdx.y counts key heads, then value heads. What bounds it is the
-// writing of the values, four times the codes' bytes in 16 bits (8192 tokens, 8 heads of 128 to bf16: 15.4 us for 43 MB,
-// 2.8 TB/s; at random slots 18.7). A lane's four bytes of a value's codes are loads of their own: the lanes of 16
+// A thread reads eight values of a vector; blockIdx.y counts key heads, then value heads. 8192 tokens, 8 heads of
+// 128 to bf16: 15.4 us for 43 MB, 2.8 TB/s (at random slots 18.7): 8192 workgroups whose threads wait for a slot, then for
+// codes and parameters, and store 16 bytes once, with nothing under way beside it but other workgroups. A lane's four bytes of a value's codes are loads of their own: the lanes of 16
 // tokens share their lines, and the same through words and LDS, as they were written, took 19 us (22).
 template <class D, int DIM>
 __global__ void __launch_bounds__(256)

@@ -20,8 +20,8 @@
 //
 // A wave's 32 x 64 scores take 208 vector instructions and 32 exponentials beside 32 products (128 values,
 // bf16), on the same SIMD: products run beside the other half's softmax, but the two overlap in part only. 2048
-// queries of 32 heads on 4096 tokens (8 heads): of 128 161 us in bf16 (640 TFLOP/s of the pairs that a causal mask
-// leaves, 53% of a large product's rate) and 191 in fp16, of 64 136 and 157. Keys and values unpacked to what they stand for
+// queries of 32 heads on 4096 tokens (8 heads): of 128 164 us in bf16 (628 TFLOP/s of the pairs that a causal mask
+// leaves, 52% of a large product's rate) and 195 in fp16, of 64 143 and 162. Keys and values unpacked to what they stand for
 // in fp16 take the parameters out of the softmax (131 us in bf16), but a key's rounding then counts with its offset and
 // outliers, in an exponent: twenty times the output's own for keys about 100.
 #include "kv4_attention.h"

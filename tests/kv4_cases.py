@@ -58,11 +58,7 @@ def bound(q, out, mag, big, lengths):
     1.9e-7), a float32 query by 2^-22 in its two fp16 parts; a score takes two more float32 roundings and
     the exponent's argument two, the exponential one. d, of a weight, counts in numerator and denominator.
     A weight's rounding to fp16 is half a step, 2^-11 (2^-22 in two parts). Sums over a lane's 16 tokens a
-    step, over steps, waves and parts: a float32 rounding each. The division and the output's rounding.
-
-    Prompts in bfloat16 round keys and values to fp16 as well, 2^-11 of each at most. A value's counts like its
-    weight's rounding; a key's D roundings reach a score with signs of their own. Neither has a term here: such
-    prompts are held to the bound without, where the output's half step of 2^-8 is the largest part."""
+    step, over steps, waves and parts: a float32 rounding each. The division and the output's rounding."""
     few = q.dtype != torch.float32
     product = 2.0 ** -20 if few else 2.0 ** -22
     d = big * (product + (0 if few else 2.0 ** -22) + 2 * U) + 2 * big * 2 * U + 2 * U
